@@ -330,6 +330,35 @@ int ptpp_layernorm_bwd_add_splitk(const float* partials, int nsplit, const int32
                                   size_t scratch_bytes, void* stream);
 
 /* ------------------------------------------------------------------ *
+ * The step between two blocks of a deep encoder: the norm behind a block, its gate and residual scale, and the norm before the
+ * next block, in one launch:
+ *   u = post norm(f)              (post_g NULL: u = f)
+ *   y = x + scale * gate * u      (x NULL: no residual; gate NULL: 1)
+ *   z = pre norm(y)               (pre_g NULL: no z)
+ * f, x, y, z: (B, T, C) contiguous, `dtype`; rms 0: LayerNorm (gamma, beta f32; a beta may be NULL), 1: v / sqrt(mean(v^2) + eps)
+ * * gamma.  gate f32: (C) (gate_rows 1) or (B, C) (gate_rows B).  Rows at or behind lengths[b] (NULL: none) are not read and give
+ * zeros.  Statistics and y are f32 inside the launch; y is rounded once, and z comes from the unrounded y.
+ * C % 4 == 0, C <= 4096.  stats (4, B * T) f32: mean and 1 / deviation of f and of y (NULL in inference).
+ * Backward recomputes y from f and x (the bytes of reading y, without its rounding): dy / dz (either may be NULL: zero) ->
+ * df, dx (NULL: not wanted), and the f32 sums dpost_g, dpost_b, dpre_g, dpre_b (C), dgate (like gate), each NULL if not wanted;
+ * added to if accumulate, else overwritten; fixed order of summation through ws (ptpp_residual_norm_ws_bytes).
+ * ------------------------------------------------------------------ */
+typedef struct ptpp_residual_norm_args {
+  const void *f, *x, *dy, *dz;
+  void *y, *z, *df, *dx;
+  const float *gate, *post_g, *post_b, *pre_g, *pre_b;
+  float *dgate, *dpost_g, *dpost_b, *dpre_g, *dpre_b, *stats;
+  const int32_t* lengths;
+  void* ws;
+  size_t ws_bytes;
+  int32_t B, T, C, rms, gate_rows, accumulate, dtype;
+  float scale, eps;
+} ptpp_residual_norm_args;
+int64_t ptpp_residual_norm_ws_bytes(const ptpp_residual_norm_args* a); /* backward; < 0: bad arguments */
+int ptpp_residual_norm_fwd(const ptpp_residual_norm_args* a, void* stream);
+int ptpp_residual_norm_bwd(const ptpp_residual_norm_args* a, void* stream);
+
+/* ------------------------------------------------------------------ *
  * Relative-position multi-head attention for short sequences
  * (esp/transformer/attention.py:63-93,142-206,237-305).
  *   q,k,v: (B,T,*) rows with stride ld, head h at columns [h*dk,(h+1)*dk)
@@ -371,6 +400,47 @@ int ptpp_attention_win_bwd(const void* q, const void* k, const void* v, const fl
                            const void* dctx, float* dS, void* dq, void* dk_out, void* dv_out, float* demb_k, float* demb_v,
                            const int32_t* lengths, int B, int T, int H, int dk, int ld, int lddctx, int lddq, int window,
                            float drop_p, uint64_t drop_seed, int dtype, void* stream);
+
+/* ------------------------------------------------------------------ *
+ * Attention over long sequences: nothing of size Tq x Tk is kept, backward recomputes the probabilities from the saved
+ * statistics.  Two operators through one argument block:
+ *   maps == 1: bucketed-bias attention    out = softmax(scale q k^T + table[bucket(j - qpos_i), h]) v
+ *   maps == 2: differential attention     out = softmax(scale q0 k0^T + bias) v - lam softmax(scale q1 k1^T + bias) v,
+ *              lam_h = exp(lam[0,h] . lam[1,h]) - exp(lam[2,h] . lam[3,h]) + lam_init       (table may be NULL)
+ *   q: (B, Tq, H * maps * dk), k: (B, Tk, Hk * maps * dk), v: (B, Tk, Hk * maps * dk), out / dout: (B, Tq, H * maps * dk): rows
+ *   of contiguous channels, row strides ld* and batch strides s* in elements, 16-byte aligned; a head's maps lie side by side.
+ *   Hk divides H: query head h reads key / value head h / (H / Hk).  dk % 8 == 0, dk <= 128 (maps == 1) / 64 (maps == 2).
+ *   k_lengths / q_lengths (B) int32: keys at or behind k_lengths[b] are never read; query rows at or behind q_lengths[b] give
+ *   zeros and receive zeros.  q_start (B) int32: position of query 0 (NULL: 0), qpos_i = q_start + i.  causal: a query sees the
+ *   keys j <= qpos_i.  A query that sees no key gives zeros.
+ *   Buckets (table (nbuckets, H) f32; Raffel et al. 2020, section 2.1): bidirectional: nbuckets / 2 for j <= qpos, the others
+ *   for j > qpos; else all for the distance qpos - j (0 for later keys).  Of such a set of n buckets the first nexact = n / 2
+ *   distances have one each, distance d >= nexact lies in bucket nexact + #{t : d >= edges[t]}; edges: HOST, ascending,
+ *   n - nexact - 1 of them, in (nexact, max_distance).  max_distance <= 1024.
+ *   lse (maps, B, H, TqP) f32, TqP = Tq rounded up to 64: statistics (base 2); NULL in inference.  out2 (B, Tq, H * 2 dk),
+ *   row stride H * 2 dk: the second map's context (maps == 2, kept for backward; NULL in inference).
+ *   Forward needs a workspace of ptpp_attention_long_ws_bytes(a, 0) bytes, backward one of ..(a, 1) (0: none); the size
+ *   depends on the shapes alone, and calls that run at the same time need their own.
+ *   Backward fills dq / dk_out / dv (every row) and ADDS to dtable (nbuckets, H) / dlam (4, lam_heads, dk) f32 if accumulate,
+ *   else overwrites them; fixed order of summation.
+ * ------------------------------------------------------------------ */
+typedef struct ptpp_attention_long_args {
+  const void *q, *k, *v, *dout;
+  void *out, *out2, *dq, *dk_out, *dv;
+  const float *table, *lam;
+  float *dtable, *dlam, *lse;
+  const int32_t *k_lengths, *q_lengths, *q_start;
+  const int32_t* edges; /* HOST */
+  void* ws;
+  size_t ws_bytes;
+  int64_t sq, sk, sv, so, sdo, sdq, sdk, sdv;
+  int32_t ldq, ldk, ldv, ldo, lddo, lddq, lddk, lddv;
+  int32_t B, Tq, Tk, H, Hk, dk, maps, nbuckets, bidirectional, causal, lam_heads, max_distance, nexact, nedges, accumulate, dtype;
+  float scale, lam_init;
+} ptpp_attention_long_args;
+int64_t ptpp_attention_long_ws_bytes(const ptpp_attention_long_args* a, int backward); /* < 0: bad arguments */
+int ptpp_attention_long_fwd(const ptpp_attention_long_args* a, void* stream);
+int ptpp_attention_long_bwd(const ptpp_attention_long_args* a, void* stream);
 
 /* ------------------------------------------------------------------ *
  * Length regulator as a gather / segment-sum instead of the reference's

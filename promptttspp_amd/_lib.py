@@ -58,6 +58,29 @@ class TtsLossArgs(Structure):
                [(n, c_float) for n in ("dec_scale", "lp_min", "ls_min")]
 
 
+class AttentionLongArgs(Structure):
+    """Mirror of ``ptpp_attention_long_args`` (include/ptpp.h)."""
+
+    _fields_ = [(n, c_void_p) for n in ("q", "k", "v", "dout", "out", "out2", "dq", "dk_out", "dv", "table", "lam", "dtable", "dlam", "lse",
+                                        "k_lengths", "q_lengths", "q_start", "edges", "ws")] + \
+               [("ws_bytes", ctypes.c_size_t)] + \
+               [(n, c_int64) for n in ("sq", "sk", "sv", "so", "sdo", "sdq", "sdk", "sdv")] + \
+               [(n, c_int32) for n in ("ldq", "ldk", "ldv", "ldo", "lddo", "lddq", "lddk", "lddv", "B", "Tq", "Tk", "H", "Hk", "dk", "maps",
+                                       "nbuckets", "bidirectional", "causal", "lam_heads", "max_distance", "nexact", "nedges", "accumulate",
+                                       "dtype")] + \
+               [("scale", c_float), ("lam_init", c_float)]
+
+
+class ResidualNormArgs(Structure):
+    """Mirror of ``ptpp_residual_norm_args`` (include/ptpp.h)."""
+
+    _fields_ = [(n, c_void_p) for n in ("f", "x", "dy", "dz", "y", "z", "df", "dx", "gate", "post_g", "post_b", "pre_g", "pre_b", "dgate",
+                                        "dpost_g", "dpost_b", "dpre_g", "dpre_b", "stats", "lengths", "ws")] + \
+               [("ws_bytes", ctypes.c_size_t)] + \
+               [(n, c_int32) for n in ("B", "T", "C", "rms", "gate_rows", "accumulate", "dtype")] + \
+               [("scale", c_float), ("eps", c_float)]
+
+
 class AmpLayerArgs(Structure):
     """Mirror of ``ptpp_amp_layer_args`` (include/ptpp.h)."""
 
@@ -367,6 +390,12 @@ SIGNATURES = {
     "ptpp_durations_cumsum": (I, [P, I, P, I, I, P]),
     "ptpp_bcast_add_rows": (I, [P, P, P, I, I, I, I, P]),
     "ptpp_rows_sum": (I, [P, P, I, I, I, I, P]),
+    "ptpp_attention_long_ws_bytes": (I64, [POINTER(AttentionLongArgs), I]),
+    "ptpp_attention_long_fwd": (I, [POINTER(AttentionLongArgs), P]),
+    "ptpp_attention_long_bwd": (I, [POINTER(AttentionLongArgs), P]),
+    "ptpp_residual_norm_ws_bytes": (I64, [POINTER(ResidualNormArgs)]),
+    "ptpp_residual_norm_fwd": (I, [POINTER(ResidualNormArgs), P]),
+    "ptpp_residual_norm_bwd": (I, [POINTER(ResidualNormArgs), P]),
     "ptpp_comm_unique_id": (I, [P]),
     "ptpp_comm_init": (I, [I, I, P, POINTER(c_void_p)]),
     "ptpp_comm_destroy": (I, [P]),

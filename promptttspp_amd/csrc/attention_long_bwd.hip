@@ -1,0 +1,550 @@
+// Backward of the attention kernels for long sequences (mathematics and layout: attention_long.h).  Two passes that each own what
+// they write -- no atomics on memory, the same bits on every run -- and one small launch for the parameter gradients:
+//   attn_long_dq_kernel   owns 128 queries, streams keys and values: dq, and D_m[i] = sum_j P_m dP in f32
+//   attn_long_dkv_kernel  owns 128 keys, streams queries and dout:   dk, dv, per-block sums of the table's gradient
+//   attn_long_fin_kernel  adds the per-block sums of dtable and dlam in a fixed order
+// The price of the second pass is 2 of 7 products (4 of 14 units with two maps); one pass would need f32 atomics on dq.
+//
+// D_m: rows of dout . out_m give it only to the rounding of the kept 16-bit context.  That is enough to centre dS, but the table's
+// gradient is a sum with heavy cancellation (every row of dS adds up to zero), so the dq pass also sums P_m (dP - D_m') in f32 and
+// the dk / dv pass uses the corrected D_m.
+#include "attention_long.h"
+
+namespace {
+
+template <typename E, int DK, int DV, int MAPS, bool BIAS>
+__global__ __launch_bounds__(256) void attn_long_dq_kernel(const LongP p) {
+  constexpr int CH = LOp<E>::CH, KS = DK / (2 * CH), VS = DV / (2 * CH), PS = 16 / CH, NT = DK / 32;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ float lred[LA_WAVES];
+  constexpr int KIMG = LA_TILE * DK, VIMG = LA_TILE * DV, BUF = MAPS * KIMG + VIMG;
+  E* const img = reinterpret_cast<E*>(smem);
+  float* const btab = reinterpret_cast<float*>(smem + 2 * BUF * sizeof(E));
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lq = lane & 31, hw = lane >> 5;
+
+  const int t = xcd_remap(blockIdx.x, gridDim.x);
+  const int qt = t % p.nqt, bh = t / p.nqt, h = bh % p.H, b = bh / p.H, hk = h / (p.H / p.Hk);
+  const int klen = la_klen(p, b), qlen = la_qlen(p, b), qs = la_qstart(p, b);
+  const int ib = qt * (LA_OWN * LA_WAVES), i0 = ib + wave * LA_OWN, iq = i0 + lq;
+  const int dv = MAPS * p.dk;
+  int kend = ib < qlen ? klen : 0;
+  if (p.causal) kend = min(kend, max(0, qs + min(ib + LA_OWN * LA_WAVES, qlen)));
+  const int nt = (kend + LA_TILE - 1) / LA_TILE;
+
+  const E* kb = reinterpret_cast<const E*>(p.k) + b * p.sk + (int64_t)hk * MAPS * p.dk;
+  const E* vb = reinterpret_cast<const E*>(p.v) + b * p.sv + (int64_t)hk * dv;
+  LTile<E, DK> kt;
+  LTile<E, DV> vt;
+  kt.init(p.ldk, p.dk, lane, wave);
+  vt.init(p.ldv, dv, lane, wave);
+  constexpr int NDMA = MAPS * LTile<E, DK>::NI + LTile<E, DV>::NI;
+  auto issue = [&](int tile, int buf) {
+    const int j0 = tile * LA_TILE;
+    E* d = img + buf * BUF;
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m) kt.issue(kb + (int64_t)j0 * p.ldk + m * p.dk, kend - j0, d + m * KIMG, lane, wave);
+    vt.issue(vb + (int64_t)j0 * p.ldv, kend - j0, d + MAPS * KIMG, lane, wave);
+  };
+  if (nt > 0) issue(0, 0);
+  if constexpr (BIAS) la_fill_btab(p, btab, h);
+  float lam = 0.f;
+  if constexpr (MAPS == 2) lam = la_lambda(p, h, lane);
+
+  uint4 qf[MAPS][KS], df[VS];
+  float Dm[MAPS], lse[MAPS], eps[MAPS];
+  {
+    const bool on = iq < qlen;
+    const E* qb = reinterpret_cast<const E*>(p.q) + b * p.sq + (int64_t)h * MAPS * p.dk + (int64_t)iq * p.ldq;
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m)
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const int c = (2 * s + hw) * CH;
+        qf[m][s] = (on && c < p.dk) ? *reinterpret_cast<const uint4*>(qb + m * p.dk + c) : uint4{0, 0, 0, 0};
+      }
+    const E* db = reinterpret_cast<const E*>(p.dout) + b * p.sdo + (int64_t)h * dv + (int64_t)iq * p.lddo;
+    const E* ob = reinterpret_cast<const E*>(p.out) + b * p.so + (int64_t)h * dv + (int64_t)iq * p.ldo;
+    const E* o2 = reinterpret_cast<const E*>(p.out2) + ((int64_t)b * p.Tq + iq) * ((int64_t)p.H * dv) + (int64_t)h * dv;
+    float d0 = 0.f, d1 = 0.f;
+#pragma unroll
+    for (int s = 0; s < VS; ++s) {
+      const int c = (2 * s + hw) * CH;
+      df[s] = uint4{0, 0, 0, 0};
+      if (on && c < dv) {
+        df[s] = *reinterpret_cast<const uint4*>(db + c);
+        d0 += la_dot<E>(df[s], *reinterpret_cast<const uint4*>(ob + c));
+        if constexpr (MAPS == 2) d1 += la_dot<E>(df[s], *reinterpret_cast<const uint4*>(o2 + c));
+      }
+    }
+    d0 = la_half_sum(d0);
+    Dm[0] = d0;
+    if constexpr (MAPS == 2) {  // out = out_0 - lam out_1
+      d1 = la_half_sum(d1);
+      Dm[0] = fmaf(lam, d1, d0);
+      Dm[MAPS - 1] = d1;
+    }
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m) {
+      lse[m] = on ? p.lse[(((int64_t)m * p.B + b) * p.H + h) * p.TqP + iq] : INFINITY;
+      eps[m] = 0.f;
+    }
+  }
+  f32x16 acc[MAPS][NT];
+#pragma unroll
+  for (int m = 0; m < MAPS; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[m][n] = f32x16{};
+  const float c2 = p.scale * LA_LOG2E;
+  const int q0 = qs + i0, D = p.max_distance;
+
+  for (int tile = 0; tile < nt; ++tile) {
+    const int buf = tile & 1;
+    if (tile + 1 < nt) {
+      issue(tile + 1, buf ^ 1);
+      glds_wait<NDMA>();
+    } else {
+      glds_wait<0>();
+    }
+    la_barrier();
+    const E* kimg = img + buf * BUF;
+    const E* vimg = kimg + MAPS * KIMG;
+#pragma unroll 1
+    for (int ks = 0; ks < 2; ++ks) {
+      const int j0 = tile * LA_TILE + 32 * ks;
+      f32x16 dp = f32x16{};
+#pragma unroll
+      for (int kk = 0; kk < VS; ++kk) dp = LOp<E>::mma(la_frag<E, DV>(vimg, 32 * ks + lq, 2 * kk + hw), df[kk], dp);
+#pragma unroll
+      for (int m = 0; m < MAPS; ++m) {
+        f32x16 s = f32x16{};
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk) s = LOp<E>::mma(la_frag<E, DK>(kimg + m * KIMG, 32 * ks + lq, 2 * kk + hw), qf[m][kk], s);
+        if constexpr (BIAS) {
+          const int dmin = j0 - (q0 + 31), dmax = j0 + 31 - q0;
+          if (dmin < D && dmax > -D) {
+            const float* bt = btab + (j0 - q0 - lq + 4 * hw + D + LA_PAD);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, bt[8 * (r >> 2) + (r & 3)]) - lse[m];
+          } else {
+            const float bc = (dmin >= D ? btab[2 * (D + LA_PAD)] : btab[0]) - lse[m];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, bc);
+          }
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, -lse[m]);
+        }
+        if (j0 + 32 > kend || (p.causal && j0 + 31 > q0)) {
+          const int jend = min(klen, p.causal ? q0 + lq + 1 : klen) - j0 - 4 * hw;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] = 8 * (r >> 2) + (r & 3) < jend ? s[r] : -INFINITY;
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[r] = la_exp2(s[r]) * (dp[r] - Dm[m]);
+          eps[m] += s[r];
+        }
+#pragma unroll
+        for (int st = 0; st < PS; ++st) {
+          const uint4 f = la_pack<E>(s, st);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) acc[m][n] = LOp<E>::mma(la_tfrag<E, DK>(kimg + m * KIMG, 32 * ks, st, n, lane), f, acc[m][n]);
+        }
+      }
+    }
+    la_barrier();
+  }
+
+#pragma unroll
+  for (int m = 0; m < MAPS; ++m) {
+    Dm[m] += la_half_sum(eps[m]);
+    if (hw == 0 && iq < p.TqP) p.D[(((int64_t)m * p.B + b) * p.H + h) * p.TqP + iq] = iq < qlen ? Dm[m] : 0.f;
+  }
+  if constexpr (MAPS == 2) {  // this block's share of dlam = -sum_i D_1
+    const float s = wave_sum(hw == 0 && iq < qlen ? Dm[MAPS - 1] : 0.f);
+    if (lane == 0) lred[wave] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) p.lam_part[(int64_t)bh * p.nqt + qt] = -((lred[0] + lred[1]) + (lred[2] + lred[3]));
+  }
+  if (iq >= p.Tq) return;
+  E* qo = reinterpret_cast<E*>(p.dq) + b * p.sdq + (int64_t)h * MAPS * p.dk + (int64_t)iq * p.lddq;
+#pragma unroll
+  for (int m = 0; m < MAPS; ++m) {
+    const float c = m == 0 ? p.scale : -lam * p.scale;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int ch = 32 * n + 8 * g + 4 * hw;
+        if (ch < p.dk)
+          la_store4<E>(qo + m * p.dk + ch, acc[m][n][4 * g] * c, acc[m][n][4 * g + 1] * c, acc[m][n][4 * g + 2] * c, acc[m][n][4 * g + 3] * c);
+      }
+  }
+}
+
+// Distances [lo, hi] of bucket bk, clipped to what the sums below hold; false: none
+__device__ __forceinline__ bool la_bucket_range(const LongP& p, int bk, int& lo, int& hi) {
+  const int far = p.max_distance + LA_PAD, half = p.bidirectional ? p.nbuckets / 2 : p.nbuckets;
+  const bool pos = bk >= half;
+  const int b = pos ? bk - half : bk;
+  const int n0 = b <= p.nexact ? b : p.edges[b - p.nexact - 1];
+  const int n1 = b < p.nexact ? b : (b - p.nexact < p.nedges ? p.edges[b - p.nexact] - 1 : far);
+  if (pos) {
+    lo = max(n0, 1);
+    hi = n1;
+  } else {
+    lo = -n1;
+    hi = (!p.bidirectional && b == 0) ? far : -n0;
+  }
+  return lo <= hi;
+}
+
+// One block = 128 keys of one (utterance, key head), a wave = 32 of them; the queries of every head of the group stream through LDS.
+// Table gradient: a wave adds dS along its patches' diagonals into its own two copies (one per half wave) of a distance-indexed
+// array in LDS -- the 32 lanes of a half wave hold 32 different distances of one register, so no two lanes ever meet -- and patches
+// beyond max_distance go into two registers.
+template <typename E, int DK, int DV, int MAPS, bool BIAS>
+__global__ __launch_bounds__(256) void attn_long_dkv_kernel(const LongP p) {
+  constexpr int CH = LOp<E>::CH, KS = DK / (2 * CH), VS = DV / (2 * CH), PS = 16 / CH, NK = DK / 32, NV = DV / 32;
+  constexpr bool F32 = sizeof(E) == 4;  // (its fragments fill the register file: the scheduler must not fetch further ahead)
+  constexpr int NBUF = sizeof(E) == 4 ? 1 : 2;  // (f32 tiles twice and the widest distance array would pass 160 KiB)
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  constexpr int QIMG = LA_TILE * DK, OIMG = LA_TILE * DV;
+  constexpr int BUFB = (MAPS * QIMG + OIMG) * (int)sizeof(E) + 1024;  // + (lse, D) of every map, 64 floats each
+  float* const btab = reinterpret_cast<float*>(smem + NBUF * BUFB);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lk = lane & 31, hw = lane >> 5;
+  const int dist_n = la_btab_len(p);
+  float* const hist = btab + ((dist_n + 3) & ~3);  // [8][dist_n]
+  float* const myhist = hist + (2 * wave + hw) * dist_n;
+
+  const int t = xcd_remap(blockIdx.x, gridDim.x);
+  const int kt = t % p.nkt, bh = t / p.nkt, hk = bh % p.Hk, b = bh / p.Hk, G = p.H / p.Hk;
+  const int klen = la_klen(p, b), qlen = la_qlen(p, b), qs = la_qstart(p, b);
+  const int jb = kt * (LA_OWN * LA_WAVES), j0 = jb + wave * LA_OWN, jk = j0 + lk;
+  const int dv = MAPS * p.dk;
+  const int t0 = p.causal ? max(0, jb - qs) / LA_TILE : 0;  // first tile with a query that sees a key of the block
+  const int ntq = jb < klen ? max(0, (qlen + LA_TILE - 1) / LA_TILE - t0) : 0;
+  const int total = ntq * G;
+
+  const E* qb = reinterpret_cast<const E*>(p.q) + b * p.sq;
+  const E* ob = reinterpret_cast<const E*>(p.dout) + b * p.sdo;
+  LTile<E, DK> qt;
+  LTile<E, DV> ot;
+  qt.init(p.ldq, p.dk, lane, wave);
+  ot.init(p.lddo, dv, lane, wave);
+  constexpr int NDMA = MAPS * LTile<E, DK>::NI + LTile<E, DV>::NI + 1;
+  auto issue = [&](int it, int buf) {
+    const int h = hk * G + it / ntq, i0 = (t0 + it % ntq) * LA_TILE;
+    char* d = smem + buf * BUFB;
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m)
+      qt.issue(qb + (int64_t)i0 * p.ldq + (h * MAPS + m) * p.dk, qlen - i0, reinterpret_cast<E*>(d) + m * QIMG, lane, wave);
+    ot.issue(ob + (int64_t)i0 * p.lddo + h * dv, qlen - i0, reinterpret_cast<E*>(d) + MAPS * QIMG, lane, wave);
+    // statistics: 16 lanes per array (lse_0, D_0, lse_1, D_1); every wave issues the same copy so that all count alike
+    const int arr = lane >> 4, m = arr >> 1;
+    const float* src = ((arr & 1) ? p.D : p.lse) + (((int64_t)m * p.B + b) * p.H + h) * p.TqP + i0 + 4 * (lane & 15);
+    glds16(m < MAPS ? (const void*)src : (const void*)g_conv_zero_page, __builtin_amdgcn_readfirstlane(lds_addr(d + (MAPS * QIMG + OIMG) * sizeof(E))));
+  };
+  if (NBUF == 2 && total > 0) issue(0, 0);
+
+  // the wave's keys and values: lane (key lk, chunk 2 s + hw)
+  uint4 kf[MAPS][KS], vf[VS];
+  {
+    const bool on = jk < klen;
+    const E* kb = reinterpret_cast<const E*>(p.k) + b * p.sk + (int64_t)hk * MAPS * p.dk + (int64_t)jk * p.ldk;
+    const E* vb = reinterpret_cast<const E*>(p.v) + b * p.sv + (int64_t)hk * dv + (int64_t)jk * p.ldv;
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m)
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const int c = (2 * s + hw) * CH;
+        kf[m][s] = (on && c < p.dk) ? *reinterpret_cast<const uint4*>(kb + m * p.dk + c) : uint4{0, 0, 0, 0};
+      }
+#pragma unroll
+    for (int s = 0; s < VS; ++s) {
+      const int c = (2 * s + hw) * CH;
+      vf[s] = (on && c < dv) ? *reinterpret_cast<const uint4*>(vb + c) : uint4{0, 0, 0, 0};
+    }
+  }
+  f32x16 ak[MAPS][NK], av[NV];
+#pragma unroll
+  for (int m = 0; m < MAPS; ++m)
+#pragma unroll
+    for (int n = 0; n < NK; ++n) ak[m][n] = f32x16{};
+#pragma unroll
+  for (int n = 0; n < NV; ++n) av[n] = f32x16{};
+  const float c2 = p.scale * LA_LOG2E;
+  const int D = p.max_distance;
+  float far_lo = 0.f, far_hi = 0.f, lam = 0.f;
+
+  // end of a head: this block's sums per bucket
+  auto flush = [&](int h) {
+    la_barrier();
+    const float lo = wave_sum(far_lo), hi = wave_sum(far_hi);
+    if (lane == 0) {  // the two outermost entries, which no near patch reaches
+      hist[2 * wave * dist_n] = lo;
+      hist[2 * wave * dist_n + dist_n - 1] = hi;
+    }
+    la_barrier();
+    for (int i = threadIdx.x; i < dist_n; i += 256) {
+      float s = 0.f;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) s += hist[c * dist_n + i];
+      hist[i] = s;
+    }
+    la_barrier();
+    for (int bk = wave; bk < p.nbuckets; bk += LA_WAVES) {
+      int lo_d, hi_d;
+      float s = 0.f;
+      if (la_bucket_range(p, bk, lo_d, hi_d))
+        for (int d = max(lo_d, -D - LA_PAD) + lane; d <= min(hi_d, D + LA_PAD); d += 64) s += hist[d + D + LA_PAD];
+      s = wave_sum(s);
+      if (lane == 0) p.tab_part[(((int64_t)b * p.nkt + kt) * p.H + h) * p.nbuckets + bk] = s;
+    }
+    la_barrier();
+  };
+
+  for (int g = 0; g < G; ++g) {
+    const int h = hk * G + g;
+    if constexpr (BIAS) {
+      la_fill_btab(p, btab, h);
+      for (int i = threadIdx.x; i < 8 * dist_n; i += 256) hist[i] = 0.f;
+      far_lo = far_hi = 0.f;
+    }
+    if constexpr (MAPS == 2) lam = la_lambda(p, h, lane);
+    for (int iq = 0; iq < ntq; ++iq) {
+      const int it = g * ntq + iq, buf = NBUF == 2 ? it & 1 : 0;
+      if (NBUF == 1) {
+        issue(it, 0);
+        glds_wait<0>();
+      } else if (it + 1 < total) {
+        issue(it + 1, buf ^ 1);
+        glds_wait<NDMA>();
+      } else {
+        glds_wait<0>();
+      }
+      la_barrier();
+      const E* qimg = reinterpret_cast<const E*>(smem + buf * BUFB);
+      const E* oimg = qimg + MAPS * QIMG;
+      const float* stat = reinterpret_cast<const float*>(oimg + OIMG);
+#pragma unroll 1
+      for (int sub = 0; sub < 2; ++sub) {
+        const int i0 = (t0 + iq) * LA_TILE + 32 * sub, q0 = qs + i0;
+        const int ln = F32 ? la_opaque(lane) : lane, lr = ln & 31, hr = ln >> 5;
+        f32x16 dp = f32x16{}, w = f32x16{}, hsum = f32x16{};
+#pragma unroll
+        for (int kk = 0; kk < VS; ++kk) {
+          dp = LOp<E>::mma(la_frag<E, DV>(oimg, 32 * sub + lr, 2 * kk + hr), vf[kk], dp);
+          if (F32 && kk % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+        }
+        const int dmin = j0 - (q0 + 31), dmax = j0 + 31 - q0;
+        const bool near = BIAS && dmin < D && dmax > -D;
+#pragma unroll
+        for (int m = 0; m < MAPS; ++m) {
+          f32x16 s = f32x16{};
+#pragma unroll
+          for (int kk = 0; kk < KS; ++kk) {
+            s = LOp<E>::mma(la_frag<E, DK>(qimg + m * QIMG, 32 * sub + lr, 2 * kk + hr), kf[m][kk], s);
+            if (F32 && kk % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+          }
+          const float* ls = stat + 2 * m * 64 + 32 * sub + 4 * hw;
+          if (near) {
+            const float* bt = btab + (jk - q0 - 4 * hw + D + LA_PAD);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, bt[-(8 * (r >> 2) + (r & 3))]) - ls[8 * (r >> 2) + (r & 3)];
+          } else {
+            const float bc = BIAS ? (dmin >= D ? btab[dist_n - 1] : btab[0]) : 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, bc - ls[8 * (r >> 2) + (r & 3)]);
+          }
+          if (p.causal && dmax > 0) {
+            const int qmin = jk - q0 - 4 * hw;  // register r's query sees the key from this row on
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = 8 * (r >> 2) + (r & 3) >= qmin ? s[r] : -INFINITY;
+          }
+          f32x16 ds;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float Dr = ls[64 + 8 * (r >> 2) + (r & 3)];
+            float pr = la_exp2(s[r]);
+            if (m == 1) pr *= -lam;
+            w[r] += pr;
+            ds[r] = pr * (dp[r] - Dr);
+            if constexpr (BIAS) hsum[r] += ds[r];
+          }
+#pragma unroll
+          for (int st = 0; st < PS; ++st) {
+            const uint4 f = la_pack<E>(ds, st);
+#pragma unroll
+            for (int n = 0; n < NK; ++n) ak[m][n] = LOp<E>::mma(la_tfrag<E, DK>(qimg + m * QIMG, 32 * sub, st, n, ln), f, ak[m][n]);
+            if (F32) __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+#pragma unroll
+        for (int st = 0; st < PS; ++st) {
+          const uint4 f = la_pack<E>(w, st);
+#pragma unroll
+          for (int n = 0; n < NV; ++n) av[n] = LOp<E>::mma(la_tfrag<E, DV>(oimg, 32 * sub, st, n, ln), f, av[n]);
+          if (F32) __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (BIAS) {
+          // (a column behind the keys holds unmasked values: it must not count; its dk / dv rows are written as zeros)
+          if (near) {
+            float* hp = myhist + (jk - q0 - 4 * hw + D + LA_PAD);
+            if (jk < klen) {
+#pragma unroll
+              for (int r = 0; r < 16; ++r) __hip_atomic_fetch_add(hp - (8 * (r >> 2) + (r & 3)), hsum[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            }
+          } else {
+            float s = 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s += hsum[r];
+            s = jk < klen ? s : 0.f;
+            if (dmin >= D) far_hi += s;
+            else far_lo += s;
+          }
+        }
+      }
+      la_barrier();
+    }
+    if constexpr (BIAS) flush(h);
+  }
+
+  if (jk >= p.Tk) return;
+  const bool on = jk < klen;
+  E* ko = reinterpret_cast<E*>(p.gk) + b * p.sdk + (int64_t)hk * MAPS * p.dk + (int64_t)jk * p.lddk;
+  E* vo = reinterpret_cast<E*>(p.gv) + b * p.sdv + (int64_t)hk * dv + (int64_t)jk * p.lddv;
+#pragma unroll
+  for (int m = 0; m < MAPS; ++m)
+#pragma unroll
+    for (int n = 0; n < NK; ++n)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int ch = 32 * n + 8 * g + 4 * hw;
+        if (ch < p.dk) {
+          float v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = on ? ak[m][n][4 * g + e] * p.scale : 0.f;
+          la_store4<E>(ko + m * p.dk + ch, v[0], v[1], v[2], v[3]);
+        }
+      }
+#pragma unroll
+  for (int n = 0; n < NV; ++n)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int ch = 32 * n + 8 * g + 4 * hw;
+      if (ch < dv) {
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = on ? av[n][4 * g + e] : 0.f;
+        la_store4<E>(vo + ch, v[0], v[1], v[2], v[3]);
+      }
+    }
+}
+
+// blocks [0, H) (with a table): one head's column of dtable; the rest: one head's (or the shared) lam vectors
+__global__ __launch_bounds__(256) void attn_long_fin_kernel(const LongP p, float* dtable, float* dlam, int accumulate) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int ntab = p.table ? p.H : 0;
+  if ((int)blockIdx.x < ntab) {
+    const int h = blockIdx.x, n = p.B * p.nkt;
+    for (int bk = wave; bk < p.nbuckets; bk += LA_WAVES) {
+      float s = 0.f;
+      for (int i = lane; i < n; i += 64) s += p.tab_part[((int64_t)i * p.H + h) * p.nbuckets + bk];
+      s = wave_sum(s);
+      float* d = dtable + (int64_t)bk * p.H + h;
+      if (lane == 0) *d = accumulate ? *d + s : s;
+    }
+    return;
+  }
+  __shared__ float red[LA_WAVES];
+  const int hh = blockIdx.x - ntab, per = p.lam_heads > 1 ? 1 : p.H;  // query heads that share these vectors
+  const int64_t n = (int64_t)p.B * per * p.nqt;
+  float s = 0.f;
+  for (int64_t i = threadIdx.x; i < n; i += 256) {
+    const int64_t b = i / (per * p.nqt), r = i % (per * p.nqt);
+    s += p.lam_part[(b * p.H + hh) * p.nqt + r];
+  }
+  s = wave_sum(s);
+  if (lane == 0) red[wave] = s;
+  __syncthreads();
+  if (wave != 0) return;
+  const float gl = (red[0] + red[1]) + (red[2] + red[3]);
+  float e1, e2;
+  la_lambda_parts(p, hh, lane, e1, e2);
+  if (lane < p.dk) {
+    const int64_t nn = (int64_t)p.lam_heads * p.dk, o = (int64_t)hh * p.dk + lane;
+    const float g[4] = {gl * e1 * p.lam[nn + o], gl * e1 * p.lam[o], -gl * e2 * p.lam[3 * nn + o], -gl * e2 * p.lam[2 * nn + o]};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float* d = dlam + i * nn + o;
+      *d = accumulate ? *d + g[i] : g[i];
+    }
+  }
+}
+
+template <typename E, int DK, int DV, int MAPS, bool BIAS>
+int launch_bwd(const LongP& p, hipStream_t st) {
+  const size_t tiles = (size_t)LA_TILE * (MAPS * DK + DV) * sizeof(E);
+  const int dn = BIAS ? 2 * (p.max_distance + LA_PAD) + 1 : 0;
+  const size_t s1 = 2 * tiles + ((dn + 3) & ~3) * sizeof(float);
+  const size_t s2 = (sizeof(E) == 4 ? 1 : 2) * (tiles + 1024) + (((dn + 3) & ~3) + 8 * (size_t)dn) * sizeof(float);
+  if (s1 > 64 * 1024 && !ptpp_lds_limit((const void*)attn_long_dq_kernel<E, DK, DV, MAPS, BIAS>, (int)s1, "attention_long_bwd")) return PTPP_ELAUNCH;
+  if (s2 > 64 * 1024 && !ptpp_lds_limit((const void*)attn_long_dkv_kernel<E, DK, DV, MAPS, BIAS>, (int)s2, "attention_long_bwd")) return PTPP_ELAUNCH;
+  hipLaunchKernelGGL((attn_long_dq_kernel<E, DK, DV, MAPS, BIAS>), dim3((unsigned)((int64_t)p.nqt * p.B * p.H)), dim3(256), s1, st, p);
+  PTPP_CHECK_LAUNCH("attention_long_bwd (dq)");
+  hipLaunchKernelGGL((attn_long_dkv_kernel<E, DK, DV, MAPS, BIAS>), dim3((unsigned)((int64_t)p.nkt * p.B * p.Hk)), dim3(256), s2, st, p);
+  PTPP_CHECK_LAUNCH("attention_long_bwd (dk, dv)");
+  return PTPP_OK;
+}
+template <typename E, int DK, int DV>
+int launch_bwd2(const LongP& p, hipStream_t st) {
+  return p.table ? launch_bwd<E, DK, DV, 2, true>(p, st) : launch_bwd<E, DK, DV, 2, false>(p, st);
+}
+template <typename E>
+int dispatch_bwd(const LongP& p, int maps, hipStream_t st) {
+  if (maps == 1) return p.dk <= 64 ? launch_bwd<E, 64, 64, 1, true>(p, st) : launch_bwd<E, 128, 128, 1, true>(p, st);
+  return p.dk <= 32 ? launch_bwd2<E, 32, 64>(p, st) : launch_bwd2<E, 64, 128>(p, st);
+}
+
+int64_t up64(int64_t n) { return (n + 63) & ~(int64_t)63; }
+// backward workspace, floats: D | lam_part | tab_part
+void bwd_layout(const LongP& p, int maps, int64_t* o_lam, int64_t* o_tab, int64_t* total) {
+  *o_lam = up64((int64_t)maps * p.B * p.H * p.TqP);
+  *o_tab = *o_lam + (maps == 2 ? up64((int64_t)p.B * p.H * p.nqt) : 0);
+  *total = *o_tab + (p.table ? up64((int64_t)p.B * p.nkt * p.H * p.nbuckets) : 0);
+}
+
+}  // namespace
+
+int64_t ptpp_attention_long_ws_bwd(const LongP& p, int maps) {
+  int64_t a, b, n;
+  bwd_layout(p, maps, &a, &b, &n);
+  return n * (int64_t)sizeof(float);
+}
+
+extern "C" int ptpp_attention_long_bwd(const ptpp_attention_long_args* a, void* stream) {
+  LongP p;
+  const int rc = ptpp_attention_long_params(a, 1, &p, "attention_long_bwd");
+  if (rc != PTPP_OK) return rc;
+  PTPP_CHECK_ARG(a->lse && (uintptr_t)a->lse % 16 == 0, "attention_long_bwd: needs the statistics of the forward pass (16-byte aligned)");
+  PTPP_CHECK_ARG(a->maps == 1 || a->out2, "attention_long_bwd: needs the second map's context");
+  PTPP_CHECK_ARG((!a->table || a->dtable) && (a->maps == 1 || a->dlam), "attention_long_bwd: null gradient");
+  int64_t o_lam, o_tab, total;
+  bwd_layout(p, a->maps, &o_lam, &o_tab, &total);
+  PTPP_CHECK_ARG(a->ws && (uintptr_t)a->ws % 16 == 0 && a->ws_bytes >= (size_t)total * sizeof(float),
+                 "attention_long_bwd: workspace of %zu bytes, needs %lld (16-byte aligned)", a->ws_bytes, (long long)(total * sizeof(float)));
+  p.D = reinterpret_cast<float*>(a->ws);
+  p.lam_part = p.D + o_lam;
+  p.tab_part = p.D + o_tab;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  int r;
+  if (a->dtype == PTPP_F32) r = dispatch_bwd<float>(p, a->maps, st);
+  else if (a->dtype == PTPP_BF16) r = dispatch_bwd<bf16_raw>(p, a->maps, st);
+  else r = dispatch_bwd<f16_raw>(p, a->maps, st);
+  if (r != PTPP_OK) return r;
+  const int blocks = (p.table ? p.H : 0) + (a->maps == 2 ? p.lam_heads : 0);
+  hipLaunchKernelGGL(attn_long_fin_kernel, dim3(blocks), dim3(256), 0, st, p, a->dtable, a->dlam, a->accumulate);
+  PTPP_CHECK_LAUNCH("attention_long_bwd (parameters)");
+  return PTPP_OK;
+}

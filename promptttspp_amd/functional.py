@@ -1004,6 +1004,179 @@ def attention(qkv, pos, bias_u, bias_v, lengths, heads, variant, drop_p=0.0):
 
 
 # ----------------------------------------------------------------------------
+# Attention over long sequences (csrc/attention_long_*.hip): O(T) memory, probabilities recomputed in backward.
+# ----------------------------------------------------------------------------
+def _param_sinks(params):
+    """The parameters themselves if every one's gradient can be accumulated in place (direct mode), else None."""
+    return params if params and all(_sink(p) is not None for p in params) else None
+
+
+class AttentionLongFn(Function):
+    @staticmethod
+    def forward(ctx, q, k, v, table, lam, cfg):
+        op = _attention_long_op(q, k, v, _f32c(table), _f32c(lam), cfg)
+        out, lse, out2 = op.forward(True)
+        ctx.cfg = cfg
+        ctx.direct = _param_sinks([p for p in (table, lam) if p is not None])
+        for p in ctx.direct or ():
+            _use(p)
+        ctx.save_for_backward(q, k, v, table, lam, out, lse, out2)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, table, lam, out, lse, out2 = ctx.saved_tensors
+        op = _attention_long_op(q, k, v, _f32c(table), _f32c(lam), ctx.cfg)
+        if not dout.is_contiguous() or dout.data_ptr() % 16:
+            dout = dout.clone(memory_format=torch.contiguous_format)
+        dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        dk = dv = None
+        if k is None:
+            parts = _split_qkv(dq, ctx.cfg)
+        else:
+            dk = torch.empty(k.shape, device=k.device, dtype=k.dtype)
+            dv = torch.empty(v.shape, device=v.device, dtype=v.dtype)
+            parts = dq, dk, dv
+        direct = ctx.direct is not None
+        grads = [None if p is None else p.grad if direct else torch.empty(p.shape, device=p.device, dtype=torch.float32) for p in (table, lam)]
+        op.backward(out, lse, out2, dout, *parts, *grads, accumulate=direct)
+        if direct:
+            for p in ctx.direct:
+                _done(p)
+            grads = [None, None]
+        dt, dl = (g if g is None or g.dtype == p.dtype else g.to(p.dtype) for g, p in zip(grads, (table, lam)))
+        return dq, dk, dv, dt, dl, None
+
+
+def _split_qkv(qkv, cfg):
+    """views of a fused (B, T, q | k | v) projection; the key / value parts are kv_heads / heads as wide as the query's"""
+    unit = qkv.shape[2] // (cfg.heads + 2 * cfg.kv_heads)
+    if qkv.shape[2] != unit * (cfg.heads + 2 * cfg.kv_heads):
+        raise ValueError(f"attention: {qkv.shape[2]} channels do not split into q of {cfg.heads} and k, v of {cfg.kv_heads} heads")
+    return qkv.split([unit * cfg.heads, unit * cfg.kv_heads, unit * cfg.kv_heads], dim=2)
+
+
+def _attention_long_op(q, k, v, table, lam, cfg):
+    if k is None:
+        q, k, v = _split_qkv(q, cfg)
+    return ops.AttentionLong(q, k, v, cfg.heads, cfg.kv_heads, cfg.maps, table=table, max_distance=cfg.max_distance,
+                             bidirectional=cfg.bidirectional, lam=lam, lam_init=cfg.lam_init, lengths=cfg.lengths, q_lengths=cfg.q_lengths,
+                             q_start=cfg.q_start, causal=cfg.causal, scale=cfg.scale)
+
+
+def _attention_long(q, k, v, table, lam, cfg):
+    if (k is None) != (v is None):
+        raise ValueError("attention: give q, k, v, or one fused q | k | v tensor and neither k nor v")
+    if k is None and cfg.q_lengths is None:
+        cfg.q_lengths = cfg.lengths
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, table, lam)):
+        return AttentionLongFn.apply(q, k, v, table, lam, cfg)
+    return _attention_long_op(q, k, v, _f32c(table), _f32c(lam), cfg).forward(False)[0]
+
+
+def attention_bucket(q, k, v, table, heads, kv_heads=None, max_distance=128, bidirectional=True, lengths=None, q_lengths=None, q_start=None,
+                     causal=False, scale=None):
+    """Attention with a learned relative-position bias by buckets: softmax(scale * q k^T + table[bucket(j - i), head]) v -> (B, Tq, H * dk).
+
+    q (B, Tq, heads * dk), k / v (B, Tk, kv_heads * dk): contiguous channels, any row and batch stride, 16-byte aligned rows (slices of
+    a fused projection as they are); ``k = v = None``: q is the fused (B, T, q | k | v) projection of self-attention.  Query head h
+    reads key / value head h // (heads // kv_heads).  dk: a multiple of 8, at most 128; f32, bf16 or f16.  ``table`` (buckets, heads):
+    bucket of a distance as ``ops.bucket_edges`` (two-sided; ``bidirectional=False``: later keys share bucket 0).
+    ``lengths`` (B): valid keys (None: all); ``q_lengths`` (B): valid queries, the others give zeros (None: as ``lengths`` for the fused
+    form, else all); rows behind them are never read.  ``q_start`` (B): position of the first query among the keys (None: 0) -- a step
+    of one query against a kept memory of n keys has ``q_start = n - 1``; ``causal``: only keys at or before the query's position.
+    A query that sees no key gives zeros.  ``scale``: positive, default dk ** -0.5.  Memory O(Tq + Tk) in both directions."""
+    if table is None:
+        raise ValueError("attention_bucket: needs a position table")
+    cfg = SimpleNamespace(heads=heads, kv_heads=kv_heads or heads, maps=1, max_distance=max_distance, bidirectional=bidirectional, lam_init=0.0,
+                          lengths=lengths, q_lengths=q_lengths, q_start=q_start, causal=causal, scale=scale)
+    return _attention_long(q, k, v, table, None, cfg)
+
+
+def attention_diff(q, k, v, lam, lam_init, heads, kv_heads=None, table=None, max_distance=128, bidirectional=True, lengths=None, q_lengths=None,
+                   q_start=None, causal=False, scale=None):
+    """Differential attention: (softmax(scale * q0 k0^T + bias) - lam_h * softmax(scale * q1 k1^T + bias)) v -> (B, Tq, H * 2 dk), with
+    lam_h = exp(lam[0, h] . lam[1, h]) - exp(lam[2, h] . lam[3, h]) + lam_init.
+
+    q (B, Tq, heads * 2 dk), k / v (B, Tk, kv_heads * 2 dk): a head's two maps lie side by side in q and k, its value is 2 dk wide; dk a
+    multiple of 8, at most 64.  ``lam`` (4, 1 or heads, dk).  ``table`` (optional): the position bias of ``attention_bucket``, the same for
+    both maps.  Everything else as there.  The norm over a head that usually follows is ``residual_norm`` without a residual."""
+    if lam is None:
+        raise ValueError("attention_diff: needs the lam vectors")
+    cfg = SimpleNamespace(heads=heads, kv_heads=kv_heads or heads, maps=2, max_distance=max_distance, bidirectional=bidirectional,
+                          lam_init=lam_init, lengths=lengths, q_lengths=q_lengths, q_start=q_start, causal=causal, scale=scale)
+    return _attention_long(q, k, v, table, lam, cfg)
+
+
+class ResidualNormFn(Function):
+    @staticmethod
+    def forward(ctx, f, x, gate, post_g, post_b, pre_g, pre_b, cfg):
+        ctx.set_materialize_grads(False)
+        f = f.contiguous()
+        x = x.contiguous() if x is not None else None
+        params = (gate, post_g, post_b, pre_g, pre_b)
+        y, z, stats = _residual_norm_op(f, x, params, cfg).forward(True)
+        ctx.cfg = cfg
+        want = [p for p, n in zip(params, ctx.needs_input_grad[2:7]) if n]
+        ctx.direct = _param_sinks(want)
+        for p in ctx.direct or ():
+            _use(p)
+        ctx.save_for_backward(f, x, *params, stats)
+        if z is None:
+            return y
+        return y, z
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dz=None):
+        f, x, *params, stats = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        op = _residual_norm_op(f, x, params, ctx.cfg)
+        dy, dz = (None if t is None else t.contiguous() for t in (dy, dz))
+        direct = ctx.direct is not None
+        sums = [None if not n else p.grad.view(_flat(p)) if direct else torch.empty(_flat(p), device=p.device, dtype=torch.float32)
+                for p, n in zip(params, need[2:7])]
+        df, dx = op.backward(stats, dy, dz, need[0], need[1], sums, accumulate=direct)
+        if direct:
+            for p in ctx.direct:
+                _done(p)
+            sums = [None] * 5
+        return (df, dx, *(None if s is None else s.view(p.shape).to(p.dtype) for s, p in zip(sums, params)), None)
+
+
+def _flat(p):
+    """a gate keeps its (B, C) rows; everything else is a vector, whatever unit dimensions the parameter carries"""
+    return tuple(p.shape) if p.dim() == 2 and p.shape[0] != 1 else (p.numel(),)
+
+
+def _residual_norm_op(f, x, params, cfg):
+    gate, post_g, post_b, pre_g, pre_b = (None if p is None else _f32c(p).reshape(_flat(p)) for p in params)
+    if gate is not None and gate.dim() == 1 and f.shape[0] > 1 and gate.numel() != f.shape[2]:
+        raise ValueError(f"residual_norm: a gate of {f.shape[2]} channels, or ({f.shape[0]}, {f.shape[2]}), expected, got {tuple(params[0].shape)}")
+    return ops.ResidualNorm(f, x, gate, (post_g, post_b), (pre_g, pre_b), cfg.scale, cfg.eps, cfg.kind, cfg.lengths)
+
+
+def residual_norm(f, x=None, gate=None, post=None, pre=None, scale=1.0, eps=1e-5, kind="layer", lengths=None):
+    """The step between two blocks: u = post(f), y = x + scale * gate * u, z = pre(y) -> (y, z), one launch each way.
+
+    f: a block's output, x: the residual stream (None: y = scale * gate * u), both (B, T, C) of one dtype (f32, bf16, f16), C a multiple
+    of 4, at most 4096.  ``post`` / ``pre``: (gamma, beta) of the norm behind the block and of the norm before the next one, or None (no
+    such norm; without ``pre`` z is None); ``kind``: "layer", or "rms" (beta None).  ``gate``: None, (C,) or one row per utterance (B, C),
+    f32.  Rows at or behind ``lengths`` (B) are not read, give zeros and get zero gradients.  y is rounded to the tensors' dtype once; z is
+    computed from the unrounded y."""
+    post_g, post_b = post if post is not None else (None, None)
+    pre_g, pre_b = pre if pre is not None else (None, None)
+    cfg = SimpleNamespace(scale=scale, eps=eps, kind=kind, lengths=lengths)
+    params = (gate, post_g, post_b, pre_g, pre_b)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (f, x, *params)):
+        r = ResidualNormFn.apply(f, x, *params, cfg)
+        return r if pre_g is not None else (r, None)
+    y, z, _ = _residual_norm_op(f.contiguous(), None if x is None else x.contiguous(), params, cfg).forward(False)
+    return y, z
+
+
+# ----------------------------------------------------------------------------
 FUSED_L1 = not os.environ.get("PTPP_NO_FUSED_L1")  # (A/B knob: the tensor-op form of the L1 losses)
 
 

@@ -9,6 +9,7 @@ Layout: activations are channels-last ``(B, T, C)`` contiguous tensors in the
 compute dtype (torch.float32 or torch.bfloat16).
 """
 import ctypes
+import functools
 import struct
 
 import torch
@@ -611,6 +612,229 @@ def attention_win_bwd(q, k, v, emb_k, emb_v, probs, dctx, lengths, heads, window
                                              int(window), float(drop_p), int(drop_seed), dtype_code(q.dtype), _stream()),
           "ptpp_attention_win_bwd")
     return dek, dev_
+
+
+# ----------------------------------------------------------------------------
+# attention over long sequences: learned bucketed position bias (maps = 1), differential (maps = 2)
+# ----------------------------------------------------------------------------
+@functools.lru_cache(maxsize=None)
+def bucket_edges(num_buckets, max_distance, bidirectional):
+    """(exact distances, int32 array of the logarithmic buckets' first distances) of a relative-position table (Raffel et al. 2020):
+    of a direction's n buckets the first e = n // 2 distances have one each; distance d >= e lies in bucket
+    e + floor(log(d / e) / log(max_distance / e) * (n - e)), at most n - 1.  Solved in whole numbers (d^(n-e) e^t >= D^t e^(n-e)),
+    so that a border never depends on how a logarithm was rounded."""
+    n = num_buckets // 2 if bidirectional else num_buckets
+    if num_buckets < 2 or num_buckets > 128 or n < 2 or (bidirectional and num_buckets % 2):
+        raise ValueError(f"relative-position buckets: {num_buckets} (2 to 128, two or more per direction, even if bidirectional)")
+    e = n // 2
+    if not e < max_distance <= 1024:
+        raise ValueError(f"relative-position buckets: max_distance {max_distance} (more than {e}, at most 1024)")
+    steps, edges, d = n - e, [], e
+    for t in range(1, steps):
+        while d ** steps * e ** t < max_distance ** t * e ** steps:
+            d += 1
+        edges.append(d)
+    return e, (ctypes.c_int32 * max(1, len(edges)))(*edges), len(edges)
+
+
+def _here(t, what):
+    """a ROCm tensor of the device that the launch goes to (the current one)"""
+    _need_gpu(t)
+    if t.device.index != torch.cuda.current_device():
+        raise _lib.PtppError(f"promptttspp_amd: {what} lies on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _rows(t, what, B, T, C, dtype):
+    """checks of a (B, T, C) operand with contiguous channels and any row / batch stride; -> (batch stride, row stride)"""
+    _here(t, what)
+    if t.dim() != 3 or tuple(t.shape) != (B, T, C) or t.dtype != dtype:
+        raise ValueError(f"{what}: expected a ({B}, {T}, {C}) {dtype} tensor, got {tuple(t.shape)} {t.dtype}")
+    if t.stride(2) != 1 and C > 1:
+        raise ValueError(f"{what}: channels must be contiguous")
+    return (t.stride(0) if B > 1 else T * t.stride(1) if T > 1 else C), (t.stride(1) if T > 1 else C)
+
+
+def _f32_operand(t, what, shape, like):
+    _here(t, what)
+    if t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{what}: expected a contiguous {shape} float32 tensor, got {tuple(t.shape)} {t.dtype}")
+    if t.device != like.device:
+        raise ValueError(f"{what}: on {t.device}, the activations on {like.device}")
+    return _ptr(t)
+
+
+def _i32_rows(t, what, B, like):
+    if t is None:
+        return None
+    if tuple(t.shape) != (B,):
+        raise ValueError(f"{what}: expected {B} entries, got {tuple(t.shape)}")
+    if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
+        raise ValueError(f"{what}: whole numbers expected, got {t.dtype}")
+    return i32(t, like.device)
+
+
+class AttentionLong:
+    """Shapes and options of one call of the long-sequence attention kernels: built once, used by forward and backward."""
+
+    def __init__(self, q, k, v, heads, kv_heads, maps, table=None, max_distance=128, bidirectional=True, lam=None, lam_init=0.0, lengths=None,
+                 q_lengths=None, q_start=None, causal=False, scale=None):
+        for t, n in ((q, "q"), (k, "k"), (v, "v")):
+            if t.dim() != 3:
+                raise ValueError(f"{n}: expected a (B, T, channels) tensor")
+        B, Tq, Cq = q.shape
+        Tk, Ck = k.shape[1], k.shape[2]
+        if heads < 1 or kv_heads < 1 or heads % kv_heads:
+            raise ValueError(f"attention: {kv_heads} key / value heads do not divide {heads} query heads")
+        dk = Cq // (heads * maps)
+        if B < 1 or Tq < 1 or Tk < 1:
+            raise ValueError("attention: empty batch or sequence")
+        if Cq != heads * maps * dk or dk % 8 or not 8 <= dk <= (128 if maps == 1 else 64):
+            raise ValueError(f"attention: {Cq} query channels for {heads} heads of {maps} map(s): the width of one map must be a multiple of 8, "
+                             f"at most {128 if maps == 1 else 64}")
+        self.shape = B, Tq, Tk, heads, kv_heads, dk, maps
+        self.width = heads * maps * dk
+        kw = kv_heads * maps * dk
+        a = self.args = _lib.AttentionLongArgs()
+        a.sq, a.ldq = _rows(q, "q", B, Tq, self.width, q.dtype)
+        a.sk, a.ldk = _rows(k, "k", B, Tk, kw, q.dtype)
+        a.sv, a.ldv = _rows(v, "v", B, Tk, kw, q.dtype)
+        a.q, a.k, a.v = _ptr(q), _ptr(k), _ptr(v)
+        a.B, a.Tq, a.Tk, a.H, a.Hk, a.dk, a.maps = B, Tq, Tk, heads, kv_heads, dk, maps
+        a.dtype = dtype_code(q.dtype)
+        a.causal = int(bool(causal))
+        a.scale = float(scale) if scale is not None else dk ** -0.5
+        if not 0.0 < a.scale < 1e30:
+            raise ValueError(f"attention: scale {scale} must be positive and finite")
+        self.table, self.lam = table, lam
+        if table is not None:
+            if table.dim() != 2 or table.shape[1] != heads:
+                raise ValueError(f"attention: a position table of shape (buckets, {heads}) expected, got {tuple(table.shape)}")
+            a.nbuckets, a.bidirectional, a.max_distance = table.shape[0], int(bool(bidirectional)), int(max_distance)
+            a.nexact, self._edges, a.nedges = bucket_edges(a.nbuckets, a.max_distance, bool(bidirectional))
+            a.edges = ctypes.addressof(self._edges)
+            a.table = _f32_operand(table, "table", tuple(table.shape), q)
+        if maps == 2:
+            if lam.dim() != 3 or lam.shape[0] != 4 or lam.shape[1] not in (1, heads) or lam.shape[2] != dk:
+                raise ValueError(f"attention: lam of shape (4, 1 or {heads}, {dk}) expected, got {tuple(lam.shape)}")
+            a.lam, a.lam_heads, a.lam_init = _f32_operand(lam, "lam", tuple(lam.shape), q), lam.shape[1], float(lam_init)
+        self._ints = [_i32_rows(t, n, B, q) for t, n in ((lengths, "lengths"), (q_lengths, "q_lengths"), (q_start, "q_start"))]
+        a.k_lengths, a.q_lengths, a.q_start = (_ptr(t) for t in self._ints)
+        self.device, self.dtype = q.device, q.dtype
+
+    def _workspace(self, backward):
+        n = _lib.load().ptpp_attention_long_ws_bytes(ctypes.byref(self.args), backward)
+        check(-1 if n < 0 else 0, "ptpp_attention_long_ws_bytes")
+        w = torch.empty(n, device=self.device, dtype=torch.uint8) if n else None  # (this call's own: two captured graphs never share it)
+        self.args.ws, self.args.ws_bytes = _ptr(w), n
+        return w
+
+    def forward(self, keep):
+        """-> (out, lse, out2); the last two only with ``keep`` (what backward needs)"""
+        B, Tq, _, H, _, dk, maps = self.shape
+        a = self.args
+        out = torch.empty((B, Tq, self.width), device=self.device, dtype=self.dtype)
+        lse = out2 = None
+        if keep:
+            lse = torch.empty((maps, B, H, (Tq + 63) // 64 * 64), device=self.device, dtype=torch.float32)
+            out2 = torch.empty_like(out) if maps == 2 else None
+        a.out, a.so, a.ldo, a.lse, a.out2 = _ptr(out), Tq * self.width, self.width, _ptr(lse), _ptr(out2)
+        ws = self._workspace(0)
+        check(_lib.load().ptpp_attention_long_fwd(ctypes.byref(a), _stream()), "ptpp_attention_long_fwd")
+        del ws
+        return out, lse, out2
+
+    def backward(self, out, lse, out2, dout, dq, dk, dv, dtable=None, dlam=None, accumulate=False):
+        """fills dq / dk / dv (views with contiguous channels) and dtable / dlam (added to with ``accumulate``)"""
+        B, Tq, Tk, H, Hk, d, maps = self.shape
+        a = self.args
+        kw = Hk * maps * d
+        a.sdo, a.lddo = _rows(dout, "dout", B, Tq, self.width, self.dtype)
+        a.so, a.ldo = _rows(out, "out", B, Tq, self.width, self.dtype)
+        a.sdq, a.lddq = _rows(dq, "dq", B, Tq, self.width, self.dtype)
+        a.sdk, a.lddk = _rows(dk, "dk", B, Tk, kw, self.dtype)
+        a.sdv, a.lddv = _rows(dv, "dv", B, Tk, kw, self.dtype)
+        a.out, a.lse, a.out2, a.dout, a.dq, a.dk_out, a.dv = (_ptr(t) for t in (out, lse, out2, dout, dq, dk, dv))
+        a.dtable = _f32_operand(dtable, "dtable", tuple(self.table.shape), dq) if self.table is not None else None
+        a.dlam = _f32_operand(dlam, "dlam", tuple(self.lam.shape), dq) if maps == 2 else None
+        a.accumulate = int(bool(accumulate))
+        ws = self._workspace(1)
+        check(_lib.load().ptpp_attention_long_bwd(ctypes.byref(a), _stream()), "ptpp_attention_long_bwd")
+        del ws
+
+
+# ----------------------------------------------------------------------------
+# norm behind a block, gate, residual scale, norm before the next block
+# ----------------------------------------------------------------------------
+class ResidualNorm:
+    """Shapes and options of one call of the residual-norm kernels: y = x + scale * gate * post(f), z = pre(y)."""
+
+    def __init__(self, f, x=None, gate=None, post=(None, None), pre=(None, None), scale=1.0, eps=1e-5, kind="layer", lengths=None):
+        if kind not in ("layer", "rms"):
+            raise ValueError(f"residual_norm: kind {kind!r} ('layer' or 'rms')")
+        if f.dim() != 3:
+            raise ValueError("residual_norm: expected a (B, T, C) tensor")
+        B, T, C = f.shape
+        if B < 1 or T < 1 or C < 1 or C % 4 or C > 4096:
+            raise ValueError(f"residual_norm: shape {tuple(f.shape)} (C a multiple of 4, at most 4096, nothing empty)")
+        if not eps > 0.0:
+            raise ValueError("residual_norm: eps must be positive")
+        a = self.args = _lib.ResidualNormArgs()
+        for t, n in ((f, "f"), (x, "x")):
+            if t is not None:
+                self._dense(t, n, f)
+        a.f, a.x = _ptr(f), _ptr(x)
+        self.f, self.x = f, x
+        if gate is not None and tuple(gate.shape) not in ((C,), (B, C)):
+            raise ValueError(f"residual_norm: a gate of shape ({C},) or ({B}, {C}) expected, got {tuple(gate.shape)}")
+        self.gate, self.post, self.pre = gate, post, pre
+        if gate is not None:
+            a.gate, a.gate_rows = _f32_operand(gate, "gate", tuple(gate.shape), f), (gate.shape[0] if gate.dim() == 2 else 1)
+        for n, (g, b) in (("post", post), ("pre", pre)):
+            if b is not None and (g is None or kind == "rms"):
+                raise ValueError(f"residual_norm: {n} beta without a gamma, or with root-mean-square norms")
+            if g is not None:
+                setattr(a, n + "_g", _f32_operand(g, n + " gamma", (C,), f))
+            if b is not None:
+                setattr(a, n + "_b", _f32_operand(b, n + " beta", (C,), f))
+        self._len = _i32_rows(lengths, "lengths", B, f)
+        a.lengths = _ptr(self._len)
+        a.B, a.T, a.C, a.rms, a.dtype = B, T, C, int(kind == "rms"), dtype_code(f.dtype)
+        a.scale, a.eps = float(scale), float(eps)
+
+    @staticmethod
+    def _dense(t, what, like):
+        _here(t, what)
+        if t.shape != like.shape or t.dtype != like.dtype or not t.is_contiguous():
+            raise ValueError(f"residual_norm: {what} must be a contiguous {tuple(like.shape)} {like.dtype} tensor, got {tuple(t.shape)} {t.dtype}")
+
+    def forward(self, keep):
+        """-> (y, z or None, statistics or None)"""
+        a, f = self.args, self.f
+        y = torch.empty_like(f)
+        z = torch.empty_like(f) if self.pre[0] is not None else None
+        stats = torch.empty((4, f.shape[0] * f.shape[1]), device=f.device, dtype=torch.float32) if keep else None
+        a.y, a.z, a.stats = _ptr(y), _ptr(z), _ptr(stats)
+        check(_lib.load().ptpp_residual_norm_fwd(ctypes.byref(a), _stream()), "ptpp_residual_norm_fwd")
+        return y, z, stats
+
+    def backward(self, stats, dy, dz, want_df, want_dx, sums, accumulate=False):
+        """``sums``: f32 buffers (or None) for (gate, post gamma, post beta, pre gamma, pre beta).  -> (df, dx)"""
+        a, f = self.args, self.f
+        for t, n in ((dy, "dy"), (dz, "dz")):
+            if t is not None:
+                self._dense(t, n, f)
+        df = torch.empty_like(f) if want_df else None
+        dx = torch.empty_like(f) if want_dx else None
+        a.dy, a.dz, a.df, a.dx, a.stats = _ptr(dy), _ptr(dz), _ptr(df), _ptr(dx), _ptr(stats)
+        for n, t, p in zip(("dgate", "dpost_g", "dpost_b", "dpre_g", "dpre_b"), sums, (self.gate, *self.post, *self.pre)):
+            setattr(a, n, _f32_operand(t, n, tuple(p.shape), f) if t is not None else None)
+        a.accumulate = int(bool(accumulate))
+        n = _lib.load().ptpp_residual_norm_ws_bytes(ctypes.byref(a))
+        check(-1 if n < 0 else 0, "ptpp_residual_norm_ws_bytes")
+        ws = torch.empty(n, device=f.device, dtype=torch.uint8) if n else None
+        a.ws, a.ws_bytes = _ptr(ws), n
+        check(_lib.load().ptpp_residual_norm_bwd(ctypes.byref(a), _stream()), "ptpp_residual_norm_bwd")
+        return df, dx
 
 
 # ----------------------------------------------------------------------------

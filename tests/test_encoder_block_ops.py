@@ -1,0 +1,855 @@
+"""Attention over long sequences (learned bucketed position bias, differential) and the norm / gate / residual step against plain
+64-bit implementations, with element-wise error bounds from the roundings that the kernels make:
+
+* u = eps / 2 of the element type: outputs are rounded once; in 16-bit types the probabilities and dS are rounded once more as
+  operands of the matrix instructions, which moves a sum over keys by at most u * sum |term|;
+* rho: the relative error of a probability computed in f32 -- a dot product of dk terms, a fused multiply-add, the statistics and
+  an exponential of an argument of size a are off by at most (dk + 16) * 2^-24 * a, which enters as a relative error of p.
+"""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from conftest import ROOT  # noqa: F401
+
+DT = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def half_ulp(dt):
+    return torch.finfo(dt).eps / 2
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# plain forms in 64 bits (CPU)
+# ---------------------------------------------------------------------------------------------------------------------
+def ref_bucket(dist, n_all, max_distance, bidirectional):
+    n = n_all // 2 if bidirectional else n_all
+    e = n // 2
+    out = torch.empty_like(dist)
+    for val in dist.unique().tolist():
+        a = abs(val) if bidirectional else max(-val, 0)
+        if a < e:
+            b = a
+        else:
+            b = e
+            while b < n - 1 and a ** (n - e) * e ** (b + 1 - e) >= max_distance ** (b + 1 - e) * e ** (n - e):
+                b += 1
+        out[dist == val] = b + (n if bidirectional and val > 0 else 0)
+    return out
+
+
+class RefAttention:
+    """Everything of one call in 64 bits, utterance by utterance and head by head, plus the sums that the error bounds need."""
+
+    def __init__(self, q, k, v, table, lam, lam_init, dout, heads, kv_heads, maps, max_distance=128, bidirectional=True, lengths=None,
+                 q_lengths=None, q_start=None, causal=False, scale=None, dt=torch.float32):
+        B, Tq, Tk = q.shape[0], q.shape[1], k.shape[1]
+        dk = q.shape[2] // heads // maps
+        dv = maps * dk
+        q = q.double().reshape(B, Tq, heads, maps, dk)
+        k = k.double().reshape(B, Tk, kv_heads, maps, dk)
+        v = v.double().reshape(B, Tk, kv_heads, dv)
+        do = dout.double().reshape(B, Tq, heads, dv) if dout is not None else None
+        u = half_ulp(dt)
+        up = u if dt != torch.float32 else 2.0 ** -24   # probabilities / dS as operands
+        f = 2.0 ** -24
+        scale = scale if scale is not None else dk ** -0.5
+        z = torch.zeros
+        self.out, self.out_b = z(B, Tq, heads, dv, dtype=torch.float64), z(B, Tq, heads, dv, dtype=torch.float64)
+        self.g = {n: torch.zeros_like(t) for n, t in (("dq", q), ("dk", k), ("dv", v))}
+        self.b = {n: torch.zeros_like(t) for n, t in (("dq", q), ("dk", k), ("dv", v))}
+        if table is not None:
+            self.g["dtable"], self.b["dtable"] = torch.zeros_like(table, dtype=torch.float64), torch.zeros_like(table, dtype=torch.float64)
+        dlam, dlam_b = z(heads, dtype=torch.float64), z(heads, dtype=torch.float64)
+        for b in range(B):
+            nk = Tk if lengths is None else min(max(int(lengths[b]), 0), Tk)
+            nq = Tq if q_lengths is None else min(max(int(q_lengths[b]), 0), Tq)
+            if nq == 0 or nk == 0:
+                continue
+            i = torch.arange(nq) + (int(q_start[b]) if q_start is not None else 0)
+            dist = torch.arange(nk)[None] - i[:, None]
+            see = torch.ones(nq, nk, dtype=torch.bool) if not causal else dist <= 0
+            bk = ref_bucket(dist, table.shape[0], max_distance, bidirectional) if table is not None else None
+            for h in range(heads):
+                kh = h // (heads // kv_heads)
+                ps, rhos = [], []
+                L = 0.0
+                if maps == 2:
+                    lv = lam.double()[:, min(h, lam.shape[1] - 1)]
+                    L = float((lv[0] @ lv[1]).exp() - (lv[2] @ lv[3]).exp() + lam_init)
+                for m in range(maps):
+                    s = q[b, :nq, h, m] @ k[b, :nk, kh, m].T * scale
+                    mag = (q[b, :nq, h, m].abs() @ k[b, :nk, kh, m].abs().T * scale).amax()
+                    if table is not None:
+                        s = s + table.double()[:, h][bk]
+                        mag = mag + table.double().abs().max()
+                    s = s.masked_fill(~see, -math.inf)
+                    mx = s.amax(-1, keepdim=True)
+                    e = (s - torch.where(mx.isfinite(), mx, torch.zeros_like(mx))).exp()
+                    l = e.sum(-1, keepdim=True)
+                    ps.append(e / torch.where(l > 0, l, torch.ones_like(l)))
+                    rhos.append(float((dk + 16) * f * (2 * mag + 4)) + nk * f * 0.05)
+                c = [1.0, -L]
+                vb = v[b, :nk, kh]
+                w = sum(c[m] * ps[m] for m in range(maps))
+                wa = sum(abs(c[m]) * ps[m] for m in range(maps))
+                rho = max(rhos)
+                self.out[b, :nq, h] = w @ vb
+                self.out_b[b, :nq, h] = (up + rho + 8 * f) * (wa @ vb.abs()) + u * (w @ vb).abs()
+                if do is None:
+                    continue
+                dob = do[b, :nq, h]
+                dp = dob @ vb.T
+                dpe = (dob.abs() @ vb.abs().T) * (dv * f)             # dP in f32
+                self.g["dv"][b, :nk, kh] += w.T @ dob
+                self.b["dv"][b, :nk, kh] += (up + rho + (16 + 0.05 * nq) * f) * (wa.T @ dob.abs())
+                oe = (u + up + rho) * (wa @ vb.abs())                  # kept contexts: what centres dS in the dq pass
+                De1 = (oe * dob.abs()).sum(-1, keepdim=True) * (1 + abs(L))
+                for m in range(maps):
+                    D = (ps[m] * dp).sum(-1, keepdim=True)
+                    ds = c[m] * ps[m] * (dp - D)
+                    mag = ps[m] * (dp.abs() + D.abs())
+                    De = (rho + 32 * f) * mag.sum(-1, keepdim=True) + (ps[m] * dpe).sum(-1, keepdim=True)   # corrected D, f32
+                    # dS in f32 (corrected D): relative error of p, the error of dP and of D
+                    dse = abs(c[m]) * (rho * mag + ps[m] * (dpe + De) + 4 * f * mag)
+                    kb, qb = k[b, :nk, kh, m], q[b, :nq, h, m]
+                    self.g["dq"][b, :nq, h, m] = scale * (ds @ kb)
+                    self.b["dq"][b, :nq, h, m] = scale * ((dse + up * (ds.abs() + abs(c[m]) * ps[m] * De1)) @ kb.abs()
+                                                          + abs(c[m]) * (ps[m] * De1) @ kb.abs()
+                                                          + (16 + 0.05 * nk) * f * ds.abs() @ kb.abs()) + u * scale * (ds @ kb).abs()
+                    self.g["dk"][b, :nk, kh, m] += scale * (ds.T @ qb)
+                    self.b["dk"][b, :nk, kh, m] += scale * ((dse + up * ds.abs() + (16 + 0.05 * nq) * f * ds.abs()).T @ qb.abs())
+                    if table is not None:
+                        nb = table.shape[0]
+                        add = lambda t: torch.zeros(nb, dtype=torch.float64).index_add_(0, bk.reshape(-1), t.reshape(-1))  # noqa: E731
+                        self.g["dtable"][:, h] += add(ds)
+                        self.b["dtable"][:, h] += add(dse + 64 * f * ds.abs())
+                    if m == 1:
+                        dlam[h] -= D.sum()
+                        dlam_b[h] += De.sum() + 64 * f * D.abs().sum()
+        for n in ("dk", "dv"):  # rounded once, after the heads that share them have been added
+            self.b[n] = self.b[n] + u * self.g[n].abs()
+        if maps == 2 and do is not None:
+            per = heads // lam.shape[1]
+            G = dlam.view(lam.shape[1], per).sum(1)[:, None] if per > 1 else dlam[:, None]
+            Gb = dlam_b.view(lam.shape[1], per).sum(1)[:, None] if per > 1 else dlam_b[:, None]
+            lv = lam.double()
+            e1, e2 = (lv[0] * lv[1]).sum(-1, keepdim=True).exp(), (lv[2] * lv[3]).sum(-1, keepdim=True).exp()
+            self.g["dlam"] = torch.stack([G * e1 * lv[1], G * e1 * lv[0], -G * e2 * lv[3], -G * e2 * lv[2]])
+            B_ = (Gb + 16 * dk * f * G.abs())
+            self.b["dlam"] = torch.stack([B_ * e1 * lv[1].abs(), B_ * e1 * lv[0].abs(), B_ * e2 * lv[3].abs(), B_ * e2 * lv[2].abs()])
+        self.out, self.out_b = self.out.flatten(2), self.out_b.flatten(2)
+        for n, fl in (("dq", (B, Tq, -1)), ("dk", (B, Tk, -1)), ("dv", (B, Tk, -1))):
+            self.g[n], self.b[n] = self.g[n].reshape(fl), self.b[n].reshape(fl)
+
+
+def within(got, ref, bound, what):
+    got = got.detach().double().cpu()
+    assert got.shape == ref.shape, (what, got.shape, ref.shape)
+    assert bool(torch.isfinite(got).all()), f"{what}: not finite"
+    bad = (got - ref).abs() - (bound + 1e-30)
+    worst = float(bad.max()) if bad.numel() else 0.0
+    at = int(bad.argmax()) if bad.numel() else 0
+    assert worst <= 0, f"{what}: off by {float((got - ref).abs().flatten()[at]):.3e} where {float(bound.flatten()[at]):.3e} is allowed (value {float(ref.flatten()[at]):.3e})"
+
+
+def make(maps, dt, B, Tq, Tk, heads, kv_heads, dk, buckets, seed=0, lam_heads=1, fused=False):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    q, k, v = r(B, Tq, heads * maps * dk).to(dt), r(B, Tk, kv_heads * maps * dk).to(dt), r(B, Tk, kv_heads * maps * dk).to(dt)
+    table = (0.7 * r(buckets, heads)) if buckets else None
+    lam = 0.3 * r(4, lam_heads, dk) if maps == 2 else None
+    return q, k, v, table, lam, r(B, Tq, heads * maps * dk).to(dt)
+
+
+def call(maps, q, k, v, table, lam, heads, **kw):
+    from promptttspp_amd import functional as PF
+
+    if maps == 2:
+        return PF.attention_diff(q, k, v, lam, 0.35, heads, table=table, **kw)
+    return PF.attention_bucket(q, k, v, table, heads, **kw)
+
+
+def check_attention(dev, maps, dtype, B, Tq, Tk, heads, kv_heads, dk, buckets, lam_heads=1, seed=0, fused=False, garbage=False, train=True, **kw):
+    dt = DT[dtype]
+    q, k, v, table, lam, dout = make(maps, dt, B, Tq, Tk, heads, kv_heads, dk, buckets, seed, lam_heads)
+    rkw = dict(kw)
+    if fused:
+        rkw.setdefault("q_lengths", kw.get("lengths"))
+    ref = RefAttention(q, k, v, table, lam, 0.35, dout if train else None, heads, kv_heads, maps, dt=dt, **rkw)
+    if garbage:  # whatever lies behind the lengths must not be read
+        for t, n in ((k, kw.get("lengths")), (v, kw.get("lengths")), (q, rkw.get("q_lengths")), (dout, rkw.get("q_lengths"))):
+            for b in range(B):
+                if n is not None:
+                    t[b, max(int(n[b]), 0):] = float("nan") if b % 2 else float("inf")
+    kwd = {n: (torch.tensor(t, device=dev, dtype=torch.int32) if isinstance(t, (list, tuple)) else t) for n, t in kw.items()}
+    if kv_heads != heads:
+        kwd["kv_heads"] = kv_heads
+    leaf = lambda t: None if t is None else t.to(dev).requires_grad_(train)  # noqa: E731
+    table_d, lam_d = leaf(table), leaf(lam)
+    if fused:
+        qkv = leaf(torch.cat([q, k, v], dim=2))
+        out = call(maps, qkv, None, None, table_d, lam_d, heads, **kwd)
+        leaves = [qkv]
+    else:
+        leaves = [leaf(q), leaf(k), leaf(v)]
+        out = call(maps, *leaves, table_d, lam_d, heads, **kwd)
+    within(out, ref.out, ref.out_b, "out")
+    if not train:
+        return
+    extra = [t for t in (table_d, lam_d) if t is not None]
+    grads = torch.autograd.grad(out, leaves + extra, dout.to(dev))
+    names = (["dtable"] if table is not None else []) + (["dlam"] if maps == 2 else [])
+    for n, t in zip(names, grads[len(leaves):]):
+        within(t, ref.g[n], ref.b[n], n)
+    parts = grads[0].split([q.shape[2], k.shape[2], v.shape[2]], dim=2) if fused else grads[:3]
+    for n, t in zip(("dq", "dk", "dv"), parts):
+        within(t, ref.g[n], ref.b[n], n)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("maps,dk", [(1, 64), (1, 128), (2, 32), (2, 64)])
+@pytest.mark.parametrize("T", [1, 2, 33, 129, 200])
+def test_self_attention_sizes(dev, dtype, maps, dk, T):
+    check_attention(dev, maps, dtype, 2, T, T, 2, 2, dk, 32, fused=True, lengths=[T, max(1, T - 37)])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("maps", [1, 2])
+@pytest.mark.parametrize("Tq,Tk", [(1, 300), (16, 65), (17, 64), (63, 1), (65, 127), (128, 31), (31, 257), (130, 128)])
+def test_cross_attention_sizes(dev, dtype, maps, Tq, Tk):
+    check_attention(dev, maps, dtype, 2, Tq, Tk, 2, 1, 32, 16, lam_heads=2, q_start=[5, -3])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("maps,dk", [(1, 8), (1, 40), (1, 80), (1, 120), (2, 8), (2, 16), (2, 40), (2, 56)])
+def test_odd_head_widths(dev, dtype, maps, dk):
+    check_attention(dev, maps, dtype, 2, 70, 90, 3, 3, dk, 8, lengths=[90, 41])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("maps", [1, 2])
+def test_rows_without_keys_and_garbage_behind_the_lengths(dev, dtype, maps):
+    """lengths of zero and one, NaN and infinities behind them, queries before the first key under the causal rule"""
+    check_attention(dev, maps, dtype, 5, 70, 140, 2, 2, 64, 32, garbage=True, lengths=[140, 0, 1, 65, 64], q_lengths=[70, 70, 1, 0, 33],
+                    q_start=[-40, 0, 0, 3, 100], causal=True)
+    check_attention(dev, maps, dtype, 4, 140, 140, 2, 2, 64, 32, fused=True, garbage=True, lengths=[140, 0, 1, 77])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("maps", [1, 2])
+@pytest.mark.parametrize("bidirectional", [True, False])
+def test_causal(dev, dtype, maps, bidirectional):
+    check_attention(dev, maps, dtype, 2, 300, 300, 2, 2, 32, 32, fused=True, lengths=[300, 211], causal=True, bidirectional=bidirectional)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("maps", [1, 2])
+@pytest.mark.parametrize("buckets,max_distance,bidirectional", [(2, 1024, False), (4, 2, True), (6, 5, True), (64, 128, True), (128, 1024, True),
+                                                                (128, 777, False), (32, 20, False)])
+def test_bucket_layouts(dev, maps, buckets, max_distance, bidirectional):
+    check_attention(dev, maps, "bf16", 2, 260, 260, 2, 2, 64, buckets, fused=True, lengths=[260, 131], max_distance=max_distance,
+                    bidirectional=bidirectional)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("maps,heads,kv_heads,lam_heads", [(1, 4, 1, 1), (1, 6, 2, 1), (2, 4, 2, 4), (2, 3, 1, 1), (2, 12, 4, 1)])
+def test_shared_key_heads(dev, dtype, maps, heads, kv_heads, lam_heads):
+    check_attention(dev, maps, dtype, 2, 75, 75, heads, kv_heads, 32, 16, fused=True, lam_heads=lam_heads, lengths=[75, 50])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_differential_without_a_table(dev, dtype):
+    check_attention(dev, 2, dtype, 3, 150, 150, 2, 2, 64, 0, fused=True, lengths=[150, 64, 1])
+
+
+@pytest.mark.gpu
+def test_positions_far_beyond_the_table_and_large_scores(dev):
+    """distances that only fit 32 bits with care, and scores whose exponentials overflow without the running maximum"""
+    check_attention(dev, 1, "bf16", 2, 40, 200, 2, 2, 64, 32, q_start=[2 ** 31 - 1, -2 ** 31], lengths=[200, 90])
+    check_attention(dev, 1, "f32", 1, 64, 200, 2, 2, 64, 32, scale=3.0)
+    check_attention(dev, 2, "bf16", 1, 64, 200, 2, 2, 32, 32, scale=2.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("maps", [1, 2])
+@pytest.mark.parametrize("dtype,dk", [("bf16", 64), ("f16", 32), ("f32", 64), ("bf16", 40)])
+@pytest.mark.parametrize("Tk", [1, 63, 500, 2100])
+def test_one_query_against_a_memory(dev, maps, dtype, dk, Tk):
+    lens = [Tk, max(1, Tk // 3), max(1, Tk - 64)]
+    check_attention(dev, maps, dtype, 3, 1, Tk, 4, 2, dk, 32, train=False, garbage=True, lengths=lens, q_start=[n - 1 for n in lens], causal=True,
+                    bidirectional=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("maps", [1, 2])
+@pytest.mark.parametrize("Tq", [2, 5, 16, 24])
+def test_few_queries_against_a_long_memory(dev, maps, Tq):
+    check_attention(dev, maps, "bf16", 2, Tq, 1500, 4, 1, 64, 32, train=False, lengths=[1500, 777], q_start=[1500 - Tq, 777 - Tq], causal=True)
+    check_attention(dev, maps, "f32", 1, Tq, 1500, 2, 2, 32, 32, train=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("maps", [1, 2])
+def test_strided_operands(dev, maps):
+    """slices of a wider tensor, batch strides that are no multiple of the rows, a key tensor shared by the whole batch"""
+    dk, H, B, T = 32, 2, 3, 70
+    q, k, v, table, lam, dout = make(maps, torch.bfloat16, B, T, T, H, H, dk, 16)
+    k = k[:1].expand(B, -1, -1).contiguous()
+    C = H * maps * dk
+    ref = RefAttention(q, k, v, table, lam, 0.35, dout, H, H, maps, dt=torch.bfloat16)
+    big = torch.zeros(B, T + 3, C + 24, dtype=torch.bfloat16, device=dev)
+    big[:, 1:T + 1, 8:C + 8] = q.to(dev)
+    qs = big[:, 1:T + 1, 8:C + 8].detach().requires_grad_()
+    k1 = k[:1].to(dev).requires_grad_()
+    vs = v.to(dev).requires_grad_()
+    out = call(maps, qs, k1.expand(B, -1, -1), vs, table.to(dev), None if lam is None else lam.to(dev), H)
+    within(out, ref.out, ref.out_b, "out")
+    dq, dk1, dv = torch.autograd.grad(out, [qs, k1, vs], dout.to(dev))
+    within(dq, ref.g["dq"], ref.b["dq"], "dq")
+    within(dv, ref.g["dv"], ref.b["dv"], "dv")
+    # torch adds the utterances' gradients of the shared keys: three bf16 values, rounded after each addition
+    s = ref.g["dk"].abs().sum(0, keepdim=True)
+    within(dk1, ref.g["dk"].sum(0, keepdim=True), ref.b["dk"].sum(0, keepdim=True) + 3 * 2.0 ** -8 * s, "dk")
+    # a gradient that torch hands over as an expanded scalar
+    (ones,) = torch.autograd.grad(call(maps, qs, k1.expand(B, -1, -1), vs, table.to(dev), None if lam is None else lam.to(dev), H).sum(), [vs])
+    ref1 = RefAttention(q, k, v, table, lam, 0.35, torch.ones_like(dout), H, H, maps, dt=torch.bfloat16)
+    within(ones, ref1.g["dv"], ref1.b["dv"], "dv of a sum")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("maps", [1, 2])
+def test_attention_gradients_against_differences(dev, maps):
+    """(L(w + h d) - L(w - h d)) / 2h along a random direction of all inputs, f32: the third-order term and the f32 rounding of L are
+    both below 1e-3 of the value at h = 1e-2"""
+    B, T, H, dk = 2, 50, 2, 32
+    q, k, v, table, lam, dout = (t if t is None else t.to(dev) for t in make(maps, torch.float32, B, T, T, H, H, dk, 16, seed=3))
+    ws = [t for t in (q, k, v, table, lam) if t is not None]
+    g = torch.Generator(device=dev).manual_seed(1)
+    ds = [torch.randn(t.shape, device=dev, generator=g) for t in ws]
+
+    def loss(step):
+        w = [(t.double() + step * d.double()).float() for t, d in zip(ws, ds)]
+        w = w + [None] * (5 - len(w))
+        return float((call(maps, w[0], w[1], w[2], w[3], w[4], H).double() * dout.double()).sum())
+
+    leaves = [t.clone().requires_grad_() for t in ws]
+    full = leaves + [None] * (5 - len(leaves))
+    out = call(maps, full[0], full[1], full[2], full[3], full[4], H)
+    ana = sum(float((gr.double() * d.double()).sum()) for gr, d in zip(torch.autograd.grad(out, leaves, dout), ds))
+    num = (loss(1e-2) - loss(-1e-2)) / 2e-2
+    num2 = (loss(5e-3) - loss(-5e-3)) / 1e-2
+    num = (4 * num2 - num) / 3  # (the h^2 term cancelled)
+    assert abs(ana - num) < 5e-3 * max(1.0, abs(ana)), (ana, num)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("maps", [1, 2])
+def test_attention_same_bits_every_run_and_on_another_stream(dev, maps):
+    q, k, v, table, lam, dout = (t if t is None else t.to(dev) for t in make(maps, torch.bfloat16, 3, 333, 333, 4, 2, 64, 32, seed=5))
+
+    def once():
+        leaves = [t.detach().requires_grad_() for t in (q, k, v, table, lam) if t is not None]
+        full = leaves + [None] * (5 - len(leaves))
+        out = call(maps, *full, 4, kv_heads=2, causal=True)
+        return [out.detach(), *torch.autograd.grad(out, leaves, dout)]
+
+    a = once()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        b = once()
+    c = once()  # (beside the other stream's call)
+    torch.cuda.synchronize()
+    for x, y, z in zip(a, b, c):
+        assert torch.equal(x, y) and torch.equal(x, z)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("maps", [1, 2])
+@pytest.mark.parametrize("Tq", [1, 70])
+def test_attention_in_captured_graphs(dev, maps, Tq):
+    """forward and backward captured, replayed with new inputs between eager calls; two graphs do not share a workspace"""
+    B, Tk, H = 2, 900, 4
+    sets = [[t if t is None else t.to(dev) for t in make(maps, torch.bfloat16, B, Tq, Tk, H, 2, 64, 32, seed=s)] for s in (1, 2, 3)]
+
+    def step(q, k, v, table, lam, dout):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v, table, lam) if t is not None]
+        full = leaves + [None] * (5 - len(leaves))
+        out = call(maps, *full, H, kv_heads=2)
+        with torch.no_grad():
+            serve = call(maps, q, k, v, table, lam, H, kv_heads=2)
+        return [serve, out.detach(), *torch.autograd.grad(out, leaves, dout)]
+
+    graphs = []
+    for n in (0, 1):
+        static = [None if t is None else t.clone() for t in sets[n]]
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            step(*static)
+        torch.cuda.current_stream().wait_stream(s)
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs = step(*static)
+        graphs.append((gr, static, outs))
+    for trip in range(3):
+        want = []
+        for n, (gr, static, outs) in enumerate(graphs):
+            src = sets[(trip + n) % 3]
+            want.append([t.clone() for t in step(*src)])
+            for d, t in zip(static, src):
+                if t is not None:
+                    d.copy_(t)
+        for gr, _, _ in graphs:
+            gr.replay()
+        torch.cuda.synchronize()
+        for (gr, _, outs), w in zip(graphs, want):
+            for o, t in zip(outs, w):
+                assert torch.equal(o, t)
+
+
+@pytest.mark.gpu
+def test_attention_only_some_inputs_need_gradients(dev):
+    from promptttspp_amd import functional as PF
+
+    q, k, v, table, lam, dout = (t if t is None else t.to(dev) for t in make(1, torch.float32, 2, 40, 40, 2, 2, 64, 16))
+    table.requires_grad_()
+    (dt,) = torch.autograd.grad(PF.attention_bucket(q, k, v, table, 2), [table], dout)
+    ref = RefAttention(q.cpu(), k.cpu(), v.cpu(), table.detach().cpu(), None, 0, dout.cpu(), 2, 2, 1)
+    within(dt, ref.g["dtable"], ref.b["dtable"], "dtable")
+
+
+@pytest.mark.gpu
+def test_long_batch_strides_pass_32_bits(dev):
+    """the second utterance of a kept memory lies more than 2^31 elements behind the first"""
+    from promptttspp_amd import functional as PF
+
+    H, dk, T = 2, 64, 100
+    room = 2 ** 31 // (H * dk) + 64  # positions of room per utterance
+    mem = torch.empty(2 * room * H * dk, device=dev, dtype=torch.bfloat16).view(2, room, H * dk)
+    q, k, v, table, _, _ = make(1, torch.bfloat16, 2, 1, T, H, H, dk, 32)
+    vals = torch.zeros(2, T, H * dk, dtype=torch.bfloat16)
+    mem[:, :T] = k.to(dev)
+    vals = v.to(dev)
+    ref = RefAttention(q, k, v, table, None, 0, None, H, H, 1, dt=torch.bfloat16, q_start=[T - 1, T - 1])
+    with torch.no_grad():
+        out = PF.attention_bucket(q.to(dev), mem[:, :T], vals, table.to(dev), H, q_start=torch.tensor([T - 1, T - 1], device=dev))
+    within(out, ref.out, ref.out_b, "out")
+
+
+def test_bucket_edges_are_the_whole_number_solution():
+    from promptttspp_amd import ops
+
+    for n, D, bi in ((32, 128, True), (32, 128, False), (64, 128, True), (8, 128, True), (128, 1024, False), (6, 5, True), (2, 1024, False), (4, 2, True)):
+        e, edges, cnt = ops.bucket_edges(n, D, bi)
+        d = torch.arange(-2 * D, 2 * D + 1)
+        want = ref_bucket(d, n, D, bi)
+        half = n // 2 if bi else n
+        a = d.abs() if bi else (-d).clamp(min=0)
+        got = torch.where(a < e, a, torch.full_like(a, e))
+        for t in range(cnt):
+            got = got + (a >= edges[t])
+        got = got + half * ((d > 0) & bi)
+        assert torch.equal(got, want), (n, D, bi)
+    for bad in ((3, 128, True), (130, 128, True), (2, 128, True), (1, 128, False), (32, 8, True), (32, 1025, True), (0, 10, False)):
+        with pytest.raises(ValueError):
+            ops.bucket_edges(*bad)
+
+
+def test_attention_refusals_on_the_host():
+    """what the C entry refuses before any launch (no GPU needed: the pointers are never followed)"""
+    from promptttspp_amd import _lib, ops
+
+    lib = _lib.load()
+    e, edges, cnt = ops.bucket_edges(32, 128, True)
+
+    def args(**kw):
+        a = _lib.AttentionLongArgs()
+        for n in ("q", "k", "v", "out", "table"):
+            setattr(a, n, 4096)
+        a.B, a.Tq, a.Tk, a.H, a.Hk, a.dk, a.maps, a.dtype = 2, 10, 10, 2, 2, 64, 1, _lib.BF16
+        a.ldq = a.ldk = a.ldv = a.ldo = a.lddo = a.lddq = a.lddk = a.lddv = 128
+        a.sq = a.sk = a.sv = a.so = a.sdo = a.sdq = a.sdk = a.sdv = 1280
+        a.nbuckets, a.bidirectional, a.max_distance, a.nexact, a.nedges, a.edges = 32, 1, 128, e, cnt, ctypes.addressof(edges)
+        a.scale = 0.125
+        for n, x in kw.items():
+            setattr(a, n, x)
+        return a
+
+    assert lib.ptpp_attention_long_ws_bytes(ctypes.byref(args()), 0) >= 0
+    back = {n: 4096 for n in ("dout", "dq", "dk_out", "dv", "dtable", "lse")}
+    assert lib.ptpp_attention_long_ws_bytes(ctypes.byref(args(**back)), 1) > 0
+    descending = (ctypes.c_int32 * 16)(*([20] + [19] * 15))
+    bad = [dict(q=None), dict(out=None), dict(dtype=7), dict(maps=3), dict(B=0), dict(Tq=0), dict(Tk=-1), dict(H=3), dict(Hk=0), dict(dk=60), dict(dk=136),
+           dict(dk=0), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(q=4098), dict(ldq=127), dict(ldk=120),
+           dict(sv=1281), dict(sk=-1280), dict(table=None), dict(maps=2, dk=72, lam=4096, lam_heads=1), dict(maps=2, dk=32), dict(maps=2, dk=32, lam=4096, lam_heads=3),
+           dict(nbuckets=31), dict(nbuckets=130), dict(nexact=9), dict(nedges=3), dict(edges=None), dict(max_distance=8), dict(max_distance=1025),
+           dict(edges=ctypes.addressof(descending)), dict(B=2 ** 30, Tq=2 ** 20)]
+    for kw in bad:
+        a = args(**kw)
+        assert lib.ptpp_attention_long_fwd(ctypes.byref(a), None) == -1, kw
+        assert lib.ptpp_attention_long_ws_bytes(ctypes.byref(a), 0) < 0, kw
+    assert lib.ptpp_attention_long_fwd(None, None) == -1
+    for kw in (dict(back, lse=None), dict(back, lse=4100), dict(back, dtable=None), dict(back, dq=None), dict(back, lddv=64), dict(back, ws=None, ws_bytes=1 << 30),
+               dict(back, ws=4096, ws_bytes=16), dict(back, ws=4104, ws_bytes=1 << 30)):
+        assert lib.ptpp_attention_long_bwd(ctypes.byref(args(**kw)), None) == -1, kw
+    assert b"attention_long" in lib.ptpp_last_error()
+
+
+def test_attention_refuses_cpu_tensors():
+    from promptttspp_amd import _lib
+    from promptttspp_amd import functional as PF
+
+    x = torch.zeros(1, 4, 3 * 64)
+    with pytest.raises(_lib.PtppError):
+        PF.attention_bucket(x, None, None, torch.zeros(32, 1), 1)
+    with pytest.raises(ValueError):
+        PF.attention_bucket(x, None, None, None, 1)
+    with pytest.raises(ValueError):
+        PF.attention_bucket(x, x, None, torch.zeros(32, 1), 1)
+    with pytest.raises(ValueError):
+        PF.attention_diff(x, None, None, None, 0.1, 1)
+    with pytest.raises(_lib.PtppError):
+        PF.residual_norm(torch.zeros(1, 4, 8))
+
+
+@pytest.mark.gpu
+def test_attention_refusals(dev):
+    from promptttspp_amd import _lib
+    from promptttspp_amd import functional as PF
+
+    z = lambda *s, dt=torch.bfloat16: torch.zeros(*s, device=dev, dtype=dt)  # noqa: E731
+    tab = z(32, 2, dt=torch.float32)
+    ok = (z(2, 5, 128), z(2, 7, 128), z(2, 7, 128), tab, 2)
+    PF.attention_bucket(*ok)
+    val = [((z(2, 5, 120), *ok[1:]), {}), ((z(2, 5, 128, dt=torch.float32), *ok[1:]), {}), ((ok[0], z(1, 7, 128), *ok[2:]), {}),
+           ((ok[0], z(2, 7, 64), *ok[2:]), {}), ((*ok[:3], z(32, 3, dt=torch.float32), 2), {}), ((*ok[:3], z(33, 2, dt=torch.float32), 2), {}),
+           (ok, {"kv_heads": 3}), (ok, {"scale": 0.0}), (ok, {"scale": -1.0}), (ok, {"max_distance": 2000}), (ok, {"max_distance": 4}),
+           (ok, {"lengths": torch.ones(3, device=dev, dtype=torch.int32)}), (ok, {"lengths": torch.ones(2, device=dev)}),
+           (ok, {"q_start": torch.ones(2, 1, device=dev, dtype=torch.int32)}), ((z(2, 128, 5).transpose(1, 2), *ok[1:]), {}),
+           ((z(2, 0, 128), *ok[1:]), {}), ((ok[0], z(2, 0, 128), z(2, 0, 128), tab, 2), {}), ((ok[0], None, ok[2], tab, 2), {}),
+           ((z(2, 5, 130), None, None, tab, 2), {})]
+    for a, kw in val:
+        with pytest.raises(ValueError):
+            PF.attention_bucket(*a, **kw)
+    with pytest.raises(TypeError):
+        PF.attention_bucket(z(2, 5, 128, dt=torch.float64), z(2, 7, 128, dt=torch.float64), z(2, 7, 128, dt=torch.float64), tab, 2)
+    with pytest.raises(_lib.PtppError):  # rows that are not 16-byte aligned
+        PF.attention_bucket(z(2, 5, 132)[:, :, 2:130], *ok[1:])
+    with pytest.raises(_lib.PtppError):
+        PF.attention_bucket(*ok[:3], tab.cpu(), 2)
+    for lam in (z(4, 3, 32, dt=torch.float32), z(3, 1, 32, dt=torch.float32), z(4, 1, 16, dt=torch.float32)):
+        with pytest.raises(ValueError):
+            PF.attention_diff(*ok[:3], lam, 0.1, 2)
+    with pytest.raises(ValueError):  # a map of 72 channels
+        PF.attention_diff(z(1, 5, 144), z(1, 5, 144), z(1, 5, 144), z(4, 1, 72, dt=torch.float32), 0.1, 1)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# norm, gate, residual, norm
+# ---------------------------------------------------------------------------------------------------------------------
+def ref_norm(f, x, gate, post, pre, scale, eps, kind, lengths, dy, dz, dt):
+    """values, gradients and bounds in 64 bits.  f32 inside the kernel: a row's mean and deviation are sums of C terms in registers and
+    over lanes (depth <= 24), so every intermediate is off by at most ~64 * 2^-24 of the magnitudes that enter it"""
+    rms, u, f32 = kind == "rms", half_ulp(dt), 64 * 2.0 ** -24
+    B, T, C = f.shape
+    d = lambda t: None if t is None else t.double()  # noqa: E731
+    rows = torch.ones(B, T, 1, dtype=torch.float64) if lengths is None else \
+        (torch.arange(T)[None] < torch.tensor(lengths)[:, None]).double()[:, :, None]
+    f = torch.where(rows > 0, f.double(), torch.zeros(())).double()
+    x = None if x is None else torch.where(rows > 0, x.double(), torch.zeros(())).double()
+    dy, dz = (None if t is None else torch.where(rows > 0, t.double(), torch.zeros(())).double() for t in (dy, dz))
+    (pg, pb), (qg, qb), gate = tuple(map(d, post)), tuple(map(d, pre)), d(gate)
+    g = 1.0 if gate is None else gate[:, None] if gate.dim() == 2 else gate
+
+    def hat(v):
+        mu = 0.0 if rms else v.mean(-1, keepdim=True)
+        r = ((v - mu).square().mean(-1, keepdim=True) + eps).rsqrt()
+        # |v| + |mean| enters the subtraction, the deviation scales everything by its own relative error
+        amp = r * (v.abs() + (0.0 if rms else v.abs().mean(-1, keepdim=True)))
+        return (v - mu) * r, r, amp
+
+    def back(gh, h, r):
+        t = gh - h * (gh * h).mean(-1, keepdim=True)
+        b = gh.abs() + h.abs() * (gh.abs() * h.abs()).mean(-1, keepdim=True) + gh.abs().mean(-1, keepdim=True)
+        return r * (t if rms else t - gh.mean(-1, keepdim=True)), r * b
+
+    if pg is not None:
+        fh, fr, fa = hat(f)
+        fa = fa + fh.abs() * (fa * fh.abs()).mean(-1, keepdim=True)
+        uu, ua = fh * pg + (0.0 if pb is None else pb), fa * pg.abs() + (0.0 if pb is None else pb.abs())
+    else:
+        fh, fr, fa, uu, ua = f, torch.ones(()).double(), f.abs(), f, f.abs()
+    y = ((0.0 if x is None else x) + scale * g * uu) * rows
+    ya = (0.0 if x is None else x.abs()) + abs(scale) * (g.abs() if torch.is_tensor(g) else g) * ua
+    res = {"y": (y, f32 * ya + u * y.abs())}
+    yh = None
+    if qg is not None:
+        yh, yr, ym = hat(y)
+        ye = yr * ya + ym                                    # error sources of the normalised y: its own, and y's
+        ye = ye + yh.abs() * (ye * yh.abs()).mean(-1, keepdim=True) + ye.mean(-1, keepdim=True)
+        z = (yh * qg + (0.0 if qb is None else qb)) * rows
+        res["z"] = (z, f32 * (ye * qg.abs() + (0.0 if qb is None else qb.abs())) + u * z.abs())
+    if dy is None and dz is None:
+        return res
+    dx = torch.zeros_like(f) if dy is None else dy.clone()
+    dxa = dx.abs()
+    if dz is not None:
+        t, ta = back(dz * qg, yh, yr)
+        te = yr * (dz * qg).abs().mean(-1, keepdim=True) * ye + ta * (1 + (ye * yh.abs()).mean(-1, keepdim=True))
+        dx, dxa = dx + t, dxa + ta + te
+        res["dpre_g"] = ((dz * yh).sum((0, 1)), f32 * (dz.abs() * (ye + yh.abs())).sum((0, 1)))
+        res["dpre_b"] = (dz.sum((0, 1)), f32 * dz.abs().sum((0, 1)))
+    dx = dx * rows
+    res["dx"] = (dx, f32 * dxa + u * dx.abs())
+    du, dua = scale * g * dx, abs(scale) * (g.abs() if torch.is_tensor(g) else g) * dxa
+    if pg is not None:
+        df, dfa = back(du * pg, fh, fr)
+        _, e1 = back(dua * pg.abs(), fh, fr)
+        dfa = dfa * (1 + (fa * fh.abs()).mean(-1, keepdim=True)) + e1 + fr * (du * pg).abs().mean(-1, keepdim=True) * fa
+        res["dpost_g"] = ((du * fh).sum((0, 1)), f32 * (dua * fh.abs() + du.abs() * fa).sum((0, 1)))
+        res["dpost_b"] = (du.sum((0, 1)), f32 * dua.sum((0, 1)))
+    else:
+        df, dfa = du, dua
+    res["df"] = (df * rows, f32 * dfa + u * df.abs())
+    if gate is not None:
+        dims = (1,) if gate.dim() == 2 else (0, 1)
+        res["dgate"] = ((scale * uu * dx).sum(dims), f32 * abs(scale) * (ua * dxa).sum(dims))
+    return res
+
+
+def check_norm(dev, dtype, B, T, C, kind="layer", gate="utt", res=True, post=True, pre=True, beta=True, lengths=None, scale=0.5, use="both", garbage=False,
+               train=True, eps=1e-5, seed=0):
+    from promptttspp_amd import functional as PF
+
+    dt = DT[dtype]
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    f, x = (2 * r(B, T, C) + 0.5).to(dt), (3 * r(B, T, C)).to(dt) if res else None
+    beta = beta and kind == "layer"
+    par = {"gate": {"utt": r(B, C), "chan": r(C), "none": None}[gate], "post_g": 1 + 0.2 * r(C) if post else None, "post_b": 0.2 * r(C) if post and beta else None,
+           "pre_g": 1 + 0.2 * r(C) if pre else None, "pre_b": 0.2 * r(C) if pre and beta else None}
+    dy, dz = r(B, T, C).to(dt), r(B, T, C).to(dt)
+    use_y, use_z = use in ("both", "y"), use in ("both", "z") and pre
+    want = ref_norm(f, x, par["gate"], (par["post_g"], par["post_b"]), (par["pre_g"], par["pre_b"]), scale, eps, kind, lengths,
+                    dy if train and use_y else None, dz if train and use_z else None, dt)
+    if garbage:
+        for t in (f, x, dy, dz):
+            if t is not None:
+                for b in range(B):
+                    t[b, lengths[b]:] = float("nan") if b % 2 else float("inf")
+    leaves = {n: t.to(dev).requires_grad_(train) for n, t in (("f", f), ("x", x), *par.items()) if t is not None}
+    y, z = PF.residual_norm(leaves["f"], leaves.get("x"), gate=leaves.get("gate"), post=(leaves["post_g"], leaves.get("post_b")) if post else None,
+                            pre=(leaves["pre_g"], leaves.get("pre_b")) if pre else None, scale=scale, eps=eps, kind=kind,
+                            lengths=None if lengths is None else torch.tensor(lengths, device=dev))
+    got = {"y": y}
+    assert (z is not None) == pre
+    if pre:
+        got["z"] = z
+    if train:
+        outs = ([y] if use_y else []) + ([z] if use_z else [])
+        gouts = ([dy.to(dev)] if use_y else []) + ([dz.to(dev)] if use_z else [])
+        for n, t in zip(leaves, torch.autograd.grad(outs, list(leaves.values()), gouts, allow_unused=True)):
+            got["d" + n] = t
+    for n, t in got.items():
+        if n in want:
+            within(t, *want[n], n)
+        else:
+            assert n in ("dpre_g", "dpre_b") and (t is None or float(t.abs().max()) == 0.0), n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("C", [4, 60, 64, 68, 128, 132, 256, 260, 512, 516, 1024, 1028, 2048, 2052, 4096])
+def test_residual_norm_widths(dev, dtype, C):
+    check_norm(dev, dtype, 2, 19, C, lengths=[19, 7])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("B,T", [(1, 1), (32, 1), (1, 5000), (3, 333), (1100, 3)])
+def test_residual_norm_row_counts(dev, dtype, B, T):
+    check_norm(dev, dtype, B, T, 64)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+@pytest.mark.parametrize("gate", ["utt", "chan", "none"])
+@pytest.mark.parametrize("res,post,pre", [(True, True, True), (True, True, False), (True, False, True), (False, True, False), (False, True, True),
+                                          (True, False, False), (False, False, True)])
+def test_residual_norm_forms(dev, kind, gate, res, post, pre):
+    check_norm(dev, "f32", 3, 21, 192, kind=kind, gate=gate, res=res, post=post, pre=pre, lengths=[21, 1, 0])
+    check_norm(dev, "bf16", 3, 21, 576, kind=kind, gate=gate, res=res, post=post, pre=pre, beta=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("use", ["y", "z"])
+def test_residual_norm_one_output_used(dev, use):
+    check_norm(dev, "bf16", 2, 30, 256, use=use, lengths=[30, 11])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_residual_norm_garbage_behind_the_lengths(dev, dtype):
+    check_norm(dev, dtype, 4, 40, 256, lengths=[40, 0, 1, 23], garbage=True)
+    check_norm(dev, dtype, 4, 40, 1500, kind="rms", lengths=[40, 0, 1, 23], garbage=True)
+    check_norm(dev, dtype, 4, 40, 256, lengths=[40, 0, 1, 23], garbage=True, train=False)
+
+
+@pytest.mark.gpu
+def test_residual_norm_inputs_off_the_beaten_path(dev):
+    """transposed and expanded inputs, (1, C, 1) parameters, an expanded gradient; parameters of another float type keep it"""
+    from promptttspp_amd import functional as PF
+
+    g = torch.Generator().manual_seed(2)
+    f = torch.randn(2, 24, 10, generator=g)
+    x = torch.randn(1, 1, 24, generator=g)
+    pg = (1 + 0.1 * torch.randn(1, 24, 1, generator=g)).to(dev).requires_grad_()
+    qg = (1 + 0.1 * torch.randn(24, generator=g)).bfloat16().to(dev).requires_grad_()
+    fd, xd = f.to(dev).requires_grad_(), x.to(dev).requires_grad_()
+    y, z = PF.residual_norm(fd.transpose(1, 2), xd.expand(2, 10, 24), post=(pg, None), pre=(qg, None), kind="rms", scale=1.0)
+    ones = torch.ones(2, 10, 24)
+    want = ref_norm(f.transpose(1, 2), x.expand(2, 10, 24), None, (pg.detach().cpu().reshape(-1), None), (qg.detach().cpu().float(), None), 1.0, 1e-5, "rms", None,
+                    ones, ones, torch.float32)
+    within(y, *want["y"], "y")
+    within(z, *want["z"], "z")
+    df, dx, dpg, dqg = torch.autograd.grad(y.sum() + z.sum(), [fd, xd, pg, qg])
+    within(df.transpose(1, 2), *want["df"], "df")
+    within(dx, want["dx"][0].sum((0, 1), keepdim=True), want["dx"][1].sum((0, 1), keepdim=True) + 32 * 2.0 ** -24 * want["dx"][0].abs().sum((0, 1), keepdim=True), "dx")
+    assert dpg.shape == pg.shape and dqg.dtype == torch.bfloat16
+    within(dpg.reshape(-1), *want["dpost_g"], "dpost_g")
+    within(dqg, want["dpre_g"][0], want["dpre_g"][1] + 2.0 ** -8 * want["dpre_g"][0].abs(), "dpre_g")
+
+
+@pytest.mark.gpu
+def test_residual_norm_gradients_against_differences(dev):
+    """central differences along a random direction, f32, the h^2 term cancelled"""
+    from promptttspp_amd import functional as PF
+
+    g = torch.Generator(device=dev).manual_seed(4)
+    r = lambda *s: torch.randn(*s, device=dev, generator=g)  # noqa: E731
+    ws = [r(2, 9, 64), r(2, 9, 64), r(2, 64), 1 + 0.2 * r(64), r(64), 1 + 0.2 * r(64), r(64)]
+    ds, dy, dz = [r(*w.shape) for w in ws], r(2, 9, 64).double(), r(2, 9, 64).double()
+
+    def run(w):
+        return PF.residual_norm(w[0], w[1], gate=w[2], post=(w[3], w[4]), pre=(w[5], w[6]), scale=0.7)
+
+    def loss(h):
+        y, z = run([(w.double() + h * d.double()).float() for w, d in zip(ws, ds)])
+        return float((y.double() * dy + z.double() * dz).sum())
+
+    leaves = [w.clone().requires_grad_() for w in ws]
+    y, z = run(leaves)
+    ana = sum(float((a.double() * d.double()).sum()) for a, d in zip(torch.autograd.grad((y, z), leaves, (dy.float(), dz.float())), ds))
+    num = (4 * (loss(5e-3) - loss(-5e-3)) / 1e-2 - (loss(1e-2) - loss(-1e-2)) / 2e-2) / 3
+    assert abs(ana - num) < 5e-3 * max(1.0, abs(ana)), (ana, num)
+
+
+@pytest.mark.gpu
+def test_residual_norm_same_bits_and_captured(dev):
+    from promptttspp_amd import functional as PF
+
+    g = torch.Generator(device=dev).manual_seed(4)
+    r = lambda *s: torch.randn(*s, device=dev, generator=g)  # noqa: E731
+    sets = [[r(5, 77, 256), r(5, 77, 256), r(5, 256), r(256), r(256), r(256), r(256), r(5, 77, 256), r(5, 77, 256)] for _ in range(2)]
+
+    def step(ts):
+        lv = [t.detach().requires_grad_() for t in ts[:7]]
+        y, z = PF.residual_norm(lv[0], lv[1], gate=lv[2], post=(lv[3], lv[4]), pre=(lv[5], lv[6]), scale=0.5)
+        return [y.detach(), z.detach(), *torch.autograd.grad((y, z), lv, (ts[7], ts[8]))]
+
+    static = [t.clone() for t in sets[0]]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step(static)
+    torch.cuda.current_stream().wait_stream(s)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        outs = step(static)
+    for trip in range(4):
+        for d, t in zip(static, sets[trip % 2]):
+            d.copy_(t)
+        gr.replay()
+        want = step(sets[trip % 2])
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            assert torch.equal(o, w)
+
+
+def test_residual_norm_refusals_on_the_host():
+    from promptttspp_amd import _lib
+
+    lib = _lib.load()
+
+    def args(**kw):
+        a = _lib.ResidualNormArgs()
+        a.f = a.x = a.y = a.z = a.gate = a.post_g = a.post_b = a.pre_g = a.pre_b = 4096
+        a.B, a.T, a.C, a.gate_rows, a.dtype, a.scale, a.eps = 2, 3, 64, 2, _lib.F32, 1.0, 1e-5
+        for n, x in kw.items():
+            setattr(a, n, x)
+        return a
+
+    for kw in (dict(f=None), dict(y=None), dict(z=None), dict(pre_g=None), dict(B=0), dict(T=0), dict(C=66), dict(C=4100), dict(C=0), dict(dtype=9), dict(gate_rows=3),
+               dict(post_g=None), dict(rms=1), dict(eps=0.0), dict(eps=float("nan")), dict(f=4104), dict(gate=4100), dict(B=2 ** 20, T=2 ** 12)):
+        assert lib.ptpp_residual_norm_fwd(ctypes.byref(args(**kw)), None) == -1, kw
+    grads = dict(dy=4096, dz=4096, df=4096, dx=4096, stats=4096, dgate=4096, dpost_g=4096)
+    n = lib.ptpp_residual_norm_ws_bytes(ctypes.byref(args(**grads)))
+    assert n > 0
+    for kw in (dict(grads, stats=None, ws=4096, ws_bytes=n), dict(grads, ws=None), dict(grads, ws=4096, ws_bytes=n - 1), dict(grads, ws=4100, ws_bytes=n),
+               dict(grads, gate=None, ws=4096, ws_bytes=n), dict(grads, dpre_g=4096, pre_g=None, pre_b=None, z=None, ws=4096, ws_bytes=1 << 20)):
+        assert lib.ptpp_residual_norm_bwd(ctypes.byref(args(**kw)), None) == -1, kw
+
+
+@pytest.mark.gpu
+def test_residual_norm_refusals(dev):
+    from promptttspp_amd import _lib
+    from promptttspp_amd import functional as PF
+
+    z = lambda *s, dt=torch.float32: torch.zeros(*s, device=dev, dtype=dt)  # noqa: E731
+    f = z(2, 3, 64)
+    for kw in (dict(x=z(2, 3, 60)), dict(x=z(2, 3, 64, dt=torch.bfloat16)), dict(gate=z(3, 64)), dict(gate=z(32)), dict(gate=z(2, 3, 64)), dict(post=(z(60), None)),
+               dict(post=(None, z(64))), dict(pre=(z(64), z(64)), kind="rms"), dict(kind="batch"), dict(eps=0.0), dict(lengths=z(2)),
+               dict(lengths=torch.ones(3, device=dev, dtype=torch.int64))):
+        with pytest.raises(ValueError):
+            PF.residual_norm(f, **kw)
+    for bad in (z(2, 3, 66), z(2, 3, 4100), z(2, 64), z(0, 3, 64)):
+        with pytest.raises(ValueError):
+            PF.residual_norm(bad)
+    with pytest.raises(TypeError):
+        PF.residual_norm(z(2, 3, 64, dt=torch.float64))
+    with pytest.raises(_lib.PtppError):
+        PF.residual_norm(f, gate=torch.zeros(64))
+
+
+def test_argument_blocks_match_the_header(tmp_path):
+    import os
+    import shutil
+    import subprocess
+
+    from promptttspp_amd import _lib
+
+    if shutil.which("gcc") is None:
+        pytest.skip("no gcc")
+    pairs = [("ptpp_attention_long_args", _lib.AttentionLongArgs), ("ptpp_residual_norm_args", _lib.ResidualNormArgs)]
+    src = tmp_path / "sz.c"
+    fields = "".join('printf("%%zu\\n", offsetof(%s, %s));' % (n, f[0]) for n, c in pairs for f in c._fields_)
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "%s"\nint main(void){%s%s return 0;}\n' % (
+        os.path.join(ROOT, "include", "ptpp.h"), "".join('printf("%%zu\\n", sizeof(%s));' % n for n, _ in pairs), fields))
+    subprocess.run(["gcc", str(src), "-o", str(tmp_path / "sz")], check=True)
+    vals = [int(v) for v in subprocess.run([str(tmp_path / "sz")], check=True, capture_output=True, text=True).stdout.split()]
+    want = [ctypes.sizeof(c) for _, c in pairs] + [getattr(c, f[0]).offset for _, c in pairs for f in c._fields_]
+    assert vals == want
