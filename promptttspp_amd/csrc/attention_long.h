@@ -28,12 +28,13 @@ struct LongP {
   const float *table, *lam;
   const int *k_lengths, *q_lengths, *q_start;
   float *lse, *D;              // (M, B, H, TqP)
-  float *lam_part, *tab_part;  // [B][H][query tiles], [B][key tiles][H][nbuckets]
-  float *part;                 // split forward: [splits][B*Hk tiles ...] partial contexts and statistics
+  float *lam_part, *tab_part;  // [B][H][query tiles], [H][nbuckets][B][key tiles]
+  float *part_o, *part_ml;     // few-row forward: [blocks][splits][M][32] rows of DV sums and their (max, sum)
   int64_t sq, sk, sv, so, sdo, sdq, sdk, sdv;  // batch strides, elements
   int ldq, ldk, ldv, ldo, lddo, lddq, lddk, lddv;
   int B, Tq, Tk, TqP, H, Hk, dk, nbuckets, bidirectional, causal, lam_heads, max_distance, nexact, nedges;
-  int nqt, nkt, splits;
+  int nqt, nkt;
+  int nh, nrb, splits;  // few-row forward: query heads of a block, row blocks per head, key ranges
   float scale, lam_init;
   int edges[LA_EDGES];
 };
@@ -164,26 +165,44 @@ __device__ __forceinline__ uint4 la_tfrag(const E* img, int row0, int s, int n, 
   }
 }
 
-// A LA_TILE x DK image fetched by LDS-DMA, NI wave instructions per wave (lane offsets kept in registers; rows >= nrows and the
-// channels that pad dk to DK come from the zero page, so nothing behind a sequence is ever read).
-template <typename E, int DK>
+// the same value, but not known to be: LDS addresses derived from it are computed where they are used instead of being kept in
+// registers across a loop (the f32 kernels have none to spare, and their matrix instructions leave the vector unit idle)
+__device__ __forceinline__ int la_opaque(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+// A ROWS x DK image fetched by LDS-DMA, by WAVES waves, NI wave instructions each (lane offsets kept in registers; rows >= nrows and
+// the channels that pad dk to DK come from the zero page, so nothing behind a sequence is ever read).
+template <typename E, int DK, int ROWS = LA_TILE, int WAVES = LA_WAVES>
 struct LTile {
-  static constexpr int CH = LOp<E>::CH, CPR = DK / CH, NI = LA_TILE * CPR / 64 / LA_WAVES;
-  static_assert(LA_TILE * CPR % (64 * LA_WAVES) == 0, "whole wave instructions");
-  int off[NI];       // element offset inside the tile, -1: padding channels
+  static constexpr int CH = LOp<E>::CH, CPR = DK / CH, NI = ROWS * CPR / 64 / WAVES;
+  static_assert(ROWS * CPR % (64 * WAVES) == 0, "whole wave instructions");
+  // element offsets inside the tile, -1: padding channels; f32 (twice the instructions, short of registers, its vector unit idle beside
+  // the matrix instructions) computes them anew each time
+  static constexpr bool KEEP = sizeof(E) == 2;
+  int off[KEEP ? NI : 1], ld_, dk_;
+  static __device__ __forceinline__ int offset(int i, int ld, int dk, int lane, int wave) {
+    const int x = (wave * NI + i) * 64 + lane, row = x / CPR, c = (x % CPR) ^ la_swz<CPR>(row);
+    return c * CH < dk ? row * ld + c * CH : -1;
+  }
   __device__ __forceinline__ void init(int ld, int dk, int lane, int wave) {
+    ld_ = ld;
+    dk_ = dk;
+    if constexpr (KEEP) {
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int x = (wave * NI + i) * 64 + lane, row = x / CPR, c = (x % CPR) ^ la_swz<CPR>(row);
-      off[i] = c * CH < dk ? row * ld + c * CH : -1;
+      for (int i = 0; i < NI; ++i) off[i] = offset(i, ld, dk, lane, wave);
     }
   }
   __device__ __forceinline__ void issue(const E* tile, int nrows, const E* img, int lane, int wave) const {
     const uint32_t dst = lds_addr(img) + wave * (NI * 1024);
+    if constexpr (!KEEP) lane = la_opaque(lane);
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int row = ((wave * NI + i) * 64 + lane) / CPR;
-      const void* src = (off[i] >= 0 && row < nrows) ? (const void*)(tile + off[i]) : (const void*)g_conv_zero_page;
+      int o;
+      if constexpr (KEEP) o = off[i];
+      else o = offset(i, ld_, dk_, lane, wave);
+      const void* src = (o >= 0 && row < nrows) ? (const void*)(tile + o) : (const void*)g_conv_zero_page;
       glds16(src, __builtin_amdgcn_readfirstlane(dst + i * 1024));
     }
   }
@@ -192,13 +211,9 @@ struct LTile {
 // every wave's LDS reads are done and every wave is here (the DMA queue is counted separately: glds_wait)
 __device__ __forceinline__ void la_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// the same value, but not known to be: LDS addresses derived from it are computed where they are used instead of being kept in
-// registers across a loop (the f32 kernels have none to spare, and their matrix instructions leave the vector unit idle)
-__device__ __forceinline__ int la_opaque(int v) {
-  asm volatile("" : "+v"(v));
-  return v;
-}
 __device__ __forceinline__ float la_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+// wave number, known to be the same in all lanes: what depends on it alone is scalar work and scalar branches
+__device__ __forceinline__ int la_wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 __device__ __forceinline__ float la_half_sum(float v) { return v + __shfl_xor(v, 32, 64); }
 __device__ __forceinline__ float la_half_max(float v) { return fmaxf(v, __shfl_xor(v, 32, 64)); }
 

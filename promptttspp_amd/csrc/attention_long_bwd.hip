@@ -13,14 +13,15 @@
 namespace {
 
 template <typename E, int DK, int DV, int MAPS, bool BIAS>
-__global__ __launch_bounds__(256) void attn_long_dq_kernel(const LongP p) {
+__global__ __launch_bounds__(256, sizeof(E) == 4 ? 1 : 2) void attn_long_dq_kernel(const LongP p) {
   constexpr int CH = LOp<E>::CH, KS = DK / (2 * CH), VS = DV / (2 * CH), PS = 16 / CH, NT = DK / 32;
+  constexpr bool TIGHT = sizeof(E) == 4 || MAPS * DV == 256;  // registers are short: LDS addresses not kept across patches
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ float lred[LA_WAVES];
   constexpr int KIMG = LA_TILE * DK, VIMG = LA_TILE * DV, BUF = MAPS * KIMG + VIMG;
   E* const img = reinterpret_cast<E*>(smem);
   float* const btab = reinterpret_cast<float*>(smem + 2 * BUF * sizeof(E));
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lq = lane & 31, hw = lane >> 5;
+  const int lane = threadIdx.x & 63, wave = la_wave(), lq = lane & 31, hw = lane >> 5;
 
   const int t = xcd_remap(blockIdx.x, gridDim.x);
   const int qt = t % p.nqt, bh = t / p.nqt, h = bh % p.H, b = bh / p.H, hk = h / (p.H / p.Hk);
@@ -111,14 +112,15 @@ __global__ __launch_bounds__(256) void attn_long_dq_kernel(const LongP p) {
 #pragma unroll 1
     for (int ks = 0; ks < 2; ++ks) {
       const int j0 = tile * LA_TILE + 32 * ks;
+      const int ln = TIGHT ? la_opaque(lane) : lane, lr = ln & 31, hr = ln >> 5;
       f32x16 dp = f32x16{};
 #pragma unroll
-      for (int kk = 0; kk < VS; ++kk) dp = LOp<E>::mma(la_frag<E, DV>(vimg, 32 * ks + lq, 2 * kk + hw), df[kk], dp);
+      for (int kk = 0; kk < VS; ++kk) dp = LOp<E>::mma(la_frag<E, DV>(vimg, 32 * ks + lr, 2 * kk + hr), df[kk], dp);
 #pragma unroll
       for (int m = 0; m < MAPS; ++m) {
         f32x16 s = f32x16{};
 #pragma unroll
-        for (int kk = 0; kk < KS; ++kk) s = LOp<E>::mma(la_frag<E, DK>(kimg + m * KIMG, 32 * ks + lq, 2 * kk + hw), qf[m][kk], s);
+        for (int kk = 0; kk < KS; ++kk) s = LOp<E>::mma(la_frag<E, DK>(kimg + m * KIMG, 32 * ks + lr, 2 * kk + hr), qf[m][kk], s);
         if constexpr (BIAS) {
           const int dmin = j0 - (q0 + 31), dmax = j0 + 31 - q0;
           if (dmin < D && dmax > -D) {
@@ -148,7 +150,7 @@ __global__ __launch_bounds__(256) void attn_long_dq_kernel(const LongP p) {
         for (int st = 0; st < PS; ++st) {
           const uint4 f = la_pack<E>(s, st);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) acc[m][n] = LOp<E>::mma(la_tfrag<E, DK>(kimg + m * KIMG, 32 * ks, st, n, lane), f, acc[m][n]);
+          for (int n = 0; n < NT; ++n) acc[m][n] = LOp<E>::mma(la_tfrag<E, DK>(kimg + m * KIMG, 32 * ks, st, n, ln), f, acc[m][n]);
         }
       }
     }
@@ -182,6 +184,30 @@ __global__ __launch_bounds__(256) void attn_long_dq_kernel(const LongP p) {
   }
 }
 
+// Sums along the diagonals of a 32 x 32 result x (columns c = lane & 31, rows q): s0: rows 0-15, lane n holds the diagonal
+// c - q = n - 15; s1: rows 16-31, c - q = n - 31; lanes >= 47 are zero.  Horner's scheme over the rows, each step one lane further
+// (the half waves hold rows 4 apart: both are spread over the whole wave first, the other half zero).
+__device__ __forceinline__ void la_diagonals(const f32x16& x, float& s0, float& s1) {
+  float acc[2] = {0.f, 0.f};
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    float lo[4], hi[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x[4 * g + e]), 0u, false, false);
+      lo[e] = __uint_as_float(r[0]);
+      hi[e] = __uint_as_float(r[1]);
+    }
+    float& a = acc[g >> 1];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) a = __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(a), 0x138, 0xf, 0xf, true)) + lo[e];  // wave_shr:1
+#pragma unroll
+    for (int e = 0; e < 4; ++e) a = __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(a), 0x138, 0xf, 0xf, true)) + hi[e];
+  }
+  s0 = acc[0];
+  s1 = acc[1];
+}
+
 // Distances [lo, hi] of bucket bk, clipped to what the sums below hold; false: none
 __device__ __forceinline__ bool la_bucket_range(const LongP& p, int bk, int& lo, int& hi) {
   const int far = p.max_distance + LA_PAD, half = p.bidirectional ? p.nbuckets / 2 : p.nbuckets;
@@ -200,11 +226,12 @@ __device__ __forceinline__ bool la_bucket_range(const LongP& p, int bk, int& lo,
 }
 
 // One block = 128 keys of one (utterance, key head), a wave = 32 of them; the queries of every head of the group stream through LDS.
-// Table gradient: a wave adds dS along its patches' diagonals into its own two copies (one per half wave) of a distance-indexed
-// array in LDS -- the 32 lanes of a half wave hold 32 different distances of one register, so no two lanes ever meet -- and patches
-// beyond max_distance go into two registers.
+// Table gradient: a wave adds dS along its patches' diagonals (la_diagonals) into its own two copies of a distance-indexed array in
+// LDS, read and written back by the one lane that holds a distance; patches beyond max_distance go into two registers.  LDS atomics
+// instead (ds_add_f32 of every element, no two lanes on one address) took about 330 cycles per wave instruction: 361 us for 24 x 1250
+// frames of 4 x 64 channels against 135 us this way.
 template <typename E, int DK, int DV, int MAPS, bool BIAS>
-__global__ __launch_bounds__(256) void attn_long_dkv_kernel(const LongP p) {
+__global__ __launch_bounds__(256, sizeof(E) == 4 || MAPS * DK == 128 ? 1 : 2) void attn_long_dkv_kernel(const LongP p) {
   constexpr int CH = LOp<E>::CH, KS = DK / (2 * CH), VS = DV / (2 * CH), PS = 16 / CH, NK = DK / 32, NV = DV / 32;
   constexpr bool F32 = sizeof(E) == 4;  // (its fragments fill the register file: the scheduler must not fetch further ahead)
   constexpr int NBUF = sizeof(E) == 4 ? 1 : 2;  // (f32 tiles twice and the widest distance array would pass 160 KiB)
@@ -212,10 +239,10 @@ __global__ __launch_bounds__(256) void attn_long_dkv_kernel(const LongP p) {
   constexpr int QIMG = LA_TILE * DK, OIMG = LA_TILE * DV;
   constexpr int BUFB = (MAPS * QIMG + OIMG) * (int)sizeof(E) + 1024;  // + (lse, D) of every map, 64 floats each
   float* const btab = reinterpret_cast<float*>(smem + NBUF * BUFB);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lk = lane & 31, hw = lane >> 5;
+  const int lane = threadIdx.x & 63, wave = la_wave(), lk = lane & 31, hw = lane >> 5;
   const int dist_n = la_btab_len(p);
   float* const hist = btab + ((dist_n + 3) & ~3);  // [8][dist_n]
-  float* const myhist = hist + (2 * wave + hw) * dist_n;
+  float* const myhist = hist + 2 * wave * dist_n;
 
   const int t = xcd_remap(blockIdx.x, gridDim.x);
   const int kt = t % p.nkt, bh = t / p.nkt, hk = bh % p.Hk, b = bh / p.Hk, G = p.H / p.Hk;
@@ -299,7 +326,7 @@ __global__ __launch_bounds__(256) void attn_long_dkv_kernel(const LongP p) {
       if (la_bucket_range(p, bk, lo_d, hi_d))
         for (int d = max(lo_d, -D - LA_PAD) + lane; d <= min(hi_d, D + LA_PAD); d += 64) s += hist[d + D + LA_PAD];
       s = wave_sum(s);
-      if (lane == 0) p.tab_part[(((int64_t)b * p.nkt + kt) * p.H + h) * p.nbuckets + bk] = s;
+      if (lane == 0) p.tab_part[((int64_t)h * p.nbuckets + bk) * ((int64_t)p.B * p.nkt) + b * p.nkt + kt] = s;
     }
     la_barrier();
   };
@@ -388,18 +415,22 @@ __global__ __launch_bounds__(256) void attn_long_dkv_kernel(const LongP p) {
           if (F32) __builtin_amdgcn_sched_barrier(0);
         }
         if constexpr (BIAS) {
-          // (a column behind the keys holds unmasked values: it must not count; its dk / dv rows are written as zeros)
-          if (near) {
-            float* hp = myhist + (jk - q0 - 4 * hw + D + LA_PAD);
-            if (jk < klen) {
+          if (j0 + 32 > klen) {  // (a column behind the keys holds unmasked values: it must not count; its dk / dv rows are written as zeros)
 #pragma unroll
-              for (int r = 0; r < 16; ++r) __hip_atomic_fetch_add(hp - (8 * (r >> 2) + (r & 3)), hsum[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            for (int r = 0; r < 16; ++r) hsum[r] = jk < klen ? hsum[r] : 0.f;
+          }
+          if (near) {
+            float s0, s1;
+            la_diagonals(hsum, s0, s1);
+            if (lane < 47) {
+              float* hp = myhist + (j0 - q0 + D + LA_PAD - 15 + lane);
+              hp[0] += s0;
+              hp[dist_n - 16] += s1;
             }
           } else {
             float s = 0.f;
 #pragma unroll
             for (int r = 0; r < 16; ++r) s += hsum[r];
-            s = jk < klen ? s : 0.f;
             if (dmin >= D) far_hi += s;
             else far_lo += s;
           }
@@ -442,19 +473,19 @@ __global__ __launch_bounds__(256) void attn_long_dkv_kernel(const LongP p) {
     }
 }
 
-// blocks [0, H) (with a table): one head's column of dtable; the rest: one head's (or the shared) lam vectors
+// waves [0, H * nbuckets) (with a table): one entry of dtable each; the last blocks: one head's (or the shared) lam vectors
 __global__ __launch_bounds__(256) void attn_long_fin_kernel(const LongP p, float* dtable, float* dlam, int accumulate) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int ntab = p.table ? p.H : 0;
+  const int lane = threadIdx.x & 63, wave = la_wave();
+  const int ntab = p.table ? (p.H * p.nbuckets + LA_WAVES - 1) / LA_WAVES : 0;
   if ((int)blockIdx.x < ntab) {
-    const int h = blockIdx.x, n = p.B * p.nkt;
-    for (int bk = wave; bk < p.nbuckets; bk += LA_WAVES) {
-      float s = 0.f;
-      for (int i = lane; i < n; i += 64) s += p.tab_part[((int64_t)i * p.H + h) * p.nbuckets + bk];
-      s = wave_sum(s);
-      float* d = dtable + (int64_t)bk * p.H + h;
-      if (lane == 0) *d = accumulate ? *d + s : s;
-    }
+    const int w = blockIdx.x * LA_WAVES + wave, h = w / p.nbuckets, bk = w % p.nbuckets, n = p.B * p.nkt;
+    if (h >= p.H) return;
+    float s = 0.f;
+#pragma unroll 8
+    for (int i = lane; i < n; i += 64) s += p.tab_part[((int64_t)h * p.nbuckets + bk) * n + i];
+    s = wave_sum(s);
+    float* d = dtable + (int64_t)bk * p.H + h;
+    if (lane == 0) *d = accumulate ? *d + s : s;
     return;
   }
   __shared__ float red[LA_WAVES];
@@ -543,7 +574,7 @@ extern "C" int ptpp_attention_long_bwd(const ptpp_attention_long_args* a, void* 
   else if (a->dtype == PTPP_BF16) r = dispatch_bwd<bf16_raw>(p, a->maps, st);
   else r = dispatch_bwd<f16_raw>(p, a->maps, st);
   if (r != PTPP_OK) return r;
-  const int blocks = (p.table ? p.H : 0) + (a->maps == 2 ? p.lam_heads : 0);
+  const int blocks = (p.table ? (p.H * p.nbuckets + LA_WAVES - 1) / LA_WAVES : 0) + (a->maps == 2 ? p.lam_heads : 0);
   hipLaunchKernelGGL(attn_long_fin_kernel, dim3(blocks), dim3(256), 0, st, p, a->dtable, a->dlam, a->accumulate);
   PTPP_CHECK_LAUNCH("attention_long_bwd (parameters)");
   return PTPP_OK;

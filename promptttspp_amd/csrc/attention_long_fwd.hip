@@ -6,17 +6,75 @@
 
 namespace {
 
+// ---- the softmax of one 32 x 32 patch of scores, a lane = one query and 16 of the keys -----------------------------------
+// No running maximum yet: far below every score that a matrix instruction of finite operands gives, and still a finite reference
+constexpr float LA_NONE = -1.0e30f;
+// The reference is raised only when a score passes it by more than this (base 2): probabilities up to 2^6 are as exact in every
+// element type, and the rescaling of the context -- as many operations as there are scores -- almost never happens.
+constexpr float LA_RAISE = 6.f;
+
+// scores in base 2 are s * mul + add afterwards.  Patches with a distance inside (-max_distance, max_distance) read the bias of every pair
+// (bt: the table at the lane's query and first key), the others share one value: no operation per element.
+template <bool BIAS>
+__device__ __forceinline__ void la_scores(f32x16& s, float c2, const float* bt, const float* table, int D, int dmin, int dmax, float& mul, float& add) {
+  mul = c2;
+  add = 0.f;
+  if constexpr (BIAS) {
+    if (dmin < D && dmax > -D) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, bt[8 * (r >> 2) + (r & 3)]);
+      mul = 1.f;
+    } else {
+      add = table[dmin >= D ? 2 * (D + LA_PAD) : 0];
+    }
+  }
+}
+__device__ __forceinline__ void la_mask(f32x16& s, int jend) {  // keys from jend on (counted from the lane's first) are not seen
+#pragma unroll
+  for (int r = 0; r < 16; ++r) s[r] = 8 * (r >> 2) + (r & 3) < jend ? s[r] : -INFINITY;
+}
+__device__ __forceinline__ float la_max16(const f32x16& s) {
+  float m = s[0];
+#pragma unroll
+  for (int r = 1; r < 16; ++r) m = fmaxf(m, s[r]);
+  return m;
+}
+template <int NT>
+__device__ __forceinline__ void la_raise(float& mx, float& l, f32x16 (&o)[NT], float tm) {
+  if (!__any(tm > mx + LA_RAISE)) return;
+  const float mn = fmaxf(mx, tm), al = la_exp2(mx - mn);
+  mx = mn;
+  l *= al;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[n][r] *= al;
+}
+// s -> 2^(s * mul + add), and their sum
+__device__ __forceinline__ float la_probs(f32x16& s, float mul, float add) {
+  float a = 0.f, b = 0.f;
+#pragma unroll
+  for (int r = 0; r < 16; r += 2) {
+    s[r] = la_exp2(fmaf(s[r], mul, add));
+    s[r + 1] = la_exp2(fmaf(s[r + 1], mul, add));
+    a += s[r];
+    b += s[r + 1];
+  }
+  return a + b;
+}
+
 // One block = 128 query rows of one (utterance, head), a wave = 32 of them; keys and values stream through LDS in tiles of 64,
 // the next tile's LDS-DMA under the current tile's products.
 template <typename E, int DK, int DV, int MAPS, bool BIAS>
-__global__ __launch_bounds__(256) void attn_long_fwd_kernel(const LongP p) {
+__global__ __launch_bounds__(256, sizeof(E) == 4 ? 1 : 2) void attn_long_fwd_kernel(const LongP p) {
   constexpr int CH = LOp<E>::CH, KS = DK / (2 * CH), PS = 16 / CH, NT = DV / 32;
-  constexpr int KSUB = sizeof(E) == 4 ? 1 : 2;  // 32-key patches taken at once (f32 fragments are twice as many registers)
+  constexpr int KSUB = sizeof(E) == 4 || MAPS * DV == 256 ? 1 : 2;  // 32-key patches taken at once (as registers allow)
+  constexpr bool TIGHT = sizeof(E) == 4 || MAPS * DV == 256;  // registers are short: LDS addresses and fragments not far ahead of use
   extern __shared__ __attribute__((aligned(16))) char smem[];
   constexpr int KIMG = LA_TILE * DK, VIMG = LA_TILE * DV, BUF = MAPS * KIMG + VIMG;
   E* const img = reinterpret_cast<E*>(smem);
   float* const btab = reinterpret_cast<float*>(smem + 2 * BUF * sizeof(E));
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lq = lane & 31, hw = lane >> 5;
+  const int lane = threadIdx.x & 63, wave = la_wave(), lq = lane & 31, hw = lane >> 5;
 
   const int t = xcd_remap(blockIdx.x, gridDim.x);
   const int qt = t % p.nqt, bh = t / p.nqt, h = bh % p.H, b = bh / p.H, hk = h / (p.H / p.Hk);
@@ -61,7 +119,7 @@ __global__ __launch_bounds__(256) void attn_long_fwd_kernel(const LongP p) {
   float mx[MAPS], l[MAPS];
 #pragma unroll
   for (int m = 0; m < MAPS; ++m) {
-    mx[m] = -INFINITY;
+    mx[m] = LA_NONE;
     l[m] = 0.f;
 #pragma unroll
     for (int n = 0; n < NT; ++n) o[m][n] = f32x16{};
@@ -84,6 +142,7 @@ __global__ __launch_bounds__(256) void attn_long_fwd_kernel(const LongP p) {
 #pragma unroll 1
     for (int sub = 0; sub < 2 / KSUB; ++sub) {
       uint4 pf[MAPS][KSUB][PS];
+      const int ln = TIGHT ? la_opaque(lane) : lane, lr = ln & 31, hr = ln >> 5;
 #pragma unroll
       for (int m = 0; m < MAPS; ++m) {
         f32x16 s[KSUB];
@@ -92,55 +151,24 @@ __global__ __launch_bounds__(256) void attn_long_fwd_kernel(const LongP p) {
           s[ks] = f32x16{};
 #pragma unroll
           for (int kk = 0; kk < KS; ++kk)
-            s[ks] = LOp<E>::mma(la_frag<E, DK>(kimg + m * KIMG, 32 * (sub * KSUB + ks) + lq, 2 * kk + hw), qf[m][kk], s[ks]);
+            s[ks] = LOp<E>::mma(la_frag<E, DK>(kimg + m * KIMG, 32 * (sub * KSUB + ks) + lr, 2 * kk + hr), qf[m][kk], s[ks]);
         }
-        float tm = -INFINITY;
+        float tm = -INFINITY, mul[KSUB], add[KSUB];
 #pragma unroll
         for (int ks = 0; ks < KSUB; ++ks) {
           const int j0 = tile * LA_TILE + 32 * (sub * KSUB + ks);
-          if constexpr (BIAS) {
-            const int dmin = j0 - (q0 + 31), dmax = j0 + 31 - q0;  // distances of this 32 x 32 patch
-            if (dmin < D && dmax > -D) {
-              const float* bt = btab + (j0 - q0 - lq + 4 * hw + D + LA_PAD);
-#pragma unroll
-              for (int r = 0; r < 16; ++r) s[ks][r] = fmaf(s[ks][r], c2, bt[8 * (r >> 2) + (r & 3)]);
-            } else {
-              const float bc = dmin >= D ? btab[2 * (D + LA_PAD)] : btab[0];
-#pragma unroll
-              for (int r = 0; r < 16; ++r) s[ks][r] = fmaf(s[ks][r], c2, bc);
-            }
-          } else {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[ks][r] *= c2;
-          }
-          if (j0 + 32 > kend || (p.causal && j0 + 31 > q0)) {
-            const int jend = min(klen, p.causal ? q0 + lq + 1 : klen) - j0 - 4 * hw;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[ks][r] = 8 * (r >> 2) + (r & 3) < jend ? s[ks][r] : -INFINITY;
-          }
-#pragma unroll
-          for (int r = 0; r < 16; ++r) tm = fmaxf(tm, s[ks][r]);
+          const float* bt = btab + (j0 - q0 - lq + 4 * hw + D + LA_PAD);
+          la_scores<BIAS>(s[ks], c2, bt, btab, D, j0 - (q0 + 31), j0 + 31 - q0, mul[ks], add[ks]);
+          if (j0 + 32 > kend || (p.causal && j0 + 31 > q0)) la_mask(s[ks], min(klen, p.causal ? q0 + lq + 1 : klen) - j0 - 4 * hw);
+          tm = fmaxf(tm, fmaf(la_max16(s[ks]), mul[ks], add[ks]));
         }
-        const float mn = fmaxf(mx[m], la_half_max(tm));
-        const float mu = mn == -INFINITY ? 0.f : mn;  // (no key seen yet: every exponent below is -inf)
-        const float al = la_exp2(mx[m] - mu);
-        mx[m] = mn;
-        float sum = 0.f;
+        la_raise<NT>(mx[m], l[m], o[m], la_half_max(tm));
 #pragma unroll
         for (int ks = 0; ks < KSUB; ++ks) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            s[ks][r] = la_exp2(s[ks][r] - mu);
-            sum += s[ks][r];
-          }
+          l[m] += la_probs(s[ks], mul[ks], add[ks] - mx[m]);
 #pragma unroll
           for (int st = 0; st < PS; ++st) pf[m][ks][st] = la_pack<E>(s[ks], st);
         }
-        l[m] = fmaf(l[m], al, sum);
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) o[m][n][r] *= al;
       }
 #pragma unroll
       for (int ks = 0; ks < KSUB; ++ks)
@@ -148,9 +176,10 @@ __global__ __launch_bounds__(256) void attn_long_fwd_kernel(const LongP p) {
         for (int st = 0; st < PS; ++st)
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            const uint4 vf = la_tfrag<E, DV>(vimg, 32 * (sub * KSUB + ks), st, n, lane);
+            const uint4 vf = la_tfrag<E, DV>(vimg, 32 * (sub * KSUB + ks), st, n, ln);
 #pragma unroll
             for (int m = 0; m < MAPS; ++m) o[m][n] = LOp<E>::mma(vf, pf[m][ks][st], o[m][n]);
+            if (TIGHT && n % 2 == 1) __builtin_amdgcn_sched_barrier(0);
           }
     }
     la_barrier();
@@ -195,21 +224,352 @@ __global__ __launch_bounds__(256) void attn_long_fwd_kernel(const LongP p) {
     }
 }
 
+// ---------------------------------------------------------------------------------------------------------------------------
+// Few query rows or few tiles: one block = 32 columns -- 32 queries of one head, or all queries of several heads that share their
+// keys (a step of one query: Tq = 1) -- and one of `splits` ranges of the keys; its W waves take 32-key chunks of the range in turn,
+// each streaming its own chunks through its own two LDS buffers (no block barrier in the loop), and join at the end.  With more
+// than one range the blocks leave unnormalised sums and (max, sum) for the join kernel.  A step is HBM-bound: every key and value is
+// read once, 64 KB in flight per CU.
+template <typename E, int DK, int DV, int MAPS>
+struct LSplit {
+  static constexpr int STAGE = 32 * (MAPS * DK + DV);                     // elements of a chunk's images
+  static constexpr int W = STAGE * (int)sizeof(E) > 16384 ? 2 : LA_WAVES;  // (f32, wide heads: 32 KB per chunk)
+  static constexpr int LDS = 2 * W * STAGE * (int)sizeof(E);
+};
+
+template <typename E, int DK, int DV, int MAPS, bool BIAS>
+__global__ __launch_bounds__((LSplit<E, DK, DV, MAPS>::W * 64), sizeof(E) == 4 || MAPS * DV == 256 ? 1 : 2) void attn_long_split_kernel(const LongP p) {
+  typedef LSplit<E, DK, DV, MAPS> S_;
+  constexpr int W = S_::W, STAGE = S_::STAGE, KIMG = 32 * DK;
+  constexpr bool TIGHT = sizeof(E) == 4 || MAPS * DV == 256;
+  constexpr int CH = LOp<E>::CH, KS = DK / (2 * CH), PS = 16 / CH, NT = DV / 32;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ float wml[W][MAPS][2][32];
+  const int lane = threadIdx.x & 63, wave = la_wave(), lq = lane & 31, hw = lane >> 5;
+  float* const btab = reinterpret_cast<float*>(smem + S_::LDS);
+  E* const img = reinterpret_cast<E*>(smem) + wave * 2 * STAGE;
+
+  // block -> (range, utterance, key head, head group, row block); ranges of one key head run on the same XCD
+  const int t = xcd_remap(blockIdx.x, gridDim.x);
+  const int sp = t % p.splits, tl = t / p.splits;  // tl: number of the 32-column block
+  const int rb = tl % p.nrb, G = p.H / p.Hk, hg = (tl / p.nrb) % (G / p.nh), bk = tl / (p.nrb * (G / p.nh));
+  const int hk = bk % p.Hk, b = bk / p.Hk, h0 = hk * G + hg * p.nh;
+  const int klen = la_klen(p, b), qlen = la_qlen(p, b), qs = la_qstart(p, b);
+  const int dv = MAPS * p.dk;
+
+  // the lane's column: query iq of head h
+  const int hcol = p.nh > 1 ? min(lq / p.Tq, p.nh - 1) : 0, h = h0 + hcol;
+  const int i0 = rb * 32, iq = p.nh > 1 ? (lq < p.nh * p.Tq ? lq % p.Tq : p.Tq) : i0 + lq;  // (Tq: no query)
+  const int ilo = i0, ihi = p.nh > 1 ? p.Tq - 1 : i0 + 31;
+  int kend = ilo < qlen ? klen : 0;
+  if (p.causal) kend = min(kend, max(0, qs + min(ihi + 1, qlen)));
+  const int nc = (kend + 31) >> 5, per = (nc + p.splits - 1) / p.splits;
+  const int c0 = sp * per, c1 = min(nc, c0 + per);
+
+  const E* kb = reinterpret_cast<const E*>(p.k) + b * p.sk + (int64_t)hk * MAPS * p.dk;
+  const E* vb = reinterpret_cast<const E*>(p.v) + b * p.sv + (int64_t)hk * dv;
+  LTile<E, DK, 32, 1> kt;
+  LTile<E, DV, 32, 1> vt;
+  kt.init(p.ldk, p.dk, lane, 0);
+  vt.init(p.ldv, dv, lane, 0);
+  constexpr int NDMA = MAPS * LTile<E, DK, 32, 1>::NI + LTile<E, DV, 32, 1>::NI;
+  auto issue = [&](int c, int buf) {
+    const int j0 = 32 * c;
+    E* d = img + buf * STAGE;
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m) kt.issue(kb + (int64_t)j0 * p.ldk + m * p.dk, kend - j0, d + m * KIMG, lane, 0);
+    vt.issue(vb + (int64_t)j0 * p.ldv, kend - j0, d + MAPS * KIMG, lane, 0);
+  };
+  int c = c0 + wave;
+  if (c < c1) issue(c, 0);
+  const int dist_n = la_btab_len(p);
+  if constexpr (BIAS)
+    for (int n = 0; n < p.nh; ++n) la_fill_btab(p, btab + n * dist_n, h0 + n);
+
+  uint4 qf[MAPS][KS];
+  {
+    const E* qb = reinterpret_cast<const E*>(p.q) + b * p.sq + (int64_t)h * MAPS * p.dk + (int64_t)iq * p.ldq;
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m)
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const int ch = (2 * s + hw) * CH;
+        qf[m][s] = (iq < qlen && ch < p.dk) ? *reinterpret_cast<const uint4*>(qb + m * p.dk + ch) : uint4{0, 0, 0, 0};
+      }
+  }
+  f32x16 o[MAPS][NT];
+  float mx[MAPS], l[MAPS];
+#pragma unroll
+  for (int m = 0; m < MAPS; ++m) {
+    mx[m] = LA_NONE;
+    l[m] = 0.f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) o[m][n] = f32x16{};
+  }
+  const float c2 = p.scale * LA_LOG2E;
+  const int D = p.max_distance, qp = qs + min(iq, ihi);  // (a column without a query reads the table within bounds)
+  if constexpr (BIAS) la_barrier();
+
+  for (int buf = 0; c < c1; c += W, buf ^= 1) {
+    if (c + W < c1) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the buffer's last reads are done
+      issue(c + W, buf ^ 1);
+      glds_wait<NDMA>();
+    } else {
+      glds_wait<0>();
+    }
+    const E* kimg = img + buf * STAGE;
+    const E* vimg = kimg + MAPS * KIMG;
+    const int j0 = 32 * c;
+    const int ln = TIGHT ? la_opaque(lane) : lane, lr = ln & 31, hr = ln >> 5;
+    uint4 pf[MAPS][PS];
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m) {
+      f32x16 s = f32x16{};
+#pragma unroll
+      for (int kk = 0; kk < KS; ++kk) {
+        s = LOp<E>::mma(la_frag<E, DK>(kimg + m * KIMG, lr, 2 * kk + hr), qf[m][kk], s);
+        if (TIGHT && kk % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      }
+      float mul, add;
+      const float* bt0 = btab + hcol * dist_n;
+      la_scores<BIAS>(s, c2, bt0 + (j0 - qp + 4 * hw + D + LA_PAD), bt0, D, j0 - (qs + ihi), j0 + 31 - (qs + ilo), mul, add);
+      if (j0 + 32 > kend || (p.causal && j0 + 31 > qs + ilo)) la_mask(s, min(klen, p.causal ? qp + 1 : klen) - j0 - 4 * hw);
+      la_raise<NT>(mx[m], l[m], o[m], la_half_max(fmaf(la_max16(s), mul, add)));
+      l[m] += la_probs(s, mul, add - mx[m]);
+#pragma unroll
+      for (int st = 0; st < PS; ++st) pf[m][st] = la_pack<E>(s, st);
+    }
+#pragma unroll
+    for (int st = 0; st < PS; ++st)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const uint4 vf = la_tfrag<E, DV>(vimg, 0, st, n, ln);
+#pragma unroll
+        for (int m = 0; m < MAPS; ++m) o[m][n] = LOp<E>::mma(vf, pf[m][st], o[m][n]);
+        if (TIGHT) __builtin_amdgcn_sched_barrier(0);
+      }
+  }
+
+  // ---- join the waves: common maximum, then each wave's sums through its own buffers ----
+#pragma unroll
+  for (int m = 0; m < MAPS; ++m) {
+    l[m] = la_half_sum(l[m]);
+    if (hw == 0) {
+      wml[wave][m][0][lq] = mx[m];
+      wml[wave][m][1][lq] = l[m];
+    }
+  }
+  la_barrier();
+  float M[MAPS], L[MAPS];
+#pragma unroll
+  for (int m = 0; m < MAPS; ++m) {
+    M[m] = LA_NONE;
+#pragma unroll
+    for (int w = 0; w < W; ++w) M[m] = fmaxf(M[m], wml[w][m][0][lq]);
+    L[m] = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) L[m] = fmaf(wml[w][m][1][lq], la_exp2(wml[w][m][0][lq] - M[m]), L[m]);
+    const float al = la_exp2(mx[m] - M[m]);
+    float* mine = reinterpret_cast<float*>(img) + m * NT * 1024 + lane;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mine[(n * 16 + r) * 64] = o[m][n][r] * al;
+  }
+  static_assert(MAPS * NT * 1024 * 4 <= 2 * STAGE * (int)sizeof(E), "a wave's sums fit its buffers");
+  la_barrier();
+  const bool row = iq < p.Tq;
+  float lam = 0.f;
+  if constexpr (MAPS == 2) lam = la_lambda(p, h, lane);
+  float inv[MAPS];
+#pragma unroll
+  for (int m = 0; m < MAPS; ++m) {
+    const bool on = iq < qlen && !(L[m] == 0.f);
+    inv[m] = on ? 1.f / L[m] : 0.f;
+    if (wave == 0 && hw == 0) {
+      if (p.splits > 1) {
+        if (row) {
+          float* ml = p.part_ml + ((((int64_t)tl * p.splits + sp) * MAPS + m) * 32 + lq) * 2;
+          ml[0] = M[m];
+          ml[1] = L[m];
+        }
+      } else if (p.lse && iq < p.TqP) {
+        p.lse[(((int64_t)m * p.B + b) * p.H + h) * p.TqP + iq] = on ? M[m] + log2f(L[m]) : INFINITY;
+      }
+    }
+  }
+  const float* all = reinterpret_cast<const float*>(smem) + lane;
+  for (int ng = wave; ng < NT * 4; ng += W) {  // registers 4 g .. 4 g + 3 of channel block n: channels 32 n + 8 g + 4 hw + (0..3)
+    const int ch = 32 * (ng >> 2) + 8 * (ng & 3) + 4 * hw;
+    float v[MAPS][4];
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[m][e] = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) v[m][e] += all[w * (2 * STAGE * (int)sizeof(E) / 4) + (m * NT * 16 + ng * 4 + e) * 64];
+      }
+    if (!row || ch >= dv) continue;
+    if (p.splits > 1) {
+#pragma unroll
+      for (int m = 0; m < MAPS; ++m)
+        *reinterpret_cast<f32x4*>(p.part_o + ((((int64_t)tl * p.splits + sp) * MAPS + m) * 32 + lq) * DV + ch) = f32x4{v[m][0], v[m][1], v[m][2], v[m][3]};
+    } else {
+      E* ob = reinterpret_cast<E*>(p.out) + b * p.so + (int64_t)iq * p.ldo + (int64_t)h * dv + ch;
+      float r[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        r[e] = v[0][e] * inv[0];
+        if constexpr (MAPS == 2) r[e] = fmaf(-lam, v[MAPS - 1][e] * inv[MAPS - 1], r[e]);
+      }
+      la_store4<E>(ob, r[0], r[1], r[2], r[3]);
+      if constexpr (MAPS == 2) {
+        if (p.out2) {
+          const float w = inv[MAPS - 1];
+          la_store4<E>(reinterpret_cast<E*>(p.out2) + ((int64_t)b * p.Tq + iq) * ((int64_t)p.H * dv) + (int64_t)h * dv + ch, v[MAPS - 1][0] * w,
+                       v[MAPS - 1][1] * w, v[MAPS - 1][2] * w, v[MAPS - 1][3] * w);
+        }
+      }
+    }
+  }
+}
+
+// join of the key ranges: one wave per (block, column)
+template <typename E, int DV, int MAPS>
+__global__ __launch_bounds__(256) void attn_long_join_kernel(const LongP p, int ncol) {
+  const int lane = threadIdx.x & 63;
+  const int64_t w = (int64_t)blockIdx.x * LA_WAVES + la_wave();
+  const int G = p.H / p.Hk, cols = p.nh > 1 ? p.nh * p.Tq : 32;
+  if (w >= (int64_t)ncol) return;
+  const int tl = (int)(w / cols), lq = (int)(w % cols);
+  const int rb = tl % p.nrb, hg = (tl / p.nrb) % (G / p.nh), bk = tl / (p.nrb * (G / p.nh));
+  const int hk = bk % p.Hk, b = bk / p.Hk, h = hk * G + hg * p.nh + (p.nh > 1 ? lq / p.Tq : 0);
+  const int iq = p.nh > 1 ? lq % p.Tq : rb * 32 + lq, dv = MAPS * p.dk;
+  float lam = 0.f;
+  if constexpr (MAPS == 2) lam = la_lambda(p, h, lane);
+  constexpr int NC = DV / 64;  // channels per lane
+  float r[MAPS][NC];
+  const bool row = iq < p.Tq;
+  const bool on = iq < la_qlen(p, b);
+#pragma unroll
+  for (int m = 0; m < MAPS; ++m) {
+    const int64_t base = (((int64_t)tl * p.splits) * MAPS + m) * 32 + lq, step = MAPS * 32;
+    float mm = LA_NONE, ll = 0.f;
+    if (row && lane < p.splits) {  // (splits <= 64)
+      mm = p.part_ml[(base + lane * step) * 2];
+      ll = p.part_ml[(base + lane * step) * 2 + 1];
+    }
+    float M = mm;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+    const float f = la_exp2(mm - M);
+    const float L = wave_sum(f * ll);
+    const bool ok = on && !(L == 0.f);
+#pragma unroll
+    for (int n = 0; n < NC; ++n) r[m][n] = 0.f;
+    if (row)
+      for (int s = 0; s < p.splits; ++s) {
+        const float fs = __shfl(f, s, 64);
+#pragma unroll
+        for (int n = 0; n < NC; ++n)
+          if (lane + 64 * n < dv) r[m][n] = fmaf(p.part_o[(base + s * step) * DV + lane + 64 * n], fs, r[m][n]);
+      }
+#pragma unroll
+    for (int n = 0; n < NC; ++n) r[m][n] *= ok ? 1.f / L : 0.f;
+    if (p.lse && lane == 0 && iq < p.TqP) p.lse[(((int64_t)m * p.B + b) * p.H + h) * p.TqP + iq] = ok ? M + log2f(L) : INFINITY;
+  }
+  if (!row) return;
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+    const int ch = lane + 64 * n;
+    if (ch >= dv) continue;
+    float v = r[0][n];
+    if constexpr (MAPS == 2) {
+      v = fmaf(-lam, r[MAPS - 1][n], v);
+      if (p.out2) Elem<E>::st(reinterpret_cast<E*>(p.out2) + ((int64_t)b * p.Tq + iq) * ((int64_t)p.H * dv) + (int64_t)h * dv + ch, r[MAPS - 1][n]);
+    }
+    Elem<E>::st(reinterpret_cast<E*>(p.out) + b * p.so + (int64_t)iq * p.ldo + (int64_t)h * dv + ch, v);
+  }
+}
+
+// The rule: 128-row tiles when they fill the chip (more than 256 blocks) and hold more than a quarter of rows; else the few-row form,
+// with as many key ranges as bring its grid to about 512 blocks of four waves (two per CU) at no fewer than two 32-key chunks per wave.
+bool few_rows(const LongP& p) { return p.Tq <= 32 || (int64_t)p.nqt * p.B * p.H <= 256; }
+// fills nh, nrb, splits; returns the number of 32-column blocks (0: too many to number)
+int plan_few(LongP& p, int waves) {
+  const int G = p.H / p.Hk;
+  p.nh = 1;
+  if (!p.lse)  // (backward's statistics are padded to whole blocks of one head's rows)
+    for (int n = 2; n <= G && n * p.Tq <= 32; ++n)
+      if (G % n == 0 && (!p.table || n * (2 * (p.max_distance + LA_PAD) + 1) <= 6144)) p.nh = n;  // (24 KB of bias tables)
+  p.nrb = p.nh > 1 ? 1 : (p.lse ? p.TqP : p.Tq + 31) / 32;
+  const int64_t blocks = (int64_t)p.B * p.Hk * (G / p.nh) * p.nrb;
+  const int64_t most = ((int64_t)p.Tk + 64 * waves - 1) / (64 * waves);
+  int64_t s = blocks ? 512 / blocks : 1;
+  if (s > most) s = most;
+  p.splits = s < 1 ? 1 : s > 64 ? 64 : (int)s;
+  return blocks * p.splits < (1ll << 31) ? (int)blocks : 0;
+}
+template <typename E>
+int few_waves(int maps, int dk) {
+  if (maps == 1) return dk <= 64 ? LSplit<E, 64, 64, 1>::W : LSplit<E, 128, 128, 1>::W;
+  return dk <= 32 ? LSplit<E, 32, 64, 2>::W : LSplit<E, 64, 128, 2>::W;
+}
+int few_waves(int dtype, int maps, int dk) {
+  return dtype == PTPP_F32 ? few_waves<float>(maps, dk) : dtype == PTPP_BF16 ? few_waves<bf16_raw>(maps, dk) : few_waves<f16_raw>(maps, dk);
+}
+int pad_dv(int maps, int dk) { return maps == 1 ? (dk <= 64 ? 64 : 128) : (dk <= 32 ? 64 : 128); }
+
 template <typename E, int DK, int DV, int MAPS>
 int launch_fwd(const LongP& p, hipStream_t st) {
-  const size_t sm = 2 * (size_t)LA_TILE * (MAPS * DK + DV) * sizeof(E) + (p.table ? (2 * (p.max_distance + LA_PAD) + 4) * sizeof(float) : 0);
-  const dim3 g((unsigned)((int64_t)p.nqt * p.B * p.H));
-  const void* kern = p.table ? (const void*)attn_long_fwd_kernel<E, DK, DV, MAPS, true> : (const void*)attn_long_fwd_kernel<E, DK, DV, MAPS, false>;
+  const size_t tab = p.table ? (2 * (p.max_distance + LA_PAD) + 1) * sizeof(float) : 0;
+  if (!p.splits) {
+    const size_t sm = 2 * (size_t)LA_TILE * (MAPS * DK + DV) * sizeof(E) + tab;
+    const dim3 g((unsigned)((int64_t)p.nqt * p.B * p.H));
+    const void* kern = p.table ? (const void*)attn_long_fwd_kernel<E, DK, DV, MAPS, true> : (const void*)attn_long_fwd_kernel<E, DK, DV, MAPS, MAPS == 1>;
+    if (sm > 64 * 1024 && !ptpp_lds_limit(kern, (int)sm, "attention_long_fwd")) return PTPP_ELAUNCH;
+    if (p.table) hipLaunchKernelGGL((attn_long_fwd_kernel<E, DK, DV, MAPS, true>), g, dim3(256), sm, st, p);
+    else if constexpr (MAPS == 2) hipLaunchKernelGGL((attn_long_fwd_kernel<E, DK, DV, MAPS, false>), g, dim3(256), sm, st, p);
+    PTPP_CHECK_LAUNCH("attention_long_fwd");
+    return PTPP_OK;
+  }
+  typedef LSplit<E, DK, DV, MAPS> S_;
+  const size_t sm = S_::LDS + p.nh * tab;
+  const int blocks = p.B * p.Hk * (p.H / p.Hk / p.nh) * p.nrb;
+  const dim3 g((unsigned)(blocks * p.splits)), t(S_::W * 64);
+  const void* kern = p.table ? (const void*)attn_long_split_kernel<E, DK, DV, MAPS, true> : (const void*)attn_long_split_kernel<E, DK, DV, MAPS, MAPS == 1>;
   if (sm > 64 * 1024 && !ptpp_lds_limit(kern, (int)sm, "attention_long_fwd")) return PTPP_ELAUNCH;
-  if (p.table) hipLaunchKernelGGL((attn_long_fwd_kernel<E, DK, DV, MAPS, true>), g, dim3(256), sm, st, p);
-  else if constexpr (MAPS == 2) hipLaunchKernelGGL((attn_long_fwd_kernel<E, DK, DV, MAPS, false>), g, dim3(256), sm, st, p);
-  PTPP_CHECK_LAUNCH("attention_long_fwd");
+  if (p.table) hipLaunchKernelGGL((attn_long_split_kernel<E, DK, DV, MAPS, true>), g, t, sm, st, p);
+  else if constexpr (MAPS == 2) hipLaunchKernelGGL((attn_long_split_kernel<E, DK, DV, MAPS, false>), g, t, sm, st, p);
+  PTPP_CHECK_LAUNCH("attention_long_fwd (few rows)");
+  if (p.splits > 1) {
+    const int ncol = blocks * (p.nh > 1 ? p.nh * p.Tq : 32);
+    hipLaunchKernelGGL((attn_long_join_kernel<E, DV, MAPS>), dim3((ncol + LA_WAVES - 1) / LA_WAVES), dim3(256), 0, st, p, ncol);
+    PTPP_CHECK_LAUNCH("attention_long_fwd (join)");
+  }
   return PTPP_OK;
 }
 template <typename E>
 int dispatch_fwd(const LongP& p, int maps, hipStream_t st) {
   if (maps == 1) return p.dk <= 64 ? launch_fwd<E, 64, 64, 1>(p, st) : launch_fwd<E, 128, 128, 1>(p, st);
   return p.dk <= 32 ? launch_fwd<E, 32, 64, 2>(p, st) : launch_fwd<E, 64, 128, 2>(p, st);
+}
+
+// forward plan: p.splits == 0: tiles.  -> bytes of workspace, < 0: refused
+int64_t plan_fwd(LongP& p, const ptpp_attention_long_args* a, int64_t* o_ml, const char* who) {
+  *o_ml = 0;
+  if (!few_rows(p)) return 0;
+  const int blocks = plan_few(p, few_waves(a->dtype, a->maps, a->dk));
+  if (!blocks) {
+    ptpp_set_error("%s: too many tiles", who);
+    return -1;
+  }
+  if (p.splits == 1) return 0;
+  const int64_t rows = (int64_t)blocks * p.splits * a->maps * 32;
+  *o_ml = rows * pad_dv(a->maps, a->dk);
+  return (*o_ml + 2 * rows) * (int64_t)sizeof(float);
 }
 
 }  // namespace
@@ -282,6 +642,13 @@ extern "C" int ptpp_attention_long_fwd(const ptpp_attention_long_args* a, void* 
   const int rc = ptpp_attention_long_params(a, 0, &p, "attention_long_fwd");
   if (rc != PTPP_OK) return rc;
   PTPP_CHECK_ARG(a->maps == 1 || !a->lse == !a->out2, "attention_long_fwd: lse and out2 are kept together");
+  int64_t o_ml;
+  const int64_t need = plan_fwd(p, a, &o_ml, "attention_long_fwd");
+  if (need < 0) return PTPP_EINVAL;
+  PTPP_CHECK_ARG(!need || (a->ws && (uintptr_t)a->ws % 16 == 0 && a->ws_bytes >= (size_t)need),
+                 "attention_long_fwd: workspace of %zu bytes, needs %lld (16-byte aligned)", a->ws_bytes, (long long)need);
+  p.part_o = reinterpret_cast<float*>(a->ws);
+  p.part_ml = p.part_o + o_ml;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (a->dtype == PTPP_F32) return dispatch_fwd<float>(p, a->maps, st);
   if (a->dtype == PTPP_BF16) return dispatch_fwd<bf16_raw>(p, a->maps, st);
@@ -292,5 +659,7 @@ int64_t ptpp_attention_long_ws_bwd(const LongP& p, int maps);
 extern "C" int64_t ptpp_attention_long_ws_bytes(const ptpp_attention_long_args* a, int backward) {
   LongP p;
   if (ptpp_attention_long_params(a, backward, &p, "attention_long_ws_bytes") != PTPP_OK) return -1;
-  return backward ? ptpp_attention_long_ws_bwd(p, a->maps) : 0;
+  if (backward) return ptpp_attention_long_ws_bwd(p, a->maps);
+  int64_t o_ml;
+  return plan_fwd(p, a, &o_ml, "attention_long_ws_bytes");
 }

@@ -1011,15 +1011,27 @@ def _param_sinks(params):
     return params if params and all(_sink(p) is not None for p in params) else None
 
 
+def _f32_view(t):
+    """``t`` as the f32 contiguous tensor that the kernels read (itself, if it is one)"""
+    return t if t is None or (t.dtype is torch.float32 and t.is_contiguous()) else t.detach().float().contiguous()
+
+
+def _still(args, names, tensors):
+    """the tensors that autograd hands back still lie where the forward launch read them (a saved-tensor hook may have moved them)"""
+    return all((0 if t is None else t.data_ptr()) == (getattr(args, n) or 0) for n, t in zip(names, tensors))
+
+
 class AttentionLongFn(Function):
     @staticmethod
     def forward(ctx, q, k, v, table, lam, cfg):
-        op = _attention_long_op(q, k, v, _f32c(table), _f32c(lam), cfg)
-        out, lse, out2 = op.forward(True)
-        ctx.cfg = cfg
-        ctx.direct = _param_sinks([p for p in (table, lam) if p is not None])
-        for p in ctx.direct or ():
-            _use(p)
+        op = _attention_long_op(q, k, v, _f32_view(table), _f32_view(lam), cfg)
+        out, lse, out2 = op.forward(q, True)
+        ctx.cfg, ctx.op = cfg, op
+        ctx.direct = None
+        if _direct["on"]:
+            ctx.direct = _param_sinks([p for p in (table, lam) if p is not None])
+            for p in ctx.direct or ():
+                _use(p)
         ctx.save_for_backward(q, k, v, table, lam, out, lse, out2)
         return out
 
@@ -1027,42 +1039,33 @@ class AttentionLongFn(Function):
     @once_differentiable
     def backward(ctx, dout):
         q, k, v, table, lam, out, lse, out2 = ctx.saved_tensors
-        op = _attention_long_op(q, k, v, _f32c(table), _f32c(lam), ctx.cfg)
+        op = ctx.op
+        if not _still(op.args, ("q", "table", "lam") if k is None else ("q", "table", "lam", "k", "v"), (q, table, lam, k, v)):
+            op = _attention_long_op(q, k, v, _f32_view(table), _f32_view(lam), ctx.cfg)
         if not dout.is_contiguous() or dout.data_ptr() % 16:
             dout = dout.clone(memory_format=torch.contiguous_format)
         dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
         dk = dv = None
-        if k is None:
-            parts = _split_qkv(dq, ctx.cfg)
-        else:
+        if k is not None:
             dk = torch.empty(k.shape, device=k.device, dtype=k.dtype)
             dv = torch.empty(v.shape, device=v.device, dtype=v.dtype)
-            parts = dq, dk, dv
         direct = ctx.direct is not None
-        grads = [None if p is None else p.grad if direct else torch.empty(p.shape, device=p.device, dtype=torch.float32) for p in (table, lam)]
-        op.backward(out, lse, out2, dout, *parts, *grads, accumulate=direct)
+        dt, dl = (None if p is None else p.grad if direct else torch.empty(p.shape, device=p.device, dtype=torch.float32) for p in (table, lam))
+        op.backward(q, k, v, table, lam, out, lse, out2, dout, dq, dk, dv, dt, dl, accumulate=direct)
         if direct:
             for p in ctx.direct:
                 _done(p)
-            grads = [None, None]
-        dt, dl = (g if g is None or g.dtype == p.dtype else g.to(p.dtype) for g, p in zip(grads, (table, lam)))
+            return dq, dk, dv, None, None, None
+        if dt is not None and table.dtype is not torch.float32:
+            dt = dt.to(table.dtype)
+        if dl is not None and lam.dtype is not torch.float32:
+            dl = dl.to(lam.dtype)
         return dq, dk, dv, dt, dl, None
 
 
-def _split_qkv(qkv, cfg):
-    """views of a fused (B, T, q | k | v) projection; the key / value parts are kv_heads / heads as wide as the query's"""
-    unit = qkv.shape[2] // (cfg.heads + 2 * cfg.kv_heads)
-    if qkv.shape[2] != unit * (cfg.heads + 2 * cfg.kv_heads):
-        raise ValueError(f"attention: {qkv.shape[2]} channels do not split into q of {cfg.heads} and k, v of {cfg.kv_heads} heads")
-    return qkv.split([unit * cfg.heads, unit * cfg.kv_heads, unit * cfg.kv_heads], dim=2)
-
-
 def _attention_long_op(q, k, v, table, lam, cfg):
-    if k is None:
-        q, k, v = _split_qkv(q, cfg)
-    return ops.AttentionLong(q, k, v, cfg.heads, cfg.kv_heads, cfg.maps, table=table, max_distance=cfg.max_distance,
-                             bidirectional=cfg.bidirectional, lam=lam, lam_init=cfg.lam_init, lengths=cfg.lengths, q_lengths=cfg.q_lengths,
-                             q_start=cfg.q_start, causal=cfg.causal, scale=cfg.scale)
+    return ops.AttentionLong(q, k, v, cfg.heads, cfg.kv_heads, cfg.maps, table, cfg.max_distance, cfg.bidirectional, lam, cfg.lam_init, cfg.lengths,
+                             cfg.q_lengths, cfg.q_start, cfg.causal, cfg.scale)
 
 
 def _attention_long(q, k, v, table, lam, cfg):
@@ -1072,7 +1075,7 @@ def _attention_long(q, k, v, table, lam, cfg):
         cfg.q_lengths = cfg.lengths
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, table, lam)):
         return AttentionLongFn.apply(q, k, v, table, lam, cfg)
-    return _attention_long_op(q, k, v, _f32c(table), _f32c(lam), cfg).forward(False)[0]
+    return _attention_long_op(q, k, v, _f32_view(table), _f32_view(lam), cfg).forward(q, False)[0]
 
 
 def attention_bucket(q, k, v, table, heads, kv_heads=None, max_distance=128, bidirectional=True, lengths=None, q_lengths=None, q_start=None,
@@ -1116,45 +1119,56 @@ class ResidualNormFn(Function):
         f = f.contiguous()
         x = x.contiguous() if x is not None else None
         params = (gate, post_g, post_b, pre_g, pre_b)
-        y, z, stats = _residual_norm_op(f, x, params, cfg).forward(True)
-        ctx.cfg = cfg
-        want = [p for p, n in zip(params, ctx.needs_input_grad[2:7]) if n]
-        ctx.direct = _param_sinks(want)
-        for p in ctx.direct or ():
-            _use(p)
+        op = _residual_norm_op(f, x, params, cfg)
+        y, z, stats = op.forward(f, True)
+        ctx.cfg, ctx.op = cfg, op
+        ctx.direct = None
+        if _direct["on"]:
+            ctx.direct = _param_sinks([p for p, n in zip(params, ctx.needs_input_grad[2:7]) if n])
+            for p in ctx.direct or ():
+                _use(p)
         ctx.save_for_backward(f, x, *params, stats)
-        if z is None:
-            return y
-        return y, z
+        return y if z is None else (y, z)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dz=None):
         f, x, *params, stats = ctx.saved_tensors
         need = ctx.needs_input_grad
-        op = _residual_norm_op(f, x, params, ctx.cfg)
+        op = ctx.op
+        if not _still(op.args, ("f", "x", "gate", "post_g", "post_b", "pre_g", "pre_b"), (f, x, *params)):
+            op = _residual_norm_op(f, x, params, ctx.cfg)
         dy, dz = (None if t is None else t.contiguous() for t in (dy, dz))
-        direct = ctx.direct is not None
-        sums = [None if not n else p.grad.view(_flat(p)) if direct else torch.empty(_flat(p), device=p.device, dtype=torch.float32)
-                for p, n in zip(params, need[2:7])]
-        df, dx = op.backward(stats, dy, dz, need[0], need[1], sums, accumulate=direct)
-        if direct:
+        if ctx.direct is not None:
+            sums = [p.grad.view(s) if n else None for p, s, n in zip(params, op.par_shapes, need[2:7])]
+            df, dx = op.backward(f, stats, dy, dz, need[0], need[1], sums, accumulate=True)
             for p in ctx.direct:
                 _done(p)
-            sums = [None] * 5
-        return (df, dx, *(None if s is None else s.view(p.shape).to(p.dtype) for s, p in zip(sums, params)), None)
+            return df, dx, None, None, None, None, None, None
+        sums = [None] * 5
+        want = [i for i in range(5) if need[2 + i]]
+        if want:  # one allocation for all of them
+            parts = torch.empty(sum(params[i].numel() for i in want), device=f.device, dtype=torch.float32).split([params[i].numel() for i in want])
+            for i, t in zip(want, parts):
+                sums[i] = t.view(op.par_shapes[i]) if len(op.par_shapes[i]) > 1 else t
+        df, dx = op.backward(f, stats, dy, dz, need[0], need[1], sums)
+        for i in want:
+            if params[i].shape != sums[i].shape:
+                sums[i] = sums[i].view(params[i].shape)
+            if params[i].dtype is not torch.float32:
+                sums[i] = sums[i].to(params[i].dtype)
+        return (df, dx, *sums, None)
 
 
 def _flat(p):
     """a gate keeps its (B, C) rows; everything else is a vector, whatever unit dimensions the parameter carries"""
-    return tuple(p.shape) if p.dim() == 2 and p.shape[0] != 1 else (p.numel(),)
+    if p is None or p.dim() == 1:
+        return _f32_view(p)
+    return _f32_view(p) if p.dim() == 2 and p.shape[0] != 1 else _f32_view(p).view(-1)
 
 
 def _residual_norm_op(f, x, params, cfg):
-    gate, post_g, post_b, pre_g, pre_b = (None if p is None else _f32c(p).reshape(_flat(p)) for p in params)
-    if gate is not None and gate.dim() == 1 and f.shape[0] > 1 and gate.numel() != f.shape[2]:
-        raise ValueError(f"residual_norm: a gate of {f.shape[2]} channels, or ({f.shape[0]}, {f.shape[2]}), expected, got {tuple(params[0].shape)}")
-    return ops.ResidualNorm(f, x, gate, (post_g, post_b), (pre_g, pre_b), cfg.scale, cfg.eps, cfg.kind, cfg.lengths)
+    return ops.ResidualNorm(f, x, *map(_flat, params), cfg.scale, cfg.eps, cfg.kind, cfg.lengths)
 
 
 def residual_norm(f, x=None, gate=None, post=None, pre=None, scale=1.0, eps=1e-5, kind="layer", lengths=None):
@@ -1172,7 +1186,8 @@ def residual_norm(f, x=None, gate=None, post=None, pre=None, scale=1.0, eps=1e-5
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (f, x, *params)):
         r = ResidualNormFn.apply(f, x, *params, cfg)
         return r if pre_g is not None else (r, None)
-    y, z, _ = _residual_norm_op(f.contiguous(), None if x is None else x.contiguous(), params, cfg).forward(False)
+    f = f.contiguous()
+    y, z, _ = _residual_norm_op(f, None if x is None else x.contiguous(), params, cfg).forward(f, False)
     return y, z
 
 

@@ -637,203 +637,245 @@ def bucket_edges(num_buckets, max_distance, bidirectional):
     return e, (ctypes.c_int32 * max(1, len(edges)))(*edges), len(edges)
 
 
-def _here(t, what):
-    """a ROCm tensor of the device that the launch goes to (the current one)"""
+def _on(t, dev, what):
+    """``t`` must lie on device number ``dev`` (the current one: that is where the launch goes)"""
+    if t.get_device() != dev:
+        _need_gpu(t)
+        raise _lib.PtppError(f"promptttspp_amd: {what} lies on {t.device}, the current device is cuda:{dev}")
+
+
+def _current(t):
     _need_gpu(t)
-    if t.device.index != torch.cuda.current_device():
-        raise _lib.PtppError(f"promptttspp_amd: {what} lies on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+    return _cur_device() if _cur_device is not None else torch.cuda.current_device()
 
 
-def _rows(t, what, B, T, C, dtype):
-    """checks of a (B, T, C) operand with contiguous channels and any row / batch stride; -> (batch stride, row stride)"""
-    _here(t, what)
-    if t.dim() != 3 or tuple(t.shape) != (B, T, C) or t.dtype != dtype:
-        raise ValueError(f"{what}: expected a ({B}, {T}, {C}) {dtype} tensor, got {tuple(t.shape)} {t.dtype}")
-    if t.stride(2) != 1 and C > 1:
+def _rows(t, what, shape, dtype, dev):
+    """(address, batch stride, row stride) of a (B, T, C) operand with contiguous channels and any other strides"""
+    if t.shape != shape or t.dtype is not dtype:
+        raise ValueError(f"{what}: expected a {tuple(shape)} {dtype} tensor, got {tuple(t.shape)} {t.dtype}")
+    _on(t, dev, what)
+    s0, s1, s2 = t.stride()
+    B, T, C = shape
+    if s2 != 1 and C > 1:
         raise ValueError(f"{what}: channels must be contiguous")
-    return (t.stride(0) if B > 1 else T * t.stride(1) if T > 1 else C), (t.stride(1) if T > 1 else C)
+    if T == 1:
+        s1 = C
+    return t.data_ptr(), (s0 if B > 1 else T * s1), s1
 
 
-def _f32_operand(t, what, shape, like):
-    _here(t, what)
-    if t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous():
-        raise ValueError(f"{what}: expected a contiguous {shape} float32 tensor, got {tuple(t.shape)} {t.dtype}")
-    if t.device != like.device:
-        raise ValueError(f"{what}: on {t.device}, the activations on {like.device}")
-    return _ptr(t)
+def _f32_operand(t, what, shape, dev):
+    if t.dtype is not torch.float32 or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{what}: expected a contiguous {tuple(shape)} float32 tensor, got {tuple(t.shape)} {t.dtype}")
+    _on(t, dev, what)
+    return t.data_ptr()
 
 
 def _i32_rows(t, what, B, like):
     if t is None:
         return None
-    if tuple(t.shape) != (B,):
+    if t.shape != (B,):
         raise ValueError(f"{what}: expected {B} entries, got {tuple(t.shape)}")
+    if t.dtype is torch.int32 and t.device == like.device and t.is_contiguous():
+        return t
     if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
         raise ValueError(f"{what}: whole numbers expected, got {t.dtype}")
     return i32(t, like.device)
 
 
 class AttentionLong:
-    """Shapes and options of one call of the long-sequence attention kernels: built once, used by forward and backward."""
+    """One call of the long-sequence attention kernels: the argument block of the forward launch, which backward copies and completes.
+    Holds no activations; ``forward`` / ``backward`` are given them."""
+
+    __slots__ = ("args", "shape", "width", "ints", "table_shape", "lam_shape", "edges", "dev", "split", "held")
 
     def __init__(self, q, k, v, heads, kv_heads, maps, table=None, max_distance=128, bidirectional=True, lam=None, lam_init=0.0, lengths=None,
                  q_lengths=None, q_start=None, causal=False, scale=None):
-        for t, n in ((q, "q"), (k, "k"), (v, "v")):
-            if t.dim() != 3:
-                raise ValueError(f"{n}: expected a (B, T, channels) tensor")
-        B, Tq, Cq = q.shape
-        Tk, Ck = k.shape[1], k.shape[2]
+        """k = v = None: q is the fused (B, T, q | k | v) projection"""
+        dev = self.dev = _current(q)
+        if q.dim() != 3 or (k is not None and (k.dim() != 3 or v.dim() != 3)):
+            raise ValueError("attention: expected (B, T, channels) tensors")
         if heads < 1 or kv_heads < 1 or heads % kv_heads:
             raise ValueError(f"attention: {kv_heads} key / value heads do not divide {heads} query heads")
-        dk = Cq // (heads * maps)
+        B, Tq, Cq = q.shape
+        parts = (heads if k is not None else heads + 2 * kv_heads) * maps
+        dk, Tk = Cq // parts, (Tq if k is None else k.shape[1])
         if B < 1 or Tq < 1 or Tk < 1:
             raise ValueError("attention: empty batch or sequence")
-        if Cq != heads * maps * dk or dk % 8 or not 8 <= dk <= (128 if maps == 1 else 64):
-            raise ValueError(f"attention: {Cq} query channels for {heads} heads of {maps} map(s): the width of one map must be a multiple of 8, "
-                             f"at most {128 if maps == 1 else 64}")
+        if Cq != parts * dk or dk % 8 or not 8 <= dk <= (128 if maps == 1 else 64):
+            raise ValueError(f"attention: {Cq} channels for {parts} parts ({heads} query heads of {maps} map(s)): the width of one map must be a "
+                             f"multiple of 8, at most {128 if maps == 1 else 64}")
         self.shape = B, Tq, Tk, heads, kv_heads, dk, maps
-        self.width = heads * maps * dk
-        kw = kv_heads * maps * dk
-        a = self.args = _lib.AttentionLongArgs()
-        a.sq, a.ldq = _rows(q, "q", B, Tq, self.width, q.dtype)
-        a.sk, a.ldk = _rows(k, "k", B, Tk, kw, q.dtype)
-        a.sv, a.ldv = _rows(v, "v", B, Tk, kw, q.dtype)
-        a.q, a.k, a.v = _ptr(q), _ptr(k), _ptr(v)
-        a.B, a.Tq, a.Tk, a.H, a.Hk, a.dk, a.maps = B, Tq, Tk, heads, kv_heads, dk, maps
-        a.dtype = dtype_code(q.dtype)
-        a.causal = int(bool(causal))
-        a.scale = float(scale) if scale is not None else dk ** -0.5
-        if not 0.0 < a.scale < 1e30:
+        wq, wk = heads * maps * dk, kv_heads * maps * dk
+        self.width, self.split = wq, k is None
+        dt = q.dtype
+        es = q.element_size()
+        pq, sq, lq = _rows(q, "q", (B, Tq, Cq), dt, dev)
+        if k is None:
+            pk, pv, sk, sv, lk, lv = pq + wq * es, pq + (wq + wk) * es, sq, sq, lq, lq
+        else:
+            pk, sk, lk = _rows(k, "k", (B, Tk, wk), dt, dev)
+            pv, sv, lv = _rows(v, "v", (B, Tk, wk), dt, dev)
+        if scale is None:
+            scale = dk ** -0.5
+        elif not 0.0 < scale < 1e30:
             raise ValueError(f"attention: scale {scale} must be positive and finite")
-        self.table, self.lam = table, lam
+        nb = nexact = nedges = 0
+        ptab = plam = edges = None
+        lam_heads = 1
+        self.table_shape = self.lam_shape = self.edges = None
         if table is not None:
             if table.dim() != 2 or table.shape[1] != heads:
                 raise ValueError(f"attention: a position table of shape (buckets, {heads}) expected, got {tuple(table.shape)}")
-            a.nbuckets, a.bidirectional, a.max_distance = table.shape[0], int(bool(bidirectional)), int(max_distance)
-            a.nexact, self._edges, a.nedges = bucket_edges(a.nbuckets, a.max_distance, bool(bidirectional))
-            a.edges = ctypes.addressof(self._edges)
-            a.table = _f32_operand(table, "table", tuple(table.shape), q)
+            self.table_shape = table.shape
+            nb, max_distance = table.shape[0], int(max_distance)
+            nexact, self.edges, nedges = bucket_edges(nb, max_distance, bool(bidirectional))
+            edges, ptab = ctypes.addressof(self.edges), _f32_operand(table, "table", table.shape, dev)
         if maps == 2:
             if lam.dim() != 3 or lam.shape[0] != 4 or lam.shape[1] not in (1, heads) or lam.shape[2] != dk:
                 raise ValueError(f"attention: lam of shape (4, 1 or {heads}, {dk}) expected, got {tuple(lam.shape)}")
-            a.lam, a.lam_heads, a.lam_init = _f32_operand(lam, "lam", tuple(lam.shape), q), lam.shape[1], float(lam_init)
-        self._ints = [_i32_rows(t, n, B, q) for t, n in ((lengths, "lengths"), (q_lengths, "q_lengths"), (q_start, "q_start"))]
-        a.k_lengths, a.q_lengths, a.q_start = (_ptr(t) for t in self._ints)
-        self.device, self.dtype = q.device, q.dtype
+            self.lam_shape = lam.shape
+            plam, lam_heads = _f32_operand(lam, "lam", lam.shape, dev), lam.shape[1]
+        self.held = table, lam  # (f32 copies of other types live until the launches that read them)
+        ints = self.ints = (_i32_rows(lengths, "lengths", B, q), _i32_rows(q_lengths, "q_lengths", B, q), _i32_rows(q_start, "q_start", B, q))
+        n, m, st = (None if t is None else t.data_ptr() for t in ints)
+        # (in the order of ptpp_attention_long_args; outputs, gradients and the workspace are filled in by forward / backward)
+        self.args = _lib.AttentionLongArgs(
+            pq, pk, pv, None, None, None, None, None, None, ptab, plam, None, None, None, n, m, st, edges, None, 0,
+            sq, sk, sv, Tq * wq, 0, 0, 0, 0, lq, lk, lv, wq, 0, 0, 0, 0, B, Tq, Tk, heads, kv_heads, dk, maps, nb, bool(bidirectional),
+            bool(causal), lam_heads, max_distance, nexact, nedges, 0, dtype_code(dt), scale, lam_init)
 
-    def _workspace(self, backward):
-        n = _lib.load().ptpp_attention_long_ws_bytes(ctypes.byref(self.args), backward)
-        check(-1 if n < 0 else 0, "ptpp_attention_long_ws_bytes")
-        w = torch.empty(n, device=self.device, dtype=torch.uint8) if n else None  # (this call's own: two captured graphs never share it)
-        self.args.ws, self.args.ws_bytes = _ptr(w), n
-        return w
-
-    def forward(self, keep):
+    def forward(self, q, keep):
         """-> (out, lse, out2); the last two only with ``keep`` (what backward needs)"""
-        B, Tq, _, H, _, dk, maps = self.shape
+        B, Tq, _, H, _, _, maps = self.shape
         a = self.args
-        out = torch.empty((B, Tq, self.width), device=self.device, dtype=self.dtype)
+        out = torch.empty((B, Tq, self.width), device=q.device, dtype=q.dtype)
         lse = out2 = None
         if keep:
-            lse = torch.empty((maps, B, H, (Tq + 63) // 64 * 64), device=self.device, dtype=torch.float32)
-            out2 = torch.empty_like(out) if maps == 2 else None
-        a.out, a.so, a.ldo, a.lse, a.out2 = _ptr(out), Tq * self.width, self.width, _ptr(lse), _ptr(out2)
-        ws = self._workspace(0)
-        check(_lib.load().ptpp_attention_long_fwd(ctypes.byref(a), _stream()), "ptpp_attention_long_fwd")
-        del ws
+            lse = torch.empty((maps, B, H, (Tq + 63) // 64 * 64), device=q.device, dtype=torch.float32)
+            a.lse = lse.data_ptr()
+            if maps == 2:
+                out2 = torch.empty_like(out)
+                a.out2 = out2.data_ptr()
+        a.out = out.data_ptr()
+        lib = _lib.load()
+        n = lib.ptpp_attention_long_ws_bytes(ctypes.byref(a), 0)
+        if n:
+            check(min(n, 0), "ptpp_attention_long_ws_bytes")
+            ws = torch.empty(n, device=q.device, dtype=torch.uint8)  # (this call's own: two captured graphs never share it)
+            a.ws, a.ws_bytes = ws.data_ptr(), n
+        check(lib.ptpp_attention_long_fwd(ctypes.byref(a), _stream()), "ptpp_attention_long_fwd")
         return out, lse, out2
 
-    def backward(self, out, lse, out2, dout, dq, dk, dv, dtable=None, dlam=None, accumulate=False):
-        """fills dq / dk / dv (views with contiguous channels) and dtable / dlam (added to with ``accumulate``)"""
-        B, Tq, Tk, H, Hk, d, maps = self.shape
-        a = self.args
-        kw = Hk * maps * d
-        a.sdo, a.lddo = _rows(dout, "dout", B, Tq, self.width, self.dtype)
-        a.so, a.ldo = _rows(out, "out", B, Tq, self.width, self.dtype)
-        a.sdq, a.lddq = _rows(dq, "dq", B, Tq, self.width, self.dtype)
-        a.sdk, a.lddk = _rows(dk, "dk", B, Tk, kw, self.dtype)
-        a.sdv, a.lddv = _rows(dv, "dv", B, Tk, kw, self.dtype)
-        a.out, a.lse, a.out2, a.dout, a.dq, a.dk_out, a.dv = (_ptr(t) for t in (out, lse, out2, dout, dq, dk, dv))
-        a.dtable = _f32_operand(dtable, "dtable", tuple(self.table.shape), dq) if self.table is not None else None
-        a.dlam = _f32_operand(dlam, "dlam", tuple(self.lam.shape), dq) if maps == 2 else None
-        a.accumulate = int(bool(accumulate))
-        ws = self._workspace(1)
-        check(_lib.load().ptpp_attention_long_bwd(ctypes.byref(a), _stream()), "ptpp_attention_long_bwd")
-        del ws
+    def backward(self, q, k, v, table, lam, out, lse, out2, dout, dq, dk, dv, dtable=None, dlam=None, accumulate=False):
+        """fills dq / dk / dv (dk = dv = None: dq is fused like q) and dtable / dlam (added to with ``accumulate``)"""
+        B, Tq, Tk, _, Hk, d, maps = self.shape
+        dev, w, wk, dt = self.dev, self.width, Hk * maps * d, q.dtype
+        a = type(self.args).from_buffer_copy(self.args)
+        a.dout, a.sdo, a.lddo = _rows(dout, "dout", (B, Tq, w), dt, dev)
+        a.out, a.so, a.ldo = _rows(out, "out", (B, Tq, w), dt, dev)
+        a.lse, a.out2 = lse.data_ptr(), _ptr(out2)
+        if self.split:
+            es = dq.element_size()
+            p, s, ld = _rows(dq, "dq", (B, Tq, w + 2 * wk), dt, dev)
+            a.dq, a.dk_out, a.dv = p, p + w * es, p + (w + wk) * es
+            a.sdq = a.sdk = a.sdv = s
+            a.lddq = a.lddk = a.lddv = ld
+        else:
+            a.dq, a.sdq, a.lddq = _rows(dq, "dq", (B, Tq, w), dt, dev)
+            a.dk_out, a.sdk, a.lddk = _rows(dk, "dk", (B, Tk, wk), dt, dev)
+            a.dv, a.sdv, a.lddv = _rows(dv, "dv", (B, Tk, wk), dt, dev)
+        if table is not None:
+            a.dtable = _f32_operand(dtable, "dtable", self.table_shape, dev)
+        if maps == 2:
+            a.dlam = _f32_operand(dlam, "dlam", self.lam_shape, dev)
+        a.accumulate = bool(accumulate)
+        lib = _lib.load()
+        n = lib.ptpp_attention_long_ws_bytes(ctypes.byref(a), 1)
+        check(min(n, 0), "ptpp_attention_long_ws_bytes")
+        ws = torch.empty(n, device=q.device, dtype=torch.uint8)
+        a.ws, a.ws_bytes = ws.data_ptr(), n
+        check(lib.ptpp_attention_long_bwd(ctypes.byref(a), _stream()), "ptpp_attention_long_bwd")
 
 
 # ----------------------------------------------------------------------------
 # norm behind a block, gate, residual scale, norm before the next block
 # ----------------------------------------------------------------------------
 class ResidualNorm:
-    """Shapes and options of one call of the residual-norm kernels: y = x + scale * gate * post(f), z = pre(y)."""
+    """One call of the residual-norm kernels, y = x + scale * gate * post(f), z = pre(y): the argument block of the forward launch, which
+    backward copies and completes.  Holds no activations."""
 
-    def __init__(self, f, x=None, gate=None, post=(None, None), pre=(None, None), scale=1.0, eps=1e-5, kind="layer", lengths=None):
-        if kind not in ("layer", "rms"):
+    __slots__ = ("args", "shape", "ints", "par_shapes", "dev", "has_z", "held")
+
+    def __init__(self, f, x=None, gate=None, post_g=None, post_b=None, pre_g=None, pre_b=None, scale=1.0, eps=1e-5, kind="layer", lengths=None):
+        dev = self.dev = _current(f)
+        if kind != "layer" and kind != "rms":
             raise ValueError(f"residual_norm: kind {kind!r} ('layer' or 'rms')")
         if f.dim() != 3:
             raise ValueError("residual_norm: expected a (B, T, C) tensor")
-        B, T, C = f.shape
+        B, T, C = self.shape = f.shape
         if B < 1 or T < 1 or C < 1 or C % 4 or C > 4096:
             raise ValueError(f"residual_norm: shape {tuple(f.shape)} (C a multiple of 4, at most 4096, nothing empty)")
         if not eps > 0.0:
             raise ValueError("residual_norm: eps must be positive")
-        a = self.args = _lib.ResidualNormArgs()
-        for t, n in ((f, "f"), (x, "x")):
-            if t is not None:
-                self._dense(t, n, f)
-        a.f, a.x = _ptr(f), _ptr(x)
-        self.f, self.x = f, x
-        if gate is not None and tuple(gate.shape) not in ((C,), (B, C)):
-            raise ValueError(f"residual_norm: a gate of shape ({C},) or ({B}, {C}) expected, got {tuple(gate.shape)}")
-        self.gate, self.post, self.pre = gate, post, pre
-        if gate is not None:
-            a.gate, a.gate_rows = _f32_operand(gate, "gate", tuple(gate.shape), f), (gate.shape[0] if gate.dim() == 2 else 1)
-        for n, (g, b) in (("post", post), ("pre", pre)):
-            if b is not None and (g is None or kind == "rms"):
+        rms, vec = kind == "rms", (C,)
+        for n, g, b in (("post", post_g, post_b), ("pre", pre_g, pre_b)):
+            if b is not None and (g is None or rms):
                 raise ValueError(f"residual_norm: {n} beta without a gamma, or with root-mean-square norms")
-            if g is not None:
-                setattr(a, n + "_g", _f32_operand(g, n + " gamma", (C,), f))
-            if b is not None:
-                setattr(a, n + "_b", _f32_operand(b, n + " beta", (C,), f))
-        self._len = _i32_rows(lengths, "lengths", B, f)
-        a.lengths = _ptr(self._len)
-        a.B, a.T, a.C, a.rms, a.dtype = B, T, C, int(kind == "rms"), dtype_code(f.dtype)
-        a.scale, a.eps = float(scale), float(eps)
+        gate_rows = 1
+        if gate is not None:
+            if gate.shape != vec and gate.shape != (B, C):
+                raise ValueError(f"residual_norm: a gate of shape ({C},) or ({B}, {C}) expected, got {tuple(gate.shape)}")
+            gate_rows = gate.shape[0] if gate.dim() == 2 else 1
+        self.held = gate, post_g, post_b, pre_g, pre_b  # (f32 copies of other types live until the launches that read them)
+        self.par_shapes = ((gate.shape if gate is not None else None), vec, vec, vec, vec)
+        par = [None if t is None else _f32_operand(t, n, s, dev)
+               for t, n, s in zip(self.held, self._NAMES, self.par_shapes)]
+        self.ints = _i32_rows(lengths, "lengths", B, f)
+        self.has_z = pre_g is not None
+        self.args = _lib.ResidualNormArgs(
+            self._dense(f, "f", f.dtype), None if x is None else self._dense(x, "x", f.dtype), None, None, None, None, None, None, *par,
+            None, None, None, None, None, None, _ptr(self.ints), None, 0, B, T, C, rms, gate_rows, 0, dtype_code(f.dtype), scale, eps)
 
-    @staticmethod
-    def _dense(t, what, like):
-        _here(t, what)
-        if t.shape != like.shape or t.dtype != like.dtype or not t.is_contiguous():
-            raise ValueError(f"residual_norm: {what} must be a contiguous {tuple(like.shape)} {like.dtype} tensor, got {tuple(t.shape)} {t.dtype}")
+    _NAMES = ("gate", "post gamma", "post beta", "pre gamma", "pre beta")
 
-    def forward(self, keep):
+    def _dense(self, t, what, dtype):
+        if t.shape != self.shape or t.dtype is not dtype or not t.is_contiguous():
+            raise ValueError(f"residual_norm: {what} must be a contiguous {tuple(self.shape)} {dtype} tensor, got {tuple(t.shape)} {t.dtype}")
+        _on(t, self.dev, what)
+        return t.data_ptr()
+
+    def forward(self, f, keep):
         """-> (y, z or None, statistics or None)"""
-        a, f = self.args, self.f
-        y = torch.empty_like(f)
-        z = torch.empty_like(f) if self.pre[0] is not None else None
-        stats = torch.empty((4, f.shape[0] * f.shape[1]), device=f.device, dtype=torch.float32) if keep else None
-        a.y, a.z, a.stats = _ptr(y), _ptr(z), _ptr(stats)
+        a = self.args
+        y, z, stats = torch.empty_like(f), None, None
+        a.y = y.data_ptr()
+        if self.has_z:
+            z = torch.empty_like(f)
+            a.z = z.data_ptr()
+        if keep:
+            stats = torch.empty((4, self.shape[0] * self.shape[1]), device=f.device, dtype=torch.float32)
+            a.stats = stats.data_ptr()
         check(_lib.load().ptpp_residual_norm_fwd(ctypes.byref(a), _stream()), "ptpp_residual_norm_fwd")
         return y, z, stats
 
-    def backward(self, stats, dy, dz, want_df, want_dx, sums, accumulate=False):
+    def backward(self, f, stats, dy, dz, want_df, want_dx, sums, accumulate=False):
         """``sums``: f32 buffers (or None) for (gate, post gamma, post beta, pre gamma, pre beta).  -> (df, dx)"""
-        a, f = self.args, self.f
-        for t, n in ((dy, "dy"), (dz, "dz")):
-            if t is not None:
-                self._dense(t, n, f)
+        a = type(self.args).from_buffer_copy(self.args)
+        dt = f.dtype
         df = torch.empty_like(f) if want_df else None
         dx = torch.empty_like(f) if want_dx else None
-        a.dy, a.dz, a.df, a.dx, a.stats = _ptr(dy), _ptr(dz), _ptr(df), _ptr(dx), _ptr(stats)
-        for n, t, p in zip(("dgate", "dpost_g", "dpost_b", "dpre_g", "dpre_b"), sums, (self.gate, *self.post, *self.pre)):
-            setattr(a, n, _f32_operand(t, n, tuple(p.shape), f) if t is not None else None)
-        a.accumulate = int(bool(accumulate))
-        n = _lib.load().ptpp_residual_norm_ws_bytes(ctypes.byref(a))
-        check(-1 if n < 0 else 0, "ptpp_residual_norm_ws_bytes")
-        ws = torch.empty(n, device=f.device, dtype=torch.uint8) if n else None
-        a.ws, a.ws_bytes = _ptr(ws), n
-        check(_lib.load().ptpp_residual_norm_bwd(ctypes.byref(a), _stream()), "ptpp_residual_norm_bwd")
+        a.dy, a.dz = (None if t is None else self._dense(t, n, dt) for t, n in ((dy, "dy"), (dz, "dz")))
+        a.df, a.dx, a.stats = _ptr(df), _ptr(dx), stats.data_ptr()
+        a.dgate, a.dpost_g, a.dpost_b, a.dpre_g, a.dpre_b = (None if t is None else _f32_operand(t, n, s, self.dev)
+                                                             for t, n, s in zip(sums, self._NAMES, self.par_shapes))
+        a.accumulate = bool(accumulate)
+        lib = _lib.load()
+        n = lib.ptpp_residual_norm_ws_bytes(ctypes.byref(a))
+        if n:
+            check(min(n, 0), "ptpp_residual_norm_ws_bytes")
+            ws = torch.empty(n, device=f.device, dtype=torch.uint8)
+            a.ws, a.ws_bytes = ws.data_ptr(), n
+        check(lib.ptpp_residual_norm_bwd(ctypes.byref(a), _stream()), "ptpp_residual_norm_bwd")
         return df, dx
 
 
