@@ -98,6 +98,50 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 ? 1 : 2) void attn_long_dq_kern
   const float c2 = p.scale * LA_LOG2E;
   const int q0 = qs + i0, D = p.max_distance;
 
+  // one 32 x 32 patch
+  auto patch = [&](const E* kimg, const E* vimg, int ks, int j0) __attribute__((always_inline)) {
+    const int ln = TIGHT ? la_opaque(lane) : lane, lr = ln & 31, hr = ln >> 5;
+    f32x16 dp = f32x16{};
+#pragma unroll
+    for (int kk = 0; kk < VS; ++kk) dp = LOp<E>::mma(la_frag<E, DV>(vimg, 32 * ks + lr, 2 * kk + hr), df[kk], dp);
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m) {
+      f32x16 s = f32x16{};
+#pragma unroll
+      for (int kk = 0; kk < KS; ++kk) s = LOp<E>::mma(la_frag<E, DK>(kimg + m * KIMG, 32 * ks + lr, 2 * kk + hr), qf[m][kk], s);
+      const int dmin = j0 - (q0 + 31), dmax = j0 + 31 - q0;
+      if (BIAS && dmin < D && dmax > -D) {
+        const float* bt = btab + (j0 - q0 - lq + 4 * hw + D + LA_PAD);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, bt[8 * (r >> 2) + (r & 3)]) - lse[m];
+      } else {
+        const float bc = (BIAS ? btab[dmin >= D ? 2 * (D + LA_PAD) : 0] : 0.f) - lse[m];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, bc);
+      }
+      if ((j0 + 32 > kend || (p.causal && j0 + 31 > q0))) {
+        const int jend = min(klen, p.causal ? q0 + lq + 1 : klen) - j0 - 4 * hw;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = 8 * (r >> 2) + (r & 3) < jend ? s[r] : -INFINITY;
+      }
+      float e0 = 0.f, e1 = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) {
+        s[r] = la_exp2(s[r]) * (dp[r] - Dm[m]);
+        s[r + 1] = la_exp2(s[r + 1]) * (dp[r + 1] - Dm[m]);
+        e0 += s[r];
+        e1 += s[r + 1];
+      }
+      eps[m] += e0 + e1;
+#pragma unroll
+      for (int st = 0; st < PS; ++st) {
+        const uint4 f = la_pack<E>(s, st);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[m][n] = LOp<E>::mma(la_tfrag<E, DK>(kimg + m * KIMG, 32 * ks, st, n, ln), f, acc[m][n]);
+      }
+    }
+  };
+
   for (int tile = 0; tile < nt; ++tile) {
     const int buf = tile & 1;
     if (tile + 1 < nt) {
@@ -109,51 +153,9 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 ? 1 : 2) void attn_long_dq_kern
     la_barrier();
     const E* kimg = img + buf * BUF;
     const E* vimg = kimg + MAPS * KIMG;
+    const int jt = tile * LA_TILE;
 #pragma unroll 1
-    for (int ks = 0; ks < 2; ++ks) {
-      const int j0 = tile * LA_TILE + 32 * ks;
-      const int ln = TIGHT ? la_opaque(lane) : lane, lr = ln & 31, hr = ln >> 5;
-      f32x16 dp = f32x16{};
-#pragma unroll
-      for (int kk = 0; kk < VS; ++kk) dp = LOp<E>::mma(la_frag<E, DV>(vimg, 32 * ks + lr, 2 * kk + hr), df[kk], dp);
-#pragma unroll
-      for (int m = 0; m < MAPS; ++m) {
-        f32x16 s = f32x16{};
-#pragma unroll
-        for (int kk = 0; kk < KS; ++kk) s = LOp<E>::mma(la_frag<E, DK>(kimg + m * KIMG, 32 * ks + lr, 2 * kk + hr), qf[m][kk], s);
-        if constexpr (BIAS) {
-          const int dmin = j0 - (q0 + 31), dmax = j0 + 31 - q0;
-          if (dmin < D && dmax > -D) {
-            const float* bt = btab + (j0 - q0 - lq + 4 * hw + D + LA_PAD);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, bt[8 * (r >> 2) + (r & 3)]) - lse[m];
-          } else {
-            const float bc = (dmin >= D ? btab[2 * (D + LA_PAD)] : btab[0]) - lse[m];
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, bc);
-          }
-        } else {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, -lse[m]);
-        }
-        if (j0 + 32 > kend || (p.causal && j0 + 31 > q0)) {
-          const int jend = min(klen, p.causal ? q0 + lq + 1 : klen) - j0 - 4 * hw;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] = 8 * (r >> 2) + (r & 3) < jend ? s[r] : -INFINITY;
-        }
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          s[r] = la_exp2(s[r]) * (dp[r] - Dm[m]);
-          eps[m] += s[r];
-        }
-#pragma unroll
-        for (int st = 0; st < PS; ++st) {
-          const uint4 f = la_pack<E>(s, st);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) acc[m][n] = LOp<E>::mma(la_tfrag<E, DK>(kimg + m * KIMG, 32 * ks, st, n, ln), f, acc[m][n]);
-        }
-      }
-    }
+    for (int ks = 0; ks < 2; ++ks) patch(kimg, vimg, ks, jt + 32 * ks);
     la_barrier();
   }
 
@@ -331,6 +333,95 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 || MAPS * DK == 128 ? 1 : 2) vo
     la_barrier();
   };
 
+  // one 32 x 32 patch
+  auto patch = [&](const E* qimg, const E* oimg, const float* stat, int sub, int q0) __attribute__((always_inline)) {
+    const int ln = F32 ? la_opaque(lane) : lane, lr = ln & 31, hr = ln >> 5;
+    const float* st0 = stat + 32 * sub + 4 * hr;
+    f32x16 dp = f32x16{}, w, hsum;
+#pragma unroll
+    for (int kk = 0; kk < VS; ++kk) {
+      dp = LOp<E>::mma(la_frag<E, DV>(oimg, 32 * sub + lr, 2 * kk + hr), vf[kk], dp);
+      if (F32 && kk % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+    }
+    const int dmin = j0 - (q0 + 31), dmax = j0 + 31 - q0;
+    const bool near = BIAS && dmin < D && dmax > -D;
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m) {
+      f32x16 s = f32x16{};
+      const float* ls = st0 + 128 * m;  // (b128 broadcasts: a half wave's rows are the same in all its lanes)
+#pragma unroll
+      for (int kk = 0; kk < KS; ++kk) {
+        s = LOp<E>::mma(la_frag<E, DK>(qimg + m * QIMG, 32 * sub + lr, 2 * kk + hr), kf[m][kk], s);
+        if (F32 && kk % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      }
+      if (near) {
+        const float* bt = btab + (jk - q0 - 4 * hw + D + LA_PAD);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, bt[-(8 * (r >> 2) + (r & 3))]) - ls[8 * (r >> 2) + (r & 3)];
+      } else {
+        const float bc = BIAS ? btab[dmin >= D ? dist_n - 1 : 0] : 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, bc - ls[8 * (r >> 2) + (r & 3)]);
+      }
+      if (p.causal && dmax > 0) {
+        const int qmin = jk - q0 - 4 * hw;  // register r's query sees the key from this row on
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = 8 * (r >> 2) + (r & 3) >= qmin ? s[r] : -INFINITY;
+      }
+      f32x16 ds;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        float pr = la_exp2(s[r]);
+        if (m == 1) pr *= -lam;
+        w[r] = m == 0 ? pr : w[r] + pr;
+        ds[r] = pr * (dp[r] - ls[64 + 8 * (r >> 2) + (r & 3)]);
+        if constexpr (BIAS) hsum[r] = m == 0 ? ds[r] : hsum[r] + ds[r];
+      }
+#pragma unroll
+      for (int st = 0; st < PS; ++st) {
+        const uint4 f = la_pack<E>(ds, st);
+#pragma unroll
+        for (int n = 0; n < NK; ++n) {
+          ak[m][n] = LOp<E>::mma(la_tfrag<E, DK>(qimg + m * QIMG, 32 * sub, st, n, ln), f, ak[m][n]);
+          if (F32) __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    }
+#pragma unroll
+    for (int st = 0; st < PS; ++st) {
+      const uint4 f = la_pack<E>(w, st);
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        av[n] = LOp<E>::mma(la_tfrag<E, DV>(oimg, 32 * sub, st, n, ln), f, av[n]);
+        if (F32) __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    if constexpr (BIAS) {
+      if (j0 + 32 > klen) {  // (a column behind the keys holds unmasked values: it must not count; its dk / dv rows are written as zeros)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) hsum[r] = jk < klen ? hsum[r] : 0.f;
+      }
+      if (near) {
+        float s0, s1;
+        la_diagonals(hsum, s0, s1);
+        if (lane < 47) {
+          float* hp = myhist + (j0 - q0 + D + LA_PAD - 15 + lane);
+          hp[0] += s0;
+          hp[dist_n - 16] += s1;
+        }
+      } else {
+        float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+          s0 += hsum[r];
+          s1 += hsum[r + 1];
+        }
+        if (dmin >= D) far_hi += s0 + s1;
+        else far_lo += s0 + s1;
+      }
+    }
+  };
+
   for (int g = 0; g < G; ++g) {
     const int h = hk * G + g;
     if constexpr (BIAS) {
@@ -354,88 +445,9 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 || MAPS * DK == 128 ? 1 : 2) vo
       const E* qimg = reinterpret_cast<const E*>(smem + buf * BUFB);
       const E* oimg = qimg + MAPS * QIMG;
       const float* stat = reinterpret_cast<const float*>(oimg + OIMG);
+      const int q0 = qs + (t0 + iq) * LA_TILE;
 #pragma unroll 1
-      for (int sub = 0; sub < 2; ++sub) {
-        const int i0 = (t0 + iq) * LA_TILE + 32 * sub, q0 = qs + i0;
-        const int ln = F32 ? la_opaque(lane) : lane, lr = ln & 31, hr = ln >> 5;
-        f32x16 dp = f32x16{}, w = f32x16{}, hsum = f32x16{};
-#pragma unroll
-        for (int kk = 0; kk < VS; ++kk) {
-          dp = LOp<E>::mma(la_frag<E, DV>(oimg, 32 * sub + lr, 2 * kk + hr), vf[kk], dp);
-          if (F32 && kk % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-        }
-        const int dmin = j0 - (q0 + 31), dmax = j0 + 31 - q0;
-        const bool near = BIAS && dmin < D && dmax > -D;
-#pragma unroll
-        for (int m = 0; m < MAPS; ++m) {
-          f32x16 s = f32x16{};
-#pragma unroll
-          for (int kk = 0; kk < KS; ++kk) {
-            s = LOp<E>::mma(la_frag<E, DK>(qimg + m * QIMG, 32 * sub + lr, 2 * kk + hr), kf[m][kk], s);
-            if (F32 && kk % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-          }
-          const float* ls = stat + 2 * m * 64 + 32 * sub + 4 * hw;
-          if (near) {
-            const float* bt = btab + (jk - q0 - 4 * hw + D + LA_PAD);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, bt[-(8 * (r >> 2) + (r & 3))]) - ls[8 * (r >> 2) + (r & 3)];
-          } else {
-            const float bc = BIAS ? (dmin >= D ? btab[dist_n - 1] : btab[0]) : 0.f;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, bc - ls[8 * (r >> 2) + (r & 3)]);
-          }
-          if (p.causal && dmax > 0) {
-            const int qmin = jk - q0 - 4 * hw;  // register r's query sees the key from this row on
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = 8 * (r >> 2) + (r & 3) >= qmin ? s[r] : -INFINITY;
-          }
-          f32x16 ds;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const float Dr = ls[64 + 8 * (r >> 2) + (r & 3)];
-            float pr = la_exp2(s[r]);
-            if (m == 1) pr *= -lam;
-            w[r] += pr;
-            ds[r] = pr * (dp[r] - Dr);
-            if constexpr (BIAS) hsum[r] += ds[r];
-          }
-#pragma unroll
-          for (int st = 0; st < PS; ++st) {
-            const uint4 f = la_pack<E>(ds, st);
-#pragma unroll
-            for (int n = 0; n < NK; ++n) ak[m][n] = LOp<E>::mma(la_tfrag<E, DK>(qimg + m * QIMG, 32 * sub, st, n, ln), f, ak[m][n]);
-            if (F32) __builtin_amdgcn_sched_barrier(0);
-          }
-        }
-#pragma unroll
-        for (int st = 0; st < PS; ++st) {
-          const uint4 f = la_pack<E>(w, st);
-#pragma unroll
-          for (int n = 0; n < NV; ++n) av[n] = LOp<E>::mma(la_tfrag<E, DV>(oimg, 32 * sub, st, n, ln), f, av[n]);
-          if (F32) __builtin_amdgcn_sched_barrier(0);
-        }
-        if constexpr (BIAS) {
-          if (j0 + 32 > klen) {  // (a column behind the keys holds unmasked values: it must not count; its dk / dv rows are written as zeros)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) hsum[r] = jk < klen ? hsum[r] : 0.f;
-          }
-          if (near) {
-            float s0, s1;
-            la_diagonals(hsum, s0, s1);
-            if (lane < 47) {
-              float* hp = myhist + (j0 - q0 + D + LA_PAD - 15 + lane);
-              hp[0] += s0;
-              hp[dist_n - 16] += s1;
-            }
-          } else {
-            float s = 0.f;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s += hsum[r];
-            if (dmin >= D) far_hi += s;
-            else far_lo += s;
-          }
-        }
-      }
+      for (int sub = 0; sub < 2; ++sub) patch(qimg, oimg, stat, sub, q0 + 32 * sub);
       la_barrier();
     }
     if constexpr (BIAS) flush(h);

@@ -1018,7 +1018,10 @@ def _f32_view(t):
 
 def _still(args, names, tensors):
     """the tensors that autograd hands back still lie where the forward launch read them (a saved-tensor hook may have moved them)"""
-    return all((0 if t is None else t.data_ptr()) == (getattr(args, n) or 0) for n, t in zip(names, tensors))
+    for n, t in zip(names, tensors):
+        if t is not None and t.data_ptr() != getattr(args, n):
+            return False
+    return True
 
 
 class AttentionLongFn(Function):
@@ -1044,14 +1047,9 @@ class AttentionLongFn(Function):
             op = _attention_long_op(q, k, v, _f32_view(table), _f32_view(lam), ctx.cfg)
         if not dout.is_contiguous() or dout.data_ptr() % 16:
             dout = dout.clone(memory_format=torch.contiguous_format)
-        dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        dk = dv = None
-        if k is not None:
-            dk = torch.empty(k.shape, device=k.device, dtype=k.dtype)
-            dv = torch.empty(v.shape, device=v.device, dtype=v.dtype)
         direct = ctx.direct is not None
-        dt, dl = (None if p is None else p.grad if direct else torch.empty(p.shape, device=p.device, dtype=torch.float32) for p in (table, lam))
-        op.backward(q, k, v, table, lam, out, lse, out2, dout, dq, dk, dv, dt, dl, accumulate=direct)
+        dt, dl = [None if p is None else p.grad if direct else lse.new_empty(p.shape) for p in (table, lam)]
+        dq, dk, dv = op.backward(q, k, v, table, lam, out, lse, out2, dout, dt, dl, accumulate=direct)
         if direct:
             for p in ctx.direct:
                 _done(p)
@@ -1140,7 +1138,7 @@ class ResidualNormFn(Function):
             op = _residual_norm_op(f, x, params, ctx.cfg)
         dy, dz = (None if t is None else t.contiguous() for t in (dy, dz))
         if ctx.direct is not None:
-            sums = [p.grad.view(s) if n else None for p, s, n in zip(params, op.par_shapes, need[2:7])]
+            sums = [p.grad.view(s) if n else None for p, s, n in zip(params, op.plan.par_shapes, need[2:7])]
             df, dx = op.backward(f, stats, dy, dz, need[0], need[1], sums, accumulate=True)
             for p in ctx.direct:
                 _done(p)
@@ -1148,9 +1146,9 @@ class ResidualNormFn(Function):
         sums = [None] * 5
         want = [i for i in range(5) if need[2 + i]]
         if want:  # one allocation for all of them
-            parts = torch.empty(sum(params[i].numel() for i in want), device=f.device, dtype=torch.float32).split([params[i].numel() for i in want])
-            for i, t in zip(want, parts):
-                sums[i] = t.view(op.par_shapes[i]) if len(op.par_shapes[i]) > 1 else t
+            sizes = [params[i].numel() for i in want]
+            for i, t in zip(want, stats.new_empty(sum(sizes)).split(sizes)):
+                sums[i] = t.view(op.plan.par_shapes[i]) if len(op.plan.par_shapes[i]) > 1 else t
         df, dx = op.backward(f, stats, dy, dz, need[0], need[1], sums)
         for i in want:
             if params[i].shape != sums[i].shape:
@@ -1168,7 +1166,7 @@ def _flat(p):
 
 
 def _residual_norm_op(f, x, params, cfg):
-    return ops.ResidualNorm(f, x, *map(_flat, params), cfg.scale, cfg.eps, cfg.kind, cfg.lengths)
+    return ops.ResidualNorm(f, x, [_flat(p) for p in params], cfg.scale, cfg.eps, cfg.kind, cfg.lengths)
 
 
 def residual_norm(f, x=None, gate=None, post=None, pre=None, scale=1.0, eps=1e-5, kind="layer", lengths=None):

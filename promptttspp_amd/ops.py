@@ -637,7 +637,7 @@ def bucket_edges(num_buckets, max_distance, bidirectional):
     return e, (ctypes.c_int32 * max(1, len(edges)))(*edges), len(edges)
 
 
-def _on(t, dev, what):
+def _on(t, dev, what):  # (get_device: -1 for a CPU tensor)
     """``t`` must lie on device number ``dev`` (the current one: that is where the launch goes)"""
     if t.get_device() != dev:
         _need_gpu(t)
@@ -649,24 +649,22 @@ def _current(t):
     return _cur_device() if _cur_device is not None else torch.cuda.current_device()
 
 
-def _rows(t, what, shape, dtype, dev):
-    """(address, batch stride, row stride) of a (B, T, C) operand with contiguous channels and any other strides"""
+def _strides(t, what, shape, dtype):
+    """(batch stride, row stride) of a (B, T, C) operand with contiguous channels and any other strides"""
     if t.shape != shape or t.dtype is not dtype:
         raise ValueError(f"{what}: expected a {tuple(shape)} {dtype} tensor, got {tuple(t.shape)} {t.dtype}")
-    _on(t, dev, what)
     s0, s1, s2 = t.stride()
     B, T, C = shape
     if s2 != 1 and C > 1:
         raise ValueError(f"{what}: channels must be contiguous")
     if T == 1:
         s1 = C
-    return t.data_ptr(), (s0 if B > 1 else T * s1), s1
+    return (s0 if B > 1 else T * s1), s1
 
 
-def _f32_operand(t, what, shape, dev):
+def _f32_operand(t, what, shape):
     if t.dtype is not torch.float32 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{what}: expected a contiguous {tuple(shape)} float32 tensor, got {tuple(t.shape)} {t.dtype}")
-    _on(t, dev, what)
     return t.data_ptr()
 
 
@@ -682,16 +680,34 @@ def _i32_rows(t, what, B, like):
     return i32(t, like.device)
 
 
-class AttentionLong:
-    """One call of the long-sequence attention kernels: the argument block of the forward launch, which backward copies and completes.
-    Holds no activations; ``forward`` / ``backward`` are given them."""
+class _Plans(dict):
+    """What depends on shapes, strides, types and options alone -- checked once, kept as a filled argument block and workspace sizes (a
+    training step calls the operators a few hundred times with the same ones).  Cleared when it grows beyond bounds (ragged batches)."""
 
-    __slots__ = ("args", "shape", "width", "ints", "table_shape", "lam_shape", "edges", "dev", "split", "held")
+    def put(self, key, plan):
+        if len(self) >= 512:
+            self.clear()
+        self[key] = plan
+        return plan
 
-    def __init__(self, q, k, v, heads, kv_heads, maps, table=None, max_distance=128, bidirectional=True, lam=None, lam_init=0.0, lengths=None,
-                 q_lengths=None, q_start=None, causal=False, scale=None):
+
+_attention_long_plans, _residual_norm_plans = _Plans(), _Plans()
+
+
+class AttentionLongPlan:
+    """Shapes and options of a call of the long-sequence attention kernels: a checked argument block without addresses."""
+
+    __slots__ = ("args", "shape", "width", "fused", "offsets", "table_shape", "lam_shape", "edges", "ws_fwd", "ws_bwd", "lse_shape")
+
+    @staticmethod
+    def of(q, k, v, heads, kv_heads, maps, table, max_distance, bidirectional, lam, lam_init, causal, scale):
         """k = v = None: q is the fused (B, T, q | k | v) projection"""
-        dev = self.dev = _current(q)
+        key = (q.shape, q.stride(), q.dtype, None if k is None else (k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype), heads, kv_heads, maps,
+               None if table is None else (table.shape, max_distance, bidirectional), None if lam is None else (lam.shape, lam_init), causal, scale)
+        return _attention_long_plans.get(key) or _attention_long_plans.put(
+            key, AttentionLongPlan(q, k, v, heads, kv_heads, maps, table, max_distance, bidirectional, lam, lam_init, causal, scale))
+
+    def __init__(self, q, k, v, heads, kv_heads, maps, table, max_distance, bidirectional, lam, lam_init, causal, scale):
         if q.dim() != 3 or (k is not None and (k.dim() != 3 or v.dim() != 3)):
             raise ValueError("attention: expected (B, T, channels) tensors")
         if heads < 1 or kv_heads < 1 or heads % kv_heads:
@@ -706,108 +722,157 @@ class AttentionLong:
                              f"multiple of 8, at most {128 if maps == 1 else 64}")
         self.shape = B, Tq, Tk, heads, kv_heads, dk, maps
         wq, wk = heads * maps * dk, kv_heads * maps * dk
-        self.width, self.split = wq, k is None
-        dt = q.dtype
-        es = q.element_size()
-        pq, sq, lq = _rows(q, "q", (B, Tq, Cq), dt, dev)
+        self.width, self.fused = wq, k is None
+        self.lse_shape = (maps, B, heads, (Tq + 63) // 64 * 64)
+        dt, es = q.dtype, q.element_size()
+        self.offsets = wq * es, (wq + wk) * es  # of k and v in a fused row
+        a = self.args = _lib.AttentionLongArgs()
+        a.sq, a.ldq = _strides(q, "q", (B, Tq, Cq), dt)
         if k is None:
-            pk, pv, sk, sv, lk, lv = pq + wq * es, pq + (wq + wk) * es, sq, sq, lq, lq
+            a.sk, a.sv, a.ldk, a.ldv = a.sq, a.sq, a.ldq, a.ldq
         else:
-            pk, sk, lk = _rows(k, "k", (B, Tk, wk), dt, dev)
-            pv, sv, lv = _rows(v, "v", (B, Tk, wk), dt, dev)
+            a.sk, a.ldk = _strides(k, "k", (B, Tk, wk), dt)
+            a.sv, a.ldv = _strides(v, "v", (B, Tk, wk), dt)
         if scale is None:
             scale = dk ** -0.5
         elif not 0.0 < scale < 1e30:
             raise ValueError(f"attention: scale {scale} must be positive and finite")
-        nb = nexact = nedges = 0
-        ptab = plam = edges = None
-        lam_heads = 1
         self.table_shape = self.lam_shape = self.edges = None
+        a.lam_heads = 1
         if table is not None:
             if table.dim() != 2 or table.shape[1] != heads:
                 raise ValueError(f"attention: a position table of shape (buckets, {heads}) expected, got {tuple(table.shape)}")
             self.table_shape = table.shape
-            nb, max_distance = table.shape[0], int(max_distance)
-            nexact, self.edges, nedges = bucket_edges(nb, max_distance, bool(bidirectional))
-            edges, ptab = ctypes.addressof(self.edges), _f32_operand(table, "table", table.shape, dev)
+            a.nbuckets, a.max_distance, a.bidirectional = table.shape[0], int(max_distance), bool(bidirectional)
+            a.nexact, self.edges, a.nedges = bucket_edges(a.nbuckets, a.max_distance, bool(bidirectional))
+            a.edges = ctypes.addressof(self.edges)
         if maps == 2:
             if lam.dim() != 3 or lam.shape[0] != 4 or lam.shape[1] not in (1, heads) or lam.shape[2] != dk:
                 raise ValueError(f"attention: lam of shape (4, 1 or {heads}, {dk}) expected, got {tuple(lam.shape)}")
             self.lam_shape = lam.shape
-            plam, lam_heads = _f32_operand(lam, "lam", lam.shape, dev), lam.shape[1]
-        self.held = table, lam  # (f32 copies of other types live until the launches that read them)
-        ints = self.ints = (_i32_rows(lengths, "lengths", B, q), _i32_rows(q_lengths, "q_lengths", B, q), _i32_rows(q_start, "q_start", B, q))
-        n, m, st = (None if t is None else t.data_ptr() for t in ints)
-        # (in the order of ptpp_attention_long_args; outputs, gradients and the workspace are filled in by forward / backward)
-        self.args = _lib.AttentionLongArgs(
-            pq, pk, pv, None, None, None, None, None, None, ptab, plam, None, None, None, n, m, st, edges, None, 0,
-            sq, sk, sv, Tq * wq, 0, 0, 0, 0, lq, lk, lv, wq, 0, 0, 0, 0, B, Tq, Tk, heads, kv_heads, dk, maps, nb, bool(bidirectional),
-            bool(causal), lam_heads, max_distance, nexact, nedges, 0, dtype_code(dt), scale, lam_init)
+            a.lam_heads, a.lam_init = lam.shape[1], lam_init
+        a.B, a.Tq, a.Tk, a.H, a.Hk, a.dk, a.maps = self.shape
+        a.causal, a.dtype, a.scale = bool(causal), dtype_code(dt), scale
+        # outputs and gradients are made here, contiguous: a fused gradient is laid out like the fused projection
+        cq = wq + 2 * wk if k is None else wq
+        a.so = a.sdo = Tq * wq
+        a.ldo = a.lddo = wq
+        a.sdq, a.lddq = Tq * cq, cq
+        a.sdk, a.lddk = (Tq * cq, cq) if k is None else (Tk * wk, wk)
+        a.sdv, a.lddv = a.sdk, a.lddk
+        # workspace sizes (the addresses only have to look like ones): without and with statistics, backward
+        b = type(a).from_buffer_copy(a)
+        b.q = b.k = b.v = b.out = b.dout = b.dq = b.dk_out = b.dv = 4096
+        b.table, b.lam = (4096 if table is not None else None), (4096 if maps == 2 else None)
+        sizes = []
+        for keep, back in ((None, 0), (4096, 0), (4096, 1)):
+            b.lse = keep
+            sizes.append(_lib.load().ptpp_attention_long_ws_bytes(ctypes.byref(b), back))
+            check(min(sizes[-1], 0), "ptpp_attention_long_ws_bytes")
+        self.ws_fwd, self.ws_bwd = sizes[:2], sizes[2]
+
+
+class AttentionLong:
+    """One call of the long-sequence attention kernels: the argument block of the forward launch, which backward copies and completes.
+    Holds no activations; ``forward`` / ``backward`` are given them."""
+
+    __slots__ = ("plan", "args", "held")
+
+    def __init__(self, q, k, v, heads, kv_heads, maps, table=None, max_distance=128, bidirectional=True, lam=None, lam_init=0.0, lengths=None,
+                 q_lengths=None, q_start=None, causal=False, scale=None):
+        dev = _current(q)
+        for t, n in ((k, "k"), (v, "v"), (table, "table"), (lam, "lam")):
+            if t is not None:
+                _on(t, dev, n)
+        if q.get_device() != dev:
+            _on(q, dev, "q")
+        plan = self.plan = AttentionLongPlan.of(q, k, v, heads, kv_heads, maps, table, max_distance, bidirectional, lam, lam_init, causal, scale)
+        a = self.args = _lib.AttentionLongArgs.from_buffer_copy(plan.args)
+        p = a.q = q.data_ptr()
+        if k is None:
+            a.k, a.v = p + plan.offsets[0], p + plan.offsets[1]
+        else:
+            a.k, a.v = k.data_ptr(), v.data_ptr()
+        B = plan.shape[0]
+        lengths, q_lengths, q_start = _i32_rows(lengths, "lengths", B, q), _i32_rows(q_lengths, "q_lengths", B, q), _i32_rows(q_start, "q_start", B, q)
+        self.held = table, lam, lengths, q_lengths, q_start  # (copies in another type live until the launches that read them)
+        if table is not None:
+            a.table = _f32_operand(table, "table", plan.table_shape)
+        if lam is not None:
+            a.lam = _f32_operand(lam, "lam", plan.lam_shape)
+        if lengths is not None:
+            a.k_lengths = lengths.data_ptr()
+        if q_lengths is not None:
+            a.q_lengths = q_lengths.data_ptr()
+        if q_start is not None:
+            a.q_start = q_start.data_ptr()
 
     def forward(self, q, keep):
         """-> (out, lse, out2); the last two only with ``keep`` (what backward needs)"""
-        B, Tq, _, H, _, _, maps = self.shape
-        a = self.args
-        out = torch.empty((B, Tq, self.width), device=q.device, dtype=q.dtype)
+        a, plan = self.args, self.plan
+        B, Tq, maps = a.B, a.Tq, a.maps
+        out = q.new_empty((B, Tq, plan.width))
         lse = out2 = None
         if keep:
-            lse = torch.empty((maps, B, H, (Tq + 63) // 64 * 64), device=q.device, dtype=torch.float32)
+            lse = q.new_empty(plan.lse_shape, dtype=torch.float32)
             a.lse = lse.data_ptr()
             if maps == 2:
-                out2 = torch.empty_like(out)
+                out2 = q.new_empty((B, Tq, plan.width))
                 a.out2 = out2.data_ptr()
         a.out = out.data_ptr()
-        lib = _lib.load()
-        n = lib.ptpp_attention_long_ws_bytes(ctypes.byref(a), 0)
+        n = plan.ws_fwd[1 if keep else 0]
         if n:
-            check(min(n, 0), "ptpp_attention_long_ws_bytes")
-            ws = torch.empty(n, device=q.device, dtype=torch.uint8)  # (this call's own: two captured graphs never share it)
+            ws = q.new_empty(n, dtype=torch.uint8)  # (this call's own: two captured graphs never share it)
             a.ws, a.ws_bytes = ws.data_ptr(), n
-        check(lib.ptpp_attention_long_fwd(ctypes.byref(a), _stream()), "ptpp_attention_long_fwd")
+        check(_lib.load().ptpp_attention_long_fwd(ctypes.byref(a), _stream()), "ptpp_attention_long_fwd")
         return out, lse, out2
 
-    def backward(self, q, k, v, table, lam, out, lse, out2, dout, dq, dk, dv, dtable=None, dlam=None, accumulate=False):
-        """fills dq / dk / dv (dk = dv = None: dq is fused like q) and dtable / dlam (added to with ``accumulate``)"""
-        B, Tq, Tk, _, Hk, d, maps = self.shape
-        dev, w, wk, dt = self.dev, self.width, Hk * maps * d, q.dtype
+    def backward(self, q, k, v, table, lam, out, lse, out2, dout, dtable=None, dlam=None, accumulate=False):
+        """-> (dq, dk, dv); k = v = None: (gradient of the fused projection, None, None).  Fills dtable / dlam (f32; added to with
+        ``accumulate``).  dout: contiguous, like out."""
+        plan = self.plan
         a = type(self.args).from_buffer_copy(self.args)
-        a.dout, a.sdo, a.lddo = _rows(dout, "dout", (B, Tq, w), dt, dev)
-        a.out, a.so, a.ldo = _rows(out, "out", (B, Tq, w), dt, dev)
-        a.lse, a.out2 = lse.data_ptr(), _ptr(out2)
-        if self.split:
-            es = dq.element_size()
-            p, s, ld = _rows(dq, "dq", (B, Tq, w + 2 * wk), dt, dev)
-            a.dq, a.dk_out, a.dv = p, p + w * es, p + (w + wk) * es
-            a.sdq = a.sdk = a.sdv = s
-            a.lddq = a.lddk = a.lddv = ld
+        if dout.shape != out.shape or dout.dtype is not out.dtype or not dout.is_contiguous():
+            raise ValueError(f"attention: a contiguous gradient of shape {tuple(out.shape)} expected, got {tuple(dout.shape)}")
+        dq = q.new_empty(q.shape)
+        dk = dv = None
+        p = a.dq = dq.data_ptr()
+        if plan.fused:
+            a.dk_out, a.dv = p + plan.offsets[0], p + plan.offsets[1]
         else:
-            a.dq, a.sdq, a.lddq = _rows(dq, "dq", (B, Tq, w), dt, dev)
-            a.dk_out, a.sdk, a.lddk = _rows(dk, "dk", (B, Tk, wk), dt, dev)
-            a.dv, a.sdv, a.lddv = _rows(dv, "dv", (B, Tk, wk), dt, dev)
+            dk, dv = k.new_empty(k.shape), v.new_empty(v.shape)
+            a.dk_out, a.dv = dk.data_ptr(), dv.data_ptr()
+        a.dout, a.out, a.lse = dout.data_ptr(), out.data_ptr(), lse.data_ptr()
+        if out2 is not None:
+            a.out2 = out2.data_ptr()
         if table is not None:
-            a.dtable = _f32_operand(dtable, "dtable", self.table_shape, dev)
-        if maps == 2:
-            a.dlam = _f32_operand(dlam, "dlam", self.lam_shape, dev)
-        a.accumulate = bool(accumulate)
-        lib = _lib.load()
-        n = lib.ptpp_attention_long_ws_bytes(ctypes.byref(a), 1)
-        check(min(n, 0), "ptpp_attention_long_ws_bytes")
-        ws = torch.empty(n, device=q.device, dtype=torch.uint8)
-        a.ws, a.ws_bytes = ws.data_ptr(), n
-        check(lib.ptpp_attention_long_bwd(ctypes.byref(a), _stream()), "ptpp_attention_long_bwd")
+            a.dtable = _f32_operand(dtable, "dtable", plan.table_shape)
+        if lam is not None:
+            a.dlam = _f32_operand(dlam, "dlam", plan.lam_shape)
+        a.accumulate = accumulate
+        ws = q.new_empty(plan.ws_bwd, dtype=torch.uint8)
+        a.ws, a.ws_bytes = ws.data_ptr(), plan.ws_bwd
+        check(_lib.load().ptpp_attention_long_bwd(ctypes.byref(a), _stream()), "ptpp_attention_long_bwd")
+        return dq, dk, dv
 
 
 # ----------------------------------------------------------------------------
 # norm behind a block, gate, residual scale, norm before the next block
 # ----------------------------------------------------------------------------
-class ResidualNorm:
-    """One call of the residual-norm kernels, y = x + scale * gate * post(f), z = pre(y): the argument block of the forward launch, which
-    backward copies and completes.  Holds no activations."""
+_RN_NAMES = ("gate", "post gamma", "post beta", "pre gamma", "pre beta")
 
-    __slots__ = ("args", "shape", "ints", "par_shapes", "dev", "has_z", "held")
 
-    def __init__(self, f, x=None, gate=None, post_g=None, post_b=None, pre_g=None, pre_b=None, scale=1.0, eps=1e-5, kind="layer", lengths=None):
-        dev = self.dev = _current(f)
+class ResidualNormPlan:
+    """Shapes and options of a call of the residual-norm kernels: a checked argument block without addresses."""
+
+    __slots__ = ("args", "shape", "par_shapes", "has_z", "stats_shape", "ws")
+
+    @staticmethod
+    def of(f, x, par, scale, eps, kind):
+        key = (f.shape, f.dtype, x is None or (x.shape, x.dtype), tuple([None if t is None else t.shape for t in par]), scale, eps, kind)
+        return _residual_norm_plans.get(key) or _residual_norm_plans.put(key, ResidualNormPlan(f, x, par, scale, eps, kind))
+
+    def __init__(self, f, x, par, scale, eps, kind):
         if kind != "layer" and kind != "rms":
             raise ValueError(f"residual_norm: kind {kind!r} ('layer' or 'rms')")
         if f.dim() != 3:
@@ -817,65 +882,98 @@ class ResidualNorm:
             raise ValueError(f"residual_norm: shape {tuple(f.shape)} (C a multiple of 4, at most 4096, nothing empty)")
         if not eps > 0.0:
             raise ValueError("residual_norm: eps must be positive")
-        rms, vec = kind == "rms", (C,)
+        if x is not None and (x.shape != f.shape or x.dtype is not f.dtype):
+            raise ValueError(f"residual_norm: x must be a {tuple(f.shape)} {f.dtype} tensor like f, got {tuple(x.shape)} {x.dtype}")
+        gate, post_g, post_b, pre_g, pre_b = par
         for n, g, b in (("post", post_g, post_b), ("pre", pre_g, pre_b)):
-            if b is not None and (g is None or rms):
+            if b is not None and (g is None or kind == "rms"):
                 raise ValueError(f"residual_norm: {n} beta without a gamma, or with root-mean-square norms")
-        gate_rows = 1
-        if gate is not None:
-            if gate.shape != vec and gate.shape != (B, C):
-                raise ValueError(f"residual_norm: a gate of shape ({C},) or ({B}, {C}) expected, got {tuple(gate.shape)}")
-            gate_rows = gate.shape[0] if gate.dim() == 2 else 1
-        self.held = gate, post_g, post_b, pre_g, pre_b  # (f32 copies of other types live until the launches that read them)
-        self.par_shapes = ((gate.shape if gate is not None else None), vec, vec, vec, vec)
-        par = [None if t is None else _f32_operand(t, n, s, dev)
-               for t, n, s in zip(self.held, self._NAMES, self.par_shapes)]
-        self.ints = _i32_rows(lengths, "lengths", B, f)
-        self.has_z = pre_g is not None
-        self.args = _lib.ResidualNormArgs(
-            self._dense(f, "f", f.dtype), None if x is None else self._dense(x, "x", f.dtype), None, None, None, None, None, None, *par,
-            None, None, None, None, None, None, _ptr(self.ints), None, 0, B, T, C, rms, gate_rows, 0, dtype_code(f.dtype), scale, eps)
+        if gate is not None and gate.shape != (C,) and gate.shape != (B, C):
+            raise ValueError(f"residual_norm: a gate of shape ({C},) or ({B}, {C}) expected, got {tuple(gate.shape)}")
+        self.par_shapes = ((gate.shape if gate is not None else None), (C,), (C,), (C,), (C,))
+        for t, n, s in zip(par, _RN_NAMES, self.par_shapes):
+            if t is not None and t.shape != s:
+                raise ValueError(f"residual_norm: {n} of shape {tuple(s)} expected, got {tuple(t.shape)}")
+        self.has_z, self.stats_shape, self.ws = pre_g is not None, (4, B * T), {}
+        a = self.args = _lib.ResidualNormArgs()
+        a.B, a.T, a.C, a.rms, a.dtype, a.scale, a.eps = B, T, C, kind == "rms", dtype_code(f.dtype), scale, eps
+        a.gate_rows = gate.shape[0] if gate is not None and gate.dim() == 2 else 1
 
-    _NAMES = ("gate", "post gamma", "post beta", "pre gamma", "pre beta")
 
-    def _dense(self, t, what, dtype):
-        if t.shape != self.shape or t.dtype is not dtype or not t.is_contiguous():
-            raise ValueError(f"residual_norm: {what} must be a contiguous {tuple(self.shape)} {dtype} tensor, got {tuple(t.shape)} {t.dtype}")
-        _on(t, self.dev, what)
-        return t.data_ptr()
+class ResidualNorm:
+    """One call of the residual-norm kernels, y = x + scale * gate * post(f), z = pre(y): the argument block of the forward launch, which
+    backward copies and completes.  Holds no activations."""
+
+    __slots__ = ("plan", "args", "held")
+
+    def __init__(self, f, x=None, par=(None,) * 5, scale=1.0, eps=1e-5, kind="layer", lengths=None):
+        """``par``: (gate, post gamma, post beta, pre gamma, pre beta), f32 or None; f and x contiguous"""
+        dev = _current(f)
+        _on(f, dev, "f")
+        plan = self.plan = ResidualNormPlan.of(f, x, par, scale, eps, kind)
+        a = self.args = _lib.ResidualNormArgs.from_buffer_copy(plan.args)
+        if not f.is_contiguous() or not (x is None or x.is_contiguous()):
+            raise ValueError("residual_norm: f and x must be contiguous")
+        a.f = f.data_ptr()
+        if x is not None:
+            _on(x, dev, "x")
+            a.x = x.data_ptr()
+        for t, n, s, field in zip(par, _RN_NAMES, plan.par_shapes, ("gate", "post_g", "post_b", "pre_g", "pre_b")):
+            if t is not None:
+                _on(t, dev, n)
+                setattr(a, field, _f32_operand(t, n, s))
+        lengths = _i32_rows(lengths, "lengths", plan.shape[0], f)
+        if lengths is not None:
+            a.lengths = lengths.data_ptr()
+        self.held = par, lengths  # (copies in another type live until the launches that read them)
 
     def forward(self, f, keep):
         """-> (y, z or None, statistics or None)"""
-        a = self.args
-        y, z, stats = torch.empty_like(f), None, None
+        a, plan = self.args, self.plan
+        y, z, stats = f.new_empty(plan.shape), None, None
         a.y = y.data_ptr()
-        if self.has_z:
-            z = torch.empty_like(f)
+        if plan.has_z:
+            z = f.new_empty(plan.shape)
             a.z = z.data_ptr()
         if keep:
-            stats = torch.empty((4, self.shape[0] * self.shape[1]), device=f.device, dtype=torch.float32)
+            stats = f.new_empty(plan.stats_shape, dtype=torch.float32)
             a.stats = stats.data_ptr()
         check(_lib.load().ptpp_residual_norm_fwd(ctypes.byref(a), _stream()), "ptpp_residual_norm_fwd")
         return y, z, stats
 
     def backward(self, f, stats, dy, dz, want_df, want_dx, sums, accumulate=False):
         """``sums``: f32 buffers (or None) for (gate, post gamma, post beta, pre gamma, pre beta).  -> (df, dx)"""
+        plan = self.plan
         a = type(self.args).from_buffer_copy(self.args)
-        dt = f.dtype
-        df = torch.empty_like(f) if want_df else None
-        dx = torch.empty_like(f) if want_dx else None
-        a.dy, a.dz = (None if t is None else self._dense(t, n, dt) for t, n in ((dy, "dy"), (dz, "dz")))
-        a.df, a.dx, a.stats = _ptr(df), _ptr(dx), stats.data_ptr()
-        a.dgate, a.dpost_g, a.dpost_b, a.dpre_g, a.dpre_b = (None if t is None else _f32_operand(t, n, s, self.dev)
-                                                             for t, n, s in zip(sums, self._NAMES, self.par_shapes))
-        a.accumulate = bool(accumulate)
-        lib = _lib.load()
-        n = lib.ptpp_residual_norm_ws_bytes(ctypes.byref(a))
-        if n:
+        for t in (dy, dz):
+            if t is not None and (t.shape != plan.shape or t.dtype is not f.dtype or not t.is_contiguous()):
+                raise ValueError(f"residual_norm: contiguous gradients of shape {tuple(plan.shape)} expected, got {tuple(t.shape)}")
+        df = dx = None
+        if want_df:
+            df = f.new_empty(plan.shape)
+            a.df = df.data_ptr()
+        if want_dx:
+            dx = f.new_empty(plan.shape)
+            a.dx = dx.data_ptr()
+        if dy is not None:
+            a.dy = dy.data_ptr()
+        if dz is not None:
+            a.dz = dz.data_ptr()
+        a.stats, a.accumulate = stats.data_ptr(), accumulate
+        wanted = 0
+        for i, (t, n, s, field) in enumerate(zip(sums, _RN_NAMES, plan.par_shapes, ("dgate", "dpost_g", "dpost_b", "dpre_g", "dpre_b"))):
+            if t is not None:
+                wanted |= 1 << i
+                setattr(a, field, _f32_operand(t, n, s))
+        n = plan.ws.get(wanted)
+        if n is None:
+            n = _lib.load().ptpp_residual_norm_ws_bytes(ctypes.byref(a))
             check(min(n, 0), "ptpp_residual_norm_ws_bytes")
-            ws = torch.empty(n, device=f.device, dtype=torch.uint8)
+            plan.ws[wanted] = n
+        if n:
+            ws = f.new_empty(n, dtype=torch.uint8)
             a.ws, a.ws_bytes = ws.data_ptr(), n
-        check(lib.ptpp_residual_norm_bwd(ctypes.byref(a), _stream()), "ptpp_residual_norm_bwd")
+        check(_lib.load().ptpp_residual_norm_bwd(ctypes.byref(a), _stream()), "ptpp_residual_norm_bwd")
         return df, dx
 
 
