@@ -28,13 +28,15 @@ struct LongP {
   const float *table, *lam;
   const int *k_lengths, *q_lengths, *q_start;
   float *lse, *D;              // (M, B, H, TqP)
-  float *lam_part, *tab_part;  // [B][H][query tiles], [H][nbuckets][B][key tiles]
+  double* lam_part;            // [B][H][query blocks]
+  float* tab_part;             // [H][nbuckets][B][key blocks]
   float *part_o, *part_ml;     // few-row forward: [blocks][splits][M][32] rows of DV sums and their (max, sum)
   int64_t sq, sk, sv, so, sdo, sdq, sdk, sdv;  // batch strides, elements
   int ldq, ldk, ldv, ldo, lddo, lddq, lddk, lddv;
   int B, Tq, Tk, TqP, H, Hk, dk, nbuckets, bidirectional, causal, lam_heads, max_distance, nexact, nedges;
-  int nqt, nkt;
+  int nqt, nkt;         // row blocks of the forward / dq and of the dk, dv launches
   int nh, nrb, splits;  // few-row forward: query heads of a block, row blocks per head, key ranges
+  int few_q, few_k;     // backward: blocks of 32 rows
   float scale, lam_init;
   int edges[LA_EDGES];
 };
@@ -173,13 +175,12 @@ __device__ __forceinline__ int la_opaque(int v) {
 }
 // A ROWS x DK image fetched by LDS-DMA, by WAVES waves, NI wave instructions each (lane offsets kept in registers; rows >= nrows and
 // the channels that pad dk to DK come from the zero page, so nothing behind a sequence is ever read).
-template <typename E, int DK, int ROWS = LA_TILE, int WAVES = LA_WAVES>
+template <typename E, int DK, int ROWS = LA_TILE, int WAVES = LA_WAVES, bool KEEP = sizeof(E) == 2>
 struct LTile {
   static constexpr int CH = LOp<E>::CH, CPR = DK / CH, NI = ROWS * CPR / 64 / WAVES;
   static_assert(ROWS * CPR % (64 * WAVES) == 0, "whole wave instructions");
-  // element offsets inside the tile, -1: padding channels; f32 (twice the instructions, short of registers, its vector unit idle beside
-  // the matrix instructions) computes them anew each time
-  static constexpr bool KEEP = sizeof(E) == 2;
+  // element offsets inside the tile, -1: padding channels.  !KEEP: computed anew each time -- f32 (twice the instructions, short of
+  // registers, its vector unit idle beside the matrix instructions) and the few-row backward
   int off[KEEP ? NI : 1], ld_, dk_;
   static __device__ __forceinline__ int offset(int i, int ld, int dk, int lane, int wave) {
     const int x = (wave * NI + i) * 64 + lane, row = x / CPR, c = (x % CPR) ^ la_swz<CPR>(row);
@@ -206,6 +207,14 @@ struct LTile {
       glds16(src, __builtin_amdgcn_readfirstlane(dst + i * 1024));
     }
   }
+};
+
+// blocks of few rows: each of W waves streams its own 32-row chunks through its own two buffers (attention_long_fwd.hip)
+template <typename E, int DK, int DV, int MAPS>
+struct LSplit {
+  static constexpr int STAGE = 32 * (MAPS * DK + DV);                     // elements of a chunk's images
+  static constexpr int W = STAGE * (int)sizeof(E) > 16384 ? 2 : LA_WAVES;  // (f32, wide heads: 32 KB per chunk)
+  static constexpr int LDS = 2 * W * STAGE * (int)sizeof(E);
 };
 
 // every wave's LDS reads are done and every wave is here (the DMA queue is counted separately: glds_wait)

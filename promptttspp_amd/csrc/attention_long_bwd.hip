@@ -12,41 +12,60 @@
 
 namespace {
 
-template <typename E, int DK, int DV, int MAPS, bool BIAS>
-__global__ __launch_bounds__(256, sizeof(E) == 4 ? 1 : 2) void attn_long_dq_kernel(const LongP p) {
+// FEW: the launch would not fill the chip with blocks of 128 rows.  A block owns 32, its W waves take 32-row chunks of the streamed side
+// in turn, each through its own two buffers, and add their sums at the end (the shape of the forward's few-row kernel).
+template <typename E, int DK, int DV, int MAPS, bool FEW>
+struct LBwd {
+  static constexpr int W = FEW ? LSplit<E, DK, DV, MAPS>::W : LA_WAVES;
+  static constexpr int ROWS = FEW ? 32 : LA_TILE;  // streamed rows of a buffer
+  static constexpr int LOADERS = FEW ? 1 : LA_WAVES;
+  static constexpr int PATCHES = ROWS / 32;
+};
+
+template <typename E, int DK, int DV, int MAPS, bool BIAS, bool FEW>
+__global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 4 ? 1 : 2) void attn_long_dq_kernel(const LongP p) {
+  typedef LBwd<E, DK, DV, MAPS, FEW> X;
+  constexpr int W = X::W, ROWS = X::ROWS;
   constexpr int CH = LOp<E>::CH, KS = DK / (2 * CH), VS = DV / (2 * CH), PS = 16 / CH, NT = DK / 32;
-  constexpr bool TIGHT = sizeof(E) == 4 || MAPS * DV == 256;  // registers are short: LDS addresses not kept across patches
+  constexpr bool TIGHT = sizeof(E) == 4 || MAPS * DV == 256 || FEW;  // registers are short: LDS addresses not kept across patches
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  __shared__ float lred[LA_WAVES];
-  constexpr int KIMG = LA_TILE * DK, VIMG = LA_TILE * DV, BUF = MAPS * KIMG + VIMG;
-  E* const img = reinterpret_cast<E*>(smem);
-  float* const btab = reinterpret_cast<float*>(smem + 2 * BUF * sizeof(E));
+  __shared__ double lred[LA_WAVES];
+  __shared__ float weps[W][MAPS][32];
+  constexpr int KIMG = ROWS * DK, VIMG = ROWS * DV, BUF = MAPS * KIMG + VIMG;
   const int lane = threadIdx.x & 63, wave = la_wave(), lq = lane & 31, hw = lane >> 5;
+  E* const img = reinterpret_cast<E*>(smem) + (FEW ? wave * 2 * BUF : 0);
+  float* const btab = reinterpret_cast<float*>(smem + (FEW ? W : 1) * 2 * BUF * sizeof(E));
 
   const int t = xcd_remap(blockIdx.x, gridDim.x);
   const int qt = t % p.nqt, bh = t / p.nqt, h = bh % p.H, b = bh / p.H, hk = h / (p.H / p.Hk);
   const int klen = la_klen(p, b), qlen = la_qlen(p, b), qs = la_qstart(p, b);
-  const int ib = qt * (LA_OWN * LA_WAVES), i0 = ib + wave * LA_OWN, iq = i0 + lq;
+  constexpr int OWN = FEW ? LA_OWN : LA_OWN * LA_WAVES;
+  const int ib = qt * OWN, i0 = ib + (FEW ? 0 : wave * LA_OWN), iq = i0 + lq;
   const int dv = MAPS * p.dk;
   int kend = ib < qlen ? klen : 0;
-  if (p.causal) kend = min(kend, max(0, qs + min(ib + LA_OWN * LA_WAVES, qlen)));
-  const int nt = (kend + LA_TILE - 1) / LA_TILE;
+  if (p.causal) kend = min(kend, max(0, qs + min(ib + OWN, qlen)));
+  const int nt = (kend + ROWS - 1) / ROWS;
 
   const E* kb = reinterpret_cast<const E*>(p.k) + b * p.sk + (int64_t)hk * MAPS * p.dk;
   const E* vb = reinterpret_cast<const E*>(p.v) + b * p.sv + (int64_t)hk * dv;
-  LTile<E, DK> kt;
-  LTile<E, DV> vt;
-  kt.init(p.ldk, p.dk, lane, wave);
-  vt.init(p.ldv, dv, lane, wave);
-  constexpr int NDMA = MAPS * LTile<E, DK>::NI + LTile<E, DV>::NI;
+  typedef LTile<E, DK, ROWS, X::LOADERS, sizeof(E) == 2 && !FEW> KT;
+  typedef LTile<E, DV, ROWS, X::LOADERS, sizeof(E) == 2 && !FEW> VT;
+  const int part = FEW ? 0 : wave;
+  KT kt;
+  VT vt;
+  kt.init(p.ldk, p.dk, lane, part);
+  vt.init(p.ldv, dv, lane, part);
+  constexpr int NDMA = MAPS * KT::NI + VT::NI;
   auto issue = [&](int tile, int buf) {
-    const int j0 = tile * LA_TILE;
+    const int j0 = tile * ROWS;
     E* d = img + buf * BUF;
 #pragma unroll
-    for (int m = 0; m < MAPS; ++m) kt.issue(kb + (int64_t)j0 * p.ldk + m * p.dk, kend - j0, d + m * KIMG, lane, wave);
-    vt.issue(vb + (int64_t)j0 * p.ldv, kend - j0, d + MAPS * KIMG, lane, wave);
+    for (int m = 0; m < MAPS; ++m) kt.issue(kb + (int64_t)j0 * p.ldk + m * p.dk, kend - j0, d + m * KIMG, lane, part);
+    vt.issue(vb + (int64_t)j0 * p.ldv, kend - j0, d + MAPS * KIMG, lane, part);
   };
-  if (nt > 0) issue(0, 0);
+  const int first = FEW ? wave : 0;
+  constexpr int STEP = FEW ? W : 1;
+  if (first < nt) issue(first, 0);
   if constexpr (BIAS) la_fill_btab(p, btab, h);
   float lam = 0.f;
   if constexpr (MAPS == 2) lam = la_lambda(p, h, lane);
@@ -142,36 +161,79 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 ? 1 : 2) void attn_long_dq_kern
     }
   };
 
-  for (int tile = 0; tile < nt; ++tile) {
-    const int buf = tile & 1;
-    if (tile + 1 < nt) {
-      issue(tile + 1, buf ^ 1);
+  if constexpr (FEW && BIAS) la_barrier();  // (the table; the loop itself has no barrier)
+  for (int tile = first, buf = 0; tile < nt; tile += STEP, buf ^= 1) {
+    if (tile + STEP < nt) {
+      if constexpr (FEW) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the buffer's last reads are done
+      issue(tile + STEP, buf ^ 1);
       glds_wait<NDMA>();
     } else {
       glds_wait<0>();
     }
-    la_barrier();
+    if constexpr (!FEW) la_barrier();
     const E* kimg = img + buf * BUF;
     const E* vimg = kimg + MAPS * KIMG;
-    const int jt = tile * LA_TILE;
 #pragma unroll 1
-    for (int ks = 0; ks < 2; ++ks) patch(kimg, vimg, ks, jt + 32 * ks);
-    la_barrier();
+    for (int ks = 0; ks < X::PATCHES; ++ks) patch(kimg, vimg, ks, tile * ROWS + 32 * ks);
+    if constexpr (!FEW) la_barrier();
   }
 
+  if constexpr (FEW) {  // the waves' sums of this row
 #pragma unroll
-  for (int m = 0; m < MAPS; ++m) {
-    Dm[m] += la_half_sum(eps[m]);
-    if (hw == 0 && iq < p.TqP) p.D[(((int64_t)m * p.B + b) * p.H + h) * p.TqP + iq] = iq < qlen ? Dm[m] : 0.f;
+    for (int m = 0; m < MAPS; ++m) {
+      const float e = la_half_sum(eps[m]);
+      if (hw == 0) weps[wave][m][lq] = e;
+      float* mine = reinterpret_cast<float*>(img) + m * NT * 1024 + lane;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mine[(n * 16 + r) * 64] = acc[m][n][r];
+    }
+    static_assert(MAPS * NT * 1024 * 4 <= 2 * BUF * (int)sizeof(E), "a wave's sums fit its buffers");
+    la_barrier();
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m)
+#pragma unroll
+      for (int w = 0; w < W; ++w) Dm[m] += weps[w][m][lq];
+  } else {
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m) Dm[m] += la_half_sum(eps[m]);
   }
-  if constexpr (MAPS == 2) {  // this block's share of dlam = -sum_i D_1
-    const float s = wave_sum(hw == 0 && iq < qlen ? Dm[MAPS - 1] : 0.f);
+  const bool stat = hw == 0 && (!FEW || wave == 0);
+#pragma unroll
+  for (int m = 0; m < MAPS; ++m)
+    if (stat && iq < p.TqP) p.D[(((int64_t)m * p.B + b) * p.H + h) * p.TqP + iq] = iq < qlen ? Dm[m] : 0.f;
+  if constexpr (MAPS == 2) {  // this block's share of dlam = -sum_i D_1 (64 bits: the rows' terms cancel)
+    double s = stat && iq < qlen ? (double)Dm[MAPS - 1] : 0.0;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
     if (lane == 0) lred[wave] = s;
     __syncthreads();
-    if (threadIdx.x == 0) p.lam_part[(int64_t)bh * p.nqt + qt] = -((lred[0] + lred[1]) + (lred[2] + lred[3]));
+    if (threadIdx.x == 0) {
+      double t = 0.0;
+#pragma unroll
+      for (int w = 0; w < W; ++w) t -= lred[w];
+      p.lam_part[(int64_t)bh * p.nqt + qt] = t;
+    }
   }
   if (iq >= p.Tq) return;
   E* qo = reinterpret_cast<E*>(p.dq) + b * p.sdq + (int64_t)h * MAPS * p.dk + (int64_t)iq * p.lddq;
+  if constexpr (FEW) {
+    const float* all = reinterpret_cast<const float*>(smem) + lane;
+    for (int g = wave; g < MAPS * NT * 4; g += W) {  // 4 registers = 4 channels at a time
+      const int m = g / (NT * 4), ch = 32 * ((g >> 2) % NT) + 8 * (g & 3) + 4 * hw;
+      const float c = m == 0 ? p.scale : -lam * p.scale;
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) v[e] += all[w * (2 * BUF * (int)sizeof(E) / 4) + (4 * g + e) * 64];
+      }
+      if (ch < p.dk) la_store4<E>(qo + m * p.dk + ch, v[0] * c, v[1] * c, v[2] * c, v[3] * c);
+    }
+    return;
+  }
 #pragma unroll
   for (int m = 0; m < MAPS; ++m) {
     const float c = m == 0 ? p.scale : -lam * p.scale;
@@ -232,49 +294,57 @@ __device__ __forceinline__ bool la_bucket_range(const LongP& p, int bk, int& lo,
 // LDS, read and written back by the one lane that holds a distance; patches beyond max_distance go into two registers.  LDS atomics
 // instead (ds_add_f32 of every element, no two lanes on one address) took about 330 cycles per wave instruction: 361 us for 24 x 1250
 // frames of 4 x 64 channels against 135 us this way.
-template <typename E, int DK, int DV, int MAPS, bool BIAS>
-__global__ __launch_bounds__(256, sizeof(E) == 4 || MAPS * DK == 128 ? 1 : 2) void attn_long_dkv_kernel(const LongP p) {
+template <typename E, int DK, int DV, int MAPS, bool BIAS, bool FEW>
+__global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 4 || MAPS * DK == 128 ? 1 : 2) void attn_long_dkv_kernel(const LongP p) {
+  typedef LBwd<E, DK, DV, MAPS, FEW> X;
+  constexpr int W = X::W, ROWS = X::ROWS;
   constexpr int CH = LOp<E>::CH, KS = DK / (2 * CH), VS = DV / (2 * CH), PS = 16 / CH, NK = DK / 32, NV = DV / 32;
+  constexpr bool AHEAD = sizeof(E) == 2 && !(MAPS == 2 && DK == 32);  // (as registers allow)
   constexpr bool F32 = sizeof(E) == 4;  // (its fragments fill the register file: the scheduler must not fetch further ahead)
-  constexpr int NBUF = sizeof(E) == 4 ? 1 : 2;  // (f32 tiles twice and the widest distance array would pass 160 KiB)
+  constexpr int NBUF = sizeof(E) == 4 && !FEW ? 1 : 2;  // (f32 tiles twice and the widest distance array would pass 160 KiB)
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  constexpr int QIMG = LA_TILE * DK, OIMG = LA_TILE * DV;
-  constexpr int BUFB = (MAPS * QIMG + OIMG) * (int)sizeof(E) + 1024;  // + (lse, D) of every map, 64 floats each
-  float* const btab = reinterpret_cast<float*>(smem + NBUF * BUFB);
+  constexpr int QIMG = ROWS * DK, OIMG = ROWS * DV;
+  constexpr int BUFB = (MAPS * QIMG + OIMG) * (int)sizeof(E) + 1024;  // + (lse, D) of every map, ROWS floats each
+  float* const btab = reinterpret_cast<float*>(smem + (FEW ? W : 1) * NBUF * BUFB);
   const int lane = threadIdx.x & 63, wave = la_wave(), lk = lane & 31, hw = lane >> 5;
   const int dist_n = la_btab_len(p);
-  float* const hist = btab + ((dist_n + 3) & ~3);  // [8][dist_n]
+  char* const bufs = smem + (FEW ? wave * NBUF * BUFB : 0);
+  float* const hist = btab + ((dist_n + 3) & ~3);  // [2 W][dist_n]
   float* const myhist = hist + 2 * wave * dist_n;
 
   const int t = xcd_remap(blockIdx.x, gridDim.x);
   const int kt = t % p.nkt, bh = t / p.nkt, hk = bh % p.Hk, b = bh / p.Hk, G = p.H / p.Hk;
   const int klen = la_klen(p, b), qlen = la_qlen(p, b), qs = la_qstart(p, b);
-  const int jb = kt * (LA_OWN * LA_WAVES), j0 = jb + wave * LA_OWN, jk = j0 + lk;
+  constexpr int OWN = FEW ? LA_OWN : LA_OWN * LA_WAVES;
+  const int jb = kt * OWN, j0 = jb + (FEW ? 0 : wave * LA_OWN), jk = j0 + lk;
   const int dv = MAPS * p.dk;
-  const int t0 = p.causal ? max(0, jb - qs) / LA_TILE : 0;  // first tile with a query that sees a key of the block
-  const int ntq = jb < klen ? max(0, (qlen + LA_TILE - 1) / LA_TILE - t0) : 0;
+  const int t0 = p.causal ? max(0, jb - qs) / ROWS : 0;  // first tile with a query that sees a key of the block
+  const int ntq = jb < klen ? max(0, (qlen + ROWS - 1) / ROWS - t0) : 0;
   const int total = ntq * G;
 
   const E* qb = reinterpret_cast<const E*>(p.q) + b * p.sq;
   const E* ob = reinterpret_cast<const E*>(p.dout) + b * p.sdo;
-  LTile<E, DK> qt;
-  LTile<E, DV> ot;
-  qt.init(p.ldq, p.dk, lane, wave);
-  ot.init(p.lddo, dv, lane, wave);
-  constexpr int NDMA = MAPS * LTile<E, DK>::NI + LTile<E, DV>::NI + 1;
+  typedef LTile<E, DK, ROWS, X::LOADERS, sizeof(E) == 2 && !FEW> QT;
+  typedef LTile<E, DV, ROWS, X::LOADERS, sizeof(E) == 2 && !FEW> OT;
+  const int part = FEW ? 0 : wave;
+  QT qt;
+  OT ot;
+  qt.init(p.ldq, p.dk, lane, part);
+  ot.init(p.lddo, dv, lane, part);
+  constexpr int NDMA = MAPS * QT::NI + OT::NI + 1;
   auto issue = [&](int it, int buf) {
-    const int h = hk * G + it / ntq, i0 = (t0 + it % ntq) * LA_TILE;
-    char* d = smem + buf * BUFB;
+    const int h = hk * G + it / ntq, i0 = (t0 + it % ntq) * ROWS;
+    char* d = bufs + buf * BUFB;
 #pragma unroll
     for (int m = 0; m < MAPS; ++m)
-      qt.issue(qb + (int64_t)i0 * p.ldq + (h * MAPS + m) * p.dk, qlen - i0, reinterpret_cast<E*>(d) + m * QIMG, lane, wave);
-    ot.issue(ob + (int64_t)i0 * p.lddo + h * dv, qlen - i0, reinterpret_cast<E*>(d) + MAPS * QIMG, lane, wave);
-    // statistics: 16 lanes per array (lse_0, D_0, lse_1, D_1); every wave issues the same copy so that all count alike
-    const int arr = lane >> 4, m = arr >> 1;
-    const float* src = ((arr & 1) ? p.D : p.lse) + (((int64_t)m * p.B + b) * p.H + h) * p.TqP + i0 + 4 * (lane & 15);
+      qt.issue(qb + (int64_t)i0 * p.ldq + (h * MAPS + m) * p.dk, qlen - i0, reinterpret_cast<E*>(d) + m * QIMG, lane, part);
+    ot.issue(ob + (int64_t)i0 * p.lddo + h * dv, qlen - i0, reinterpret_cast<E*>(d) + MAPS * QIMG, lane, part);
+    // statistics: ROWS / 4 lanes per array (lse_0, D_0, lse_1, D_1); every wave issues the same copy so that all count alike
+    const int arr = lane / (ROWS / 4), m = arr >> 1;
+    const float* src = ((arr & 1) ? p.D : p.lse) + (((int64_t)m * p.B + b) * p.H + h) * p.TqP + i0 + 4 * (lane % (ROWS / 4));
     glds16(m < MAPS ? (const void*)src : (const void*)g_conv_zero_page, __builtin_amdgcn_readfirstlane(lds_addr(d + (MAPS * QIMG + OIMG) * sizeof(E))));
   };
-  if (NBUF == 2 && total > 0) issue(0, 0);
+  if (!FEW && NBUF == 2 && total > 0) issue(0, 0);
 
   // the wave's keys and values: lane (key lk, chunk 2 s + hw)
   uint4 kf[MAPS][KS], vf[VS];
@@ -315,14 +385,14 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 || MAPS * DK == 128 ? 1 : 2) vo
       hist[2 * wave * dist_n + dist_n - 1] = hi;
     }
     la_barrier();
-    for (int i = threadIdx.x; i < dist_n; i += 256) {
+    for (int i = threadIdx.x; i < dist_n; i += W * 64) {
       float s = 0.f;
 #pragma unroll
-      for (int c = 0; c < 8; ++c) s += hist[c * dist_n + i];
+      for (int c = 0; c < 2 * W; ++c) s += hist[c * dist_n + i];
       hist[i] = s;
     }
     la_barrier();
-    for (int bk = wave; bk < p.nbuckets; bk += LA_WAVES) {
+    for (int bk = wave; bk < p.nbuckets; bk += W) {
       int lo_d, hi_d;
       float s = 0.f;
       if (la_bucket_range(p, bk, lo_d, hi_d))
@@ -335,64 +405,97 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 || MAPS * DK == 128 ? 1 : 2) vo
 
   // one 32 x 32 patch
   auto patch = [&](const E* qimg, const E* oimg, const float* stat, int sub, int q0) __attribute__((always_inline)) {
-    const int ln = F32 ? la_opaque(lane) : lane, lr = ln & 31, hr = ln >> 5;
-    const float* st0 = stat + 32 * sub + 4 * hr;
-    f32x16 dp = f32x16{}, w, hsum;
+    const int ln = F32 || FEW ? la_opaque(lane) : lane, lr = ln & 31, hr = ln >> 5;
+    const float* st0 = stat + 32 * sub + 4 * hr;  // [m][lse, D][ROWS]; b128 broadcasts: a half wave's rows are the same in all its lanes
+    f32x16 dp = f32x16{}, s[MAPS], hsum;
 #pragma unroll
     for (int kk = 0; kk < VS; ++kk) {
       dp = LOp<E>::mma(la_frag<E, DV>(oimg, 32 * sub + lr, 2 * kk + hr), vf[kk], dp);
       if (F32 && kk % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
-    const int dmin = j0 - (q0 + 31), dmax = j0 + 31 - q0;
-    const bool near = BIAS && dmin < D && dmax > -D;
 #pragma unroll
     for (int m = 0; m < MAPS; ++m) {
-      f32x16 s = f32x16{};
-      const float* ls = st0 + 128 * m;  // (b128 broadcasts: a half wave's rows are the same in all its lanes)
+      s[m] = f32x16{};
 #pragma unroll
       for (int kk = 0; kk < KS; ++kk) {
-        s = LOp<E>::mma(la_frag<E, DK>(qimg + m * QIMG, 32 * sub + lr, 2 * kk + hr), kf[m][kk], s);
+        s[m] = LOp<E>::mma(la_frag<E, DK>(qimg + m * QIMG, 32 * sub + lr, 2 * kk + hr), kf[m][kk], s[m]);
         if (F32 && kk % 4 == 3) __builtin_amdgcn_sched_barrier(0);
       }
-      if (near) {
-        const float* bt = btab + (jk - q0 - 4 * hw + D + LA_PAD);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, bt[-(8 * (r >> 2) + (r & 3))]) - ls[8 * (r >> 2) + (r & 3)];
-      } else {
-        const float bc = BIAS ? btab[dmin >= D ? dist_n - 1 : 0] : 0.f;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, bc - ls[8 * (r >> 2) + (r & 3)]);
-      }
-      if (p.causal && dmax > 0) {
-        const int qmin = jk - q0 - 4 * hw;  // register r's query sees the key from this row on
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = 8 * (r >> 2) + (r & 3) >= qmin ? s[r] : -INFINITY;
-      }
-      f32x16 ds;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        float pr = la_exp2(s[r]);
-        if (m == 1) pr *= -lam;
-        w[r] = m == 0 ? pr : w[r] + pr;
-        ds[r] = pr * (dp[r] - ls[64 + 8 * (r >> 2) + (r & 3)]);
-        if constexpr (BIAS) hsum[r] = m == 0 ? ds[r] : hsum[r] + ds[r];
-      }
+    }
+    // the transposed operands of the last products are fetched before the softmax, which hides their way
+    uint4 tq[AHEAD ? MAPS : 1][AHEAD ? PS : 1][AHEAD ? NK : 1], to[AHEAD ? PS : 1][AHEAD ? NV : 1];
+    if constexpr (AHEAD) {
 #pragma unroll
       for (int st = 0; st < PS; ++st) {
-        const uint4 f = la_pack<E>(ds, st);
+#pragma unroll
+        for (int m = 0; m < MAPS; ++m)
+#pragma unroll
+          for (int n = 0; n < NK; ++n) tq[m][st][n] = la_tfrag<E, DK>(qimg + m * QIMG, 32 * sub, st, n, ln);
+#pragma unroll
+        for (int n = 0; n < NV; ++n) to[st][n] = la_tfrag<E, DV>(oimg, 32 * sub, st, n, ln);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    const int dmin = j0 - (q0 + 31), dmax = j0 + 31 - q0;
+    const bool near = BIAS && dmin < D && dmax > -D;
+    if (near) {
+      const float* bt = btab + (jk - q0 - 4 * hw + D + LA_PAD);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float bv = bt[-(8 * (r >> 2) + (r & 3))];
+#pragma unroll
+        for (int m = 0; m < MAPS; ++m) s[m][r] = fmaf(s[m][r], c2, bv);
+      }
+    } else {
+      const float bc = BIAS ? btab[dmin >= D ? dist_n - 1 : 0] : 0.f;
+#pragma unroll
+      for (int m = 0; m < MAPS; ++m)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[m][r] = fmaf(s[m][r], c2, bc);
+    }
+    if (p.causal && dmax > 0) {
+      const int qmin = jk - q0 - 4 * hw;  // register r's query sees the key from this row on
+#pragma unroll
+      for (int m = 0; m < MAPS; ++m)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[m][r] = 8 * (r >> 2) + (r & 3) >= qmin ? s[m][r] : -INFINITY;
+    }
+    f32x16 w;
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m) {
+      const float* ls = st0 + 2 * ROWS * m;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        float pr = la_exp2(s[m][r] - ls[8 * (r >> 2) + (r & 3)]);
+        if (m == 1) pr *= -lam;
+        w[r] = m == 0 ? pr : w[r] + pr;
+        s[m][r] = pr * (dp[r] - ls[ROWS + 8 * (r >> 2) + (r & 3)]);
+        if constexpr (BIAS) hsum[r] = m == 0 ? s[m][r] : hsum[r] + s[m][r];
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m)
+#pragma unroll
+      for (int st = 0; st < PS; ++st) {
+        const uint4 f = la_pack<E>(s[m], st);
 #pragma unroll
         for (int n = 0; n < NK; ++n) {
-          ak[m][n] = LOp<E>::mma(la_tfrag<E, DK>(qimg + m * QIMG, 32 * sub, st, n, ln), f, ak[m][n]);
+          uint4 t;
+          if constexpr (AHEAD) t = tq[m][st][n];
+          else t = la_tfrag<E, DK>(qimg + m * QIMG, 32 * sub, st, n, ln);
+          ak[m][n] = LOp<E>::mma(t, f, ak[m][n]);
           if (F32) __builtin_amdgcn_sched_barrier(0);
         }
       }
-    }
 #pragma unroll
     for (int st = 0; st < PS; ++st) {
       const uint4 f = la_pack<E>(w, st);
 #pragma unroll
       for (int n = 0; n < NV; ++n) {
-        av[n] = LOp<E>::mma(la_tfrag<E, DV>(oimg, 32 * sub, st, n, ln), f, av[n]);
+        uint4 t;
+        if constexpr (AHEAD) t = to[st][n];
+        else t = la_tfrag<E, DV>(oimg, 32 * sub, st, n, ln);
+        av[n] = LOp<E>::mma(t, f, av[n]);
         if (F32) __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -426,37 +529,82 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 || MAPS * DK == 128 ? 1 : 2) vo
     const int h = hk * G + g;
     if constexpr (BIAS) {
       la_fill_btab(p, btab, h);
-      for (int i = threadIdx.x; i < 8 * dist_n; i += 256) hist[i] = 0.f;
+      for (int i = threadIdx.x; i < 2 * W * dist_n; i += W * 64) hist[i] = 0.f;
       far_lo = far_hi = 0.f;
     }
     if constexpr (MAPS == 2) lam = la_lambda(p, h, lane);
-    for (int iq = 0; iq < ntq; ++iq) {
-      const int it = g * ntq + iq, buf = NBUF == 2 ? it & 1 : 0;
+    if constexpr (FEW) {
+      if (wave < ntq) issue(g * ntq + wave, 0);
+      if constexpr (BIAS) la_barrier();  // (the table and the cleared sums; the loop itself has no barrier)
+    }
+    constexpr int STEP = FEW ? W : 1;
+    for (int iq = FEW ? wave : 0, fb = 0; iq < ntq; iq += STEP, fb ^= 1) {
+      const int it = g * ntq + iq, buf = FEW ? fb : NBUF == 2 ? it & 1 : 0;
       if (NBUF == 1) {
         issue(it, 0);
         glds_wait<0>();
-      } else if (it + 1 < total) {
-        issue(it + 1, buf ^ 1);
+      } else if (FEW ? iq + STEP < ntq : it + 1 < total) {
+        if constexpr (FEW) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the buffer's last reads are done
+        issue(it + STEP, buf ^ 1);
         glds_wait<NDMA>();
       } else {
         glds_wait<0>();
       }
-      la_barrier();
-      const E* qimg = reinterpret_cast<const E*>(smem + buf * BUFB);
+      if constexpr (!FEW) la_barrier();
+      const E* qimg = reinterpret_cast<const E*>(bufs + buf * BUFB);
       const E* oimg = qimg + MAPS * QIMG;
       const float* stat = reinterpret_cast<const float*>(oimg + OIMG);
-      const int q0 = qs + (t0 + iq) * LA_TILE;
+      const int q0 = qs + (t0 + iq) * ROWS;
 #pragma unroll 1
-      for (int sub = 0; sub < 2; ++sub) patch(qimg, oimg, stat, sub, q0 + 32 * sub);
-      la_barrier();
+      for (int sub = 0; sub < X::PATCHES; ++sub) patch(qimg, oimg, stat, sub, q0 + 32 * sub);
+      if constexpr (!FEW) la_barrier();
     }
+    if constexpr (FEW) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the next head's first chunk goes into buffer 0)
     if constexpr (BIAS) flush(h);
   }
 
+  if constexpr (FEW) {  // every wave's sums into its own buffers
+    constexpr int NS = (MAPS * NK + NV) * 1024;
+    static_assert(NS * 4 <= NBUF * BUFB, "a wave's sums fit its buffers");
+    float* mine = reinterpret_cast<float*>(bufs) + lane;
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m)
+#pragma unroll
+      for (int n = 0; n < NK; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mine[((m * NK + n) * 16 + r) * 64] = ak[m][n][r];
+#pragma unroll
+    for (int n = 0; n < NV; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mine[((MAPS * NK + n) * 16 + r) * 64] = av[n][r];
+    la_barrier();
+  }
   if (jk >= p.Tk) return;
   const bool on = jk < klen;
   E* ko = reinterpret_cast<E*>(p.gk) + b * p.sdk + (int64_t)hk * MAPS * p.dk + (int64_t)jk * p.lddk;
   E* vo = reinterpret_cast<E*>(p.gv) + b * p.sdv + (int64_t)hk * dv + (int64_t)jk * p.lddv;
+  if constexpr (FEW) {
+    const float* all = reinterpret_cast<const float*>(smem) + lane;
+    for (int g = wave; g < (MAPS * NK + NV) * 4; g += W) {  // 4 registers = 4 channels at a time: dk's, then dv's
+      const int n = g >> 2, ch0 = 8 * (g & 3) + 4 * hw;
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) v[e] += all[w * (NBUF * BUFB / 4) + (4 * g + e) * 64];
+        v[e] = on ? (n < MAPS * NK ? v[e] * p.scale : v[e]) : 0.f;
+      }
+      if (n < MAPS * NK) {
+        const int ch = 32 * (n % NK) + ch0;
+        if (ch < p.dk) la_store4<E>(ko + (n / NK) * p.dk + ch, v[0], v[1], v[2], v[3]);
+      } else {
+        const int ch = 32 * (n - MAPS * NK) + ch0;
+        if (ch < dv) la_store4<E>(vo + ch, v[0], v[1], v[2], v[3]);
+      }
+    }
+    return;
+  }
 #pragma unroll
   for (int m = 0; m < MAPS; ++m)
 #pragma unroll
@@ -500,19 +648,20 @@ __global__ __launch_bounds__(256) void attn_long_fin_kernel(const LongP p, float
     if (lane == 0) *d = accumulate ? *d + s : s;
     return;
   }
-  __shared__ float red[LA_WAVES];
+  __shared__ double red[LA_WAVES];
   const int hh = blockIdx.x - ntab, per = p.lam_heads > 1 ? 1 : p.H;  // query heads that share these vectors
   const int64_t n = (int64_t)p.B * per * p.nqt;
-  float s = 0.f;
+  double s = 0.0;
   for (int64_t i = threadIdx.x; i < n; i += 256) {
     const int64_t b = i / (per * p.nqt), r = i % (per * p.nqt);
     s += p.lam_part[(b * p.H + hh) * p.nqt + r];
   }
-  s = wave_sum(s);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
   if (lane == 0) red[wave] = s;
   __syncthreads();
   if (wave != 0) return;
-  const float gl = (red[0] + red[1]) + (red[2] + red[3]);
+  const float gl = (float)((red[0] + red[1]) + (red[2] + red[3]));
   float e1, e2;
   la_lambda_parts(p, hh, lane, e1, e2);
   if (lane < p.dk) {
@@ -526,19 +675,62 @@ __global__ __launch_bounds__(256) void attn_long_fin_kernel(const LongP p, float
   }
 }
 
-template <typename E, int DK, int DV, int MAPS, bool BIAS>
-int launch_bwd(const LongP& p, hipStream_t st) {
-  const size_t tiles = (size_t)LA_TILE * (MAPS * DK + DV) * sizeof(E);
-  const int dn = BIAS ? 2 * (p.max_distance + LA_PAD) + 1 : 0;
-  const size_t s1 = 2 * tiles + ((dn + 3) & ~3) * sizeof(float);
-  const size_t s2 = (sizeof(E) == 4 ? 1 : 2) * (tiles + 1024) + (((dn + 3) & ~3) + 8 * (size_t)dn) * sizeof(float);
-  if (s1 > 64 * 1024 && !ptpp_lds_limit((const void*)attn_long_dq_kernel<E, DK, DV, MAPS, BIAS>, (int)s1, "attention_long_bwd")) return PTPP_ELAUNCH;
-  if (s2 > 64 * 1024 && !ptpp_lds_limit((const void*)attn_long_dkv_kernel<E, DK, DV, MAPS, BIAS>, (int)s2, "attention_long_bwd")) return PTPP_ELAUNCH;
-  hipLaunchKernelGGL((attn_long_dq_kernel<E, DK, DV, MAPS, BIAS>), dim3((unsigned)((int64_t)p.nqt * p.B * p.H)), dim3(256), s1, st, p);
+// The rule (as in forward): blocks of 32 rows where that gives at most 256 of them (one round of the chip), else of 128 -- also where the
+// few-row form's buffers and the distance sums of a wide table do not fit LDS together.
+constexpr size_t LDS_MAX = 160 * 1024;
+template <typename E, int DK, int DV, int MAPS>
+size_t lds_dq(bool few, int dn) {
+  return 2 * (few ? LSplit<E, DK, DV, MAPS>::W * 32 : LA_TILE) * (size_t)(MAPS * DK + DV) * sizeof(E) + ((dn + 3) & ~3) * sizeof(float);
+}
+template <typename E, int DK, int DV, int MAPS>
+size_t lds_dkv(bool few, int dn) {
+  const int W = few ? LSplit<E, DK, DV, MAPS>::W : LA_WAVES;
+  const size_t buf = (few ? 32 : LA_TILE) * (size_t)(MAPS * DK + DV) * sizeof(E) + 1024;
+  return (few ? 2 * W : sizeof(E) == 4 ? 1 : 2) * buf + (((dn + 3) & ~3) + 2 * W * (size_t)dn) * sizeof(float);
+}
+// chooses the launch shape and sets the row-block counts
+template <typename E, int DK, int DV, int MAPS>
+void plan_bwd(LongP& p) {
+  const int dn = p.table ? 2 * (p.max_distance + LA_PAD) + 1 : 0;
+  p.few_q = (int64_t)(p.TqP / 32) * p.B * p.H <= 256;
+  p.few_k = (int64_t)((p.Tk + 31) / 32) * p.B * p.Hk <= 256 && lds_dkv<E, DK, DV, MAPS>(true, dn) + 1024 <= LDS_MAX;
+  if (p.few_q) p.nqt = p.TqP / 32;  // (D is written up to the padding of its rows)
+  if (p.few_k) p.nkt = (p.Tk + 31) / 32;
+}
+template <typename E>
+void plan_bwd(LongP& p, int maps) {
+  if (maps == 1) p.dk <= 64 ? plan_bwd<E, 64, 64, 1>(p) : plan_bwd<E, 128, 128, 1>(p);
+  else p.dk <= 32 ? plan_bwd<E, 32, 64, 2>(p) : plan_bwd<E, 64, 128, 2>(p);
+}
+void plan_bwd(LongP& p, int maps, int dtype) {
+  if (dtype == PTPP_F32) plan_bwd<float>(p, maps);
+  else if (dtype == PTPP_BF16) plan_bwd<bf16_raw>(p, maps);
+  else plan_bwd<f16_raw>(p, maps);
+}
+
+template <typename E, int DK, int DV, int MAPS, bool BIAS, bool FEW>
+int launch_dq(const LongP& p, size_t sm, hipStream_t st) {
+  if (sm > 64 * 1024 && !ptpp_lds_limit((const void*)attn_long_dq_kernel<E, DK, DV, MAPS, BIAS, FEW>, (int)sm, "attention_long_bwd")) return PTPP_ELAUNCH;
+  hipLaunchKernelGGL((attn_long_dq_kernel<E, DK, DV, MAPS, BIAS, FEW>), dim3((unsigned)((int64_t)p.nqt * p.B * p.H)), dim3(LBwd<E, DK, DV, MAPS, FEW>::W * 64), sm,
+                     st, p);
   PTPP_CHECK_LAUNCH("attention_long_bwd (dq)");
-  hipLaunchKernelGGL((attn_long_dkv_kernel<E, DK, DV, MAPS, BIAS>), dim3((unsigned)((int64_t)p.nkt * p.B * p.Hk)), dim3(256), s2, st, p);
+  return PTPP_OK;
+}
+template <typename E, int DK, int DV, int MAPS, bool BIAS, bool FEW>
+int launch_dkv(const LongP& p, size_t sm, hipStream_t st) {
+  if (sm > 64 * 1024 && !ptpp_lds_limit((const void*)attn_long_dkv_kernel<E, DK, DV, MAPS, BIAS, FEW>, (int)sm, "attention_long_bwd")) return PTPP_ELAUNCH;
+  hipLaunchKernelGGL((attn_long_dkv_kernel<E, DK, DV, MAPS, BIAS, FEW>), dim3((unsigned)((int64_t)p.nkt * p.B * p.Hk)), dim3(LBwd<E, DK, DV, MAPS, FEW>::W * 64),
+                     sm, st, p);
   PTPP_CHECK_LAUNCH("attention_long_bwd (dk, dv)");
   return PTPP_OK;
+}
+template <typename E, int DK, int DV, int MAPS, bool BIAS>
+int launch_bwd(const LongP& p, hipStream_t st) {
+  const int dn = BIAS ? 2 * (p.max_distance + LA_PAD) + 1 : 0;
+  const size_t s1 = lds_dq<E, DK, DV, MAPS>(p.few_q, dn), s2 = lds_dkv<E, DK, DV, MAPS>(p.few_k, dn);
+  const int r = p.few_q ? launch_dq<E, DK, DV, MAPS, BIAS, true>(p, s1, st) : launch_dq<E, DK, DV, MAPS, BIAS, false>(p, s1, st);
+  if (r != PTPP_OK) return r;
+  return p.few_k ? launch_dkv<E, DK, DV, MAPS, BIAS, true>(p, s2, st) : launch_dkv<E, DK, DV, MAPS, BIAS, false>(p, s2, st);
 }
 template <typename E, int DK, int DV>
 int launch_bwd2(const LongP& p, hipStream_t st) {
@@ -554,14 +746,15 @@ int64_t up64(int64_t n) { return (n + 63) & ~(int64_t)63; }
 // backward workspace, floats: D | lam_part | tab_part
 void bwd_layout(const LongP& p, int maps, int64_t* o_lam, int64_t* o_tab, int64_t* total) {
   *o_lam = up64((int64_t)maps * p.B * p.H * p.TqP);
-  *o_tab = *o_lam + (maps == 2 ? up64((int64_t)p.B * p.H * p.nqt) : 0);
+  *o_tab = *o_lam + (maps == 2 ? up64(2 * (int64_t)p.B * p.H * p.nqt) : 0);  // (64-bit sums)
   *total = *o_tab + (p.table ? up64((int64_t)p.B * p.nkt * p.H * p.nbuckets) : 0);
 }
 
 }  // namespace
 
-int64_t ptpp_attention_long_ws_bwd(const LongP& p, int maps) {
+int64_t ptpp_attention_long_ws_bwd(LongP p, int maps, int dtype) {
   int64_t a, b, n;
+  plan_bwd(p, maps, dtype);
   bwd_layout(p, maps, &a, &b, &n);
   return n * (int64_t)sizeof(float);
 }
@@ -574,11 +767,12 @@ extern "C" int ptpp_attention_long_bwd(const ptpp_attention_long_args* a, void* 
   PTPP_CHECK_ARG(a->maps == 1 || a->out2, "attention_long_bwd: needs the second map's context");
   PTPP_CHECK_ARG((!a->table || a->dtable) && (a->maps == 1 || a->dlam), "attention_long_bwd: null gradient");
   int64_t o_lam, o_tab, total;
+  plan_bwd(p, a->maps, a->dtype);
   bwd_layout(p, a->maps, &o_lam, &o_tab, &total);
   PTPP_CHECK_ARG(a->ws && (uintptr_t)a->ws % 16 == 0 && a->ws_bytes >= (size_t)total * sizeof(float),
                  "attention_long_bwd: workspace of %zu bytes, needs %lld (16-byte aligned)", a->ws_bytes, (long long)(total * sizeof(float)));
   p.D = reinterpret_cast<float*>(a->ws);
-  p.lam_part = p.D + o_lam;
+  p.lam_part = reinterpret_cast<double*>(p.D + o_lam);
   p.tab_part = p.D + o_tab;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   int r;

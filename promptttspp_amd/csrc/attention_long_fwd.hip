@@ -230,13 +230,6 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 ? 1 : 2) void attn_long_fwd_ker
 // each streaming its own chunks through its own two LDS buffers (no block barrier in the loop), and join at the end.  With more
 // than one range the blocks leave unnormalised sums and (max, sum) for the join kernel.  A step is HBM-bound: every key and value is
 // read once, 64 KB in flight per CU.
-template <typename E, int DK, int DV, int MAPS>
-struct LSplit {
-  static constexpr int STAGE = 32 * (MAPS * DK + DV);                     // elements of a chunk's images
-  static constexpr int W = STAGE * (int)sizeof(E) > 16384 ? 2 : LA_WAVES;  // (f32, wide heads: 32 KB per chunk)
-  static constexpr int LDS = 2 * W * STAGE * (int)sizeof(E);
-};
-
 template <typename E, int DK, int DV, int MAPS, bool BIAS>
 __global__ __launch_bounds__((LSplit<E, DK, DV, MAPS>::W * 64), sizeof(E) == 4 || MAPS * DV == 256 ? 1 : 2) void attn_long_split_kernel(const LongP p) {
   typedef LSplit<E, DK, DV, MAPS> S_;
@@ -494,9 +487,9 @@ __global__ __launch_bounds__(256) void attn_long_join_kernel(const LongP p, int 
   }
 }
 
-// The rule: 128-row tiles when they fill the chip (more than 256 blocks) and hold more than a quarter of rows; else the few-row form,
-// with as many key ranges as bring its grid to about 512 blocks of four waves (two per CU) at no fewer than two 32-key chunks per wave.
-bool few_rows(const LongP& p) { return p.Tq <= 32 || (int64_t)p.nqt * p.B * p.H <= 256; }
+// The rule: blocks of 128 rows, unless there are at most 32 rows, or blocks of 32 make at most 256 (one round of the chip); then as many
+// key ranges as bring the grid to about 512 blocks of four waves (two per CU) at no fewer than two 32-key chunks per wave.
+bool few_rows(const LongP& p) { return p.Tq <= 32 || (int64_t)((p.Tq + 31) / 32) * p.B * p.H <= 256; }
 // fills nh, nrb, splits; returns the number of 32-column blocks (0: too many to number)
 int plan_few(LongP& p, int waves) {
   const int G = p.H / p.Hk;
@@ -655,11 +648,11 @@ extern "C" int ptpp_attention_long_fwd(const ptpp_attention_long_args* a, void* 
   return dispatch_fwd<f16_raw>(p, a->maps, st);
 }
 
-int64_t ptpp_attention_long_ws_bwd(const LongP& p, int maps);
+int64_t ptpp_attention_long_ws_bwd(LongP p, int maps, int dtype);
 extern "C" int64_t ptpp_attention_long_ws_bytes(const ptpp_attention_long_args* a, int backward) {
   LongP p;
   if (ptpp_attention_long_params(a, backward, &p, "attention_long_ws_bytes") != PTPP_OK) return -1;
-  if (backward) return ptpp_attention_long_ws_bwd(p, a->maps);
+  if (backward) return ptpp_attention_long_ws_bwd(p, a->maps, a->dtype);
   int64_t o_ml;
   return plan_fwd(p, a, &o_ml, "attention_long_ws_bytes");
 }

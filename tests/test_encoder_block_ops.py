@@ -55,6 +55,9 @@ class RefAttention:
         u = half_ulp(dt)
         up = u if dt != torch.float32 else 2.0 ** -24   # probabilities / dS as operands
         f = 2.0 ** -24
+        # below 2^-14 the f16 values are 2^-24 apart: a rounding there is off by up to half of that, 2^-25, whatever the value.  It enters
+        # once per output and, for the operands P (divided by a sum of at least 1) and dS, once per term of a sum
+        tiny = 2.0 ** -25 if dt == torch.float16 else 0.0
         scale = scale if scale is not None else dk ** -0.5
         z = torch.zeros
         self.out, self.out_b = z(B, Tq, heads, dv, dtype=torch.float64), z(B, Tq, heads, dv, dtype=torch.float64)
@@ -97,14 +100,14 @@ class RefAttention:
                 wa = sum(abs(c[m]) * ps[m] for m in range(maps))
                 rho = max(rhos)
                 self.out[b, :nq, h] = w @ vb
-                self.out_b[b, :nq, h] = (up + rho + 8 * f) * (wa @ vb.abs()) + u * (w @ vb).abs()
+                self.out_b[b, :nq, h] = (up + rho + 8 * f) * (wa @ vb.abs()) + u * (w @ vb).abs() + tiny * (1 + (1 + abs(L)) * vb.abs().sum(0))
                 if do is None:
                     continue
                 dob = do[b, :nq, h]
                 dp = dob @ vb.T
                 dpe = (dob.abs() @ vb.abs().T) * (dv * f)             # dP in f32
                 self.g["dv"][b, :nk, kh] += w.T @ dob
-                self.b["dv"][b, :nk, kh] += (up + rho + (16 + 0.05 * nq) * f) * (wa.T @ dob.abs())
+                self.b["dv"][b, :nk, kh] += (up + rho + (16 + 0.05 * nq) * f) * (wa.T @ dob.abs()) + tiny * dob.abs().sum(0)
                 oe = (u + up + rho) * (wa @ vb.abs())                  # kept contexts: what centres dS in the dq pass
                 De1 = (oe * dob.abs()).sum(-1, keepdim=True) * (1 + abs(L))
                 for m in range(maps):
@@ -118,9 +121,10 @@ class RefAttention:
                     self.g["dq"][b, :nq, h, m] = scale * (ds @ kb)
                     self.b["dq"][b, :nq, h, m] = scale * ((dse + up * (ds.abs() + abs(c[m]) * ps[m] * De1)) @ kb.abs()
                                                           + abs(c[m]) * (ps[m] * De1) @ kb.abs()
-                                                          + (16 + 0.05 * nk) * f * ds.abs() @ kb.abs()) + u * scale * (ds @ kb).abs()
+                                                          + (16 + 0.05 * nk) * f * ds.abs() @ kb.abs()) + u * scale * (ds @ kb).abs() \
+                        + tiny * (1 + scale * max(1.0, abs(L)) * kb.abs().sum(0))
                     self.g["dk"][b, :nk, kh, m] += scale * (ds.T @ qb)
-                    self.b["dk"][b, :nk, kh, m] += scale * ((dse + up * ds.abs() + (16 + 0.05 * nq) * f * ds.abs()).T @ qb.abs())
+                    self.b["dk"][b, :nk, kh, m] += scale * ((dse + up * ds.abs() + (16 + 0.05 * nq) * f * ds.abs()).T @ qb.abs()) + tiny * scale * qb.abs().sum(0)
                     if table is not None:
                         nb = table.shape[0]
                         add = lambda t: torch.zeros(nb, dtype=torch.float64).index_add_(0, bk.reshape(-1), t.reshape(-1))  # noqa: E731
@@ -130,7 +134,7 @@ class RefAttention:
                         dlam[h] -= D.sum()
                         dlam_b[h] += De.sum() + 64 * f * D.abs().sum()
         for n in ("dk", "dv"):  # rounded once, after the heads that share them have been added
-            self.b[n] = self.b[n] + u * self.g[n].abs()
+            self.b[n] = self.b[n] + u * self.g[n].abs() + tiny
         if maps == 2 and do is not None:
             per = heads // lam.shape[1]
             G = dlam.view(lam.shape[1], per).sum(1)[:, None] if per > 1 else dlam[:, None]
@@ -299,6 +303,26 @@ def test_one_query_against_a_memory(dev, maps, dtype, dk, Tk):
 def test_few_queries_against_a_long_memory(dev, maps, Tq):
     check_attention(dev, maps, "bf16", 2, Tq, 1500, 4, 1, 64, 32, train=False, lengths=[1500, 777], q_start=[1500 - Tq, 777 - Tq], causal=True)
     check_attention(dev, maps, "f32", 1, Tq, 1500, 2, 2, 32, 32, train=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("maps,dk", [(1, 64), (1, 128), (2, 32), (2, 64)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_batches_that_fill_the_chip(dev, dtype, maps, dk, causal):
+    """more than 256 blocks of 128 rows: the launch shapes of full batches (few rows take others), lengths of zero and garbage included"""
+    B = 66 if dk != 128 else 44
+    lens = [(37 * b) % 150 for b in range(B)]
+    lens[1] = 149
+    check_attention(dev, maps, dtype, B, 149, 149, 6 if dk == 128 else 4, 2, dk, 32, fused=True, garbage=True, lengths=lens, causal=causal, bidirectional=not causal)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("maps", [1, 2])
+def test_full_batches_of_unequal_sides(dev, maps):
+    """few queries against many keys and the other way round in batches large enough for either launch shape of either pass"""
+    check_attention(dev, maps, "bf16", 150, 140, 30, 2, 2, 40, 16, q_start=[b - 70 for b in range(150)])
+    check_attention(dev, maps, "bf16", 150, 33, 260, 2, 1, 40, 16, causal=True, q_start=[2 * b for b in range(150)])
 
 
 @pytest.mark.gpu
