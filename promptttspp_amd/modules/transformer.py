@@ -12,6 +12,11 @@ kernels with the band terms as index arithmetic); the tensor-op form it replaced
 Masking note: the reference fills masked scores with -1e4 (not -inf), which gives PADDED query rows a uniform
 attention over all positions; every layer ends in ``x * mask`` and every convolution reads ``x * mask``, so padded
 rows never reach a valid row or the output.  The PLAIN kernel writes zeros there instead: outputs are identical.
+
+Beyond the reference, for long inputs (memory linear in the sequence length): ``attention="bucket"`` -- a learned relative-position
+bias by buckets -- and ``attention="diff"`` -- differential attention with a norm per head --, and ``norm="sandwich"``: a residual
+stream with a norm before and behind every sub-layer, a gate (learned, or from the conditioning vector) and a residual scale, one
+launch between two sub-layers.  The defaults are the reference's.
 """
 import math
 
@@ -126,6 +131,59 @@ class RelativeMultiHeadAttention(nn.Module):
         return ops.btc_to_bct(self.forward_cl(ops.bct_to_btc(x, compute_dtype()), lengths))
 
 
+class BucketAttention(nn.Module):
+    """Self-attention with a learned bias per head and relative-position bucket (``PF.attention_bucket``).  ``kv_heads`` < ``n_heads``:
+    key / value heads shared by groups of query heads.  Dropout applies to the output projection."""
+
+    def __init__(self, channels, n_heads, dropout, num_buckets=32, max_distance=128, kv_heads=None):
+        super().__init__()
+        assert channels % n_heads == 0
+        self.n_heads, self.kv_heads, self.max_distance = n_heads, kv_heads or n_heads, max_distance
+        width = channels // n_heads
+        self.qkv = nn.Conv1d(channels, (n_heads + 2 * self.kv_heads) * width, 1)
+        self.out = nn.Conv1d(channels, channels, 1)
+        self.rel_bias = nn.Parameter(torch.randn(num_buckets, n_heads) * 0.02)
+        self.drop = nn.Dropout(dropout)
+
+    def _context(self, x, lengths):
+        qkv = PF.conv1d(x, self.qkv.weight, self.qkv.bias)
+        return PF.attention_bucket(qkv, None, None, self.rel_bias, self.n_heads, kv_heads=self.kv_heads, max_distance=self.max_distance,
+                                   lengths=lengths)
+
+    def forward_cl(self, x, lengths):
+        return PF.conv1d(self._context(x, lengths), self.out.weight, self.out.bias, drop_p=float(self.drop.p) if self.training else 0.0)
+
+    def forward(self, x, mask):
+        lengths = None if mask is None else mask[:, 0].amax(dim=1).sum(dim=-1).to(torch.int32)
+        return ops.btc_to_bct(self.forward_cl(ops.bct_to_btc(x, compute_dtype()), lengths))
+
+
+class DifferentialAttention(BucketAttention):
+    """Differential self-attention (``PF.attention_diff``; Ye et al. 2024): every head is the difference of two softmax maps with learned
+    lam (vectors shared by the heads, lam_init from the layer's depth), then a root-mean-square norm per head scaled by 1 - lam_init
+    (``PF.residual_norm`` without a residual).  ``num_buckets`` = 0: no position bias."""
+
+    def __init__(self, channels, n_heads, dropout, num_buckets=32, max_distance=128, kv_heads=None, depth=0):
+        super().__init__(channels, n_heads, dropout, max(num_buckets, 1), max_distance, kv_heads)
+        if not num_buckets:
+            del self.rel_bias
+            self.rel_bias = None
+        self.head_width = channels // n_heads
+        assert self.head_width % 2 == 0
+        self.lam_init = 0.8 - 0.6 * math.exp(-0.3 * depth)
+        self.lam = nn.Parameter(torch.randn(4, 1, self.head_width // 2) * 0.1)
+        self.sub_norm = nn.Parameter(torch.ones(self.head_width))
+
+    def _context(self, x, lengths):
+        B, T, _ = x.shape
+        qkv = PF.conv1d(x, self.qkv.weight, self.qkv.bias)
+        ctx = PF.attention_diff(qkv, None, None, self.lam, self.lam_init, self.n_heads, kv_heads=self.kv_heads, table=self.rel_bias,
+                                max_distance=self.max_distance, lengths=lengths)
+        y, _ = PF.residual_norm(ctx.view(B, T * self.n_heads, self.head_width), post=(self.sub_norm, None), kind="rms", scale=1.0 - self.lam_init,
+                                lengths=None if lengths is None else lengths * self.n_heads)
+        return y.view(B, T, -1)
+
+
 class FFN(nn.Module):
     def __init__(self, channels, kernel_size, dropout, scale):
         super().__init__()
@@ -133,12 +191,12 @@ class FFN(nn.Module):
         self.conv2 = nn.Conv1d(channels * scale, channels, 1)
         self.drop = nn.Dropout(dropout)
 
-    def forward_cl(self, x, lengths):
-        """conv2(drop(relu(conv1(x * m))) * m) * m"""
+    def forward_cl(self, x, lengths, drop_out=0.0):
+        """drop_out(conv2(drop(relu(conv1(x * m))) * m)) * m"""
         k = self.conv1.kernel_size[0]
         h = PF.conv1d(x, self.conv1.weight, self.conv1.bias, ks=k, pad=k // 2, act="relu", lengths=lengths, in_mask=True,
                       drop_p=float(self.drop.p) if self.training else 0.0)
-        return PF.conv1d(h, self.conv2.weight, self.conv2.bias, lengths=lengths, in_mask=True, out_mask=True)
+        return PF.conv1d(h, self.conv2.weight, self.conv2.bias, lengths=lengths, in_mask=True, out_mask=True, drop_p=drop_out)
 
     def forward(self, x, x_mask):
         return ops.btc_to_bct(self.forward_cl(ops.bct_to_btc(x, compute_dtype()), _lengths_of(x_mask)))
@@ -189,10 +247,32 @@ class FFNLayer(nn.Module):
         return ops.btc_to_bct(self.forward_cl(ops.bct_to_btc(x, compute_dtype()), _lengths_of(mask)))
 
 
-class TransformerLayer(nn.Module):
-    def __init__(self, channels, num_head, kernel_size, dropout, scale, window_size=None, use_rel=False):
+class LongAttentionLayer(_AttnSubLayer):
+    """x = norm(x + dropout(attention(x))) around ``BucketAttention`` / ``DifferentialAttention`` (built without a dropout of their own)"""
+
+    def __init__(self, channels, attention, dropout):
         super().__init__()
-        if use_rel:
+        self.attention_layer = attention
+        self.norm = LayerNorm(channels)
+        self.dropout = nn.Dropout(dropout)
+
+
+def long_attention(kind, channels, num_head, dropout, depth, num_buckets, max_distance, kv_heads):
+    if kind == "bucket":
+        return BucketAttention(channels, num_head, dropout, num_buckets, max_distance, kv_heads)
+    if kind == "diff":
+        return DifferentialAttention(channels, num_head, dropout, num_buckets, max_distance, kv_heads, depth)
+    raise ValueError(f"attention {kind!r}: None (plain, or windowed with use_rel), 'bucket' or 'diff'")
+
+
+class TransformerLayer(nn.Module):
+    def __init__(self, channels, num_head, kernel_size, dropout, scale, window_size=None, use_rel=False, attention=None, depth=0, num_buckets=32,
+                 max_distance=128, kv_heads=None):
+        super().__init__()
+        if attention is not None:
+            self.attention = LongAttentionLayer(channels, long_attention(attention, channels, num_head, 0.0, depth, num_buckets, max_distance, kv_heads),
+                                                dropout)
+        elif use_rel:
             self.attention = RelativeAttentionLayer(channels, num_head, dropout, window_size)
         else:
             self.attention = AttentionLayer(channels, num_head, dropout)
@@ -205,16 +285,85 @@ class TransformerLayer(nn.Module):
         return ops.btc_to_bct(self.forward_cl(ops.bct_to_btc(x, compute_dtype()), _lengths_of(mask)))
 
 
+class _SandwichNorms(nn.Module):
+    """What stands between two sub-layers of a ``norm="sandwich"`` stack: the norm behind the first, its gate, the norm before the next"""
+
+    def __init__(self, channels):
+        super().__init__()
+        self.post, self.pre = LayerNorm(channels), LayerNorm(channels)
+        self.gate = nn.Parameter(torch.ones(channels))
+
+    def step(self, f, x, gate, scale, lengths):
+        return PF.residual_norm(f, x, gate=gate, post=(self.post.gamma, self.post.beta), pre=(self.pre.gamma, self.pre.beta), scale=scale,
+                                eps=self.post.eps, lengths=lengths)
+
+
+class SandwichStack(nn.Module):
+    """The layers of ``Transformer(norm="sandwich")``: z = norm(x); then for every attention and feed-forward sub-layer
+    x <- x + residual_scale * gate * norm(sub-layer(z)), z <- norm(x) in one launch; the last z is the output.
+
+    ``cond_channels``: the conditioning vector g (B, 1, cond_channels) gates every sub-layer through one projection (zero at the start:
+    the learned gates alone), gate = learned + projection(g)."""
+
+    def __init__(self, channels, num_head, num_layers, kernel_size, dropout, scale, attention, num_buckets, max_distance, kv_heads, residual_scale,
+                 cond_channels):
+        super().__init__()
+        self.residual_scale = residual_scale
+        self.attentions = nn.ModuleList([long_attention(attention, channels, num_head, dropout, i, num_buckets, max_distance, kv_heads)
+                                         for i in range(num_layers)])
+        self.ffns = nn.ModuleList([FFN(channels, kernel_size, dropout, scale) for _ in range(num_layers)])
+        self.drop = nn.Dropout(dropout)
+        self.norm = LayerNorm(channels)
+        self.steps = nn.ModuleList([_SandwichNorms(channels) for _ in range(2 * num_layers)])
+        self.cond = None
+        if cond_channels:
+            self.cond = nn.Linear(cond_channels, 2 * num_layers * channels)
+            nn.init.zeros_(self.cond.weight)
+            nn.init.zeros_(self.cond.bias)
+
+    def _gates(self, g):
+        if g is None:
+            return [s.gate for s in self.steps]
+        if self.cond is None or g.shape[1] != 1:
+            raise ValueError("norm='sandwich' takes its conditioning as one vector per utterance, through gates (cond_channels)")
+        c = PF.linear(g.contiguous(), self.cond.weight, self.cond.bias).float()              # (B, 1, steps * C)
+        c = c.view(g.shape[0], len(self.steps), -1).transpose(0, 1).contiguous()              # (steps, B, C)
+        return [c[i] + s.gate for i, s in enumerate(self.steps)]
+
+    def forward_cl(self, x, lengths, g=None):
+        gates = self._gates(g)
+        z = self.norm.forward_cl(x, lengths=lengths, out_mask=True)
+        for i, (attention, ffn) in enumerate(zip(self.attentions, self.ffns)):
+            x, z = self.steps[2 * i].step(attention.forward_cl(z, lengths), x, gates[2 * i], self.residual_scale, lengths)
+            f = ffn.forward_cl(z, lengths, drop_out=float(self.drop.p) if self.training else 0.0)
+            x, z = self.steps[2 * i + 1].step(f, x, gates[2 * i + 1], self.residual_scale, lengths)
+        return z
+
+
 class Transformer(nn.Module):
-    def __init__(self, channels, num_head, num_layers, kernel_size, dropout, scale=4, window_size=None, use_rel=False):
+    """``attention``: None (the reference's: plain, or windowed relative with ``use_rel``), "bucket" or "diff"; ``norm``: "post" (the
+    reference's) or "sandwich".  ``num_buckets`` / ``max_distance`` / ``kv_heads``: of the two long forms; ``residual_scale`` /
+    ``cond_channels``: of the sandwich (see ``SandwichStack``)."""
+
+    def __init__(self, channels, num_head, num_layers, kernel_size, dropout, scale=4, window_size=None, use_rel=False, attention=None, norm="post",
+                 num_buckets=32, max_distance=128, kv_heads=None, residual_scale=1.0, cond_channels=None):
         super().__init__()
         self.channels = channels
-        self.layers = nn.ModuleList([TransformerLayer(channels, num_head, kernel_size, dropout, scale, window_size, use_rel)
-                                     for _ in range(num_layers)])
+        self.norm_form = norm
+        if norm == "sandwich":
+            self.stack = SandwichStack(channels, num_head, num_layers, kernel_size, dropout, scale, attention, num_buckets, max_distance, kv_heads,
+                                       residual_scale, cond_channels)
+        elif norm == "post":
+            self.layers = nn.ModuleList([TransformerLayer(channels, num_head, kernel_size, dropout, scale, window_size, use_rel, attention, i, num_buckets,
+                                                          max_distance, kv_heads) for i in range(num_layers)])
+        else:
+            raise ValueError(f"norm {norm!r}: 'post' or 'sandwich'")
 
     def forward_cl(self, x, lengths, g=None):
         """x (B,T,C) channels-last in the compute dtype; g: optional (B,1,C) / (B,T,C) conditioning added before
-        every layer (transformer.py:258-260)."""
+        every layer (transformer.py:258-260); with ``norm="sandwich"`` (B,1,cond_channels), through the gates."""
+        if self.norm_form == "sandwich":
+            return self.stack.forward_cl(x, lengths, g)
         for layer in self.layers:
             if g is not None:
                 x = x + g
