@@ -1114,8 +1114,10 @@ class ResidualNormFn(Function):
     @staticmethod
     def forward(ctx, f, x, gate, post_g, post_b, pre_g, pre_b, cfg):
         ctx.set_materialize_grads(False)
-        f = f.contiguous()
-        x = x.contiguous() if x is not None else None
+        if not f.is_contiguous():
+            f = f.contiguous()
+        if x is not None and not x.is_contiguous():
+            x = x.contiguous()
         params = (gate, post_g, post_b, pre_g, pre_b)
         op = _residual_norm_op(f, x, params, cfg)
         y, z, stats = op.forward(f, True)
@@ -1136,26 +1138,27 @@ class ResidualNormFn(Function):
         op = ctx.op
         if not _still(op.args, ("f", "x", "gate", "post_g", "post_b", "pre_g", "pre_b"), (f, x, *params)):
             op = _residual_norm_op(f, x, params, ctx.cfg)
-        dy, dz = (None if t is None else t.contiguous() for t in (dy, dz))
+        if dy is not None and not dy.is_contiguous():
+            dy = dy.contiguous()
+        if dz is not None and not dz.is_contiguous():
+            dz = dz.contiguous()
+        want = need[2:7]
         if ctx.direct is not None:
-            sums = [p.grad.view(s) if n else None for p, s, n in zip(params, op.plan.par_shapes, need[2:7])]
-            df, dx = op.backward(f, stats, dy, dz, need[0], need[1], sums, accumulate=True)
+            into = [p.grad if p.dim() == 2 and p.shape[0] != 1 else p.grad.view(-1) for p in ctx.direct]
+            df, dx, _ = op.backward(f, stats, dy, dz, need[0], need[1], want, into)
             for p in ctx.direct:
                 _done(p)
             return df, dx, None, None, None, None, None, None
-        sums = [None] * 5
-        want = [i for i in range(5) if need[2 + i]]
-        if want:  # one allocation for all of them
-            sizes = [params[i].numel() for i in want]
-            for i, t in zip(want, stats.new_empty(sum(sizes)).split(sizes)):
-                sums[i] = t.view(op.plan.par_shapes[i]) if len(op.plan.par_shapes[i]) > 1 else t
-        df, dx = op.backward(f, stats, dy, dz, need[0], need[1], sums)
-        for i in want:
-            if params[i].shape != sums[i].shape:
-                sums[i] = sums[i].view(params[i].shape)
-            if params[i].dtype is not torch.float32:
-                sums[i] = sums[i].to(params[i].dtype)
-        return (df, dx, *sums, None)
+        df, dx, fresh = op.backward(f, stats, dy, dz, need[0], need[1], want)
+        grads, i = [df, dx, None, None, None, None, None, None], 0
+        for k, p in enumerate(params):
+            if want[k]:
+                g = fresh[i]
+                i += 1
+                if p.dim() != 1:
+                    g = g.view(p.shape)
+                grads[2 + k] = g if p.dtype is torch.float32 else g.to(p.dtype)
+        return tuple(grads)
 
 
 def _flat(p):

@@ -10,6 +10,7 @@ compute dtype (torch.float32 or torch.bfloat16).
 """
 import ctypes
 import functools
+import math
 import struct
 
 import torch
@@ -662,9 +663,11 @@ def _strides(t, what, shape, dtype):
     return (s0 if B > 1 else T * s1), s1
 
 
-def _f32_operand(t, what, shape):
+def _f32_operand(t, what, shape, dev):
     if t.dtype is not torch.float32 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{what}: expected a contiguous {tuple(shape)} float32 tensor, got {tuple(t.shape)} {t.dtype}")
+    if t.get_device() != dev:
+        _on(t, dev, what)
     return t.data_ptr()
 
 
@@ -781,11 +784,10 @@ class AttentionLong:
     def __init__(self, q, k, v, heads, kv_heads, maps, table=None, max_distance=128, bidirectional=True, lam=None, lam_init=0.0, lengths=None,
                  q_lengths=None, q_start=None, causal=False, scale=None):
         dev = _current(q)
-        for t, n in ((k, "k"), (v, "v"), (table, "table"), (lam, "lam")):
-            if t is not None:
-                _on(t, dev, n)
-        if q.get_device() != dev:
-            _on(q, dev, "q")
+        _on(q, dev, "q")
+        if k is not None:
+            _on(k, dev, "k")
+            _on(v, dev, "v")
         plan = self.plan = AttentionLongPlan.of(q, k, v, heads, kv_heads, maps, table, max_distance, bidirectional, lam, lam_init, causal, scale)
         a = self.args = _lib.AttentionLongArgs.from_buffer_copy(plan.args)
         p = a.q = q.data_ptr()
@@ -797,9 +799,9 @@ class AttentionLong:
         lengths, q_lengths, q_start = _i32_rows(lengths, "lengths", B, q), _i32_rows(q_lengths, "q_lengths", B, q), _i32_rows(q_start, "q_start", B, q)
         self.held = table, lam, lengths, q_lengths, q_start  # (copies in another type live until the launches that read them)
         if table is not None:
-            a.table = _f32_operand(table, "table", plan.table_shape)
+            a.table = _f32_operand(table, "table", plan.table_shape, dev)
         if lam is not None:
-            a.lam = _f32_operand(lam, "lam", plan.lam_shape)
+            a.lam = _f32_operand(lam, "lam", plan.lam_shape, dev)
         if lengths is not None:
             a.k_lengths = lengths.data_ptr()
         if q_lengths is not None:
@@ -845,10 +847,11 @@ class AttentionLong:
         a.dout, a.out, a.lse = dout.data_ptr(), out.data_ptr(), lse.data_ptr()
         if out2 is not None:
             a.out2 = out2.data_ptr()
+        dev = q.get_device()
         if table is not None:
-            a.dtable = _f32_operand(dtable, "dtable", plan.table_shape)
+            a.dtable = _f32_operand(dtable, "dtable", plan.table_shape, dev)
         if lam is not None:
-            a.dlam = _f32_operand(dlam, "dlam", plan.lam_shape)
+            a.dlam = _f32_operand(dlam, "dlam", plan.lam_shape, dev)
         a.accumulate = accumulate
         ws = q.new_empty(plan.ws_bwd, dtype=torch.uint8)
         a.ws, a.ws_bytes = ws.data_ptr(), plan.ws_bwd
@@ -859,13 +862,10 @@ class AttentionLong:
 # ----------------------------------------------------------------------------
 # norm behind a block, gate, residual scale, norm before the next block
 # ----------------------------------------------------------------------------
-_RN_NAMES = ("gate", "post gamma", "post beta", "pre gamma", "pre beta")
-
-
 class ResidualNormPlan:
     """Shapes and options of a call of the residual-norm kernels: a checked argument block without addresses."""
 
-    __slots__ = ("args", "shape", "par_shapes", "has_z", "stats_shape", "ws")
+    __slots__ = ("args", "shape", "par_shapes", "has_z", "stats_shape", "sums")
 
     @staticmethod
     def of(f, x, par, scale, eps, kind):
@@ -890,11 +890,11 @@ class ResidualNormPlan:
                 raise ValueError(f"residual_norm: {n} beta without a gamma, or with root-mean-square norms")
         if gate is not None and gate.shape != (C,) and gate.shape != (B, C):
             raise ValueError(f"residual_norm: a gate of shape ({C},) or ({B}, {C}) expected, got {tuple(gate.shape)}")
-        self.par_shapes = ((gate.shape if gate is not None else None), (C,), (C,), (C,), (C,))
-        for t, n, s in zip(par, _RN_NAMES, self.par_shapes):
-            if t is not None and t.shape != s:
-                raise ValueError(f"residual_norm: {n} of shape {tuple(s)} expected, got {tuple(t.shape)}")
-        self.has_z, self.stats_shape, self.ws = pre_g is not None, (4, B * T), {}
+        self.par_shapes = (gate.shape if gate is not None else None), (C,)  # of the gate, of every other parameter
+        for t, n in zip(par[1:], ("post gamma", "post beta", "pre gamma", "pre beta")):
+            if t is not None and t.shape != (C,):
+                raise ValueError(f"residual_norm: {n} of shape ({C},) expected, got {tuple(t.shape)}")
+        self.has_z, self.stats_shape, self.sums = pre_g is not None, (4, B * T), {}
         a = self.args = _lib.ResidualNormArgs()
         a.B, a.T, a.C, a.rms, a.dtype, a.scale, a.eps = B, T, C, kind == "rms", dtype_code(f.dtype), scale, eps
         a.gate_rows = gate.shape[0] if gate is not None and gate.dim() == 2 else 1
@@ -918,10 +918,18 @@ class ResidualNorm:
         if x is not None:
             _on(x, dev, "x")
             a.x = x.data_ptr()
-        for t, n, s, field in zip(par, _RN_NAMES, plan.par_shapes, ("gate", "post_g", "post_b", "pre_g", "pre_b")):
-            if t is not None:
-                _on(t, dev, n)
-                setattr(a, field, _f32_operand(t, n, s))
+        gate, post_g, post_b, pre_g, pre_b = par
+        s0, s1 = plan.par_shapes
+        if gate is not None:
+            a.gate = _f32_operand(gate, "gate", s0, dev)
+        if post_g is not None:
+            a.post_g = _f32_operand(post_g, "post gamma", s1, dev)
+        if post_b is not None:
+            a.post_b = _f32_operand(post_b, "post beta", s1, dev)
+        if pre_g is not None:
+            a.pre_g = _f32_operand(pre_g, "pre gamma", s1, dev)
+        if pre_b is not None:
+            a.pre_b = _f32_operand(pre_b, "pre beta", s1, dev)
         lengths = _i32_rows(lengths, "lengths", plan.shape[0], f)
         if lengths is not None:
             a.lengths = lengths.data_ptr()
@@ -941,40 +949,62 @@ class ResidualNorm:
         check(_lib.load().ptpp_residual_norm_fwd(ctypes.byref(a), _stream()), "ptpp_residual_norm_fwd")
         return y, z, stats
 
-    def backward(self, f, stats, dy, dz, want_df, want_dx, sums, accumulate=False):
-        """``sums``: f32 buffers (or None) for (gate, post gamma, post beta, pre gamma, pre beta).  -> (df, dx)"""
+    _GRADS = ("dgate", "dpost_g", "dpost_b", "dpre_g", "dpre_b")
+
+    def _wanted(self, want):
+        """per set of wanted sums: (fields, sizes, byte offsets, shapes inside one buffer, workspace bytes)"""
+        plan = self.plan
+        s0, s1 = plan.par_shapes
+        fields = [n for n, w in zip(self._GRADS, want) if w]
+        shapes = [s0 if n == "dgate" else s1 for n in fields]
+        sizes = [math.prod(s) for s in shapes]
+        a = type(self.args).from_buffer_copy(self.args)
+        for n in fields:
+            setattr(a, n, 4096)
+        n = _lib.load().ptpp_residual_norm_ws_bytes(ctypes.byref(a))
+        check(min(n, 0), "ptpp_residual_norm_ws_bytes")
+        r = plan.sums[want] = fields, sizes, [4 * sum(sizes[:i]) for i in range(len(sizes))], shapes, n
+        return r
+
+    def backward(self, f, stats, dy, dz, want_df, want_dx, want, into=None):
+        """``want``: which of (gate, post gamma, post beta, pre gamma, pre beta) get a gradient; ``into``: f32 buffers to add them to, in that
+        order (None: fresh ones).  -> (df, dx, [the fresh sums])"""
         plan = self.plan
         a = type(self.args).from_buffer_copy(self.args)
-        for t in (dy, dz):
-            if t is not None and (t.shape != plan.shape or t.dtype is not f.dtype or not t.is_contiguous()):
-                raise ValueError(f"residual_norm: contiguous gradients of shape {tuple(plan.shape)} expected, got {tuple(t.shape)}")
-        df = dx = None
-        if want_df:
-            df = f.new_empty(plan.shape)
-            a.df = df.data_ptr()
-        if want_dx:
-            dx = f.new_empty(plan.shape)
-            a.dx = dx.data_ptr()
+        shape, dt = plan.shape, f.dtype
         if dy is not None:
+            if dy.shape != shape or dy.dtype is not dt or not dy.is_contiguous():
+                raise ValueError(f"residual_norm: contiguous gradients of shape {tuple(shape)} expected, got {tuple(dy.shape)}")
             a.dy = dy.data_ptr()
         if dz is not None:
+            if dz.shape != shape or dz.dtype is not dt or not dz.is_contiguous():
+                raise ValueError(f"residual_norm: contiguous gradients of shape {tuple(shape)} expected, got {tuple(dz.shape)}")
             a.dz = dz.data_ptr()
-        a.stats, a.accumulate = stats.data_ptr(), accumulate
-        wanted = 0
-        for i, (t, n, s, field) in enumerate(zip(sums, _RN_NAMES, plan.par_shapes, ("dgate", "dpost_g", "dpost_b", "dpre_g", "dpre_b"))):
-            if t is not None:
-                wanted |= 1 << i
-                setattr(a, field, _f32_operand(t, n, s))
-        n = plan.ws.get(wanted)
-        if n is None:
-            n = _lib.load().ptpp_residual_norm_ws_bytes(ctypes.byref(a))
-            check(min(n, 0), "ptpp_residual_norm_ws_bytes")
-            plan.ws[wanted] = n
+        df = dx = None
+        if want_df:
+            df = f.new_empty(shape)
+            a.df = df.data_ptr()
+        if want_dx:
+            dx = f.new_empty(shape)
+            a.dx = dx.data_ptr()
+        a.stats = stats.data_ptr()
+        fields, sizes, offsets, shapes, n = plan.sums.get(want) or self._wanted(want)
+        fresh = ()
+        if into is not None:
+            a.accumulate = 1
+            dev = f.get_device()
+            for name, t, s in zip(fields, into, shapes):
+                setattr(a, name, _f32_operand(t, name, s, dev))
+        elif fields:  # one allocation for all of them
+            buf = stats.new_empty(offsets[-1] // 4 + sizes[-1])
+            p, fresh = buf.data_ptr(), buf.split(sizes)
+            for name, o in zip(fields, offsets):
+                setattr(a, name, p + o)
         if n:
             ws = f.new_empty(n, dtype=torch.uint8)
             a.ws, a.ws_bytes = ws.data_ptr(), n
         check(_lib.load().ptpp_residual_norm_bwd(ctypes.byref(a), _stream()), "ptpp_residual_norm_bwd")
-        return df, dx
+        return df, dx, fresh
 
 
 # ----------------------------------------------------------------------------
