@@ -173,6 +173,13 @@ __device__ __forceinline__ int la_opaque(int v) {
   asm volatile("" : "+v"(v));
   return v;
 }
+// an address that is the same in all lanes, as the scalar it is
+__device__ __forceinline__ const void* la_uniform(const void* p) {
+  const uint64_t v = (uint64_t)(uintptr_t)p;
+  const uint64_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)v), hi = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+  return (const void*)(uintptr_t)(lo | (hi << 32));
+}
+
 // A ROWS x DK image fetched by LDS-DMA, by WAVES waves, NI wave instructions each (lane offsets kept in registers; rows >= nrows and
 // the channels that pad dk to DK come from the zero page, so nothing behind a sequence is ever read).
 template <typename E, int DK, int ROWS = LA_TILE, int WAVES = LA_WAVES, bool KEEP = sizeof(E) == 2>
@@ -182,6 +189,7 @@ struct LTile {
   // element offsets inside the tile, -1: padding channels.  !KEEP: computed anew each time -- f32 (twice the instructions, short of
   // registers, its vector unit idle beside the matrix instructions) and the few-row backward
   int off[KEEP ? NI : 1], ld_, dk_;
+  bool whole;  // no padding channels, and every byte offset of a tile fits 31 bits
   static __device__ __forceinline__ int offset(int i, int ld, int dk, int lane, int wave) {
     const int x = (wave * NI + i) * 64 + lane, row = x / CPR, c = (x % CPR) ^ la_swz<CPR>(row);
     return c * CH < dk ? row * ld + c * CH : -1;
@@ -189,14 +197,23 @@ struct LTile {
   __device__ __forceinline__ void init(int ld, int dk, int lane, int wave) {
     ld_ = ld;
     dk_ = dk;
+    whole = dk == DK && ld < (1 << 22);
     if constexpr (KEEP) {
 #pragma unroll
       for (int i = 0; i < NI; ++i) off[i] = offset(i, ld, dk, lane, wave);
     }
   }
+  // whole tiles: one scalar address and the kept lane offsets, no vector work at all; the last tile of a sequence: row by row
   __device__ __forceinline__ void issue(const E* tile, int nrows, const E* img, int lane, int wave) const {
-    const uint32_t dst = lds_addr(img) + wave * (NI * 1024);
-    if constexpr (!KEEP) lane = la_opaque(lane);
+    const uint32_t dst = __builtin_amdgcn_readfirstlane(lds_addr(img) + wave * (NI * 1024));
+    if constexpr (KEEP) {
+      if (whole && nrows >= ROWS) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) glds16_s(la_uniform(tile), (uint32_t)off[i] * (uint32_t)sizeof(E), dst + i * 1024);
+        return;
+      }
+    }
+    lane = la_opaque(lane);
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int row = ((wave * NI + i) * 64 + lane) / CPR;
@@ -204,7 +221,7 @@ struct LTile {
       if constexpr (KEEP) o = off[i];
       else o = offset(i, ld_, dk_, lane, wave);
       const void* src = (o >= 0 && row < nrows) ? (const void*)(tile + o) : (const void*)g_conv_zero_page;
-      glds16(src, __builtin_amdgcn_readfirstlane(dst + i * 1024));
+      glds16(src, dst + i * 1024);
     }
   }
 };
@@ -223,8 +240,14 @@ __device__ __forceinline__ void la_barrier() { asm volatile("s_waitcnt lgkmcnt(0
 __device__ __forceinline__ float la_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 // wave number, known to be the same in all lanes: what depends on it alone is scalar work and scalar branches
 __device__ __forceinline__ int la_wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
-__device__ __forceinline__ float la_half_sum(float v) { return v + __shfl_xor(v, 32, 64); }
-__device__ __forceinline__ float la_half_max(float v) { return fmaxf(v, __shfl_xor(v, 32, 64)); }
+__device__ __forceinline__ float la_half_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float la_half_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
 
 // bucket of a distance d = key position - query position (Raffel et al. 2020: half of the buckets per direction, the first
 // nexact distances one each, then logarithmic steps up to max_distance; the steps' first distances come from the host as whole
@@ -246,6 +269,16 @@ __device__ __forceinline__ void la_fill_btab(const LongP& p, float* bt, int h) {
     const int d = min(max(i - D - LA_PAD, -D), D);
     bt[i] = p.table[(int64_t)la_bucket(p, d) * p.H + h] * LA_LOG2E;
   }
+}
+
+// block -> (tile, pair), a pair being one (utterance, head) with `tiles` blocks; `pairs` of them.  Tiles of a pair run on one XCD (they share
+// keys and values in its L2), and an XCD gets every 8th pair: lengths differ from utterance to utterance, and consecutive pairs are one
+// utterance's heads -- with contiguous ranges of pairs the XCD of the longest utterance ran on alone.
+__device__ __forceinline__ void la_block(int tiles, int pairs, int& tile, int& pair) {
+  const int t = xcd_remap(blockIdx.x, gridDim.x), pos = t / tiles;
+  tile = t - pos * tiles;
+  const int q = pairs >> 3, rem = pairs & 7, big = rem * (q + 1);
+  pair = pos < big ? pos / (q + 1) + 8 * (pos % (q + 1)) : rem + (pos - big) / max(q, 1) + 8 * ((pos - big) % max(q, 1));
 }
 
 // lam of head h (every lane of a wave calls it; dk <= 64)

@@ -36,8 +36,10 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
   E* const img = reinterpret_cast<E*>(smem) + (FEW ? wave * 2 * BUF : 0);
   float* const btab = reinterpret_cast<float*>(smem + (FEW ? W : 1) * 2 * BUF * sizeof(E));
 
-  const int t = xcd_remap(blockIdx.x, gridDim.x);
-  const int qt = t % p.nqt, bh = t / p.nqt, h = bh % p.H, b = bh / p.H, hk = h / (p.H / p.Hk);
+  int qt, bh;
+  la_block(p.nqt, p.B * p.H, qt, bh);
+  if (p.causal) qt = p.nqt - 1 - qt;  // (the longest rows first)
+  const int h = bh % p.H, b = bh / p.H, hk = h / (p.H / p.Hk);
   const int klen = la_klen(p, b), qlen = la_qlen(p, b), qs = la_qstart(p, b);
   constexpr int OWN = FEW ? LA_OWN : LA_OWN * LA_WAVES;
   const int ib = qt * OWN, i0 = ib + (FEW ? 0 : wave * LA_OWN), iq = i0 + lq;
@@ -122,7 +124,10 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
     const int ln = TIGHT ? la_opaque(lane) : lane, lr = ln & 31, hr = ln >> 5;
     f32x16 dp = f32x16{};
 #pragma unroll
-    for (int kk = 0; kk < VS; ++kk) dp = LOp<E>::mma(la_frag<E, DV>(vimg, 32 * ks + lr, 2 * kk + hr), df[kk], dp);
+    for (int kk = 0; kk < VS; ++kk) {
+      dp = LOp<E>::mma(la_frag<E, DV>(vimg, 32 * ks + lr, 2 * kk + hr), df[kk], dp);
+      if (TIGHT && kk % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+    }
 #pragma unroll
     for (int m = 0; m < MAPS; ++m) {
       f32x16 s = f32x16{};
@@ -130,7 +135,7 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
       for (int kk = 0; kk < KS; ++kk) s = LOp<E>::mma(la_frag<E, DK>(kimg + m * KIMG, 32 * ks + lr, 2 * kk + hr), qf[m][kk], s);
       const int dmin = j0 - (q0 + 31), dmax = j0 + 31 - q0;
       if (BIAS && dmin < D && dmax > -D) {
-        const float* bt = btab + (j0 - q0 - lq + 4 * hw + D + LA_PAD);
+        const float* bt = btab + (j0 - q0 - lr + 4 * hr + D + LA_PAD);
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, bt[8 * (r >> 2) + (r & 3)]) - lse[m];
       } else {
@@ -139,25 +144,24 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
         for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, bc);
       }
       if ((j0 + 32 > kend || (p.causal && j0 + 31 > q0))) {
-        const int jend = min(klen, p.causal ? q0 + lq + 1 : klen) - j0 - 4 * hw;
+        const int jend = min(klen, p.causal ? q0 + lr + 1 : klen) - j0 - 4 * hr;
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = 8 * (r >> 2) + (r & 3) < jend ? s[r] : -INFINITY;
       }
-      float e0 = 0.f, e1 = 0.f;
+      float e = 0.f;
 #pragma unroll
-      for (int r = 0; r < 16; r += 2) {
+      for (int r = 0; r < 16; ++r) {
         s[r] = la_exp2(s[r]) * (dp[r] - Dm[m]);
-        s[r + 1] = la_exp2(s[r + 1]) * (dp[r + 1] - Dm[m]);
-        e0 += s[r];
-        e1 += s[r + 1];
+        e += s[r];
       }
-      eps[m] += e0 + e1;
+      eps[m] += e;
 #pragma unroll
       for (int st = 0; st < PS; ++st) {
         const uint4 f = la_pack<E>(s, st);
 #pragma unroll
         for (int n = 0; n < NT; ++n) acc[m][n] = LOp<E>::mma(la_tfrag<E, DK>(kimg + m * KIMG, 32 * ks, st, n, ln), f, acc[m][n]);
       }
+      if (TIGHT) __builtin_amdgcn_sched_barrier(0);
     }
   };
 
@@ -312,8 +316,9 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
   float* const hist = btab + ((dist_n + 3) & ~3);  // [2 W][dist_n]
   float* const myhist = hist + 2 * wave * dist_n;
 
-  const int t = xcd_remap(blockIdx.x, gridDim.x);
-  const int kt = t % p.nkt, bh = t / p.nkt, hk = bh % p.Hk, b = bh / p.Hk, G = p.H / p.Hk;
+  int kt, bh;
+  la_block(p.nkt, p.B * p.Hk, kt, bh);
+  const int hk = bh % p.Hk, b = bh / p.Hk, G = p.H / p.Hk;
   const int klen = la_klen(p, b), qlen = la_qlen(p, b), qs = la_qstart(p, b);
   constexpr int OWN = FEW ? LA_OWN : LA_OWN * LA_WAVES;
   const int jb = kt * OWN, j0 = jb + (FEW ? 0 : wave * LA_OWN), jk = j0 + lk;
@@ -405,7 +410,7 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
 
   // one 32 x 32 patch
   auto patch = [&](const E* qimg, const E* oimg, const float* stat, int sub, int q0) __attribute__((always_inline)) {
-    const int ln = F32 || FEW ? la_opaque(lane) : lane, lr = ln & 31, hr = ln >> 5;
+    const int ln = F32 || FEW || (MAPS == 2 && DK == 32) ? la_opaque(lane) : lane, lr = ln & 31, hr = ln >> 5;
     const float* st0 = stat + 32 * sub + 4 * hr;  // [m][lse, D][ROWS]; b128 broadcasts: a half wave's rows are the same in all its lanes
     f32x16 dp = f32x16{}, s[MAPS], hsum;
 #pragma unroll

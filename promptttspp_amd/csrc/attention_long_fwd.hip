@@ -76,8 +76,10 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 ? 1 : 2) void attn_long_fwd_ker
   float* const btab = reinterpret_cast<float*>(smem + 2 * BUF * sizeof(E));
   const int lane = threadIdx.x & 63, wave = la_wave(), lq = lane & 31, hw = lane >> 5;
 
-  const int t = xcd_remap(blockIdx.x, gridDim.x);
-  const int qt = t % p.nqt, bh = t / p.nqt, h = bh % p.H, b = bh / p.H, hk = h / (p.H / p.Hk);
+  int qt, bh;
+  la_block(p.nqt, p.B * p.H, qt, bh);
+  if (p.causal) qt = p.nqt - 1 - qt;  // (the longest rows first)
+  const int h = bh % p.H, b = bh / p.H, hk = h / (p.H / p.Hk);
   const int klen = la_klen(p, b), qlen = la_qlen(p, b), qs = la_qstart(p, b);
   const int ib = qt * (LA_OWN * LA_WAVES), i0 = ib + wave * LA_OWN, iq = i0 + lq;
   const int dv = MAPS * p.dk;
@@ -429,12 +431,14 @@ __global__ __launch_bounds__((LSplit<E, DK, DV, MAPS>::W * 64), sizeof(E) == 4 |
   }
 }
 
+// columns of a block that the join has to look at: its queries (with statistics also the rows that pad them)
+__host__ __device__ __forceinline__ int join_cols(const LongP& p) { return p.nh > 1 ? p.nh * p.Tq : p.nrb > 1 || p.lse ? 32 : min(p.Tq, 32); }
 // join of the key ranges: one wave per (block, column)
 template <typename E, int DV, int MAPS>
 __global__ __launch_bounds__(256) void attn_long_join_kernel(const LongP p, int ncol) {
   const int lane = threadIdx.x & 63;
   const int64_t w = (int64_t)blockIdx.x * LA_WAVES + la_wave();
-  const int G = p.H / p.Hk, cols = p.nh > 1 ? p.nh * p.Tq : 32;
+  const int G = p.H / p.Hk, cols = join_cols(p);
   if (w >= (int64_t)ncol) return;
   const int tl = (int)(w / cols), lq = (int)(w % cols);
   const int rb = tl % p.nrb, hg = (tl / p.nrb) % (G / p.nh), bk = tl / (p.nrb * (G / p.nh));
@@ -538,7 +542,7 @@ int launch_fwd(const LongP& p, hipStream_t st) {
   else if constexpr (MAPS == 2) hipLaunchKernelGGL((attn_long_split_kernel<E, DK, DV, MAPS, false>), g, t, sm, st, p);
   PTPP_CHECK_LAUNCH("attention_long_fwd (few rows)");
   if (p.splits > 1) {
-    const int ncol = blocks * (p.nh > 1 ? p.nh * p.Tq : 32);
+    const int ncol = blocks * join_cols(p);
     hipLaunchKernelGGL((attn_long_join_kernel<E, DV, MAPS>), dim3((ncol + LA_WAVES - 1) / LA_WAVES), dim3(256), 0, st, p, ncol);
     PTPP_CHECK_LAUNCH("attention_long_fwd (join)");
   }
