@@ -230,8 +230,10 @@ struct LTile {
 template <typename E, int DK, int DV, int MAPS>
 struct LSplit {
   static constexpr int STAGE = 32 * (MAPS * DK + DV);                     // elements of a chunk's images
-  static constexpr int W = STAGE * (int)sizeof(E) > 16384 ? 2 : LA_WAVES;  // (f32, wide heads: 32 KB per chunk)
-  static constexpr int LDS = 2 * W * STAGE * (int)sizeof(E);
+  // (f32, wide heads: 32 KB per chunk.  One buffer and four waves: four SIMDs' matrix units against the fetch that two waves with two
+  // buffers would hide -- 64 x 64 k multiply-adds per lane of a 16th-rate instruction outweigh it)
+  static constexpr int W = LA_WAVES, NB = STAGE * (int)sizeof(E) > 16384 ? 1 : 2;
+  static constexpr int LDS = NB * W * STAGE * (int)sizeof(E);
 };
 
 // every wave's LDS reads are done and every wave is here (the DMA queue is counted separately: glds_wait)

@@ -20,12 +20,13 @@ struct LBwd {
   static constexpr int ROWS = FEW ? 32 : LA_TILE;  // streamed rows of a buffer
   static constexpr int LOADERS = FEW ? 1 : LA_WAVES;
   static constexpr int PATCHES = ROWS / 32;
+  static constexpr int NB = FEW ? LSplit<E, DK, DV, MAPS>::NB : 2;
 };
 
 template <typename E, int DK, int DV, int MAPS, bool BIAS, bool FEW>
 __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 4 ? 1 : 2) void attn_long_dq_kernel(const LongP p) {
   typedef LBwd<E, DK, DV, MAPS, FEW> X;
-  constexpr int W = X::W, ROWS = X::ROWS;
+  constexpr int W = X::W, ROWS = X::ROWS, NB = X::NB;
   constexpr int CH = LOp<E>::CH, KS = DK / (2 * CH), VS = DV / (2 * CH), PS = 16 / CH, NT = DK / 32;
   constexpr bool TIGHT = sizeof(E) == 4 || MAPS * DV == 256 || FEW;  // registers are short: LDS addresses not kept across patches
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -33,8 +34,8 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
   __shared__ float weps[W][MAPS][32];
   constexpr int KIMG = ROWS * DK, VIMG = ROWS * DV, BUF = MAPS * KIMG + VIMG;
   const int lane = threadIdx.x & 63, wave = la_wave(), lq = lane & 31, hw = lane >> 5;
-  E* const img = reinterpret_cast<E*>(smem) + (FEW ? wave * 2 * BUF : 0);
-  float* const btab = reinterpret_cast<float*>(smem + (FEW ? W : 1) * 2 * BUF * sizeof(E));
+  E* const img = reinterpret_cast<E*>(smem) + (FEW ? wave * NB * BUF : 0);
+  float* const btab = reinterpret_cast<float*>(smem + (FEW ? W : 1) * NB * BUF * sizeof(E));
 
   int qt, bh;
   la_block(p.nqt, p.B * p.H, qt, bh);
@@ -67,7 +68,7 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
   };
   const int first = FEW ? wave : 0;
   constexpr int STEP = FEW ? W : 1;
-  if (first < nt) issue(first, 0);
+  if (NB == 2 && first < nt) issue(first, 0);
   if constexpr (BIAS) la_fill_btab(p, btab, h);
   float lam = 0.f;
   if constexpr (MAPS == 2) lam = la_lambda(p, h, lane);
@@ -166,9 +167,12 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
   };
 
   if constexpr (FEW && BIAS) la_barrier();  // (the table; the loop itself has no barrier)
-  for (int tile = first, buf = 0; tile < nt; tile += STEP, buf ^= 1) {
-    if (tile + STEP < nt) {
-      if constexpr (FEW) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the buffer's last reads are done
+  for (int tile = first, buf = 0; tile < nt; tile += STEP, buf ^= NB - 1) {
+    if constexpr (FEW) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the next buffer's last reads are done
+    if (NB == 1) {
+      issue(tile, 0);
+      glds_wait<0>();
+    } else if (tile + STEP < nt) {
       issue(tile + STEP, buf ^ 1);
       glds_wait<NDMA>();
     } else {
@@ -193,7 +197,7 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
 #pragma unroll
         for (int r = 0; r < 16; ++r) mine[(n * 16 + r) * 64] = acc[m][n][r];
     }
-    static_assert(MAPS * NT * 1024 * 4 <= 2 * BUF * (int)sizeof(E), "a wave's sums fit its buffers");
+    static_assert(MAPS * NT * 1024 * 4 <= NB * BUF * (int)sizeof(E), "a wave's sums fit its buffers");
     la_barrier();
 #pragma unroll
     for (int m = 0; m < MAPS; ++m)
@@ -232,7 +236,7 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
       for (int e = 0; e < 4; ++e) {
         v[e] = 0.f;
 #pragma unroll
-        for (int w = 0; w < W; ++w) v[e] += all[w * (2 * BUF * (int)sizeof(E) / 4) + (4 * g + e) * 64];
+        for (int w = 0; w < W; ++w) v[e] += all[w * (NB * BUF * (int)sizeof(E) / 4) + (4 * g + e) * 64];
       }
       if (ch < p.dk) la_store4<E>(qo + m * p.dk + ch, v[0] * c, v[1] * c, v[2] * c, v[3] * c);
     }
@@ -301,11 +305,11 @@ __device__ __forceinline__ bool la_bucket_range(const LongP& p, int bk, int& lo,
 template <typename E, int DK, int DV, int MAPS, bool BIAS, bool FEW>
 __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 4 || MAPS * DK == 128 ? 1 : 2) void attn_long_dkv_kernel(const LongP p) {
   typedef LBwd<E, DK, DV, MAPS, FEW> X;
-  constexpr int W = X::W, ROWS = X::ROWS;
+  constexpr int W = X::W, ROWS = X::ROWS, NB = X::NB;
   constexpr int CH = LOp<E>::CH, KS = DK / (2 * CH), VS = DV / (2 * CH), PS = 16 / CH, NK = DK / 32, NV = DV / 32;
   constexpr bool AHEAD = sizeof(E) == 2 && !(MAPS == 2 && DK == 32);  // (as registers allow)
   constexpr bool F32 = sizeof(E) == 4;  // (its fragments fill the register file: the scheduler must not fetch further ahead)
-  constexpr int NBUF = sizeof(E) == 4 && !FEW ? 1 : 2;  // (f32 tiles twice and the widest distance array would pass 160 KiB)
+  constexpr int NBUF = FEW ? NB : sizeof(E) == 4 ? 1 : 2;  // (f32 tiles twice and the widest distance array would pass 160 KiB)
   extern __shared__ __attribute__((aligned(16))) char smem[];
   constexpr int QIMG = ROWS * DK, OIMG = ROWS * DV;
   constexpr int BUFB = (MAPS * QIMG + OIMG) * (int)sizeof(E) + 1024;  // + (lse, D) of every map, ROWS floats each
@@ -539,17 +543,17 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
     }
     if constexpr (MAPS == 2) lam = la_lambda(p, h, lane);
     if constexpr (FEW) {
-      if (wave < ntq) issue(g * ntq + wave, 0);
+      if (NBUF == 2 && wave < ntq) issue(g * ntq + wave, 0);
       if constexpr (BIAS) la_barrier();  // (the table and the cleared sums; the loop itself has no barrier)
     }
     constexpr int STEP = FEW ? W : 1;
-    for (int iq = FEW ? wave : 0, fb = 0; iq < ntq; iq += STEP, fb ^= 1) {
+    for (int iq = FEW ? wave : 0, fb = 0; iq < ntq; iq += STEP, fb ^= NBUF - 1) {
       const int it = g * ntq + iq, buf = FEW ? fb : NBUF == 2 ? it & 1 : 0;
+      if constexpr (FEW) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the next buffer's last reads are done
       if (NBUF == 1) {
         issue(it, 0);
         glds_wait<0>();
       } else if (FEW ? iq + STEP < ntq : it + 1 < total) {
-        if constexpr (FEW) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the buffer's last reads are done
         issue(it + STEP, buf ^ 1);
         glds_wait<NDMA>();
       } else {
@@ -685,13 +689,14 @@ __global__ __launch_bounds__(256) void attn_long_fin_kernel(const LongP p, float
 constexpr size_t LDS_MAX = 160 * 1024;
 template <typename E, int DK, int DV, int MAPS>
 size_t lds_dq(bool few, int dn) {
-  return 2 * (few ? LSplit<E, DK, DV, MAPS>::W * 32 : LA_TILE) * (size_t)(MAPS * DK + DV) * sizeof(E) + ((dn + 3) & ~3) * sizeof(float);
+  typedef LSplit<E, DK, DV, MAPS> S_;
+  return (few ? S_::NB * S_::W * 32 : 2 * LA_TILE) * (size_t)(MAPS * DK + DV) * sizeof(E) + ((dn + 3) & ~3) * sizeof(float);
 }
 template <typename E, int DK, int DV, int MAPS>
 size_t lds_dkv(bool few, int dn) {
   const int W = few ? LSplit<E, DK, DV, MAPS>::W : LA_WAVES;
   const size_t buf = (few ? 32 : LA_TILE) * (size_t)(MAPS * DK + DV) * sizeof(E) + 1024;
-  return (few ? 2 * W : sizeof(E) == 4 ? 1 : 2) * buf + (((dn + 3) & ~3) + 2 * W * (size_t)dn) * sizeof(float);
+  return (few ? LSplit<E, DK, DV, MAPS>::NB * W : sizeof(E) == 4 ? 1 : 2) * buf + (((dn + 3) & ~3) + 2 * W * (size_t)dn) * sizeof(float);
 }
 // chooses the launch shape and sets the row-block counts
 template <typename E, int DK, int DV, int MAPS>

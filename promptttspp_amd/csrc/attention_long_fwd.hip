@@ -235,14 +235,14 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 ? 1 : 2) void attn_long_fwd_ker
 template <typename E, int DK, int DV, int MAPS, bool BIAS>
 __global__ __launch_bounds__((LSplit<E, DK, DV, MAPS>::W * 64), sizeof(E) == 4 || MAPS * DV == 256 ? 1 : 2) void attn_long_split_kernel(const LongP p) {
   typedef LSplit<E, DK, DV, MAPS> S_;
-  constexpr int W = S_::W, STAGE = S_::STAGE, KIMG = 32 * DK;
+  constexpr int W = S_::W, NB = S_::NB, STAGE = S_::STAGE, KIMG = 32 * DK;
   constexpr bool TIGHT = sizeof(E) == 4 || MAPS * DV == 256;
   constexpr int CH = LOp<E>::CH, KS = DK / (2 * CH), PS = 16 / CH, NT = DV / 32;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ float wml[W][MAPS][2][32];
   const int lane = threadIdx.x & 63, wave = la_wave(), lq = lane & 31, hw = lane >> 5;
   float* const btab = reinterpret_cast<float*>(smem + S_::LDS);
-  E* const img = reinterpret_cast<E*>(smem) + wave * 2 * STAGE;
+  E* const img = reinterpret_cast<E*>(smem) + wave * NB * STAGE;
 
   // block -> (range, utterance, key head, head group, row block); ranges of one key head run on the same XCD
   const int t = xcd_remap(blockIdx.x, gridDim.x);
@@ -267,16 +267,20 @@ __global__ __launch_bounds__((LSplit<E, DK, DV, MAPS>::W * 64), sizeof(E) == 4 |
   LTile<E, DV, 32, 1> vt;
   kt.init(p.ldk, p.dk, lane, 0);
   vt.init(p.ldv, dv, lane, 0);
-  constexpr int NDMA = MAPS * LTile<E, DK, 32, 1>::NI + LTile<E, DV, 32, 1>::NI;
-  auto issue = [&](int c, int buf) {
-    const int j0 = 32 * c;
-    E* d = img + buf * STAGE;
+  constexpr int NK = MAPS * LTile<E, DK, 32, 1>::NI, NV = LTile<E, DV, 32, 1>::NI;
+  auto issue_k = [&](int c, int buf) {
 #pragma unroll
-    for (int m = 0; m < MAPS; ++m) kt.issue(kb + (int64_t)j0 * p.ldk + m * p.dk, kend - j0, d + m * KIMG, lane, 0);
-    vt.issue(vb + (int64_t)j0 * p.ldv, kend - j0, d + MAPS * KIMG, lane, 0);
+    for (int m = 0; m < MAPS; ++m)
+      kt.issue(kb + (int64_t)(32 * c) * p.ldk + m * p.dk, kend - 32 * c, img + buf * STAGE + m * KIMG, lane, 0);
   };
+  auto issue_v = [&](int c, int buf) { vt.issue(vb + (int64_t)(32 * c) * p.ldv, kend - 32 * c, img + buf * STAGE + MAPS * KIMG, lane, 0); };
   int c = c0 + wave;
-  if (c < c1) issue(c, 0);
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (NB == 2 && c + i * W < c1) {
+      issue_k(c + i * W, i);
+      issue_v(c + i * W, i);
+    }
   const int dist_n = la_btab_len(p);
   if constexpr (BIAS)
     for (int n = 0; n < p.nh; ++n) la_fill_btab(p, btab + n * dist_n, h0 + n);
@@ -305,36 +309,53 @@ __global__ __launch_bounds__((LSplit<E, DK, DV, MAPS>::W * 64), sizeof(E) == 4 |
   const int D = p.max_distance, qp = qs + min(iq, ihi);  // (a column without a query reads the table within bounds)
   if constexpr (BIAS) la_barrier();
 
-  for (int buf = 0; c < c1; c += W, buf ^= 1) {
-    if (c + W < c1) {
+  // Two chunks are on their way ahead of the one in hand: the keys' half of a buffer is refilled as soon as the scores are computed, the
+  // values' half after the second product.  The waits count what was asked for later (in order: V, K', V', K'').
+  for (int buf = 0; c < c1; c += W, buf ^= NB - 1) {
+    const bool one = c + W < c1, two = c + 2 * W < c1;
+    if (NB == 1) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the buffer's last reads are done
-      issue(c + W, buf ^ 1);
-      glds_wait<NDMA>();
+      issue_k(c, 0);
+      issue_v(c, 0);
+      glds_wait<NV>();
+    } else if (one) {
+      glds_wait<NK + 2 * NV>();
     } else {
-      glds_wait<0>();
+      glds_wait<NV>();
     }
     const E* kimg = img + buf * STAGE;
     const E* vimg = kimg + MAPS * KIMG;
     const int j0 = 32 * c;
     const int ln = TIGHT ? la_opaque(lane) : lane, lr = ln & 31, hr = ln >> 5;
     uint4 pf[MAPS][PS];
+    f32x16 s[MAPS];
 #pragma unroll
     for (int m = 0; m < MAPS; ++m) {
-      f32x16 s = f32x16{};
+      s[m] = f32x16{};
 #pragma unroll
       for (int kk = 0; kk < KS; ++kk) {
-        s = LOp<E>::mma(la_frag<E, DK>(kimg + m * KIMG, lr, 2 * kk + hr), qf[m][kk], s);
+        s[m] = LOp<E>::mma(la_frag<E, DK>(kimg + m * KIMG, lr, 2 * kk + hr), qf[m][kk], s[m]);
         if (TIGHT && kk % 4 == 3) __builtin_amdgcn_sched_barrier(0);
       }
+    }
+    if (NB == 2 && two) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the keys' last reads are done
+      issue_k(c + 2 * W, buf);
+    }
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m) {
       float mul, add;
       const float* bt0 = btab + hcol * dist_n;
-      la_scores<BIAS>(s, c2, bt0 + (j0 - qp + 4 * hw + D + LA_PAD), bt0, D, j0 - (qs + ihi), j0 + 31 - (qs + ilo), mul, add);
-      if (j0 + 32 > kend || (p.causal && j0 + 31 > qs + ilo)) la_mask(s, min(klen, p.causal ? qp + 1 : klen) - j0 - 4 * hw);
-      la_raise<NT>(mx[m], l[m], o[m], la_half_max(fmaf(la_max16(s), mul, add)));
-      l[m] += la_probs(s, mul, add - mx[m]);
+      la_scores<BIAS>(s[m], c2, bt0 + (j0 - qp + 4 * hw + D + LA_PAD), bt0, D, j0 - (qs + ihi), j0 + 31 - (qs + ilo), mul, add);
+      if (j0 + 32 > kend || (p.causal && j0 + 31 > qs + ilo)) la_mask(s[m], min(klen, p.causal ? qp + 1 : klen) - j0 - 4 * hw);
+      la_raise<NT>(mx[m], l[m], o[m], la_half_max(fmaf(la_max16(s[m]), mul, add)));
+      l[m] += la_probs(s[m], mul, add - mx[m]);
 #pragma unroll
-      for (int st = 0; st < PS; ++st) pf[m][st] = la_pack<E>(s, st);
+      for (int st = 0; st < PS; ++st) pf[m][st] = la_pack<E>(s[m], st);
     }
+    if (NB == 2 && two) glds_wait<2 * NK + NV>();
+    else if (NB == 2 && one) glds_wait<NK + NV>();
+    else glds_wait<0>();
 #pragma unroll
     for (int st = 0; st < PS; ++st)
 #pragma unroll
@@ -344,6 +365,10 @@ __global__ __launch_bounds__((LSplit<E, DK, DV, MAPS>::W * 64), sizeof(E) == 4 |
         for (int m = 0; m < MAPS; ++m) o[m][n] = LOp<E>::mma(vf, pf[m][st], o[m][n]);
         if (TIGHT) __builtin_amdgcn_sched_barrier(0);
       }
+    if (NB == 2 && two) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the values' last reads are done
+      issue_v(c + 2 * W, buf);
+    }
   }
 
   // ---- join the waves: common maximum, then each wave's sums through its own buffers ----
@@ -372,7 +397,7 @@ __global__ __launch_bounds__((LSplit<E, DK, DV, MAPS>::W * 64), sizeof(E) == 4 |
 #pragma unroll
       for (int r = 0; r < 16; ++r) mine[(n * 16 + r) * 64] = o[m][n][r] * al;
   }
-  static_assert(MAPS * NT * 1024 * 4 <= 2 * STAGE * (int)sizeof(E), "a wave's sums fit its buffers");
+  static_assert(MAPS * NT * 1024 * 4 <= NB * STAGE * (int)sizeof(E), "a wave's sums fit its buffers");
   la_barrier();
   const bool row = iq < p.Tq;
   float lam = 0.f;
@@ -404,7 +429,7 @@ __global__ __launch_bounds__((LSplit<E, DK, DV, MAPS>::W * 64), sizeof(E) == 4 |
       for (int e = 0; e < 4; ++e) {
         v[m][e] = 0.f;
 #pragma unroll
-        for (int w = 0; w < W; ++w) v[m][e] += all[w * (2 * STAGE * (int)sizeof(E) / 4) + (m * NT * 16 + ng * 4 + e) * 64];
+        for (int w = 0; w < W; ++w) v[m][e] += all[w * (NB * STAGE * (int)sizeof(E) / 4) + (m * NT * 16 + ng * 4 + e) * 64];
       }
     if (!row || ch >= dv) continue;
     if (p.splits > 1) {
@@ -492,10 +517,10 @@ __global__ __launch_bounds__(256) void attn_long_join_kernel(const LongP p, int 
 }
 
 // The rule: blocks of 128 rows, unless there are at most 32 rows, or blocks of 32 make at most 256 (one round of the chip); then as many
-// key ranges as bring the grid to about 512 blocks of four waves (two per CU) at no fewer than two 32-key chunks per wave.
+// key ranges as fill the chip once -- one or two blocks per CU, as their buffers fit -- at no fewer than two 32-key chunks per wave.
 bool few_rows(const LongP& p) { return p.Tq <= 32 || (int64_t)((p.Tq + 31) / 32) * p.B * p.H <= 256; }
 // fills nh, nrb, splits; returns the number of 32-column blocks (0: too many to number)
-int plan_few(LongP& p, int waves) {
+int plan_few(LongP& p, int lds) {
   const int G = p.H / p.Hk;
   p.nh = 1;
   if (!p.lse)  // (backward's statistics are padded to whole blocks of one head's rows)
@@ -503,20 +528,18 @@ int plan_few(LongP& p, int waves) {
       if (G % n == 0 && (!p.table || n * (2 * (p.max_distance + LA_PAD) + 1) <= 6144)) p.nh = n;  // (24 KB of bias tables)
   p.nrb = p.nh > 1 ? 1 : (p.lse ? p.TqP : p.Tq + 31) / 32;
   const int64_t blocks = (int64_t)p.B * p.Hk * (G / p.nh) * p.nrb;
-  const int64_t most = ((int64_t)p.Tk + 64 * waves - 1) / (64 * waves);
-  int64_t s = blocks ? 512 / blocks : 1;
+  const int64_t most = ((int64_t)p.Tk + 64 * LA_WAVES - 1) / (64 * LA_WAVES);
+  int64_t s = blocks ? (lds > 72 * 1024 ? 256 : 512) / blocks : 1;  // (72 KB: two blocks per CU with their tables and statistics)
   if (s > most) s = most;
   p.splits = s < 1 ? 1 : s > 64 ? 64 : (int)s;
   return blocks * p.splits < (1ll << 31) ? (int)blocks : 0;
 }
 template <typename E>
-int few_waves(int maps, int dk) {
-  if (maps == 1) return dk <= 64 ? LSplit<E, 64, 64, 1>::W : LSplit<E, 128, 128, 1>::W;
-  return dk <= 32 ? LSplit<E, 32, 64, 2>::W : LSplit<E, 64, 128, 2>::W;
+int few_lds(int maps, int dk) {
+  if (maps == 1) return dk <= 64 ? LSplit<E, 64, 64, 1>::LDS : LSplit<E, 128, 128, 1>::LDS;
+  return dk <= 32 ? LSplit<E, 32, 64, 2>::LDS : LSplit<E, 64, 128, 2>::LDS;
 }
-int few_waves(int dtype, int maps, int dk) {
-  return dtype == PTPP_F32 ? few_waves<float>(maps, dk) : dtype == PTPP_BF16 ? few_waves<bf16_raw>(maps, dk) : few_waves<f16_raw>(maps, dk);
-}
+int few_lds(int dtype, int maps, int dk) { return dtype == PTPP_F32 ? few_lds<float>(maps, dk) : few_lds<bf16_raw>(maps, dk); }  // (f16 as bf16)
 int pad_dv(int maps, int dk) { return maps == 1 ? (dk <= 64 ? 64 : 128) : (dk <= 32 ? 64 : 128); }
 
 template <typename E, int DK, int DV, int MAPS>
@@ -558,7 +581,7 @@ int dispatch_fwd(const LongP& p, int maps, hipStream_t st) {
 int64_t plan_fwd(LongP& p, const ptpp_attention_long_args* a, int64_t* o_ml, const char* who) {
   *o_ml = 0;
   if (!few_rows(p)) return 0;
-  const int blocks = plan_few(p, few_waves(a->dtype, a->maps, a->dk));
+  const int blocks = plan_few(p, few_lds(a->dtype, a->maps, a->dk));
   if (!blocks) {
     ptpp_set_error("%s: too many tiles", who);
     return -1;
