@@ -236,6 +236,16 @@ struct LSplit {
   static constexpr int LDS = NB * W * STAGE * (int)sizeof(E);
 };
 
+// Blocks use up to 158 KB of dynamic LDS beside at most 2 KB of named arrays.  The limit is raised once per kernel and device: the runtime's
+// call costs the host as much as a launch.
+constexpr int LA_LDS = 158 * 1024;
+inline bool la_lds_limit(const void* kern, size_t bytes, const char* who) {
+  if (bytes <= 64 * 1024 || lds_limit_raised(kern)) return true;
+  if (!ptpp_lds_limit(kern, LA_LDS, who)) return false;
+  lds_limit_mark(kern);
+  return true;
+}
+
 // every wave's LDS reads are done and every wave is here (the DMA queue is counted separately: glds_wait)
 __device__ __forceinline__ void la_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 

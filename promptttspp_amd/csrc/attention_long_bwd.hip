@@ -686,7 +686,6 @@ __global__ __launch_bounds__(256) void attn_long_fin_kernel(const LongP p, float
 
 // The rule (as in forward): blocks of 32 rows where that gives at most 256 of them (one round of the chip), else of 128 -- also where the
 // few-row form's buffers and the distance sums of a wide table do not fit LDS together.
-constexpr size_t LDS_MAX = 160 * 1024;
 template <typename E, int DK, int DV, int MAPS>
 size_t lds_dq(bool few, int dn) {
   typedef LSplit<E, DK, DV, MAPS> S_;
@@ -703,7 +702,7 @@ template <typename E, int DK, int DV, int MAPS>
 void plan_bwd(LongP& p) {
   const int dn = p.table ? 2 * (p.max_distance + LA_PAD) + 1 : 0;
   p.few_q = (int64_t)(p.TqP / 32) * p.B * p.H <= 256;
-  p.few_k = (int64_t)((p.Tk + 31) / 32) * p.B * p.Hk <= 256 && lds_dkv<E, DK, DV, MAPS>(true, dn) + 1024 <= LDS_MAX;
+  p.few_k = (int64_t)((p.Tk + 31) / 32) * p.B * p.Hk <= 256 && lds_dkv<E, DK, DV, MAPS>(true, dn) <= LA_LDS;
   if (p.few_q) p.nqt = p.TqP / 32;  // (D is written up to the padding of its rows)
   if (p.few_k) p.nkt = (p.Tk + 31) / 32;
 }
@@ -720,7 +719,7 @@ void plan_bwd(LongP& p, int maps, int dtype) {
 
 template <typename E, int DK, int DV, int MAPS, bool BIAS, bool FEW>
 int launch_dq(const LongP& p, size_t sm, hipStream_t st) {
-  if (sm > 64 * 1024 && !ptpp_lds_limit((const void*)attn_long_dq_kernel<E, DK, DV, MAPS, BIAS, FEW>, (int)sm, "attention_long_bwd")) return PTPP_ELAUNCH;
+  if (!la_lds_limit((const void*)attn_long_dq_kernel<E, DK, DV, MAPS, BIAS, FEW>, sm, "attention_long_bwd")) return PTPP_ELAUNCH;
   hipLaunchKernelGGL((attn_long_dq_kernel<E, DK, DV, MAPS, BIAS, FEW>), dim3((unsigned)((int64_t)p.nqt * p.B * p.H)), dim3(LBwd<E, DK, DV, MAPS, FEW>::W * 64), sm,
                      st, p);
   PTPP_CHECK_LAUNCH("attention_long_bwd (dq)");
@@ -728,7 +727,7 @@ int launch_dq(const LongP& p, size_t sm, hipStream_t st) {
 }
 template <typename E, int DK, int DV, int MAPS, bool BIAS, bool FEW>
 int launch_dkv(const LongP& p, size_t sm, hipStream_t st) {
-  if (sm > 64 * 1024 && !ptpp_lds_limit((const void*)attn_long_dkv_kernel<E, DK, DV, MAPS, BIAS, FEW>, (int)sm, "attention_long_bwd")) return PTPP_ELAUNCH;
+  if (!la_lds_limit((const void*)attn_long_dkv_kernel<E, DK, DV, MAPS, BIAS, FEW>, sm, "attention_long_bwd")) return PTPP_ELAUNCH;
   hipLaunchKernelGGL((attn_long_dkv_kernel<E, DK, DV, MAPS, BIAS, FEW>), dim3((unsigned)((int64_t)p.nkt * p.B * p.Hk)), dim3(LBwd<E, DK, DV, MAPS, FEW>::W * 64),
                      sm, st, p);
   PTPP_CHECK_LAUNCH("attention_long_bwd (dk, dv)");

@@ -532,7 +532,7 @@ int plan_few(LongP& p, int lds) {
   int64_t s = blocks ? (lds > 72 * 1024 ? 256 : 512) / blocks : 1;  // (72 KB: two blocks per CU with their tables and statistics)
   if (s > most) s = most;
   p.splits = s < 1 ? 1 : s > 64 ? 64 : (int)s;
-  return blocks * p.splits < (1ll << 31) ? (int)blocks : 0;
+  return blocks * p.splits < (1ll << 24) ? (int)blocks : 0;  // (a launch holds fewer than 2^32 threads)
 }
 template <typename E>
 int few_lds(int maps, int dk) {
@@ -549,7 +549,7 @@ int launch_fwd(const LongP& p, hipStream_t st) {
     const size_t sm = 2 * (size_t)LA_TILE * (MAPS * DK + DV) * sizeof(E) + tab;
     const dim3 g((unsigned)((int64_t)p.nqt * p.B * p.H));
     const void* kern = p.table ? (const void*)attn_long_fwd_kernel<E, DK, DV, MAPS, true> : (const void*)attn_long_fwd_kernel<E, DK, DV, MAPS, MAPS == 1>;
-    if (sm > 64 * 1024 && !ptpp_lds_limit(kern, (int)sm, "attention_long_fwd")) return PTPP_ELAUNCH;
+    if (!la_lds_limit(kern, sm, "attention_long_fwd")) return PTPP_ELAUNCH;
     if (p.table) hipLaunchKernelGGL((attn_long_fwd_kernel<E, DK, DV, MAPS, true>), g, dim3(256), sm, st, p);
     else if constexpr (MAPS == 2) hipLaunchKernelGGL((attn_long_fwd_kernel<E, DK, DV, MAPS, false>), g, dim3(256), sm, st, p);
     PTPP_CHECK_LAUNCH("attention_long_fwd");
@@ -560,7 +560,7 @@ int launch_fwd(const LongP& p, hipStream_t st) {
   const int blocks = p.B * p.Hk * (p.H / p.Hk / p.nh) * p.nrb;
   const dim3 g((unsigned)(blocks * p.splits)), t(S_::W * 64);
   const void* kern = p.table ? (const void*)attn_long_split_kernel<E, DK, DV, MAPS, true> : (const void*)attn_long_split_kernel<E, DK, DV, MAPS, MAPS == 1>;
-  if (sm > 64 * 1024 && !ptpp_lds_limit(kern, (int)sm, "attention_long_fwd")) return PTPP_ELAUNCH;
+  if (!la_lds_limit(kern, sm, "attention_long_fwd")) return PTPP_ELAUNCH;
   if (p.table) hipLaunchKernelGGL((attn_long_split_kernel<E, DK, DV, MAPS, true>), g, t, sm, st, p);
   else if constexpr (MAPS == 2) hipLaunchKernelGGL((attn_long_split_kernel<E, DK, DV, MAPS, false>), g, t, sm, st, p);
   PTPP_CHECK_LAUNCH("attention_long_fwd (few rows)");
@@ -642,7 +642,8 @@ int ptpp_attention_long_params(const ptpp_attention_long_args* a, int backward, 
     }
   }
   const int64_t nqt = ((int64_t)a->Tq + 127) / 128, nkt = ((int64_t)a->Tk + 127) / 128;
-  PTPP_CHECK_ARG(nqt * a->B * a->H < (1ll << 31) && nkt * a->B * a->H < (1ll << 31), "%s: too many tiles", who);
+  // (a launch holds fewer than 2^32 threads: 2^24 blocks of 256)
+  PTPP_CHECK_ARG(nqt * a->B * a->H < (1ll << 24) && nkt * a->B * a->Hk < (1ll << 24), "%s: too many tiles", who);
   o->q = a->q; o->k = a->k; o->v = a->v; o->dout = a->dout; o->out = a->out; o->out2 = a->out2; o->dq = a->dq;
   o->gk = a->dk_out; o->gv = a->dv;
   o->table = a->table; o->lam = a->lam; o->k_lengths = a->k_lengths; o->q_lengths = a->q_lengths; o->q_start = a->q_start;

@@ -316,6 +316,7 @@ __global__ __launch_bounds__(1024) void residual_norm_fin_kernel(const RnP p, co
   const int lo = per_utt ? ub * p.chunks : 0, n = per_utt ? p.chunks : p.B * p.chunks;
   float s = 0.f;
   if (c < p.C)
+#pragma unroll 8
     for (int i = r; i < n; i += 32) s += p.part[((int64_t)(lo + i) * p.nslots + p.slot[k]) * p.C + c];
   red[r][cl] = s;
   __syncthreads();
@@ -333,7 +334,7 @@ int check(const ptpp_residual_norm_args* a, int backward, RnP* p, const char* wh
   PTPP_CHECK_ARG(a->dtype == PTPP_F32 || a->dtype == PTPP_BF16 || a->dtype == PTPP_F16, "%s: bad dtype %d", who, a->dtype);
   PTPP_CHECK_ARG(a->B > 0 && a->T > 0 && a->C > 0 && a->C % 4 == 0 && a->C <= 4096, "%s: bad shape (B %d, T %d, C %d: a multiple of 4, at most 4096)",
                  who, a->B, a->T, a->C);
-  PTPP_CHECK_ARG((int64_t)a->B * a->T < (1ll << 31), "%s: too many rows", who);
+  PTPP_CHECK_ARG((int64_t)a->B * a->T < (1ll << 28), "%s: too many rows", who);
   PTPP_CHECK_ARG(a->f && (backward || a->y), "%s: null tensor", who);
   PTPP_CHECK_ARG(backward || !a->pre_g == !a->z, "%s: z and the pre norm come together", who);
   PTPP_CHECK_ARG(!a->gate || a->gate_rows == 1 || a->gate_rows == a->B, "%s: a gate of %d rows (1 or %d)", who, a->gate_rows, a->B);
@@ -358,7 +359,6 @@ int check(const ptpp_residual_norm_args* a, int backward, RnP* p, const char* wh
     rpc = (rpc + 15) & ~15;
     p->rows_per_chunk = rpc;
     p->chunks = (a->T + rpc - 1) / rpc;
-    PTPP_CHECK_ARG((int64_t)p->chunks * a->B < (1ll << 31), "%s: too many rows", who);
     const float* want_p[] = {a->dpre_g, a->dpre_b, a->dpost_g, a->dpost_b, a->dgate};
     const float* have_p[] = {a->pre_g, a->pre_b, a->post_g, a->post_b, a->gate};
     for (int k = 0; k < 5; ++k) {
@@ -372,13 +372,14 @@ int check(const ptpp_residual_norm_args* a, int backward, RnP* p, const char* wh
 template <typename E, int NT, int LPR, int NV>
 int launch(const RnP& p, bool bwd, hipStream_t st) {
   constexpr int RPB = NT / LPR;
-  const int64_t rows = (int64_t)p.B * p.T;
+  const int64_t rows = (int64_t)p.B * p.T, blocks = bwd ? (int64_t)p.B * p.chunks : (rows + RPB - 1) / RPB;
+  PTPP_CHECK_ARG(blocks * NT < (1ll << 32), "residual_norm: too many rows");
   if (!bwd) {
-    hipLaunchKernelGGL((residual_norm_fwd_kernel<E, NT, LPR, NV>), dim3((unsigned)((rows + RPB - 1) / RPB)), dim3(NT), 0, st, p);
+    hipLaunchKernelGGL((residual_norm_fwd_kernel<E, NT, LPR, NV>), dim3((unsigned)blocks), dim3(NT), 0, st, p);
     PTPP_CHECK_LAUNCH("residual_norm_fwd");
   } else {
     const size_t sm = RPB > 1 ? (size_t)RPB * p.C * sizeof(float) : 0;
-    hipLaunchKernelGGL((residual_norm_bwd_kernel<E, NT, LPR, NV>), dim3((unsigned)(p.B * p.chunks)), dim3(NT), sm, st, p);
+    hipLaunchKernelGGL((residual_norm_bwd_kernel<E, NT, LPR, NV>), dim3((unsigned)blocks), dim3(NT), sm, st, p);
     PTPP_CHECK_LAUNCH("residual_norm_bwd");
   }
   return PTPP_OK;
@@ -425,12 +426,12 @@ extern "C" int ptpp_residual_norm_bwd(const ptpp_residual_norm_args* a, void* st
   PTPP_CHECK_ARG(!need || (a->ws && (uintptr_t)a->ws % 16 == 0 && (int64_t)a->ws_bytes >= need), "residual_norm_bwd: workspace of %zu bytes, needs %lld (16-byte aligned)",
                  a->ws_bytes, (long long)need);
   p.part = reinterpret_cast<float*>(a->ws);
+  const int ny = p.nslots - (p.slot[4] >= 0 ? 1 : 0) + (p.slot[4] >= 0 ? p.gate_rows : 0);
+  PTPP_CHECK_ARG(ny <= 65535, "residual_norm_bwd: a gate of %d rows", p.gate_rows);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const int r = run(p, true, a->dtype, st);
   if (r != PTPP_OK || !p.nslots) return r;
   const RnDst d = {{a->dpre_g, a->dpre_b, a->dpost_g, a->dpost_b, a->dgate}};
-  const int ny = p.nslots - (p.slot[4] >= 0 ? 1 : 0) + (p.slot[4] >= 0 ? p.gate_rows : 0);
-  PTPP_CHECK_ARG(ny <= 65535, "residual_norm_bwd: a gate of %d rows", p.gate_rows);
   hipLaunchKernelGGL(residual_norm_fin_kernel, dim3((p.C + 31) / 32, ny), dim3(1024), 0, st, p, d, a->accumulate);
   PTPP_CHECK_LAUNCH("residual_norm_bwd (sums)");
   return PTPP_OK;

@@ -7,6 +7,7 @@ import ctypes
 import math
 import os
 import weakref
+from operator import index
 from types import SimpleNamespace
 
 import torch
@@ -1024,6 +1025,24 @@ def _still(args, names, tensors):
     return True
 
 
+def _number(x, what):
+    """``x`` as the plain number that the kernels take by value (a tensor in its place would lose its gradient)"""
+    if torch.is_tensor(x) and x.requires_grad:
+        raise ValueError(f"{what} is a number, not something to learn")
+    return float(x)
+
+
+def _packed(t):
+    """``t``, or a contiguous copy on its own 16-byte boundary"""
+    return t if t is None or (t.is_contiguous() and not t.data_ptr() & 15) else t.clone(memory_format=torch.contiguous_format)
+
+
+def _attention_cfg(maps, heads, kv_heads, max_distance, bidirectional, lam_init, lengths, q_lengths, q_start, causal, scale):
+    return SimpleNamespace(heads=index(heads), kv_heads=index(heads if kv_heads is None else kv_heads), maps=maps, max_distance=index(max_distance),
+                           bidirectional=bool(bidirectional), lam_init=_number(lam_init, "attention: lam_init"), lengths=lengths, q_lengths=q_lengths,
+                           q_start=q_start, causal=bool(causal), scale=None if scale is None else _number(scale, "attention: scale"))
+
+
 class AttentionLongFn(Function):
     @staticmethod
     def forward(ctx, q, k, v, table, lam, cfg):
@@ -1045,8 +1064,7 @@ class AttentionLongFn(Function):
         op = ctx.op
         if not _still(op.args, ("q", "table", "lam") if k is None else ("q", "table", "lam", "k", "v"), (q, table, lam, k, v)):
             op = _attention_long_op(q, k, v, _f32_view(table), _f32_view(lam), ctx.cfg)
-        if not dout.is_contiguous() or dout.data_ptr() % 16:
-            dout = dout.clone(memory_format=torch.contiguous_format)
+        dout = _packed(dout)
         direct = ctx.direct is not None
         dt, dl = [None if p is None else p.grad if direct else lse.new_empty(p.shape) for p in (table, lam)]
         dq, dk, dv = op.backward(q, k, v, table, lam, out, lse, out2, dout, dt, dl, accumulate=direct)
@@ -1087,11 +1105,12 @@ def attention_bucket(q, k, v, table, heads, kv_heads=None, max_distance=128, bid
     ``lengths`` (B): valid keys (None: all); ``q_lengths`` (B): valid queries, the others give zeros (None: as ``lengths`` for the fused
     form, else all); rows behind them are never read.  ``q_start`` (B): position of the first query among the keys (None: 0) -- a step
     of one query against a kept memory of n keys has ``q_start = n - 1``; ``causal``: only keys at or before the query's position.
-    A query that sees no key gives zeros.  ``scale``: positive, default dk ** -0.5.  Memory O(Tq + Tk) in both directions."""
+    A query that sees no key gives zeros; a table entry of -inf (or below -1e30) hides its keys like a mask.  Keys behind the lengths, and for
+    ``causal`` keys behind the last query, are not read in forward; a value that only ``causal`` hides from an earlier query has to be finite,
+    as has a gradient: it may still be multiplied by zero.  ``scale``: positive, default dk ** -0.5.  Memory O(Tq + Tk) in both directions."""
     if table is None:
         raise ValueError("attention_bucket: needs a position table")
-    cfg = SimpleNamespace(heads=heads, kv_heads=kv_heads or heads, maps=1, max_distance=max_distance, bidirectional=bidirectional, lam_init=0.0,
-                          lengths=lengths, q_lengths=q_lengths, q_start=q_start, causal=causal, scale=scale)
+    cfg = _attention_cfg(1, heads, kv_heads, max_distance, bidirectional, 0.0, lengths, q_lengths, q_start, causal, scale)
     return _attention_long(q, k, v, table, None, cfg)
 
 
@@ -1105,8 +1124,7 @@ def attention_diff(q, k, v, lam, lam_init, heads, kv_heads=None, table=None, max
     both maps.  Everything else as there.  The norm over a head that usually follows is ``residual_norm`` without a residual."""
     if lam is None:
         raise ValueError("attention_diff: needs the lam vectors")
-    cfg = SimpleNamespace(heads=heads, kv_heads=kv_heads or heads, maps=2, max_distance=max_distance, bidirectional=bidirectional,
-                          lam_init=lam_init, lengths=lengths, q_lengths=q_lengths, q_start=q_start, causal=causal, scale=scale)
+    cfg = _attention_cfg(2, heads, kv_heads, max_distance, bidirectional, lam_init, lengths, q_lengths, q_start, causal, scale)
     return _attention_long(q, k, v, table, lam, cfg)
 
 
@@ -1114,10 +1132,7 @@ class ResidualNormFn(Function):
     @staticmethod
     def forward(ctx, f, x, gate, post_g, post_b, pre_g, pre_b, cfg):
         ctx.set_materialize_grads(False)
-        if not f.is_contiguous():
-            f = f.contiguous()
-        if x is not None and not x.is_contiguous():
-            x = x.contiguous()
+        f, x = _packed(f), _packed(x)
         params = (gate, post_g, post_b, pre_g, pre_b)
         op = _residual_norm_op(f, x, params, cfg)
         y, z, stats = op.forward(f, True)
@@ -1138,10 +1153,7 @@ class ResidualNormFn(Function):
         op = ctx.op
         if not _still(op.args, ("f", "x", "gate", "post_g", "post_b", "pre_g", "pre_b"), (f, x, *params)):
             op = _residual_norm_op(f, x, params, ctx.cfg)
-        if dy is not None and not dy.is_contiguous():
-            dy = dy.contiguous()
-        if dz is not None and not dz.is_contiguous():
-            dz = dz.contiguous()
+        dy, dz = _packed(dy), _packed(dz)
         want = need[2:7]
         if ctx.direct is not None:
             into = [p.grad if p.dim() == 2 and p.shape[0] != 1 else p.grad.view(-1) for p in ctx.direct]
@@ -1163,9 +1175,12 @@ class ResidualNormFn(Function):
 
 def _flat(p):
     """a gate keeps its (B, C) rows; everything else is a vector, whatever unit dimensions the parameter carries"""
-    if p is None or p.dim() == 1:
-        return _f32_view(p)
-    return _f32_view(p) if p.dim() == 2 and p.shape[0] != 1 else _f32_view(p).view(-1)
+    if p is None:
+        return p
+    if p.dtype is not torch.float32 or not p.is_contiguous() or p.data_ptr() & 15:
+        p = _packed(p.detach().float())
+    n = p.dim()
+    return p if n == 1 or (n == 2 and p.shape[0] != 1) else p.view(-1)
 
 
 def _residual_norm_op(f, x, params, cfg):
@@ -1182,13 +1197,13 @@ def residual_norm(f, x=None, gate=None, post=None, pre=None, scale=1.0, eps=1e-5
     computed from the unrounded y."""
     post_g, post_b = post if post is not None else (None, None)
     pre_g, pre_b = pre if pre is not None else (None, None)
-    cfg = SimpleNamespace(scale=scale, eps=eps, kind=kind, lengths=lengths)
+    cfg = SimpleNamespace(scale=_number(scale, "residual_norm: scale"), eps=_number(eps, "residual_norm: eps"), kind=kind, lengths=lengths)
     params = (gate, post_g, post_b, pre_g, pre_b)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (f, x, *params)):
         r = ResidualNormFn.apply(f, x, *params, cfg)
         return r if pre_g is not None else (r, None)
-    f = f.contiguous()
-    y, z, _ = _residual_norm_op(f, None if x is None else x.contiguous(), params, cfg).forward(f, False)
+    f = _packed(f)
+    y, z, _ = _residual_norm_op(f, _packed(x), params, cfg).forward(f, False)
     return y, z
 
 

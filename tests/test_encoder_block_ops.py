@@ -533,6 +533,34 @@ def test_attention_refusals_on_the_host():
     assert b"attention_long" in lib.ptpp_last_error()
 
 
+def test_launches_beyond_the_grid_are_refused():
+    """a launch holds fewer than 2^32 threads: more one-query blocks, or more rows of a norm, are refused before any launch"""
+    from promptttspp_amd import _lib, ops
+
+    lib = _lib.load()
+    e, edges, cnt = ops.bucket_edges(32, 128, True)
+    a = _lib.AttentionLongArgs()
+    for n in ("q", "k", "v", "out", "table"):
+        setattr(a, n, 4096)
+    a.Tq, a.Tk, a.H, a.Hk, a.dk, a.maps, a.dtype = 1, 1, 16, 16, 64, 1, _lib.BF16
+    a.ldq = a.ldk = a.ldv = a.ldo = a.sq = a.sk = a.sv = a.so = 1024
+    a.nbuckets, a.bidirectional, a.max_distance, a.nexact, a.nedges, a.edges = 32, 1, 128, e, cnt, ctypes.addressof(edges)
+    a.scale = 0.125
+    a.B = 2 ** 20 - 1
+    assert lib.ptpp_attention_long_ws_bytes(ctypes.byref(a), 0) >= 0
+    a.B = 2 ** 20
+    assert lib.ptpp_attention_long_ws_bytes(ctypes.byref(a), 0) < 0
+    assert lib.ptpp_attention_long_fwd(ctypes.byref(a), None) == -1
+    n = _lib.ResidualNormArgs()
+    n.f = n.y = 4096
+    n.B, n.T, n.C, n.gate_rows, n.dtype, n.scale, n.eps = 2 ** 12, 2 ** 13, 1024, 1, _lib.BF16, 1.0, 1e-5
+    assert lib.ptpp_residual_norm_fwd(ctypes.byref(n), None) == -1
+    # a gate row per utterance: one block of the finishing launch each
+    n.B, n.T, n.C, n.gate, n.gate_rows, n.dy, n.stats, n.dgate = 65536, 1, 4, 4096, 65536, 4096, 4096, 4096
+    n.ws, n.ws_bytes = 4096, lib.ptpp_residual_norm_ws_bytes(ctypes.byref(n))
+    assert lib.ptpp_residual_norm_bwd(ctypes.byref(n), None) == -1
+
+
 def test_attention_refuses_cpu_tensors():
     from promptttspp_amd import _lib
     from promptttspp_amd import functional as PF
@@ -548,6 +576,71 @@ def test_attention_refuses_cpu_tensors():
         PF.attention_diff(x, None, None, None, 0.1, 1)
     with pytest.raises(_lib.PtppError):
         PF.residual_norm(torch.zeros(1, 4, 8))
+    # what is given by value cannot be learned, and is not cut off
+    one = torch.ones((), requires_grad=True)
+    with pytest.raises(ValueError):
+        PF.attention_bucket(x, None, None, torch.zeros(32, 1), 1, scale=one)
+    with pytest.raises(ValueError):
+        PF.attention_diff(x, None, None, torch.zeros(4, 1, 32), one, 1)
+    with pytest.raises(ValueError):
+        PF.residual_norm(torch.zeros(1, 4, 8), scale=one)
+    with pytest.raises(TypeError):
+        PF.attention_bucket(x, None, None, torch.zeros(32, 1), 1, max_distance=128.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("maps", [1, 2])
+@pytest.mark.parametrize("Tq,start", [(1, 0), (1, 299), (5, 300), (40, 256)])
+def test_memory_behind_the_last_query_is_not_read(dev, maps, Tq, start):
+    """a step against a preallocated memory: with ``causal`` what lies behind the last query is not read, lengths or not"""
+    B, Tk, heads, dk = 2, 700, 2, 64 // maps
+    q, k, v, table, lam, _ = make(maps, torch.bfloat16, B, Tq, Tk, heads, heads, dk, 32, seed=9)
+    ref = RefAttention(q, k, v, table, lam, 0.35, None, heads, heads, maps, causal=True, q_start=[start, start], dt=torch.bfloat16)
+    k[:, start + Tq:], v[:, start + Tq:] = float("nan"), float("inf")
+    d = lambda t: None if t is None else t.to(dev)  # noqa: E731
+    out = call(maps, d(q), d(k), d(v), d(table), d(lam), heads, causal=True, q_start=torch.full((B,), start, device=dev, dtype=torch.int32))
+    within(out, ref.out, ref.out_b, "out")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("maps", [1, 2])
+@pytest.mark.parametrize("hide", [float("-inf"), -3.4028234663852886e38])
+@pytest.mark.parametrize("Tq,Tk", [(150, 150), (3, 200)])
+def test_table_entries_that_hide_keys(dev, maps, hide, Tq, Tk):
+    """buckets of the lowest values: their keys count for nothing, in every direction; a row that sees only such keys gives zeros"""
+    heads, dk, B = 2, 64 // maps, 2
+    q, k, v, table, lam, dout = make(maps, torch.bfloat16, B, Tq, Tk, heads, heads, dk, 32, seed=5)
+    finite = table.clone()
+    table[15, 0] = table[31, 0] = hide      # head 0: everything far away (in either direction)
+    table[:, 1] = hide                      # head 1: all keys
+    dist = torch.arange(Tk)[None] - torch.arange(Tq)[:, None]
+    bk = ref_bucket(dist, 32, 128, True)
+    seen = (bk != 15) & (bk != 31)
+    f = 2.0 ** -24
+    leaves = [t.to(dev).requires_grad_() for t in (q, k, v, table) + ((lam,) if maps == 2 else ())]
+    out = call(maps, *leaves[:4], leaves[4] if maps == 2 else None, heads)
+    assert not out[:, :, 64:].any()
+    qd, kd, vd = (t.double().view(B, -1, heads, 64)[:, :, 0] for t in (q, k, v))
+    for b in range(B):
+        ps, rhos = [], []
+        for m in range(maps):
+            s = dk ** -0.5 * qd[b, :, m * dk:(m + 1) * dk] @ kd[b, :, m * dk:(m + 1) * dk].T + finite.double()[bk, 0]
+            rhos.append((dk + 16) * f * float(s.abs().max()))
+            ps.append(s.masked_fill(~seen, float("-inf")).softmax(-1))
+        c = [1.0]
+        if maps == 2:
+            lv = lam.double()
+            c.append(-float((lv[0, 0] @ lv[1, 0]).exp() - (lv[2, 0] @ lv[3, 0]).exp() + 0.35))
+        w, wa = sum(x * p for x, p in zip(c, ps)), sum(abs(x) * p for x, p in zip(c, ps))
+        u = 2.0 ** -8
+        want = w @ vd[b]
+        within(out[b, :, :64], want, (u + 2 * max(rhos) + 8 * f) * (wa @ vd[b].abs()) + u * want.abs(), "out")
+    grads = torch.autograd.grad(out, leaves, dout.to(dev))
+    assert all(bool(torch.isfinite(t).all()) for t in grads)
+    dt = grads[3]
+    assert not dt[:, 1].any() and not dt[15].any() and not dt[31].any() and dt[:, 0].any()
+    for t in grads[:3]:
+        assert not t[:, :, 64:].any()
 
 
 @pytest.mark.gpu
@@ -756,6 +849,32 @@ def test_residual_norm_inputs_off_the_beaten_path(dev):
     assert dpg.shape == pg.shape and dqg.dtype == torch.bfloat16
     within(dpg.reshape(-1), *want["dpost_g"], "dpost_g")
     within(dqg, want["dpre_g"][0], want["dpre_g"][1] + 2.0 ** -8 * want["dpre_g"][0].abs(), "dpre_g")
+
+
+@pytest.mark.gpu
+def test_residual_norm_off_the_16_byte_grid(dev):
+    """contiguous operands, parameters and gradients that start anywhere"""
+    from promptttspp_amd import functional as PF
+
+    g = torch.Generator().manual_seed(8)
+    f, x = torch.randn(2, 2, 7, 12, generator=g).bfloat16()
+    pg, dy = 1 + 0.1 * torch.randn(12, generator=g), torch.randn(2, 7, 12, generator=g).bfloat16()
+    want = ref_norm(f, x, None, (pg, None), (None, None), 1.0, 1e-5, "rms", None, dy, None, torch.bfloat16)
+
+    def off(t):
+        return torch.cat([t.new_zeros(1), t.reshape(-1)]).to(dev).requires_grad_()
+
+    fd, xd, pd = off(f), off(x), off(pg)
+    y, _ = PF.residual_norm(fd[1:].view(2, 7, 12), xd[1:].view(2, 7, 12), post=(pd[1:], None), kind="rms")
+    within(y, *want["y"], "y")
+    joined = torch.cat([y.new_zeros(1), y.reshape(-1)])  # (its backward hands a gradient one element off)
+    df, dx, dp = torch.autograd.grad(joined, [fd, xd, pd], torch.cat([dy.new_zeros(1), dy.reshape(-1)]).to(dev))
+    within(df[1:].view(2, 7, 12), *want["df"], "df")
+    within(dx[1:].view(2, 7, 12), *want["dx"], "dx")
+    within(dp[1:], *want["dpost_g"], "dpost_g")
+    with torch.no_grad():
+        y2, _ = PF.residual_norm(fd[1:].view(2, 7, 12), xd[1:].view(2, 7, 12), post=(pd[1:], None), kind="rms")
+    assert torch.equal(y, y2)
 
 
 @pytest.mark.gpu
