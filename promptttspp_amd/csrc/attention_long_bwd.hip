@@ -40,7 +40,7 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
   int qt, bh;
   la_block(p.nqt, p.B * p.H, qt, bh);
   if (p.causal) qt = p.nqt - 1 - qt;  // (the longest rows first)
-  const int h = bh % p.H, b = bh / p.H, hk = h / (p.H / p.Hk);
+  const int h = bh % p.H, b = FEW ? bh / p.H : la_longest(p, p.k_lengths, bh / p.H, lane), hk = h / (p.H / p.Hk);
   const int klen = la_klen(p, b), qlen = la_qlen(p, b), qs = la_qstart(p, b);
   constexpr int OWN = FEW ? LA_OWN : LA_OWN * LA_WAVES;
   const int ib = qt * OWN, i0 = ib + (FEW ? 0 : wave * LA_OWN), iq = i0 + lq;
@@ -221,7 +221,7 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
       double t = 0.0;
 #pragma unroll
       for (int w = 0; w < W; ++w) t -= lred[w];
-      p.lam_part[(int64_t)bh * p.nqt + qt] = t;
+      p.lam_part[((int64_t)b * p.H + h) * p.nqt + qt] = t;
     }
   }
   if (iq >= p.Tq) return;
@@ -322,7 +322,7 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
 
   int kt, bh;
   la_block(p.nkt, p.B * p.Hk, kt, bh);
-  const int hk = bh % p.Hk, b = bh / p.Hk, G = p.H / p.Hk;
+  const int hk = bh % p.Hk, b = FEW ? bh / p.Hk : la_longest(p, p.q_lengths, bh / p.Hk, lane), G = p.H / p.Hk;
   const int klen = la_klen(p, b), qlen = la_qlen(p, b), qs = la_qstart(p, b);
   constexpr int OWN = FEW ? LA_OWN : LA_OWN * LA_WAVES;
   const int jb = kt * OWN, j0 = jb + (FEW ? 0 : wave * LA_OWN), jk = j0 + lk;

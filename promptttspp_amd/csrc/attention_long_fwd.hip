@@ -79,7 +79,7 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 ? 1 : 2) void attn_long_fwd_ker
   int qt, bh;
   la_block(p.nqt, p.B * p.H, qt, bh);
   if (p.causal) qt = p.nqt - 1 - qt;  // (the longest rows first)
-  const int h = bh % p.H, b = bh / p.H, hk = h / (p.H / p.Hk);
+  const int h = bh % p.H, b = la_longest(p, p.k_lengths, bh / p.H, lane), hk = h / (p.H / p.Hk);
   const int klen = la_klen(p, b), qlen = la_qlen(p, b), qs = la_qstart(p, b);
   const int ib = qt * (LA_OWN * LA_WAVES), i0 = ib + wave * LA_OWN, iq = i0 + lq;
   const int dv = MAPS * p.dk;
