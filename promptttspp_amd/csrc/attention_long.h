@@ -334,5 +334,15 @@ __device__ __forceinline__ int la_qstart(const LongP& p, int b) {
 
 }  // namespace
 
+// host side: blocks of 32 rows (their four waves share the streamed side) instead of 128, up to which number of them.  Two rounds of the chip
+// where a block's buffers take a CU but its waves four times as long per row (f32), or where two blocks fit a CU (heads of up to 64
+// channels in all maps); one round for wide 16-bit heads.  128 -> 32 rows, forward / dq / dk, dv, us:
+//   16-bit, 64 channels:     384 blocks (6 x 512)  17 -> 12 / 21 -> 16 / 32 -> 34, 512 (4 x 1024) 25 -> 16 / 31 -> 23 / 49 -> 48,
+//                            768 (12 x 512) 17 -> 18 / 21 -> 25 / 33 -> 50
+//   f32, 64 channels:        512 (8 x 512) 56 -> 43 / 71 -> 55 / 98 -> 70, 768 (12 x 512) 57 -> 63 / 73 -> 81 / 100 -> 105
+//   f32, 128 channels:       512 (4 x 1024) 175 -> 129 / 246 -> 164 / 330 -> 209
+//   16-bit, 128 channels:    256 (4 x 512) 19 -> 13 / 27 -> 19 / 41 -> 24, 384 (6 x 512) 20 -> 22 / 28 -> 33 / 42 -> 46
+static inline int64_t la_few_blocks(int dtype, int maps, int dk) { return dtype == PTPP_F32 || maps * dk <= 64 ? 512 : 256; }
+
 // host side (attention_long_fwd.hip): argument checks shared by both directions; fills the kernel parameters
 int ptpp_attention_long_params(const ptpp_attention_long_args* a, int backward, LongP* out, const char* who);

@@ -684,8 +684,8 @@ __global__ __launch_bounds__(256) void attn_long_fin_kernel(const LongP p, float
   }
 }
 
-// The rule (as in forward): blocks of 32 rows where that gives at most 256 of them (one round of the chip), else of 128 -- also where the
-// few-row form's buffers and the distance sums of a wide table do not fit LDS together.
+// The rule (as in forward): blocks of 32 rows where that gives few of them (la_few_blocks), else of 128 -- also where the few-row form's
+// buffers and the distance sums of a wide table do not fit LDS together.
 template <typename E, int DK, int DV, int MAPS>
 size_t lds_dq(bool few, int dn) {
   typedef LSplit<E, DK, DV, MAPS> S_;
@@ -701,8 +701,9 @@ size_t lds_dkv(bool few, int dn) {
 template <typename E, int DK, int DV, int MAPS>
 void plan_bwd(LongP& p) {
   const int dn = p.table ? 2 * (p.max_distance + LA_PAD) + 1 : 0;
-  p.few_q = (int64_t)(p.TqP / 32) * p.B * p.H <= 256;
-  p.few_k = (int64_t)((p.Tk + 31) / 32) * p.B * p.Hk <= 256 && lds_dkv<E, DK, DV, MAPS>(true, dn) <= LA_LDS;
+  const int64_t few = la_few_blocks(sizeof(E) == 4 ? PTPP_F32 : PTPP_BF16, MAPS, p.dk);
+  p.few_q = (int64_t)(p.TqP / 32) * p.B * p.H <= few;
+  p.few_k = (int64_t)((p.Tk + 31) / 32) * p.B * p.Hk <= few && lds_dkv<E, DK, DV, MAPS>(true, dn) <= LA_LDS;
   if (p.few_q) p.nqt = p.TqP / 32;  // (D is written up to the padding of its rows)
   if (p.few_k) p.nkt = (p.Tk + 31) / 32;
 }

@@ -516,11 +516,15 @@ __global__ __launch_bounds__(256) void attn_long_join_kernel(const LongP p, int 
   }
 }
 
-// The rule: blocks of 128 rows, unless there are at most 32 rows, or blocks of 32 make at most 256 (one round of the chip); then as many
-// key ranges as fill the chip once -- one or two blocks per CU, as their buffers fit -- at no fewer than two 32-key chunks per wave.
-bool few_rows(const LongP& p) { return p.Tq <= 32 || (int64_t)((p.Tq + 31) / 32) * p.B * p.H <= 256; }
+// The rule: blocks of 128 rows, unless there are at most 32 rows, or few blocks (la_few_blocks); then as many key ranges as fill the chip
+// once -- one or two blocks per CU, as their buffers fit -- at no fewer than four 32-key chunks per wave (f32: two), which is what the join
+// of many rows costs: 4 x 512 rows of 4 x 64 channels 10.1 us in one range, 10.5 + 7 us in two; one query against 8000 keys of 8 x 64
+// channels 16.3 us this way, 19.3 us from two chunks on.
+bool few_rows(const LongP& p, int dtype, int maps) {
+  return p.Tq <= 32 || (int64_t)((p.Tq + 31) / 32) * p.B * p.H <= la_few_blocks(dtype, maps, p.dk);
+}
 // fills nh, nrb, splits; returns the number of 32-column blocks (0: too many to number)
-int plan_few(LongP& p, int lds) {
+int plan_few(LongP& p, int lds, int dtype) {
   const int G = p.H / p.Hk;
   p.nh = 1;
   if (!p.lse)  // (backward's statistics are padded to whole blocks of one head's rows)
@@ -528,7 +532,7 @@ int plan_few(LongP& p, int lds) {
       if (G % n == 0 && (!p.table || n * (2 * (p.max_distance + LA_PAD) + 1) <= 6144)) p.nh = n;  // (24 KB of bias tables)
   p.nrb = p.nh > 1 ? 1 : (p.lse ? p.TqP : p.Tq + 31) / 32;
   const int64_t blocks = (int64_t)p.B * p.Hk * (G / p.nh) * p.nrb;
-  const int64_t most = ((int64_t)p.Tk + 64 * LA_WAVES - 1) / (64 * LA_WAVES);
+  const int64_t range = (dtype == PTPP_F32 ? 2 : 4) * 32 * LA_WAVES, most = (p.Tk + range - 1) / range;
   int64_t s = blocks ? (lds > 72 * 1024 ? 256 : 512) / blocks : 1;  // (72 KB: two blocks per CU with their tables and statistics)
   if (s > most) s = most;
   p.splits = s < 1 ? 1 : s > 64 ? 64 : (int)s;
@@ -580,8 +584,8 @@ int dispatch_fwd(const LongP& p, int maps, hipStream_t st) {
 // forward plan: p.splits == 0: tiles.  -> bytes of workspace, < 0: refused
 int64_t plan_fwd(LongP& p, const ptpp_attention_long_args* a, int64_t* o_ml, const char* who) {
   *o_ml = 0;
-  if (!few_rows(p)) return 0;
-  const int blocks = plan_few(p, few_lds(a->dtype, a->maps, a->dk));
+  if (!few_rows(p, a->dtype, a->maps)) return 0;
+  const int blocks = plan_few(p, few_lds(a->dtype, a->maps, a->dk), a->dtype);
   if (!blocks) {
     ptpp_set_error("%s: too many tiles", who);
     return -1;
