@@ -106,6 +106,15 @@ __device__ __forceinline__ uint4 la_pack(const f32x16& v, int s) {
                  LOp<E>::pk(v[8 * s + 6], v[8 * s + 7])};
   }
 }
+// what la_pack's rounding took from registers [CH s, CH s + CH) of v, in the same layout (16-bit elements)
+template <typename E>
+__device__ __forceinline__ uint4 la_pack_rest(const f32x16& v, int s, uint4 f) {
+  const uint32_t r[4] = {f.x, f.y, f.z, f.w};
+  uint32_t o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = LOp<E>::pk(v[8 * s + 2 * i] - LOp<E>::lo(r[i]), v[8 * s + 2 * i + 1] - LOp<E>::hi(r[i]));
+  return uint4{o[0], o[1], o[2], o[3]};
+}
 // dot product of two fragments in f32
 template <typename E>
 __device__ __forceinline__ float la_dot(uint4 a, uint4 b) {

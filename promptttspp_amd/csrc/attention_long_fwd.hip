@@ -232,10 +232,14 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 ? 1 : 2) void attn_long_fwd_ker
 // each streaming its own chunks through its own two LDS buffers (no block barrier in the loop), and join at the end.  With more
 // than one range the blocks leave unnormalised sums and (max, sum) for the join kernel.  A step is HBM-bound: every key and value is
 // read once, 64 KB in flight per CU.
-template <typename E, int DK, int DV, int MAPS, bool BIAS>
+template <typename E, int DK, int DV, int MAPS, bool BIAS, bool REST>
 __global__ __launch_bounds__((LSplit<E, DK, DV, MAPS>::W * 64), sizeof(E) == 4 || MAPS * DV == 256 ? 1 : 2) void attn_long_split_kernel(const LongP p) {
   typedef LSplit<E, DK, DV, MAPS> S_;
   constexpr int W = S_::W, NB = S_::NB, STAGE = S_::STAGE, KIMG = 32 * DK;
+  // REST: 16-bit probabilities as two operands, the rounded value and what the rounding took: the matrix units wait for memory here, and the
+  // context has the accuracy of f32 probabilities (against 64 bits one f16 query on 4001 keys, differential: 3.1e-4 -> 2.1e-4, the output's
+  // own rounding) for 50.5 instead of 46.8 us, 40.2 instead of 39.3 us for one bf16 query on 8191 keys.  Not where backward follows, which
+  // rounds the same probabilities once.
   constexpr bool TIGHT = sizeof(E) == 4 || MAPS * DV == 256;
   constexpr int CH = LOp<E>::CH, KS = DK / (2 * CH), PS = 16 / CH, NT = DV / 32;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -327,7 +331,7 @@ __global__ __launch_bounds__((LSplit<E, DK, DV, MAPS>::W * 64), sizeof(E) == 4 |
     const E* vimg = kimg + MAPS * KIMG;
     const int j0 = 32 * c;
     const int ln = TIGHT ? la_opaque(lane) : lane, lr = ln & 31, hr = ln >> 5;
-    uint4 pf[MAPS][PS];
+    uint4 pf[MAPS][PS], pr[REST ? MAPS : 1][REST ? PS : 1];
     f32x16 s[MAPS];
 #pragma unroll
     for (int m = 0; m < MAPS; ++m) {
@@ -351,7 +355,10 @@ __global__ __launch_bounds__((LSplit<E, DK, DV, MAPS>::W * 64), sizeof(E) == 4 |
       la_raise<NT>(mx[m], l[m], o[m], la_half_max(fmaf(la_max16(s[m]), mul, add)));
       l[m] += la_probs(s[m], mul, add - mx[m]);
 #pragma unroll
-      for (int st = 0; st < PS; ++st) pf[m][st] = la_pack<E>(s[m], st);
+      for (int st = 0; st < PS; ++st) {
+        pf[m][st] = la_pack<E>(s[m], st);
+        if constexpr (REST) pr[m][st] = la_pack_rest<E>(s[m], st, pf[m][st]);
+      }
     }
     if (NB == 2 && two) glds_wait<2 * NK + NV>();
     else if (NB == 2 && one) glds_wait<NK + NV>();
@@ -363,7 +370,11 @@ __global__ __launch_bounds__((LSplit<E, DK, DV, MAPS>::W * 64), sizeof(E) == 4 |
         const uint4 vf = la_tfrag<E, DV>(vimg, 0, st, n, ln);
 #pragma unroll
         for (int m = 0; m < MAPS; ++m) o[m][n] = LOp<E>::mma(vf, pf[m][st], o[m][n]);
-        if (TIGHT) __builtin_amdgcn_sched_barrier(0);
+        if constexpr (REST) {
+#pragma unroll
+          for (int m = 0; m < MAPS; ++m) o[m][n] = LOp<E>::mma(vf, pr[m][st], o[m][n]);
+        }
+        if (TIGHT && (!REST || n % 2 == 1)) __builtin_amdgcn_sched_barrier(0);
       }
     if (NB == 2 && two) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the values' last reads are done
@@ -546,6 +557,19 @@ int few_lds(int maps, int dk) {
 int few_lds(int dtype, int maps, int dk) { return dtype == PTPP_F32 ? few_lds<float>(maps, dk) : few_lds<bf16_raw>(maps, dk); }  // (f16 as bf16)
 int pad_dv(int maps, int dk) { return maps == 1 ? (dk <= 64 ? 64 : 128) : (dk <= 32 ? 64 : 128); }
 
+template <typename E, int DK, int DV, int MAPS, bool BIAS, bool REST>
+int launch_split(const LongP& p, unsigned blocks, size_t sm, hipStream_t st) {
+  if (!la_lds_limit((const void*)attn_long_split_kernel<E, DK, DV, MAPS, BIAS, REST>, sm, "attention_long_fwd")) return PTPP_ELAUNCH;
+  hipLaunchKernelGGL((attn_long_split_kernel<E, DK, DV, MAPS, BIAS, REST>), dim3(blocks), dim3(LSplit<E, DK, DV, MAPS>::W * 64), sm, st, p);
+  PTPP_CHECK_LAUNCH("attention_long_fwd (few rows)");
+  return PTPP_OK;
+}
+template <typename E, int DK, int DV, int MAPS, bool BIAS>
+int launch_split(const LongP& p, unsigned blocks, size_t sm, hipStream_t st) {
+  if constexpr (sizeof(E) == 2)
+    if (!p.lse) return launch_split<E, DK, DV, MAPS, BIAS, true>(p, blocks, sm, st);
+  return launch_split<E, DK, DV, MAPS, BIAS, false>(p, blocks, sm, st);
+}
 template <typename E, int DK, int DV, int MAPS>
 int launch_fwd(const LongP& p, hipStream_t st) {
   const size_t tab = p.table ? (2 * (p.max_distance + LA_PAD) + 1) * sizeof(float) : 0;
@@ -562,12 +586,10 @@ int launch_fwd(const LongP& p, hipStream_t st) {
   typedef LSplit<E, DK, DV, MAPS> S_;
   const size_t sm = S_::LDS + p.nh * tab;
   const int blocks = p.B * p.Hk * (p.H / p.Hk / p.nh) * p.nrb;
-  const dim3 g((unsigned)(blocks * p.splits)), t(S_::W * 64);
-  const void* kern = p.table ? (const void*)attn_long_split_kernel<E, DK, DV, MAPS, true> : (const void*)attn_long_split_kernel<E, DK, DV, MAPS, MAPS == 1>;
-  if (!la_lds_limit(kern, sm, "attention_long_fwd")) return PTPP_ELAUNCH;
-  if (p.table) hipLaunchKernelGGL((attn_long_split_kernel<E, DK, DV, MAPS, true>), g, t, sm, st, p);
-  else if constexpr (MAPS == 2) hipLaunchKernelGGL((attn_long_split_kernel<E, DK, DV, MAPS, false>), g, t, sm, st, p);
-  PTPP_CHECK_LAUNCH("attention_long_fwd (few rows)");
+  int r = PTPP_OK;
+  if (p.table) r = launch_split<E, DK, DV, MAPS, true>(p, (unsigned)(blocks * p.splits), sm, st);
+  else if constexpr (MAPS == 2) r = launch_split<E, DK, DV, MAPS, false>(p, (unsigned)(blocks * p.splits), sm, st);
+  if (r != PTPP_OK) return r;
   if (p.splits > 1) {
     const int ncol = blocks * join_cols(p);
     hipLaunchKernelGGL((attn_long_join_kernel<E, DV, MAPS>), dim3((ncol + LA_WAVES - 1) / LA_WAVES), dim3(256), 0, st, p, ncol);
