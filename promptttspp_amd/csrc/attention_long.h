@@ -304,7 +304,7 @@ __device__ __forceinline__ void la_block(int tiles, int pairs, int& tile, int& p
   pair = pos < big ? pos / (q + 1) + 8 * (pos % (q + 1)) : rem + (pos - big) / max(q, 1) + 8 * ((pos - big) % max(q, 1));
 }
 
-// lam of head h (every lane of a wave calls it; dk <= 64)
+// lam of head h (every lane of a wave calls it, all with the same h: lane c takes channel c of that head's vectors; dk <= 64)
 __device__ __forceinline__ void la_lambda_parts(const LongP& p, int h, int lane, float& e1, float& e2) {
   const int hh = p.lam_heads > 1 ? h : 0;
   float a = 0.f, b = 0.f;

@@ -416,7 +416,13 @@ __global__ __launch_bounds__((LSplit<E, DK, DV, MAPS>::W * 64), sizeof(E) == 4 |
   la_barrier();
   const bool row = iq < p.Tq;
   float lam = 0.f;
-  if constexpr (MAPS == 2) lam = la_lambda(p, h, lane);
+  if constexpr (MAPS == 2) {
+    if (p.splits == 1)  // (with more ranges the join applies it)
+      for (int n = 0; n < (p.lam_heads > 1 ? p.nh : 1); ++n) {  // one head after the other: a whole wave computes one value
+        const float l = la_lambda(p, h0 + n, lane);
+        if (p.lam_heads == 1 || n == hcol) lam = l;
+      }
+  }
   float inv[MAPS];
 #pragma unroll
   for (int m = 0; m < MAPS; ++m) {

@@ -298,6 +298,17 @@ def test_one_query_against_a_memory(dev, maps, dtype, dk, Tk):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,dk", [("bf16", 64), ("f16", 32), ("f32", 64)])
+@pytest.mark.parametrize("B,Tq,Tk,heads,kv_heads", [(3, 1, 63, 4, 2), (3, 1, 2100, 4, 2), (2, 5, 200, 6, 2), (2, 1, 120, 12, 1), (150, 1, 600, 4, 2)])
+def test_lam_per_head_where_a_block_takes_several_heads(dev, dtype, dk, B, Tq, Tk, heads, kv_heads):
+    """few queries without gradients: heads that share their keys lie side by side in one block, each with its own lam -- short memories and
+    large batches (one range of keys per block) and long memories (ranges joined afterwards)"""
+    lens = [max(Tq, Tk - 37 * b % Tk) for b in range(B)]
+    check_attention(dev, 2, dtype, B, Tq, Tk, heads, kv_heads, dk, 16, lam_heads=heads, train=False, garbage=True, lengths=lens,
+                    q_start=[n - Tq for n in lens], causal=True)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("maps", [1, 2])
 @pytest.mark.parametrize("Tq", [2, 5, 16, 24])
 def test_few_queries_against_a_long_memory(dev, maps, Tq):
