@@ -1008,8 +1008,9 @@ def attention(qkv, pos, bias_u, bias_v, lengths, heads, variant, drop_p=0.0):
 # Attention over long sequences (csrc/attention_long_*.hip): O(T) memory, probabilities recomputed in backward.
 # ----------------------------------------------------------------------------
 def _param_sinks(params):
-    """The parameters themselves if every one's gradient can be accumulated in place (direct mode), else None."""
-    return params if params and all(_sink(p) is not None for p in params) else None
+    """The parameters themselves if every one's gradient can be accumulated in place (direct mode), else None.  One that is given twice (a
+    norm that stands behind and before a block) goes through autograd's sum: one launch must not add to the same buffer from two blocks."""
+    return params if params and len({id(p) for p in params}) == len(params) and all(_sink(p) is not None for p in params) else None
 
 
 def _f32_view(t):

@@ -178,6 +178,50 @@ def test_gradients_land_in_the_flat_buffer(dev):
             PF.enable_direct_grads(False)
 
 
+def test_a_parameter_given_twice_is_not_added_to_in_place():
+    """in the flat buffer's mode one launch would add to the same gradient from two blocks at once"""
+    from promptttspp_amd import functional as PF
+
+    a, b = (torch.nn.Parameter(torch.ones(8)) for _ in range(2))
+    a.grad, b.grad = torch.zeros(8), torch.zeros(8)
+    on = PF._direct["on"]
+    PF._direct["on"] = True
+    try:
+        assert PF._param_sinks([a, b]) == [a, b]
+        assert PF._param_sinks([a, b, a]) is None
+    finally:
+        PF._direct["on"] = on
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(2, 60, 256), (40, 33, 64)])
+def test_one_norm_behind_and_before_a_block(dev, shape):
+    """the same (gamma, beta) as post and pre norm: the flat buffer gets the sum of both gradients, which is what the norms given
+    separately get"""
+    from promptttspp_amd import functional as PF
+    from promptttspp_amd.parallel import FlatGradReducer
+
+    B, T, C = shape
+    gen = torch.Generator(device=dev).manual_seed(3)
+    r = lambda *s: torch.randn(*s, device=dev, generator=gen)  # noqa: E731
+    f, x, dy, dz = r(B, T, C), r(B, T, C), r(B, T, C), r(B, T, C)
+    gamma, beta = torch.nn.Parameter(1 + 0.1 * r(C)), torch.nn.Parameter(0.1 * r(C))
+    apart = [p.detach().clone().requires_grad_() for p in (gamma, beta, gamma, beta)]
+    want = torch.autograd.grad(PF.residual_norm(f, x, post=tuple(apart[:2]), pre=tuple(apart[2:])), apart, (dy, dz))
+    try:
+        red = FlatGradReducer([gamma, beta])
+        red.zero_grad()
+        for _ in range(2):
+            torch.autograd.backward(PF.residual_norm(f, x, post=(gamma, beta), pre=(gamma, beta)), (dy, dz))
+        red.finish()
+        torch.cuda.synchronize()
+        for p, a, b in ((gamma, want[0], want[2]), (beta, want[1], want[3])):
+            # each sum is the same f32 value in both calls: three additions of them remain
+            assert bool(((p.grad - 2 * (a + b)).abs() <= 4 * 2.0 ** -24 * 2 * (a.abs() + b.abs())).all())
+    finally:
+        PF.enable_direct_grads(False)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("form", [1, 3])
 def test_training_mode_runs_with_dropout(dev, form):
