@@ -211,11 +211,14 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
     for (int m = 0; m < MAPS; ++m) Dm[m] += la_half_sum(eps[m]);
   }
   const bool stat = hw == 0 && (!FEW || wave == 0);
+  bool live[MAPS];  // rows that are none, or see no key: zeros by selection, as in forward
 #pragma unroll
-  for (int m = 0; m < MAPS; ++m)
-    if (stat && iq < p.TqP) p.D[(((int64_t)m * p.B + b) * p.H + h) * p.TqP + iq] = iq < qlen ? Dm[m] : 0.f;
+  for (int m = 0; m < MAPS; ++m) {
+    live[m] = iq < qlen && !(lse[m] == INFINITY);
+    if (stat && iq < p.TqP) p.D[(((int64_t)m * p.B + b) * p.H + h) * p.TqP + iq] = live[m] ? Dm[m] : 0.f;
+  }
   if constexpr (MAPS == 2) {  // this block's share of dlam = -sum_i D_1 (64 bits: the rows' terms cancel)
-    double s = stat && iq < qlen ? (double)Dm[MAPS - 1] : 0.0;
+    double s = stat && live[MAPS - 1] ? (double)Dm[MAPS - 1] : 0.0;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
     if (lane == 0) lred[wave] = s;
@@ -234,14 +237,16 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
     for (int g = wave; g < MAPS * NT * 4; g += W) {  // 4 registers = 4 channels at a time
       const int m = g / (NT * 4), ch = 32 * ((g >> 2) % NT) + 8 * (g & 3) + 4 * hw;
       const float c = m == 0 ? p.scale : -lam * p.scale;
+      const bool on = m == 0 ? live[0] : live[MAPS - 1];
       float v[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         v[e] = 0.f;
 #pragma unroll
         for (int w = 0; w < W; ++w) v[e] += all[w * (NB * BUF * (int)sizeof(E) / 4) + (4 * g + e) * 64];
+        v[e] = on ? v[e] * c : 0.f;
       }
-      if (ch < p.dk) la_store4<E>(qo + m * p.dk + ch, v[0] * c, v[1] * c, v[2] * c, v[3] * c);
+      if (ch < p.dk) la_store4<E>(qo + m * p.dk + ch, v[0], v[1], v[2], v[3]);
     }
     return;
   }
@@ -253,8 +258,10 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const int ch = 32 * n + 8 * g + 4 * hw;
-        if (ch < p.dk)
-          la_store4<E>(qo + m * p.dk + ch, acc[m][n][4 * g] * c, acc[m][n][4 * g + 1] * c, acc[m][n][4 * g + 2] * c, acc[m][n][4 * g + 3] * c);
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = live[m] ? acc[m][n][4 * g + e] * c : 0.f;
+        if (ch < p.dk) la_store4<E>(qo + m * p.dk + ch, v[0], v[1], v[2], v[3]);
       }
   }
 }

@@ -192,13 +192,14 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 ? 1 : 2) void attn_long_fwd_ker
 
   // ---- epilogue: lane (query lq) holds channels 32 n + 8 g + 4 hw + (0..3) ----
   float inv[MAPS];
+  bool on[MAPS];  // a row that is none, or sees no key, gives zeros by selection: its sums may hold NaN from infinite keys or values
 #pragma unroll
   for (int m = 0; m < MAPS; ++m) {
     l[m] = la_half_sum(l[m]);
-    const bool on = iq < qlen && !(l[m] == 0.f);  // (a NaN sum passes: it belongs in the output)
-    inv[m] = on ? 1.f / l[m] : 0.f;
+    on[m] = iq < qlen && !(l[m] == 0.f);  // (a NaN sum passes: it belongs in the output)
+    inv[m] = 1.f / l[m];
     if (p.lse && hw == 0 && iq < p.TqP)
-      p.lse[(((int64_t)m * p.B + b) * p.H + h) * p.TqP + iq] = on ? mx[m] + log2f(l[m]) : INFINITY;
+      p.lse[(((int64_t)m * p.B + b) * p.H + h) * p.TqP + iq] = on[m] ? mx[m] + log2f(l[m]) : INFINITY;
   }
   float lam = 0.f;
   if constexpr (MAPS == 2) lam = la_lambda(p, h, lane);
@@ -211,19 +212,16 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 ? 1 : 2) void attn_long_fwd_ker
     for (int g = 0; g < 4; ++g) {
       const int c = 32 * n + 8 * g + 4 * hw;
       if (c < dv) {
-        float v[4];
+        float v[4], w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          v[e] = o[0][n][4 * g + e] * inv[0];
-          if constexpr (MAPS == 2) v[e] = fmaf(-lam, o[MAPS - 1][n][4 * g + e] * inv[MAPS - 1], v[e]);
+          v[e] = on[0] ? o[0][n][4 * g + e] * inv[0] : 0.f;
+          w[e] = on[MAPS - 1] ? o[MAPS - 1][n][4 * g + e] * inv[MAPS - 1] : 0.f;
+          if constexpr (MAPS == 2) v[e] = fmaf(-lam, w[e], v[e]);
         }
-        // (a row that sees nothing has all-zero probabilities, and V rows behind the keys are never loaded: v is 0, not NaN)
         la_store4<E>(ob + c, v[0], v[1], v[2], v[3]);
         if constexpr (MAPS == 2) {
-          if (o2) {
-            const float w = inv[MAPS - 1];
-            la_store4<E>(o2 + c, o[MAPS - 1][n][4 * g] * w, o[MAPS - 1][n][4 * g + 1] * w, o[MAPS - 1][n][4 * g + 2] * w, o[MAPS - 1][n][4 * g + 3] * w);
-          }
+          if (o2) la_store4<E>(o2 + c, w[0], w[1], w[2], w[3]);
         }
       }
     }
@@ -424,10 +422,11 @@ __global__ __launch_bounds__((LSplit<E, DK, DV, MAPS>::W * 64), sizeof(E) == 4 |
       }
   }
   float inv[MAPS];
+  bool on[MAPS];
 #pragma unroll
   for (int m = 0; m < MAPS; ++m) {
-    const bool on = iq < qlen && !(L[m] == 0.f);
-    inv[m] = on ? 1.f / L[m] : 0.f;
+    on[m] = iq < qlen && !(L[m] == 0.f);
+    inv[m] = 1.f / L[m];
     if (wave == 0 && hw == 0) {
       if (p.splits > 1) {
         if (row) {
@@ -436,7 +435,7 @@ __global__ __launch_bounds__((LSplit<E, DK, DV, MAPS>::W * 64), sizeof(E) == 4 |
           ml[1] = L[m];
         }
       } else if (p.lse && iq < p.TqP) {
-        p.lse[(((int64_t)m * p.B + b) * p.H + h) * p.TqP + iq] = on ? M[m] + log2f(L[m]) : INFINITY;
+        p.lse[(((int64_t)m * p.B + b) * p.H + h) * p.TqP + iq] = on[m] ? M[m] + log2f(L[m]) : INFINITY;
       }
     }
   }
@@ -459,19 +458,17 @@ __global__ __launch_bounds__((LSplit<E, DK, DV, MAPS>::W * 64), sizeof(E) == 4 |
         *reinterpret_cast<f32x4*>(p.part_o + ((((int64_t)tl * p.splits + sp) * MAPS + m) * 32 + lq) * DV + ch) = f32x4{v[m][0], v[m][1], v[m][2], v[m][3]};
     } else {
       E* ob = reinterpret_cast<E*>(p.out) + b * p.so + (int64_t)iq * p.ldo + (int64_t)h * dv + ch;
-      float r[4];
+      float r[4], w[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        r[e] = v[0][e] * inv[0];
-        if constexpr (MAPS == 2) r[e] = fmaf(-lam, v[MAPS - 1][e] * inv[MAPS - 1], r[e]);
+        r[e] = on[0] ? v[0][e] * inv[0] : 0.f;
+        w[e] = on[MAPS - 1] ? v[MAPS - 1][e] * inv[MAPS - 1] : 0.f;
+        if constexpr (MAPS == 2) r[e] = fmaf(-lam, w[e], r[e]);
       }
       la_store4<E>(ob, r[0], r[1], r[2], r[3]);
       if constexpr (MAPS == 2) {
-        if (p.out2) {
-          const float w = inv[MAPS - 1];
-          la_store4<E>(reinterpret_cast<E*>(p.out2) + ((int64_t)b * p.Tq + iq) * ((int64_t)p.H * dv) + (int64_t)h * dv + ch, v[MAPS - 1][0] * w,
-                       v[MAPS - 1][1] * w, v[MAPS - 1][2] * w, v[MAPS - 1][3] * w);
-        }
+        if (p.out2)
+          la_store4<E>(reinterpret_cast<E*>(p.out2) + ((int64_t)b * p.Tq + iq) * ((int64_t)p.H * dv) + (int64_t)h * dv + ch, w[0], w[1], w[2], w[3]);
       }
     }
   }
@@ -520,7 +517,7 @@ __global__ __launch_bounds__(256) void attn_long_join_kernel(const LongP p, int 
           if (lane + 64 * n < dv) r[m][n] = fmaf(p.part_o[(base + s * step) * DV + lane + 64 * n], fs, r[m][n]);
       }
 #pragma unroll
-    for (int n = 0; n < NC; ++n) r[m][n] *= ok ? 1.f / L : 0.f;
+    for (int n = 0; n < NC; ++n) r[m][n] = ok ? r[m][n] * (1.f / L) : 0.f;
     if (p.lse && lane == 0 && iq < p.TqP) p.lse[(((int64_t)m * p.B + b) * p.H + h) * p.TqP + iq] = ok ? M + log2f(L) : INFINITY;
   }
   if (!row) return;

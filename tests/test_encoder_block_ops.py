@@ -250,6 +250,36 @@ def test_rows_without_keys_and_garbage_behind_the_lengths(dev, dtype, maps):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("maps", [1, 2])
+@pytest.mark.parametrize("B,T", [(2, 70), (2, 600), (70, 140)])
+def test_rows_behind_the_queries_stay_zero_beside_infinities(dev, dtype, maps, B, T):
+    """infinities and NaN among the valid keys and values reach the rows of valid queries only: outputs and query gradients behind
+    ``q_lengths`` are exact zeros, as are those of a row that sees no key (few rows, many, and without gradients)"""
+    dt, H, dk = DT[dtype], 2, 32
+    q, k, v, table, lam, dout = make(maps, dt, B, T, T, H, H, dk, 16, seed=2)
+    v[0, 3], k[1, 5], v[1, 40] = float("inf"), float("nan"), float("nan")
+    n = [T - 21, T - 40] + [T] * (B - 2)
+    kw = dict(q_lengths=torch.tensor(n, device=dev, dtype=torch.int32))
+    leaves = [t.to(dev).requires_grad_() for t in (q, k, v, table) + ((lam,) if maps == 2 else ())]
+    full = leaves + [None] * (5 - len(leaves))
+    out = call(maps, *full, H, **kw)
+    dq, dk_, dv = torch.autograd.grad(out, leaves[:3], dout.to(dev))
+    with torch.no_grad():
+        few = call(maps, full[0][:, :24].contiguous(), *full[1:], H, q_lengths=torch.full((B,), 9, device=dev))
+    for b in range(2):
+        for t in (out, dq):
+            assert not t[b, n[b]:].any()
+            assert not bool(torch.isfinite(t[b, :n[b]]).all())
+        assert not few[b, 9:].any() and not bool(torch.isfinite(few[b, :9]).all())
+    assert bool(torch.isfinite(out[2:]).all()) and bool(torch.isfinite(dk_[2:]).all())
+    # rows before the first key under the causal rule see nothing
+    with torch.no_grad():
+        a = call(maps, *full, H, causal=True, q_start=torch.full((B,), -10, device=dev, dtype=torch.int32))
+    assert not a[:, :10].any() and not bool(torch.isfinite(a[0, 20:]).all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("maps", [1, 2])
 @pytest.mark.parametrize("bidirectional", [True, False])
