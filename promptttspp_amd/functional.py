@@ -1026,6 +1026,12 @@ def _still(args, names, tensors):
     return True
 
 
+def _saved_rows(rows):
+    """whole numbers per utterance as save_for_backward takes them: refilling one in place before backward raises there, as for any saved
+    tensor, instead of masking with other lengths than forward did (one from inference mode has no version to compare: a copy)"""
+    return [t.clone() if t is not None and t.is_inference() else t for t in rows]
+
+
 def _number(x, what):
     """``x`` as the plain number that the kernels take by value (a tensor in its place would lose its gradient)"""
     if torch.is_tensor(x) and x.requires_grad:
@@ -1055,16 +1061,17 @@ class AttentionLongFn(Function):
             ctx.direct = _param_sinks([p for p in (table, lam) if p is not None])
             for p in ctx.direct or ():
                 _use(p)
-        ctx.save_for_backward(q, k, v, table, lam, out, lse, out2)
+        ctx.save_for_backward(q, k, v, table, lam, out, lse, out2, *_saved_rows(op.rows))
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, table, lam, out, lse, out2 = ctx.saved_tensors
+        q, k, v, table, lam, out, lse, out2, *rows = ctx.saved_tensors
         op = ctx.op
-        if not _still(op.args, ("q", "table", "lam") if k is None else ("q", "table", "lam", "k", "v"), (q, table, lam, k, v)):
-            op = _attention_long_op(q, k, v, _f32_view(table), _f32_view(lam), ctx.cfg)
+        names = ("q", "table", "lam", "k_lengths", "q_lengths", "q_start") if k is None else ("q", "table", "lam", "k_lengths", "q_lengths", "q_start", "k", "v")
+        if not _still(op.args, names, (q, table, lam, *rows, k, v)):
+            op = _attention_long_op(q, k, v, _f32_view(table), _f32_view(lam), ctx.cfg, rows)
         dout = _packed(dout)
         direct = ctx.direct is not None
         dt, dl = [None if p is None else p.grad if direct else lse.new_empty(p.shape) for p in (table, lam)]
@@ -1080,9 +1087,10 @@ class AttentionLongFn(Function):
         return dq, dk, dv, dt, dl, None
 
 
-def _attention_long_op(q, k, v, table, lam, cfg):
-    return ops.AttentionLong(q, k, v, cfg.heads, cfg.kv_heads, cfg.maps, table, cfg.max_distance, cfg.bidirectional, lam, cfg.lam_init, cfg.lengths,
-                             cfg.q_lengths, cfg.q_start, cfg.causal, cfg.scale)
+def _attention_long_op(q, k, v, table, lam, cfg, rows=None):
+    lengths, q_lengths, q_start = (cfg.lengths, cfg.q_lengths, cfg.q_start) if rows is None else rows
+    return ops.AttentionLong(q, k, v, cfg.heads, cfg.kv_heads, cfg.maps, table, cfg.max_distance, cfg.bidirectional, lam, cfg.lam_init, lengths,
+                             q_lengths, q_start, cfg.causal, cfg.scale)
 
 
 def _attention_long(q, k, v, table, lam, cfg):
@@ -1135,7 +1143,7 @@ class ResidualNormFn(Function):
         ctx.set_materialize_grads(False)
         f, x = _packed(f), _packed(x)
         params = (gate, post_g, post_b, pre_g, pre_b)
-        op = _residual_norm_op(f, x, params, cfg)
+        op = _residual_norm_op(f, x, params, cfg, cfg.lengths)
         y, z, stats = op.forward(f, True)
         ctx.cfg, ctx.op = cfg, op
         ctx.direct = None
@@ -1143,17 +1151,17 @@ class ResidualNormFn(Function):
             ctx.direct = _param_sinks([p for p, n in zip(params, ctx.needs_input_grad[2:7]) if n])
             for p in ctx.direct or ():
                 _use(p)
-        ctx.save_for_backward(f, x, *params, stats)
+        ctx.save_for_backward(f, x, *params, stats, *_saved_rows(op.rows))
         return y if z is None else (y, z)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dz=None):
-        f, x, *params, stats = ctx.saved_tensors
+        f, x, *params, stats, lengths = ctx.saved_tensors
         need = ctx.needs_input_grad
         op = ctx.op
-        if not _still(op.args, ("f", "x", "gate", "post_g", "post_b", "pre_g", "pre_b"), (f, x, *params)):
-            op = _residual_norm_op(f, x, params, ctx.cfg)
+        if not _still(op.args, ("f", "x", "gate", "post_g", "post_b", "pre_g", "pre_b", "lengths"), (f, x, *params, lengths)):
+            op = _residual_norm_op(f, x, params, ctx.cfg, lengths)
         dy, dz = _packed(dy), _packed(dz)
         want = need[2:7]
         if ctx.direct is not None:
@@ -1184,8 +1192,8 @@ def _flat(p):
     return p if n == 1 or (n == 2 and p.shape[0] != 1) else p.view(-1)
 
 
-def _residual_norm_op(f, x, params, cfg):
-    return ops.ResidualNorm(f, x, [_flat(p) for p in params], cfg.scale, cfg.eps, cfg.kind, cfg.lengths)
+def _residual_norm_op(f, x, params, cfg, lengths):
+    return ops.ResidualNorm(f, x, [_flat(p) for p in params], cfg.scale, cfg.eps, cfg.kind, lengths)
 
 
 def residual_norm(f, x=None, gate=None, post=None, pre=None, scale=1.0, eps=1e-5, kind="layer", lengths=None):
@@ -1204,7 +1212,7 @@ def residual_norm(f, x=None, gate=None, post=None, pre=None, scale=1.0, eps=1e-5
         r = ResidualNormFn.apply(f, x, *params, cfg)
         return r if pre_g is not None else (r, None)
     f = _packed(f)
-    y, z, _ = _residual_norm_op(f, _packed(x), params, cfg).forward(f, False)
+    y, z, _ = _residual_norm_op(f, _packed(x), params, cfg, cfg.lengths).forward(f, False)
     return y, z
 
 

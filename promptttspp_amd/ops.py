@@ -777,9 +777,9 @@ class AttentionLongPlan:
 
 class AttentionLong:
     """One call of the long-sequence attention kernels: the argument block of the forward launch, which backward copies and completes.
-    Holds no activations; ``forward`` / ``backward`` are given them."""
+    Holds no activations; ``forward`` / ``backward`` are given them.  ``rows``: (lengths, q_lengths, q_start) as the kernels read them."""
 
-    __slots__ = ("plan", "args", "held")
+    __slots__ = ("plan", "args", "held", "rows")
 
     def __init__(self, q, k, v, heads, kv_heads, maps, table=None, max_distance=128, bidirectional=True, lam=None, lam_init=0.0, lengths=None,
                  q_lengths=None, q_start=None, causal=False, scale=None):
@@ -797,7 +797,8 @@ class AttentionLong:
             a.k, a.v = k.data_ptr(), v.data_ptr()
         B = plan.shape[0]
         lengths, q_lengths, q_start = _i32_rows(lengths, "lengths", B, q), _i32_rows(q_lengths, "q_lengths", B, q), _i32_rows(q_start, "q_start", B, q)
-        self.held = table, lam, lengths, q_lengths, q_start  # (copies in another type live until the launches that read them)
+        self.rows = lengths, q_lengths, q_start
+        self.held = table, lam  # (copies in another type live until the launches that read them)
         if table is not None:
             a.table = _f32_operand(table, "table", plan.table_shape, dev)
         if lam is not None:
@@ -902,9 +903,9 @@ class ResidualNormPlan:
 
 class ResidualNorm:
     """One call of the residual-norm kernels, y = x + scale * gate * post(f), z = pre(y): the argument block of the forward launch, which
-    backward copies and completes.  Holds no activations."""
+    backward copies and completes.  Holds no activations.  ``rows``: the lengths as the kernels read them."""
 
-    __slots__ = ("plan", "args", "held")
+    __slots__ = ("plan", "args", "held", "rows")
 
     def __init__(self, f, x=None, par=(None,) * 5, scale=1.0, eps=1e-5, kind="layer", lengths=None):
         """``par``: (gate, post gamma, post beta, pre gamma, pre beta), f32 or None; f and x contiguous"""
@@ -933,7 +934,8 @@ class ResidualNorm:
         lengths = _i32_rows(lengths, "lengths", plan.shape[0], f)
         if lengths is not None:
             a.lengths = lengths.data_ptr()
-        self.held = par, lengths  # (copies in another type live until the launches that read them)
+        self.rows = (lengths,)
+        self.held = par  # (copies in another type live until the launches that read them)
 
     def forward(self, f, keep):
         """-> (y, z or None, statistics or None)"""

@@ -515,6 +515,61 @@ def test_long_batch_strides_pass_32_bits(dev):
     within(out, ref.out, ref.out_b, "out")
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("maps", [1, 2])
+@pytest.mark.parametrize("name", ["lengths", "q_lengths", "q_start"])
+def test_attention_rows_refilled_before_backward_are_refused(dev, maps, name):
+    """lengths and positions that forward read are saved like any other tensor: refilled in place, backward raises; one of another type was
+    copied, and one refilled after backward, or restored by a hook at another address, changes nothing"""
+    q, k, v, table, lam, dout = (t if t is None else t.to(dev) for t in make(maps, torch.bfloat16, 2, 40, 40, 2, 2, 32, 16, seed=8))
+    full = [t if t is None else t.requires_grad_() for t in (q, k, v, table, lam)]
+    leaves = [t for t in full if t is not None]
+
+    def run(rows, touch=None):
+        out = call(maps, *full, 2, causal=name == "q_start", **{name: rows})
+        if touch is not None:
+            rows.fill_(touch)
+        return torch.autograd.grad(out, leaves, dout)
+
+    i32 = lambda *n: torch.tensor(n, device=dev, dtype=torch.int32)  # noqa: E731
+    want = run(i32(30, 17))
+    with pytest.raises(RuntimeError, match="inplace"):
+        run(i32(30, 17), touch=5)
+    for got in (run(i32(30, 17).long(), touch=5), run(torch.tensor([30, 17]), touch=5)):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with torch.inference_mode():
+        rows = i32(30, 17)
+    assert all(torch.equal(a, b) for a, b in zip(run(rows), want))
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), lambda t: t.clone()):
+        assert all(torch.equal(a, b) for a, b in zip(run(i32(30, 17)), want))
+
+
+@pytest.mark.gpu
+def test_residual_norm_lengths_refilled_before_backward_are_refused(dev):
+    from promptttspp_amd import functional as PF
+
+    g = torch.Generator(device=dev).manual_seed(4)
+    r = lambda *s: torch.randn(*s, device=dev, generator=g)  # noqa: E731
+    leaves = [r(2, 30, 64).requires_grad_(), r(2, 30, 64).requires_grad_(), r(64).requires_grad_(), r(64).requires_grad_()]
+    dy, dz = r(2, 30, 64), r(2, 30, 64)
+
+    def run(rows, touch=None):
+        out = PF.residual_norm(leaves[0], leaves[1], post=(leaves[2], None), pre=(leaves[3], None), lengths=rows)
+        if touch is not None:
+            rows.fill_(touch)
+        return torch.autograd.grad(out, leaves, (dy, dz))
+
+    want = run(torch.tensor([22, 9], device=dev, dtype=torch.int32))
+    with pytest.raises(RuntimeError, match="inplace"):
+        run(torch.tensor([22, 9], device=dev, dtype=torch.int32), touch=30)
+    with torch.inference_mode():
+        rows = torch.tensor([22, 9], device=dev, dtype=torch.int32)
+    for got in (run(torch.tensor([22, 9], device=dev), touch=30), run(rows)):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), lambda t: t.clone()):
+        assert all(torch.equal(a, b) for a, b in zip(run(torch.tensor([22, 9], device=dev, dtype=torch.int32)), want))
+
+
 def test_bucket_edges_are_the_whole_number_solution():
     from promptttspp_amd import ops
 
