@@ -11,7 +11,7 @@ from operator import index
 from types import SimpleNamespace
 
 import torch
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
@@ -1032,6 +1032,28 @@ def _saved_rows(rows):
     return [t.clone() if t is not None and t.is_inference() else t for t in rows]
 
 
+def _watched(tensors):
+    """Whether a call has to be an autograd node: a gradient is wanted, a trace records it (a launch on bare addresses leaves no trace), or a
+    forward-mode level is open (the node refuses a tangent that a bare launch would drop)"""
+    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) or torch._C._is_tracing() \
+        or forward_ad._current_level >= 0
+
+
+class _untraced:
+    """While a call's arguments are checked a trace is put aside: the sizes of its tensors are plain numbers then, as ctypes needs them"""
+
+    __slots__ = ("state",)
+
+    def __enter__(self):
+        self.state = torch._C._get_tracing_state()
+        if self.state is not None:
+            torch._C._set_tracing_state(None)
+
+    def __exit__(self, *exc):
+        if self.state is not None:
+            torch._C._set_tracing_state(self.state)
+
+
 def _number(x, what):
     """``x`` as the plain number that the kernels take by value (a tensor in its place would lose its gradient)"""
     if torch.is_tensor(x) and x.requires_grad:
@@ -1044,17 +1066,17 @@ def _packed(t):
     return t if t is None or (t.is_contiguous() and not t.data_ptr() & 15) else t.clone(memory_format=torch.contiguous_format)
 
 
-def _attention_cfg(maps, heads, kv_heads, max_distance, bidirectional, lam_init, lengths, q_lengths, q_start, causal, scale):
+def _attention_cfg(maps, heads, kv_heads, max_distance, bidirectional, lam_init, causal, scale):
     return SimpleNamespace(heads=index(heads), kv_heads=index(heads if kv_heads is None else kv_heads), maps=maps, max_distance=index(max_distance),
-                           bidirectional=bool(bidirectional), lam_init=_number(lam_init, "attention: lam_init"), lengths=lengths, q_lengths=q_lengths,
-                           q_start=q_start, causal=bool(causal), scale=None if scale is None else _number(scale, "attention: scale"))
+                           bidirectional=bool(bidirectional), lam_init=_number(lam_init, "attention: lam_init"), causal=bool(causal),
+                           scale=None if scale is None else _number(scale, "attention: scale"))
 
 
 class AttentionLongFn(Function):
     @staticmethod
-    def forward(ctx, q, k, v, table, lam, cfg):
-        op = _attention_long_op(q, k, v, _f32_view(table), _f32_view(lam), cfg)
-        out, lse, out2 = op.forward(q, True)
+    def forward(ctx, q, k, v, table, lam, lengths, q_lengths, q_start, cfg):
+        op = _attention_long_op(q, k, v, _f32_view(table), _f32_view(lam), (lengths, q_lengths, q_start), cfg)
+        out, lse, out2 = op.forward(q, any(ctx.needs_input_grad))
         ctx.cfg, ctx.op = cfg, op
         ctx.direct = None
         if _direct["on"]:
@@ -1071,7 +1093,7 @@ class AttentionLongFn(Function):
         op = ctx.op
         names = ("q", "table", "lam", "k_lengths", "q_lengths", "q_start") if k is None else ("q", "table", "lam", "k_lengths", "q_lengths", "q_start", "k", "v")
         if not _still(op.args, names, (q, table, lam, *rows, k, v)):
-            op = _attention_long_op(q, k, v, _f32_view(table), _f32_view(lam), ctx.cfg, rows)
+            op = _attention_long_op(q, k, v, _f32_view(table), _f32_view(lam), rows, ctx.cfg)
         dout = _packed(dout)
         direct = ctx.direct is not None
         dt, dl = [None if p is None else p.grad if direct else lse.new_empty(p.shape) for p in (table, lam)]
@@ -1079,28 +1101,28 @@ class AttentionLongFn(Function):
         if direct:
             for p in ctx.direct:
                 _done(p)
-            return dq, dk, dv, None, None, None
+            return dq, dk, dv, None, None, None, None, None, None
         if dt is not None and table.dtype is not torch.float32:
             dt = dt.to(table.dtype)
         if dl is not None and lam.dtype is not torch.float32:
             dl = dl.to(lam.dtype)
-        return dq, dk, dv, dt, dl, None
+        return dq, dk, dv, dt, dl, None, None, None, None
 
 
-def _attention_long_op(q, k, v, table, lam, cfg, rows=None):
-    lengths, q_lengths, q_start = (cfg.lengths, cfg.q_lengths, cfg.q_start) if rows is None else rows
-    return ops.AttentionLong(q, k, v, cfg.heads, cfg.kv_heads, cfg.maps, table, cfg.max_distance, cfg.bidirectional, lam, cfg.lam_init, lengths,
-                             q_lengths, q_start, cfg.causal, cfg.scale)
+def _attention_long_op(q, k, v, table, lam, rows, cfg):
+    with _untraced():
+        return ops.AttentionLong(q, k, v, cfg.heads, cfg.kv_heads, cfg.maps, table, cfg.max_distance, cfg.bidirectional, lam, cfg.lam_init, *rows,
+                                 cfg.causal, cfg.scale)
 
 
-def _attention_long(q, k, v, table, lam, cfg):
+def _attention_long(q, k, v, table, lam, lengths, q_lengths, q_start, cfg):
     if (k is None) != (v is None):
         raise ValueError("attention: give q, k, v, or one fused q | k | v tensor and neither k nor v")
-    if k is None and cfg.q_lengths is None:
-        cfg.q_lengths = cfg.lengths
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, table, lam)):
-        return AttentionLongFn.apply(q, k, v, table, lam, cfg)
-    return _attention_long_op(q, k, v, _f32_view(table), _f32_view(lam), cfg).forward(q, False)[0]
+    if k is None and q_lengths is None:
+        q_lengths = lengths
+    if _watched((q, k, v, table, lam)):
+        return AttentionLongFn.apply(q, k, v, table, lam, lengths, q_lengths, q_start, cfg)
+    return _attention_long_op(q, k, v, _f32_view(table), _f32_view(lam), (lengths, q_lengths, q_start), cfg).forward(q, False)[0]
 
 
 def attention_bucket(q, k, v, table, heads, kv_heads=None, max_distance=128, bidirectional=True, lengths=None, q_lengths=None, q_start=None,
@@ -1119,8 +1141,8 @@ def attention_bucket(q, k, v, table, heads, kv_heads=None, max_distance=128, bid
     as has a gradient: it may still be multiplied by zero.  ``scale``: positive, default dk ** -0.5.  Memory O(Tq + Tk) in both directions."""
     if table is None:
         raise ValueError("attention_bucket: needs a position table")
-    cfg = _attention_cfg(1, heads, kv_heads, max_distance, bidirectional, 0.0, lengths, q_lengths, q_start, causal, scale)
-    return _attention_long(q, k, v, table, None, cfg)
+    cfg = _attention_cfg(1, heads, kv_heads, max_distance, bidirectional, 0.0, causal, scale)
+    return _attention_long(q, k, v, table, None, lengths, q_lengths, q_start, cfg)
 
 
 def attention_diff(q, k, v, lam, lam_init, heads, kv_heads=None, table=None, max_distance=128, bidirectional=True, lengths=None, q_lengths=None,
@@ -1133,18 +1155,18 @@ def attention_diff(q, k, v, lam, lam_init, heads, kv_heads=None, table=None, max
     both maps.  Everything else as there.  The norm over a head that usually follows is ``residual_norm`` without a residual."""
     if lam is None:
         raise ValueError("attention_diff: needs the lam vectors")
-    cfg = _attention_cfg(2, heads, kv_heads, max_distance, bidirectional, lam_init, lengths, q_lengths, q_start, causal, scale)
-    return _attention_long(q, k, v, table, lam, cfg)
+    cfg = _attention_cfg(2, heads, kv_heads, max_distance, bidirectional, lam_init, causal, scale)
+    return _attention_long(q, k, v, table, lam, lengths, q_lengths, q_start, cfg)
 
 
 class ResidualNormFn(Function):
     @staticmethod
-    def forward(ctx, f, x, gate, post_g, post_b, pre_g, pre_b, cfg):
+    def forward(ctx, f, x, gate, post_g, post_b, pre_g, pre_b, lengths, cfg):
         ctx.set_materialize_grads(False)
         f, x = _packed(f), _packed(x)
         params = (gate, post_g, post_b, pre_g, pre_b)
-        op = _residual_norm_op(f, x, params, cfg, cfg.lengths)
-        y, z, stats = op.forward(f, True)
+        op = _residual_norm_op(f, x, params, lengths, cfg)
+        y, z, stats = op.forward(f, any(ctx.needs_input_grad))
         ctx.cfg, ctx.op = cfg, op
         ctx.direct = None
         if _direct["on"]:
@@ -1161,7 +1183,7 @@ class ResidualNormFn(Function):
         need = ctx.needs_input_grad
         op = ctx.op
         if not _still(op.args, ("f", "x", "gate", "post_g", "post_b", "pre_g", "pre_b", "lengths"), (f, x, *params, lengths)):
-            op = _residual_norm_op(f, x, params, ctx.cfg, lengths)
+            op = _residual_norm_op(f, x, params, lengths, ctx.cfg)
         dy, dz = _packed(dy), _packed(dz)
         want = need[2:7]
         if ctx.direct is not None:
@@ -1169,9 +1191,9 @@ class ResidualNormFn(Function):
             df, dx, _ = op.backward(f, stats, dy, dz, need[0], need[1], want, into)
             for p in ctx.direct:
                 _done(p)
-            return df, dx, None, None, None, None, None, None
+            return df, dx, None, None, None, None, None, None, None
         df, dx, fresh = op.backward(f, stats, dy, dz, need[0], need[1], want)
-        grads, i = [df, dx, None, None, None, None, None, None], 0
+        grads, i = [df, dx, None, None, None, None, None, None, None], 0
         for k, p in enumerate(params):
             if want[k]:
                 g = fresh[i]
@@ -1192,8 +1214,9 @@ def _flat(p):
     return p if n == 1 or (n == 2 and p.shape[0] != 1) else p.view(-1)
 
 
-def _residual_norm_op(f, x, params, cfg, lengths):
-    return ops.ResidualNorm(f, x, [_flat(p) for p in params], cfg.scale, cfg.eps, cfg.kind, lengths)
+def _residual_norm_op(f, x, params, lengths, cfg):
+    with _untraced():
+        return ops.ResidualNorm(f, x, [_flat(p) for p in params], cfg.scale, cfg.eps, cfg.kind, lengths)
 
 
 def residual_norm(f, x=None, gate=None, post=None, pre=None, scale=1.0, eps=1e-5, kind="layer", lengths=None):
@@ -1206,13 +1229,13 @@ def residual_norm(f, x=None, gate=None, post=None, pre=None, scale=1.0, eps=1e-5
     computed from the unrounded y."""
     post_g, post_b = post if post is not None else (None, None)
     pre_g, pre_b = pre if pre is not None else (None, None)
-    cfg = SimpleNamespace(scale=_number(scale, "residual_norm: scale"), eps=_number(eps, "residual_norm: eps"), kind=kind, lengths=lengths)
+    cfg = SimpleNamespace(scale=_number(scale, "residual_norm: scale"), eps=_number(eps, "residual_norm: eps"), kind=kind)
     params = (gate, post_g, post_b, pre_g, pre_b)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (f, x, *params)):
-        r = ResidualNormFn.apply(f, x, *params, cfg)
+    if _watched((f, x, *params)):
+        r = ResidualNormFn.apply(f, x, *params, lengths, cfg)
         return r if pre_g is not None else (r, None)
     f = _packed(f)
-    y, z, _ = _residual_norm_op(f, _packed(x), params, cfg, cfg.lengths).forward(f, False)
+    y, z, _ = _residual_norm_op(f, _packed(x), params, lengths, cfg).forward(f, False)
     return y, z
 
 

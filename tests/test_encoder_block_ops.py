@@ -570,6 +570,77 @@ def test_residual_norm_lengths_refilled_before_backward_are_refused(dev):
         assert all(torch.equal(a, b) for a, b in zip(run(torch.tensor([22, 9], device=dev, dtype=torch.int32)), want))
 
 
+def _tangent_calls(dev):
+    """every operator with one input that carries a tangent and nothing that requires a gradient"""
+    from promptttspp_amd import functional as PF
+
+    z = lambda *s: torch.zeros(*s, device=dev)  # noqa: E731
+    dual = lambda t: torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+    return [lambda: PF.attention_bucket(dual(z(1, 4, 96)), None, None, z(16, 1), 1), lambda: PF.attention_bucket(z(1, 4, 96), None, None, dual(z(16, 1)), 1),
+            lambda: PF.attention_diff(z(1, 4, 96), None, None, dual(z(4, 1, 16)), 0.1, 1), lambda: PF.residual_norm(dual(z(1, 4, 32)), pre=(z(32), None)),
+            lambda: PF.residual_norm(z(1, 4, 32), gate=dual(z(32)))]
+
+
+def test_open_forward_levels_and_traces_make_nodes(monkeypatch):
+    """(no GPU: where the calls go) a tangent or a trace never meets a launch that passes autograd by"""
+    from promptttspp_amd import functional as PF
+
+    class Node(Exception):
+        pass
+
+    def node(*a):
+        raise Node
+
+    for fn in (PF.AttentionLongFn, PF.ResidualNormFn):
+        monkeypatch.setattr(fn, "apply", node)
+    with torch.autograd.forward_ad.dual_level():
+        for f in _tangent_calls("cpu"):
+            with pytest.raises(Node):
+                f()
+    t = torch.zeros(16, 1)
+    for f in (lambda x: PF.attention_bucket(x, None, None, t, 1), lambda x: PF.residual_norm(x)[0]):
+        with torch.no_grad(), pytest.raises(Node):
+            torch.jit.trace(f, (torch.zeros(1, 4, 96),), check_trace=False)
+
+
+@pytest.mark.gpu
+def test_tangents_are_refused(dev):
+    with torch.autograd.forward_ad.dual_level():
+        for f in _tangent_calls(dev):
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                f()
+    for f in _tangent_calls(dev):  # (no level open: make_dual refuses, nothing else is left behind)
+        with pytest.raises(RuntimeError):
+            f()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("grad", [False, True])
+def test_traced_calls_run_the_kernels(dev, grad):
+    """a traced function computes what the function computes, with other inputs, other lengths and their gradients too"""
+    from promptttspp_amd import functional as PF
+
+    g = torch.Generator(device=dev).manual_seed(6)
+    r = lambda *s: torch.randn(*s, device=dev, generator=g)  # noqa: E731
+    ws = [t.requires_grad_(grad) for t in (r(16, 2), 0.2 * r(4, 1, 32), r(2, 128), r(128))]
+
+    def fun(x, lengths, table, lam, gate, w):  # (torch takes nothing that requires a gradient as a constant of a trace)
+        a = PF.attention_bucket(x, None, None, table, 2, lengths=lengths)
+        b = PF.attention_diff(x, None, None, lam, 0.3, 2, lengths=lengths, causal=True)
+        return PF.residual_norm(a, b, gate=gate, post=(w, None), pre=(w, None), kind="rms", lengths=lengths)
+
+    inputs = [(r(2, 50, 384), torch.tensor(n, device=dev, dtype=torch.int32)) for n in ([50, 31], [7, 50], [0, 1])]
+    with torch.set_grad_enabled(grad):
+        traced = torch.jit.trace(fun, (*inputs[0], *ws), check_trace=False)
+        for x, n in inputs:
+            got, want = traced(x, n, *ws), fun(x, n, *ws)
+            for a, b in zip(got, want):
+                assert torch.equal(a, b)
+            if grad:
+                for a, b in zip(torch.autograd.grad(got[0].sum() + got[1].square().sum(), ws), torch.autograd.grad(want[0].sum() + want[1].square().sum(), ws)):
+                    assert torch.equal(a, b)
+
+
 def test_bucket_edges_are_the_whole_number_solution():
     from promptttspp_amd import ops
 
