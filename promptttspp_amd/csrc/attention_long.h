@@ -96,7 +96,8 @@ struct LOp<float> {
 };
 
 // CH consecutive registers of a 32 x 32 result -> a fragment.  16-bit: probabilities and dS are rounded to the element type
-// (to nearest) because the matrix instruction takes both operands in it; their sums (softmax denominator, D) use the f32 values.
+// (to nearest; dS in f16 scaled: LScale) because the matrix instruction takes both operands in it; their sums (softmax denominator, D)
+// use the f32 values.
 template <typename E>
 __device__ __forceinline__ uint4 la_pack(const f32x16& v, int s) {
   if constexpr (sizeof(E) == 4) {
@@ -115,6 +116,53 @@ __device__ __forceinline__ uint4 la_pack_rest(const f32x16& v, int s, uint4 f) {
   for (int i = 0; i < 4; ++i) o[i] = LOp<E>::pk(v[8 * s + 2 * i] - LOp<E>::lo(r[i]), v[8 * s + 2 * i + 1] - LOp<E>::hi(r[i]));
   return uint4{o[0], o[1], o[2], o[3]};
 }
+__device__ __forceinline__ float la_half_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float la_half_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// f16: dS as an operand.  dS = P (dP - D) is about 1 / keys of the gradient that arrives, and f16 ends at 2^-24 (2^-14 with all its bits) and
+// 65504: unscaled, gradients of 1e-4 on 2000 keys kept four bits, smaller ones none.  A column of dS -- one query in dq, one key in dk --
+// goes through the product times a power of two, its accumulators with it: the column's largest value so far lies in [2^11, 2^15], so a
+// term loses at most 2^-36 of it beside its own rounding.  The scale is set by the first patch and lowered when a later one passes 2^15 (the
+// accumulators follow, exactly); the other element types have f32's range and take none.  P needs none either: its rows add up to one.
+// Price: backward of 24 x 833-1250 of 4 x 64 206 -> 220 us, of 8 x 1333-2000 differential 391 -> 410 us, of 32 x 145-217 of 2 x 128 none.
+template <typename E>
+struct LScale {
+  template <int NT>
+  __device__ __forceinline__ void apply(f32x16&, f32x16 (&)[NT]) {}
+  __device__ __forceinline__ float undo(float v) const { return v; }
+};
+template <>
+struct LScale<f16_raw> {
+  float mul = 1.f, lim = 0.f;  // values up to lim stay below 2^15 when scaled
+  template <int NT>
+  __device__ __forceinline__ void apply(f32x16& s, f32x16 (&acc)[NT]) {
+    float m = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) m = fmaxf(m, fabsf(s[r]));
+    m = la_half_max(m);
+    if (__any(m > lim)) {
+      const int old = (int)(__float_as_uint(mul) >> 23), e = (int)(__float_as_uint(m) >> 23);  // exponents with their offset of 127
+      const int now = m > lim ? min(127 + 11 - (e - 127), 227) : old;                          // (10 .. 227: an infinity has e = 255)
+      mul = __uint_as_float((uint32_t)now << 23);
+      lim = m > lim ? __uint_as_float((uint32_t)min(127 + 15 - (now - 127), 254) << 23) : lim;
+      const float ratio = __uint_as_float((uint32_t)min(max(now - old + 127, 0), 254) << 23);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[n][r] *= ratio;
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] *= mul;
+  }
+  __device__ __forceinline__ float undo(float v) const { return v * __uint_as_float((254u << 23) - __float_as_uint(mul)); }
+};
+
 // dot product of two fragments in f32
 template <typename E>
 __device__ __forceinline__ float la_dot(uint4 a, uint4 b) {
@@ -262,15 +310,6 @@ __device__ __forceinline__ void la_barrier() { asm volatile("s_waitcnt lgkmcnt(0
 __device__ __forceinline__ float la_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 // wave number, known to be the same in all lanes: what depends on it alone is scalar work and scalar branches
 __device__ __forceinline__ int la_wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
-__device__ __forceinline__ float la_half_sum(float v) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-__device__ __forceinline__ float la_half_max(float v) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-
 // bucket of a distance d = key position - query position (Raffel et al. 2020: half of the buckets per direction, the first
 // nexact distances one each, then logarithmic steps up to max_distance; the steps' first distances come from the host as whole
 // numbers, so no logarithm is rounded here)

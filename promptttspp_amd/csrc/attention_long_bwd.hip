@@ -120,6 +120,7 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
   for (int m = 0; m < MAPS; ++m)
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[m][n] = f32x16{};
+  LScale<E> sc[MAPS];
   const float c2 = p.scale * LA_LOG2E;
   const int q0 = qs + i0, D = p.max_distance;
 
@@ -159,6 +160,7 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
         e += s[r];
       }
       eps[m] += e;
+      sc[m].apply(s, acc[m]);
 #pragma unroll
       for (int st = 0; st < PS; ++st) {
         const uint4 f = la_pack<E>(s, st);
@@ -198,7 +200,7 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) mine[(n * 16 + r) * 64] = acc[m][n][r];
+        for (int r = 0; r < 16; ++r) mine[(n * 16 + r) * 64] = sc[m].undo(acc[m][n][r]);
     }
     static_assert(MAPS * NT * 1024 * 4 <= NB * BUF * (int)sizeof(E), "a wave's sums fit its buffers");
     la_barrier();
@@ -260,7 +262,7 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
         const int ch = 32 * n + 8 * g + 4 * hw;
         float v[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = live[m] ? acc[m][n][4 * g + e] * c : 0.f;
+        for (int e = 0; e < 4; ++e) v[e] = live[m] ? sc[m].undo(acc[m][n][4 * g + e]) * c : 0.f;
         if (ch < p.dk) la_store4<E>(qo + m * p.dk + ch, v[0], v[1], v[2], v[3]);
       }
   }
@@ -391,6 +393,7 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
     for (int n = 0; n < NK; ++n) ak[m][n] = f32x16{};
 #pragma unroll
   for (int n = 0; n < NV; ++n) av[n] = f32x16{};
+  LScale<E> sc[MAPS];
   const float c2 = p.scale * LA_LOG2E;
   const int D = p.max_distance;
   float far_lo = 0.f, far_hi = 0.f, lam = 0.f;
@@ -493,7 +496,8 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
       }
     }
 #pragma unroll
-    for (int m = 0; m < MAPS; ++m)
+    for (int m = 0; m < MAPS; ++m) {
+      sc[m].apply(s[m], ak[m]);
 #pragma unroll
       for (int st = 0; st < PS; ++st) {
         const uint4 f = la_pack<E>(s[m], st);
@@ -506,6 +510,7 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
           if (F32) __builtin_amdgcn_sched_barrier(0);
         }
       }
+    }
 #pragma unroll
     for (int st = 0; st < PS; ++st) {
       const uint4 f = la_pack<E>(w, st);
@@ -591,7 +596,7 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
 #pragma unroll
       for (int n = 0; n < NK; ++n)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) mine[((m * NK + n) * 16 + r) * 64] = ak[m][n][r];
+        for (int r = 0; r < 16; ++r) mine[((m * NK + n) * 16 + r) * 64] = sc[m].undo(ak[m][n][r]);
 #pragma unroll
     for (int n = 0; n < NV; ++n)
 #pragma unroll
@@ -634,7 +639,7 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
         if (ch < p.dk) {
           float v[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = on ? ak[m][n][4 * g + e] * p.scale : 0.f;
+          for (int e = 0; e < 4; ++e) v[e] = on ? sc[m].undo(ak[m][n][4 * g + e]) * p.scale : 0.f;
           la_store4<E>(ko + m * p.dk + ch, v[0], v[1], v[2], v[3]);
         }
       }

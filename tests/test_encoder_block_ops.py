@@ -359,6 +359,34 @@ def test_batches_that_fill_the_chip(dev, dtype, maps, dk, causal):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("maps,dk", [(1, 64), (1, 128), (2, 32), (2, 64)])
+@pytest.mark.parametrize("B,T", [(1, 700), (16, 500)])
+@pytest.mark.parametrize("power", [-14, -9, 12])
+def test_f16_gradients_of_any_size(dev, maps, dk, B, T, power):
+    """Gradients that arrive at 2^-14 (what they are without a loss scale) to 2^12 keep the accuracy of those of order one.  The bounds are those
+    of the same gradient times 2^20, divided by it -- dS is an operand whose 2^-25 per term then counts for nothing, since a column of it
+    is scaled to 2^11 and more, and its error is 2^-36 of the column's largest term -- and the output's own rounding, 2^-25 below 2^-14."""
+    H = 2
+    q, k, v, table, lam, dout = make(maps, torch.float16, B, T, T, H, H, dk, 32, seed=4)
+    dout = (dout.double() * 2.0 ** power).half()
+    lens = [T - 11 * b for b in range(B)]
+    up = 2.0 ** 20
+    ref = RefAttention(q, k, v, table, lam, 0.35, dout.double() * up, H, H, maps, dt=torch.float16, lengths=lens, q_lengths=lens)
+    out_tiny = 2.0 ** -25
+    leaves = [t.to(dev).requires_grad_() for t in (q, k, v, table) + ((lam,) if maps == 2 else ())]
+    full = leaves + [None] * (5 - len(leaves))
+    rows = torch.tensor(lens, device=dev, dtype=torch.int32)
+    out = call(maps, *full, H, lengths=rows, q_lengths=rows)
+    grads = torch.autograd.grad(out, leaves, dout.to(dev))
+    for n, t in zip(("dq", "dk", "dtable") + (("dlam",) if maps == 2 else ()), grads[:2] + grads[3:]):
+        within(t, ref.g[n] / up, ref.b[n] / up + (out_tiny if n in ("dq", "dk") else 0.0), n)
+    # P is not scaled: a term of dv is off by half a step of f16, 2^-25, of the gradient that it weighs
+    weigh = dout.double().abs().view(B, T, H, -1) * (torch.arange(T)[None] < torch.tensor(lens)[:, None])[:, :, None, None]
+    c = 1.0 if maps == 1 else 2.0 * (1.0 + float(((lam.double()[0] * lam.double()[1]).sum(-1).exp() + (lam.double()[2] * lam.double()[3]).sum(-1).exp()).max()))
+    within(grads[2], ref.g["dv"] / up, ref.b["dv"] / up + out_tiny * (1 + c * weigh.sum(1, keepdim=True).expand(B, T, H, -1).reshape(B, T, -1)), "dv")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("maps", [1, 2])
 def test_full_batches_of_unequal_sides(dev, maps):
     """few queries against many keys and the other way round in batches large enough for either launch shape of either pass"""
