@@ -303,7 +303,8 @@ class SandwichStack(nn.Module):
     x <- x + residual_scale * gate * norm(sub-layer(z)), z <- norm(x) in one launch; the last z is the output.
 
     ``cond_channels``: the conditioning vector g (B, 1, cond_channels) gates every sub-layer through one projection (zero at the start:
-    the learned gates alone), gate = learned + projection(g)."""
+    the learned gates alone), gate = learned + projection(g).  Such a stack is always called with g; the acoustic model's encoder slot has
+    none to give, so there the gates are the learned ones (no ``cond_channels``)."""
 
     def __init__(self, channels, num_head, num_layers, kernel_size, dropout, scale, attention, num_buckets, max_distance, kv_heads, residual_scale,
                  cond_channels):
@@ -323,6 +324,8 @@ class SandwichStack(nn.Module):
 
     def _gates(self, g):
         if g is None:
+            if self.cond is not None:
+                raise ValueError("norm='sandwich' was built with cond_channels: it needs the conditioning vector (its projection would never learn)")
             return [s.gate for s in self.steps]
         if self.cond is None or g.shape[1] != 1:
             raise ValueError("norm='sandwich' takes its conditioning as one vector per utterance, through gates (cond_channels)")

@@ -271,3 +271,14 @@ def test_forms_and_defaults():
     for kw in (dict(attention="other"), dict(norm="other"), dict(norm="sandwich"), dict(norm="sandwich", attention=None)):
         with pytest.raises(ValueError):
             Transformer(256, 2, 1, 3, 0.1, **kw)
+
+
+def test_a_conditioned_stack_needs_its_conditioning():
+    from promptttspp_amd.modules.transformer import Transformer
+
+    x, g = torch.zeros(2, 5, 64), torch.zeros(2, 1, 16)
+    kw = dict(attention="bucket", norm="sandwich")
+    with pytest.raises(ValueError, match="conditioning vector"):
+        Transformer(64, 2, 1, 3, 0.1, cond_channels=16, **kw).forward_cl(x, None)
+    with pytest.raises(ValueError, match="cond_channels"):
+        Transformer(64, 2, 1, 3, 0.1, **kw).forward_cl(x, None, g)
