@@ -526,6 +526,44 @@ def test_attention_only_some_inputs_need_gradients(dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("maps,buckets,lam_heads", [(1, 32, 1), (2, 32, 1), (2, 32, 4), (2, 0, 4), (2, 0, 1)])
+@pytest.mark.parametrize("B,T", [(2, 70), (40, 140)])
+def test_parameter_gradients_added_in_place(dev, maps, buckets, lam_heads, B, T):
+    """with the flat gradient buffer two passes leave exactly twice the gradient of the table and of the lam vectors (the sums have a fixed order,
+    and doubling is exact); the inputs' gradients come back as ever, and a parameter that is frozen stays out"""
+    from promptttspp_amd import functional as PF
+    from promptttspp_amd.parallel import FlatGradReducer
+
+    heads = 4
+    q, k, v, table, lam, dout = (t if t is None else t.to(dev) for t in make(maps, torch.float32, B, T, T, heads, 2, 32, buckets, seed=7, lam_heads=lam_heads))
+    table, lam = (None if t is None else torch.nn.Parameter(t) for t in (table, lam))
+    params = [p for p in (table, lam) if p is not None]
+    q.requires_grad_()
+    want = torch.autograd.grad(call(maps, q, k, v, table, lam, heads, kv_heads=2, causal=True), [q, *params], dout)
+    assert all(bool(g.any()) for g in want)
+    try:
+        red = FlatGradReducer(params)
+        red.zero_grad()
+        for _ in range(2):
+            q.grad = None
+            call(maps, q, k, v, table, lam, heads, kv_heads=2, causal=True).backward(dout)
+        red.finish()
+        torch.cuda.synchronize()
+        assert torch.equal(q.grad, want[0])
+        for p, w in zip(params, want[1:]):
+            assert torch.equal(p.grad, 2 * w)
+        if len(params) == 2:
+            red.zero_grad()
+            table.requires_grad_(False)
+            call(maps, q, k, v, table, lam, heads, kv_heads=2, causal=True).backward(dout)
+            red.finish()
+            torch.cuda.synchronize()
+            assert torch.equal(lam.grad, want[2]) and not table.grad.any()
+    finally:
+        PF.enable_direct_grads(False)
+
+
+@pytest.mark.gpu
 def test_long_batch_strides_pass_32_bits(dev):
     """the second utterance of a kept memory lies more than 2^31 elements behind the first"""
     from promptttspp_amd import functional as PF
