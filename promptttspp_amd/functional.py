@@ -1075,7 +1075,8 @@ def _attention_cfg(maps, heads, kv_heads, max_distance, bidirectional, lam_init,
 class AttentionLongFn(Function):
     @staticmethod
     def forward(ctx, q, k, v, table, lam, lengths, q_lengths, q_start, cfg):
-        op = _attention_long_op(q, k, v, _f32_view(table), _f32_view(lam), (lengths, q_lengths, q_start), cfg)
+        with _untraced():
+            op = _attention_long_op(q, k, v, _f32_view(table), _f32_view(lam), (lengths, q_lengths, q_start), cfg)
         out, lse, out2 = op.forward(q, any(ctx.needs_input_grad))
         ctx.cfg, ctx.op = cfg, op
         ctx.direct = None
@@ -1110,9 +1111,8 @@ class AttentionLongFn(Function):
 
 
 def _attention_long_op(q, k, v, table, lam, rows, cfg):
-    with _untraced():
-        return ops.AttentionLong(q, k, v, cfg.heads, cfg.kv_heads, cfg.maps, table, cfg.max_distance, cfg.bidirectional, lam, cfg.lam_init, *rows,
-                                 cfg.causal, cfg.scale)
+    return ops.AttentionLong(q, k, v, cfg.heads, cfg.kv_heads, cfg.maps, table, cfg.max_distance, cfg.bidirectional, lam, cfg.lam_init, *rows,
+                             cfg.causal, cfg.scale)
 
 
 def _attention_long(q, k, v, table, lam, lengths, q_lengths, q_start, cfg):
@@ -1165,7 +1165,8 @@ class ResidualNormFn(Function):
         ctx.set_materialize_grads(False)
         f, x = _packed(f), _packed(x)
         params = (gate, post_g, post_b, pre_g, pre_b)
-        op = _residual_norm_op(f, x, params, lengths, cfg)
+        with _untraced():
+            op = _residual_norm_op(f, x, params, lengths, cfg)
         y, z, stats = op.forward(f, any(ctx.needs_input_grad))
         ctx.cfg, ctx.op = cfg, op
         ctx.direct = None
@@ -1215,8 +1216,7 @@ def _flat(p):
 
 
 def _residual_norm_op(f, x, params, lengths, cfg):
-    with _untraced():
-        return ops.ResidualNorm(f, x, [_flat(p) for p in params], cfg.scale, cfg.eps, cfg.kind, lengths)
+    return ops.ResidualNorm(f, x, [_flat(p) for p in params], cfg.scale, cfg.eps, cfg.kind, lengths)
 
 
 def residual_norm(f, x=None, gate=None, post=None, pre=None, scale=1.0, eps=1e-5, kind="layer", lengths=None):
