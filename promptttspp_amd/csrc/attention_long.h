@@ -128,8 +128,8 @@ __device__ __forceinline__ float la_half_max(float v) {
 // f16: dS as an operand.  dS = P (dP - D) is about 1 / keys of the gradient that arrives, and f16 ends at 2^-24 (2^-14 with all its bits) and
 // 65504: unscaled, gradients of 1e-4 on 2000 keys kept four bits, smaller ones none.  A column of dS -- one query in dq, one key in dk --
 // goes through the product times a power of two, its accumulators with it: the column's largest value so far lies in [2^11, 2^15], so a
-// term loses at most 2^-36 of it beside its own rounding.  The scale is set by the first patch and lowered when a later one passes 2^15 (the
-// accumulators follow, exactly); the other element types have f32's range and take none.  P needs none either: its rows add up to one.
+// term loses at most 2^-36 of it beside its own rounding.  The scale starts at 2^100 and is lowered when a patch passes 2^15 (the accumulators
+// follow, exactly); the other element types have f32's range and take none.  P needs none either: its rows add up to one.
 // Price: backward of 24 x 833-1250 of 4 x 64 206 -> 220 us, of 8 x 1333-2000 differential 391 -> 410 us, of 32 x 145-217 of 2 x 128 none.
 template <typename E>
 struct LScale {
@@ -139,19 +139,19 @@ struct LScale {
 };
 template <>
 struct LScale<f16_raw> {
-  float mul = 1.f, lim = 0.f;  // values up to lim stay below 2^15 when scaled
+  float mul = 0x1p100f;  // (the first value above 2^-85 lowers it)
   template <int NT>
   __device__ __forceinline__ void apply(f32x16& s, f32x16 (&acc)[NT]) {
     float m = 0.f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) m = fmaxf(m, fabsf(s[r]));
     m = la_half_max(m);
-    if (__any(m > lim)) {
-      const int old = (int)(__float_as_uint(mul) >> 23), e = (int)(__float_as_uint(m) >> 23);  // exponents with their offset of 127
-      const int now = m > lim ? min(127 + 11 - (e - 127), 227) : old;                          // (10 .. 227: an infinity has e = 255)
-      mul = __uint_as_float((uint32_t)now << 23);
-      lim = m > lim ? __uint_as_float((uint32_t)min(127 + 15 - (now - 127), 254) << 23) : lim;
-      const float ratio = __uint_as_float((uint32_t)min(max(now - old + 127, 0), 254) << 23);
+    const uint32_t old = __float_as_uint(mul) >> 23;  // exponents with their offset of 127
+    const bool over = m > __uint_as_float(min(127 + 15 + 127 - old, 254u) << 23);  // 2^15 / mul
+    if (__any(over)) {
+      const uint32_t now = over ? 127 + 11 + 127 - (__float_as_uint(m) >> 23) : old;  // (at least 10: an infinity's exponent is 255)
+      mul = __uint_as_float(now << 23);
+      const float ratio = __uint_as_float((uint32_t)max((int)(now - old) + 127, 0) << 23);  // (now <= old)
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll

@@ -10,7 +10,15 @@
 //
 // D_m: rows of dout . out_m give it only to the rounding of the kept 16-bit context.  That is enough to centre dS, but the table's
 // gradient is a sum with heavy cancellation (every row of dS adds up to zero), so the dq pass also sums P_m (dP - D_m') in f32 and
-// the dk / dv pass uses the corrected D_m.
+// the dk / dv pass uses the corrected D_m.  lam's gradient adds the D_1 of all rows (50000 of 8 x 1317-2000, of either sign), and takes that
+// sum as exact as its terms are, at no operation per pair (EXACT; error of such a D_1 against 64 bits 1.7e-7 -> 0.9e-7, of dlam 1.8e-4 -> 0.34e-4
+// where plain f32 has 0.9e-4; backward of 8 x 1333-2000 bf16 385 -> 389 us):
+//   - D' rounded to the grid of dP's largest values (la_grid): dP - D' is then exact, else it is rounded the same way for all pairs of a row;
+//   - P taken against lse - log2(keys) / 2, a whole number, instead of lse (la_half_lse): a row spread over n keys has scores log2(n) below lse,
+//     whose rounding would grow with that; the factor is applied to the row's sums;
+//   - the patches' sums added with their rounding errors carried along;
+//   - 16-bit: dP of every other row as the product with -dout.  The matrix instruction's 16-bit sums are rounded with a bias that does not
+//     follow their sign (D_1 came out 1.6e-9 too small on average, with dout and with -dout; f32 has none).
 #include "attention_long.h"
 
 namespace {
@@ -26,12 +34,20 @@ struct LBwd {
   static constexpr int NB = FEW ? LSplit<E, DK, DV, MAPS>::NB : 2;
 };
 
+// x rounded to the steps that f32 has at `size` (both f32; no excess precision or reassociation in the compiler's defaults)
+__device__ __forceinline__ float la_grid(float x, float size) {
+  const float c = 1.5f * __uint_as_float((uint32_t)min((int)(__float_as_uint(size) >> 23) + 1, 254) << 23);
+  return (x + c) - c;
+}
+__device__ __forceinline__ float la_half_lse(float lse, int keys) { return rintf(lse - 0.5f * log2f((float)max(keys, 1))); }
+
 template <typename E, int DK, int DV, int MAPS, bool BIAS, bool FEW>
 __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 4 ? 1 : 2) void attn_long_dq_kernel(const LongP p) {
   typedef LBwd<E, DK, DV, MAPS, FEW> X;
   constexpr int W = X::W, ROWS = X::ROWS, NB = X::NB;
   constexpr int CH = LOp<E>::CH, KS = DK / (2 * CH), VS = DV / (2 * CH), PS = 16 / CH, NT = DK / 32;
   constexpr bool TIGHT = sizeof(E) == 4 || MAPS * DV == 256 || FEW;  // registers are short: LDS addresses not kept across patches
+  constexpr bool EXACT = MAPS == 2, FLIP = EXACT && sizeof(E) == 2;  // D_1 as exact as its terms (head of this file)
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ double lred[LA_WAVES];
   __shared__ float weps[W][MAPS][32];
@@ -77,7 +93,7 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
   if constexpr (MAPS == 2) lam = la_lambda(p, h, lane);
 
   uint4 qf[MAPS][KS], df[VS];
-  float Dm[MAPS], lse[MAPS], eps[MAPS];
+  float Dm[MAPS], ref[MAPS], eps[MAPS], low = 0.f;  // ref: lse or its stand-in; eps, low: the sum and what its roundings left
   {
     const bool on = iq < qlen;
     const E* qb = reinterpret_cast<const E*>(p.q) + b * p.sq + (int64_t)h * MAPS * p.dk + (int64_t)iq * p.ldq;
@@ -91,13 +107,22 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
     const E* db = reinterpret_cast<const E*>(p.dout) + b * p.sdo + (int64_t)h * dv + (int64_t)iq * p.lddo;
     const E* ob = reinterpret_cast<const E*>(p.out) + b * p.so + (int64_t)h * dv + (int64_t)iq * p.ldo;
     const E* o2 = reinterpret_cast<const E*>(p.out2) + ((int64_t)b * p.Tq + iq) * ((int64_t)p.H * dv) + (int64_t)h * dv;
-    float d0 = 0.f, d1 = 0.f;
+    float d0 = 0.f, d1 = 0.f, dn = 0.f, vn = 0.f;
+    uint4 vf[EXACT ? VS : 1];
+    if constexpr (EXACT) {  // |v| of the first 32 keys and |dout|: dP's size
+#pragma unroll
+      for (int s = 0; s < VS; ++s) {
+        const int c = (2 * s + hw) * CH;
+        vf[s] = *(lq < kend && c < dv ? reinterpret_cast<const uint4*>(vb + (int64_t)lq * p.ldv + c) : g_conv_zero_page);
+      }
+    }
 #pragma unroll
     for (int s = 0; s < VS; ++s) {
       const int c = (2 * s + hw) * CH;
       df[s] = uint4{0, 0, 0, 0};
       if (on && c < dv) {
         df[s] = *reinterpret_cast<const uint4*>(db + c);
+        if constexpr (EXACT) dn += la_dot<E>(df[s], df[s]);
         d0 += la_dot<E>(df[s], *reinterpret_cast<const uint4*>(ob + c));
         if constexpr (MAPS == 2) d1 += la_dot<E>(df[s], *reinterpret_cast<const uint4*>(o2 + c));
       }
@@ -109,9 +134,27 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
       Dm[0] = fmaf(lam, d1, d0);
       Dm[MAPS - 1] = d1;
     }
+    float size = 0.f;
+    if constexpr (EXACT) {
+#pragma unroll
+      for (int s = 0; s < VS; ++s) vn += la_dot<E>(vf[s], vf[s]);
+      vn = la_half_sum(vn);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) vn = fmaxf(vn, __shfl_xor(vn, o, 64));
+      size = sqrtf(la_half_sum(dn)) * sqrtf(vn);
+    }
+    if constexpr (FLIP) {
+      const uint32_t flip = lq & 1 ? 0x80008000u : 0u;
+#pragma unroll
+      for (int s = 0; s < VS; ++s) df[s] = uint4{df[s].x ^ flip, df[s].y ^ flip, df[s].z ^ flip, df[s].w ^ flip};
+    }
 #pragma unroll
     for (int m = 0; m < MAPS; ++m) {
-      lse[m] = on ? p.lse[(((int64_t)m * p.B + b) * p.H + h) * p.TqP + iq] : INFINITY;
+      ref[m] = on ? p.lse[(((int64_t)m * p.B + b) * p.H + h) * p.TqP + iq] : INFINITY;
+      if (EXACT && m == MAPS - 1) {
+        ref[m] = la_half_lse(ref[m], klen);
+        Dm[m] = la_grid(Dm[m], size);
+      }
       eps[m] = 0.f;
     }
   }
@@ -121,7 +164,7 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[m][n] = f32x16{};
   LScale<E> sc[MAPS];
-  const float c2 = p.scale * LA_LOG2E;
+  const float c2 = p.scale * LA_LOG2E, sign = lq & 1 ? -1.f : 1.f;
   const int q0 = qs + i0, D = p.max_distance;
 
   // one 32 x 32 patch
@@ -142,9 +185,9 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
       if (BIAS && dmin < D && dmax > -D) {
         const float* bt = btab + (j0 - q0 - lr + 4 * hr + D + LA_PAD);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, bt[8 * (r >> 2) + (r & 3)]) - lse[m];
+        for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, bt[8 * (r >> 2) + (r & 3)]) - ref[m];
       } else {
-        const float bc = (BIAS ? btab[dmin >= D ? 2 * (D + LA_PAD) : 0] : 0.f) - lse[m];
+        const float bc = (BIAS ? btab[dmin >= D ? 2 * (D + LA_PAD) : 0] : 0.f) - ref[m];
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, bc);
       }
@@ -153,13 +196,15 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = 8 * (r >> 2) + (r & 3) < jend ? s[r] : -INFINITY;
       }
-      float e = 0.f;
+      float e[4] = {};
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        s[r] = la_exp2(s[r]) * (dp[r] - Dm[m]);
-        e += s[r];
+        s[r] = la_exp2(s[r]) * (FLIP ? fmaf(dp[r], sign, -Dm[m]) : dp[r] - Dm[m]);
+        e[r & 3] += s[r];
       }
-      eps[m] += e;
+      const float y = (e[0] + e[1]) + (e[2] + e[3]) - (EXACT && m == MAPS - 1 ? low : 0.f), t = eps[m] + y;
+      if (EXACT && m == MAPS - 1) low = (t - eps[m]) - y;  // (compensated: what the addition rounded away)
+      eps[m] = t;
       sc[m].apply(s, acc[m]);
 #pragma unroll
       for (int st = 0; st < PS; ++st) {
@@ -205,22 +250,28 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
     static_assert(MAPS * NT * 1024 * 4 <= NB * BUF * (int)sizeof(E), "a wave's sums fit its buffers");
     la_barrier();
 #pragma unroll
-    for (int m = 0; m < MAPS; ++m)
+    for (int m = 0; m < MAPS; ++m) {
+      eps[m] = 0.f;
 #pragma unroll
-      for (int w = 0; w < W; ++w) Dm[m] += weps[w][m][lq];
+      for (int w = 0; w < W; ++w) eps[m] += weps[w][m][lq];
+    }
   } else {
 #pragma unroll
-    for (int m = 0; m < MAPS; ++m) Dm[m] += la_half_sum(eps[m]);
+    for (int m = 0; m < MAPS; ++m) eps[m] = la_half_sum(eps[m]);
   }
   const bool stat = hw == 0 && (!FEW || wave == 0);
+  float fac[MAPS];  // from the stand-in to lse (read anew: the loop has no register to spare)
   bool live[MAPS];  // rows that are none, or see no key: zeros by selection, as in forward
 #pragma unroll
   for (int m = 0; m < MAPS; ++m) {
-    live[m] = iq < qlen && !(lse[m] == INFINITY);
-    if (stat && iq < p.TqP) p.D[(((int64_t)m * p.B + b) * p.H + h) * p.TqP + iq] = live[m] ? Dm[m] : 0.f;
+    const int64_t at = (((int64_t)m * p.B + b) * p.H + h) * p.TqP + iq;
+    const float lse = iq < qlen ? p.lse[at] : INFINITY;
+    live[m] = iq < qlen && !(lse == INFINITY);
+    fac[m] = EXACT && m == MAPS - 1 ? la_exp2(ref[m] - lse) : 1.f;
+    if (stat && iq < p.TqP) p.D[at] = live[m] ? fmaf(fac[m], eps[m], Dm[m]) : 0.f;
   }
   if constexpr (MAPS == 2) {  // this block's share of dlam = -sum_i D_1 (64 bits: the rows' terms cancel)
-    double s = stat && live[MAPS - 1] ? (double)Dm[MAPS - 1] : 0.0;
+    double s = stat && live[MAPS - 1] ? (double)Dm[MAPS - 1] + (double)fac[MAPS - 1] * (double)eps[MAPS - 1] : 0.0;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
     if (lane == 0) lred[wave] = s;
@@ -238,7 +289,7 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
     const float* all = reinterpret_cast<const float*>(smem) + lane;
     for (int g = wave; g < MAPS * NT * 4; g += W) {  // 4 registers = 4 channels at a time
       const int m = g / (NT * 4), ch = 32 * ((g >> 2) % NT) + 8 * (g & 3) + 4 * hw;
-      const float c = m == 0 ? p.scale : -lam * p.scale;
+      const float c = (m == 0 ? p.scale : -lam * p.scale) * (m == 0 ? fac[0] : fac[MAPS - 1]);
       const bool on = m == 0 ? live[0] : live[MAPS - 1];
       float v[4];
 #pragma unroll
@@ -254,7 +305,7 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
   }
 #pragma unroll
   for (int m = 0; m < MAPS; ++m) {
-    const float c = m == 0 ? p.scale : -lam * p.scale;
+    const float c = (m == 0 ? p.scale : -lam * p.scale) * fac[m];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll

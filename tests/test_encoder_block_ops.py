@@ -387,6 +387,24 @@ def test_f16_gradients_of_any_size(dev, maps, dk, B, T, power):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("dk", [32, 64])
+@pytest.mark.parametrize("B", [4, 12])
+def test_lam_gradient_follows_the_sign_of_the_gradient(dev, dtype, dk, B):
+    """Every rounding of the gradient of lam has to follow the sign of what arrives: a bias that does not adds up over all rows.  With each query
+    given twice (rows 2 i and 2 i + 1) the pairs' roundings are each other's mirror image, whatever the matrix instructions do: the gradient of
+    -dout is the negative one up to the order of a sum in 64 bits and one rounding to f32, 2^-24 of it"""
+    T, H = 700, 4
+    q, k, v, _, lam, dout = make(2, DT[dtype], B, T, T, H, H, dk, 0, seed=11)
+    q, dout = (t[:, ::2].repeat_interleave(2, dim=1).to(dev) for t in (q, dout))
+    k, v = k.to(dev), v.to(dev)
+    lam = lam.to(dev).requires_grad_()
+    out = call(2, q, k, v, None, lam, H)
+    plus, minus = (torch.autograd.grad(out, lam, g, retain_graph=True)[0] for g in (dout, -dout))
+    assert bool(((plus + minus).abs() <= 2.0 ** -22 * plus.abs()).all()), float(((plus + minus) / plus).abs().max())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("maps", [1, 2])
 def test_full_batches_of_unequal_sides(dev, maps):
     """few queries against many keys and the other way round in batches large enough for either launch shape of either pass"""
