@@ -8,7 +8,9 @@
 // differential: 132 and 265 us (dk / dv: its accumulators leave one wave per SIMD).  Counters of the former dk / dv: vector unit 33 %, matrix
 // 18 %, LDS 17 % busy, no bank conflicts, 1.45 waves per SIMD on average -- the second, partly empty round of blocks.
 //
-// D_m: rows of dout . out_m give it only to the rounding of the kept 16-bit context.  That is enough to centre dS, but the table's
+// D_m: rows of dout . out_m give it only to the rounding of the kept 16-bit context.  That is enough to centre dS where a row sees many keys
+// (in dq the centre's error is multiplied by the mean of their k), not where it sees few: up to LA_TWICE of them a first sweep of the block
+// corrects it.  But the table's
 // gradient is a sum with heavy cancellation (every row of dS adds up to zero), so the dq pass also sums P_m (dP - D_m') in f32 and
 // the dk / dv pass uses the corrected D_m.  lam's gradient adds the D_1 of all rows (50000 of 8 x 1317-2000, of either sign), and takes that
 // sum as exact as its terms are, at no operation per pair (EXACT; error of such a D_1 against 64 bits 1.7e-7 -> 0.9e-7, of dlam 1.8e-4 -> 0.34e-4
@@ -19,6 +21,8 @@
 //   - the patches' sums added with their rounding errors carried along;
 //   - 16-bit: dP of every other row as the product with -dout.  The matrix instruction's 16-bit sums are rounded with a bias that does not
 //     follow their sign (D_1 came out 1.6e-9 too small on average, with dout and with -dout; f32 has none).
+#include <type_traits>
+
 #include "attention_long.h"
 
 namespace {
@@ -33,6 +37,11 @@ struct LBwd {
   static constexpr int PATCHES = ROWS / 32;
   static constexpr int NB = FEW ? LSplit<E, DK, DV, MAPS>::NB : 2;
 };
+
+// Most keys of a block, 16-bit, for which the centre is corrected before dq is summed.  Error of dq against 64 bits, in units of its output's
+// rounding, without and with: 2-12 keys 1.6-3.4 and 1.4, 16-41 keys 1.5-1.6 and 1.4, 63-128 keys 1.5 and 1.4.  Backward, us: 32 x 64 of
+// 2 x 128 27.8 and 29.9, 200 x 64 of 4 x 64 49 and 53; up to 128 keys 200 x 128 of 4 x 64 would go from 74 to 82.
+constexpr int LA_TWICE = 64;
 
 // x rounded to the steps that f32 has at `size` (both f32; no excess precision or reassociation in the compiler's defaults)
 __device__ __forceinline__ float la_grid(float x, float size) {
@@ -93,7 +102,7 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
   if constexpr (MAPS == 2) lam = la_lambda(p, h, lane);
 
   uint4 qf[MAPS][KS], df[VS];
-  float Dm[MAPS], ref[MAPS], eps[MAPS], low = 0.f;  // ref: lse or its stand-in; eps, low: the sum and what its roundings left
+  float Dm[MAPS], ref[MAPS], eps[MAPS], low = 0.f, size = 0.f;  // ref: lse or its stand-in; eps, low: the sum and what its roundings left
   {
     const bool on = iq < qlen;
     const E* qb = reinterpret_cast<const E*>(p.q) + b * p.sq + (int64_t)h * MAPS * p.dk + (int64_t)iq * p.ldq;
@@ -134,7 +143,6 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
       Dm[0] = fmaf(lam, d1, d0);
       Dm[MAPS - 1] = d1;
     }
-    float size = 0.f;
     if constexpr (EXACT) {
 #pragma unroll
       for (int s = 0; s < VS; ++s) vn += la_dot<E>(vf[s], vf[s]);
@@ -167,8 +175,8 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
   const float c2 = p.scale * LA_LOG2E, sign = lq & 1 ? -1.f : 1.f;
   const int q0 = qs + i0, D = p.max_distance;
 
-  // one 32 x 32 patch
-  auto patch = [&](const E* kimg, const E* vimg, int ks, int j0) __attribute__((always_inline)) {
+  // one 32 x 32 patch; `sums`: only what corrects D'
+  auto patch = [&](auto sums, const E* kimg, const E* vimg, int ks, int j0) __attribute__((always_inline)) {
     const int ln = TIGHT ? la_opaque(lane) : lane, lr = ln & 31, hr = ln >> 5;
     f32x16 dp = f32x16{};
 #pragma unroll
@@ -205,36 +213,71 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
       const float y = (e[0] + e[1]) + (e[2] + e[3]) - (EXACT && m == MAPS - 1 ? low : 0.f), t = eps[m] + y;
       if (EXACT && m == MAPS - 1) low = (t - eps[m]) - y;  // (compensated: what the addition rounded away)
       eps[m] = t;
-      sc[m].apply(s, acc[m]);
+      if constexpr (!decltype(sums)::value) {
+        sc[m].apply(s, acc[m]);
 #pragma unroll
-      for (int st = 0; st < PS; ++st) {
-        const uint4 f = la_pack<E>(s, st);
+        for (int st = 0; st < PS; ++st) {
+          const uint4 f = la_pack<E>(s, st);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) acc[m][n] = LOp<E>::mma(la_tfrag<E, DK>(kimg + m * KIMG, 32 * ks, st, n, ln), f, acc[m][n]);
+          for (int n = 0; n < NT; ++n) acc[m][n] = LOp<E>::mma(la_tfrag<E, DK>(kimg + m * KIMG, 32 * ks, st, n, ln), f, acc[m][n]);
+        }
       }
       if (TIGHT) __builtin_amdgcn_sched_barrier(0);
     }
   };
 
-  if constexpr (FEW && BIAS) la_barrier();  // (the table; the loop itself has no barrier)
-  for (int tile = first, buf = 0; tile < nt; tile += STEP, buf ^= NB - 1) {
-    if constexpr (FEW) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the next buffer's last reads are done
-    if (NB == 1) {
-      issue(tile, 0);
-      glds_wait<0>();
-    } else if (tile + STEP < nt) {
-      issue(tile + STEP, buf ^ 1);
-      glds_wait<NDMA>();
-    } else {
-      glds_wait<0>();
-    }
-    if constexpr (!FEW) la_barrier();
-    const E* kimg = img + buf * BUF;
-    const E* vimg = kimg + MAPS * KIMG;
+  auto sweep = [&](auto sums) __attribute__((always_inline)) {
+    for (int tile = first, buf = 0; tile < nt; tile += STEP, buf ^= NB - 1) {
+      if constexpr (FEW) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the next buffer's last reads are done
+      if (NB == 1) {
+        issue(tile, 0);
+        glds_wait<0>();
+      } else if (tile + STEP < nt) {
+        issue(tile + STEP, buf ^ 1);
+        glds_wait<NDMA>();
+      } else {
+        glds_wait<0>();
+      }
+      if constexpr (!FEW) la_barrier();
+      const E* kimg = img + buf * BUF;
+      const E* vimg = kimg + MAPS * KIMG;
 #pragma unroll 1
-    for (int ks = 0; ks < X::PATCHES; ++ks) patch(kimg, vimg, ks, tile * ROWS + 32 * ks);
-    if constexpr (!FEW) la_barrier();
+      for (int ks = 0; ks < X::PATCHES; ++ks) patch(sums, kimg, vimg, ks, tile * ROWS + 32 * ks);
+      if constexpr (!FEW) la_barrier();
+    }
+  };
+  if constexpr (FEW && BIAS) la_barrier();  // (the table; the loop itself has no barrier)
+  if constexpr (sizeof(E) == 2) {
+    if (kend <= LA_TWICE) {  // (the whole block: kend is the same in all its waves)
+      sweep(std::true_type{});
+#pragma unroll
+      for (int m = 0; m < MAPS; ++m) {
+        eps[m] = la_half_sum(eps[m]);
+        if (FEW && hw == 0) weps[wave][m][lq] = eps[m];
+      }
+      if constexpr (FEW) {
+        la_barrier();
+#pragma unroll
+        for (int m = 0; m < MAPS; ++m) {
+          eps[m] = 0.f;
+#pragma unroll
+          for (int w = 0; w < W; ++w) eps[m] += weps[w][m][lq];
+        }
+        la_barrier();  // (weps is written again at the end)
+      }
+#pragma unroll
+      for (int m = 0; m < MAPS; ++m) {
+        const float lse = iq < qlen ? p.lse[(((int64_t)m * p.B + b) * p.H + h) * p.TqP + iq] : INFINITY;
+        const float d = EXACT && m == MAPS - 1 ? eps[m] * la_exp2(ref[m] - lse) : eps[m];
+        if (!(lse == INFINITY)) Dm[m] += d;
+        if (EXACT && m == MAPS - 1) Dm[m] = la_grid(Dm[m], size);
+        eps[m] = 0.f;
+      }
+      low = 0.f;
+      if (NB == 2 && first < nt) issue(first, 0);
+    }
   }
+  sweep(std::false_type{});
 
   if constexpr (FEW) {  // the waves' sums of this row
 #pragma unroll

@@ -387,6 +387,41 @@ def test_f16_gradients_of_any_size(dev, maps, dk, B, T, power):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("maps,dk", [(1, 64), (1, 128), (2, 32), (2, 64)])
+@pytest.mark.parametrize("B,T", [(3, 2), (3, 7), (3, 33), (3, 64), (90, 64)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_query_gradients_of_short_rows(dev, dtype, maps, dk, B, T, causal):
+    """Where a row sees few keys the centre D of dS must not carry the rounding of the kept 16-bit context: dq is off by the f32 errors (those of
+    the f32 form), by dS rounded once as an operand -- half a step of sum |dS| |k| -- and by its own rounding; a row with one key gives next
+    to nothing"""
+    dt, H = DT[dtype], 2
+    u, tiny = half_ulp(dt), 2.0 ** -25 if dtype == "f16" else 0.0
+    q, k, v, _, lam, dout = make(maps, dt, B, T, T, H, H, dk, 0, seed=13)
+    table = torch.zeros(4, H) if maps == 1 else None
+    lens = [max(1, T - 5 * b % T) for b in range(B)]
+    kw = dict(lengths=lens, q_lengths=lens, causal=causal)
+    ref = RefAttention(q, k, v, table, lam, 0.35, dout, H, H, maps, dt=torch.float32, **kw)
+    half = torch.zeros(B, T, H, maps, dk, dtype=torch.float64)
+    split = lambda t, *n: t.double().view(B, T, H, *n)  # noqa: E731
+    Q, K, V, G = split(q, maps, dk), split(k, maps, dk), split(v, -1), split(dout, -1)
+    L = 0.0 if maps == 1 else float((lam.double()[0, 0] @ lam.double()[1, 0]).exp() - (lam.double()[2, 0] @ lam.double()[3, 0]).exp() + 0.35)
+    for b, n in enumerate(lens):
+        see = torch.ones(n, n, dtype=torch.bool).tril() if causal else torch.ones(n, n, dtype=torch.bool)
+        for h in range(H):
+            dp = G[b, :n, h] @ V[b, :n, h].T
+            for m in range(maps):
+                P = (Q[b, :n, h, m] @ K[b, :n, h, m].T * dk ** -0.5).masked_fill(~see, -math.inf).softmax(-1)
+                dS = (1.0, -L)[m] * P * (dp - (P * dp).sum(-1, keepdim=True))
+                half[b, :n, h, m] = dk ** -0.5 * (u * dS.abs()) @ K[b, :n, h, m].abs()
+    leaves = [t.to(dev).requires_grad_() for t in (q, k, v)]
+    rows = torch.tensor(lens, device=dev, dtype=torch.int32)
+    out = call(maps, *leaves, None if table is None else table.to(dev), None if lam is None else lam.to(dev), H, lengths=rows, q_lengths=rows, causal=causal)
+    (dq,) = torch.autograd.grad(out, leaves[:1], dout.to(dev))
+    within(dq, ref.g["dq"], ref.b["dq"] + half.reshape(B, T, -1) + u * ref.g["dq"].abs() + tiny, "dq")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("dk", [32, 64])
 @pytest.mark.parametrize("B", [4, 12])
