@@ -1029,7 +1029,7 @@ def _still(args, names, tensors):
 def _saved_rows(rows):
     """whole numbers per utterance as save_for_backward takes them: refilling one in place before backward raises there, as for any saved
     tensor, instead of masking with other lengths than forward did (one from inference mode has no version to compare: a copy)"""
-    return [t.clone() if t is not None and t.is_inference() else t for t in rows]
+    return [t if t is None or not t.is_inference() else t.clone() for t in rows]
 
 
 def _watched(tensors):
@@ -1039,19 +1039,17 @@ def _watched(tensors):
         or forward_ad._current_level >= 0
 
 
-class _untraced:
-    """While a call's arguments are checked a trace is put aside: the sizes of its tensors are plain numbers then, as ctypes needs them"""
-
-    __slots__ = ("state",)
-
-    def __enter__(self):
-        self.state = torch._C._get_tracing_state()
-        if self.state is not None:
-            torch._C._set_tracing_state(None)
-
-    def __exit__(self, *exc):
-        if self.state is not None:
-            torch._C._set_tracing_state(self.state)
+def _untraced(make, *args):
+    """``make(*args)``; while the arguments of a call are checked a trace is put aside: the sizes of its tensors are plain numbers then, as
+    ctypes needs them"""
+    if not torch._C._is_tracing():
+        return make(*args)
+    state = torch._C._get_tracing_state()
+    torch._C._set_tracing_state(None)
+    try:
+        return make(*args)
+    finally:
+        torch._C._set_tracing_state(state)
 
 
 def _number(x, what):
@@ -1075,8 +1073,7 @@ def _attention_cfg(maps, heads, kv_heads, max_distance, bidirectional, lam_init,
 class AttentionLongFn(Function):
     @staticmethod
     def forward(ctx, q, k, v, table, lam, lengths, q_lengths, q_start, cfg):
-        with _untraced():
-            op = _attention_long_op(q, k, v, _f32_view(table), _f32_view(lam), (lengths, q_lengths, q_start), cfg)
+        op = _untraced(_attention_long_op, q, k, v, _f32_view(table), _f32_view(lam), (lengths, q_lengths, q_start), cfg)
         out, lse, out2 = op.forward(q, any(ctx.needs_input_grad))
         ctx.cfg, ctx.op = cfg, op
         ctx.direct = None
@@ -1165,8 +1162,7 @@ class ResidualNormFn(Function):
         ctx.set_materialize_grads(False)
         f, x = _packed(f), _packed(x)
         params = (gate, post_g, post_b, pre_g, pre_b)
-        with _untraced():
-            op = _residual_norm_op(f, x, params, lengths, cfg)
+        op = _untraced(_residual_norm_op, f, x, params, lengths, cfg)
         y, z, stats = op.forward(f, any(ctx.needs_input_grad))
         ctx.cfg, ctx.op = cfg, op
         ctx.direct = None
