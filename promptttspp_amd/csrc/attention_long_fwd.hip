@@ -655,6 +655,9 @@ int ptpp_attention_long_params(const ptpp_attention_long_args* a, int backward, 
     PTPP_CHECK_ARG(r.ld >= r.w && r.ld < (1 << 24), "%s: row stride %d of %s (rows are %d wide)", who, r.ld, r.n, r.w);
     PTPP_CHECK_ARG(r.s >= 0, "%s: negative batch stride of %s", who, r.n);
   }
+  PTPP_CHECK_ARG((uintptr_t)a->out2 % 16 == 0, "%s: the second map's context is not 16-byte aligned", who);  // (stored like out)
+  const void* words[] = {a->table, a->lam, a->dtable, a->dlam, a->lse, a->k_lengths, a->q_lengths, a->q_start, a->edges};
+  for (const void* w : words) PTPP_CHECK_ARG((uintptr_t)w % 4 == 0, "%s: tables, statistics and lengths must be 4-byte aligned", who);
   if (a->maps == 1) PTPP_CHECK_ARG(a->table, "%s: the bucketed form needs a table", who);
   if (a->maps == 2) {
     PTPP_CHECK_ARG(a->lam, "%s: null lam", who);

@@ -345,6 +345,8 @@ int check(const ptpp_residual_norm_args* a, int backward, RnP* p, const char* wh
   const int al = a->dtype == PTPP_F32 ? 16 : 8;
   const void* ten[] = {a->f, a->x, a->dy, a->dz, a->y, a->z, a->df, a->dx};
   for (const void* q : ten) PTPP_CHECK_ARG((uintptr_t)q % al == 0, "%s: tensors must be %d-byte aligned", who, al);
+  const void* words[] = {a->stats, a->lengths, a->dgate, a->dpost_g, a->dpost_b, a->dpre_g, a->dpre_b};
+  for (const void* w : words) PTPP_CHECK_ARG((uintptr_t)w % 4 == 0, "%s: statistics, lengths and sums must be 4-byte aligned", who);
   const void* par[] = {a->gate, a->post_g, a->post_b, a->pre_g, a->pre_b};
   for (const void* q : par) PTPP_CHECK_ARG((uintptr_t)q % 16 == 0, "%s: parameters must be 16-byte aligned", who);
   *p = RnP{};

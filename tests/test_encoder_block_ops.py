@@ -819,6 +819,37 @@ def test_attention_refusals_on_the_host():
     assert b"attention_long" in lib.ptpp_last_error()
 
 
+def test_misaligned_side_arguments_are_refused():
+    """the second map's context is stored in 16-byte pieces like the output; tables, statistics and lengths are words"""
+    from promptttspp_amd import _lib
+
+    lib = _lib.load()
+
+    def attention(**kw):
+        a = _lib.AttentionLongArgs()
+        for n in ("q", "k", "v", "out", "lam", "lse", "out2"):
+            setattr(a, n, 4096)
+        a.B, a.Tq, a.Tk, a.H, a.Hk, a.dk, a.maps, a.lam_heads, a.dtype, a.scale = 2, 600, 10, 2, 2, 64, 2, 1, _lib.BF16, 0.125
+        a.ldq = a.ldk = a.ldv = a.ldo = 256
+        a.sq = a.so = 600 * 256
+        a.sk = a.sv = 2560
+        for n, x in kw.items():
+            setattr(a, n, x)
+        return a
+
+    assert lib.ptpp_attention_long_ws_bytes(ctypes.byref(attention()), 0) >= 0
+    for kw in (dict(out2=4104), dict(lam=4097), dict(lse=4098), dict(k_lengths=4097), dict(q_lengths=4097), dict(q_start=4098), dict(table=4098)):
+        assert lib.ptpp_attention_long_ws_bytes(ctypes.byref(attention(**kw)), 0) < 0, kw
+        assert lib.ptpp_attention_long_fwd(ctypes.byref(attention(**kw)), None) == -1, kw
+    for kw in (dict(stats=4098), dict(lengths=4097)):
+        n = _lib.ResidualNormArgs()
+        n.f = n.y = 4096
+        n.B, n.T, n.C, n.gate_rows, n.dtype, n.scale, n.eps = 2, 3, 64, 1, _lib.F32, 1.0, 1e-5
+        for k, x in kw.items():
+            setattr(n, k, x)
+        assert lib.ptpp_residual_norm_fwd(ctypes.byref(n), None) == -1, kw
+
+
 def test_launches_beyond_the_grid_are_refused():
     """a launch holds fewer than 2^32 threads: more one-query blocks, or more rows of a norm, are refused before any launch"""
     from promptttspp_amd import _lib, ops
