@@ -411,14 +411,15 @@ int ptpp_attention_win_bwd(const void* q, const void* k, const void* v, const fl
  *   of contiguous channels, row strides ld* and batch strides s* in elements, 16-byte aligned; a head's maps lie side by side.
  *   Hk divides H: query head h reads key / value head h / (H / Hk).  dk % 8 == 0, dk <= 128 (maps == 1) / 64 (maps == 2).
  *   k_lengths / q_lengths (B) int32: keys at or behind k_lengths[b] are never read; query rows at or behind q_lengths[b] give
- *   zeros and receive zeros.  q_start (B) int32: position of query 0 (NULL: 0), qpos_i = q_start + i.  causal: a query sees the
+ *   zeros and receive zeros, whatever the keys hold.  q_start (B) int32: position of query 0 (NULL: 0), qpos_i = q_start + i.  causal: a query sees the
  *   keys j <= qpos_i.  A query that sees no key gives zeros.
  *   Buckets (table (nbuckets, H) f32; Raffel et al. 2020, section 2.1): bidirectional: nbuckets / 2 for j <= qpos, the others
  *   for j > qpos; else all for the distance qpos - j (0 for later keys).  Of such a set of n buckets the first nexact = n / 2
  *   distances have one each, distance d >= nexact lies in bucket nexact + #{t : d >= edges[t]}; edges: HOST, ascending,
- *   n - nexact - 1 of them, in (nexact, max_distance).  max_distance <= 1024.
+ *   n - nexact - 1 of them, in [nexact, max_distance].  max_distance <= 1024.  An entry of -inf, or of -1e30 and lower, hides its keys.
+ *   bf16 / f16: scores, statistics and sums are f32; probabilities and dS are rounded once as matrix operands (dS in f16 scaled).
  *   lse (maps, B, H, TqP) f32, TqP = Tq rounded up to 64: statistics (base 2); NULL in inference.  out2 (B, Tq, H * 2 dk),
- *   row stride H * 2 dk: the second map's context (maps == 2, kept for backward; NULL in inference).
+ *   row stride H * 2 dk, 16-byte aligned: the second map's context (maps == 2, kept for backward; NULL in inference).
  *   Forward needs a workspace of ptpp_attention_long_ws_bytes(a, 0) bytes, backward one of ..(a, 1) (0: none); the size
  *   depends on the shapes alone, and calls that run at the same time need their own.
  *   Backward fills dq / dk_out / dv (every row) and ADDS to dtable (nbuckets, H) / dlam (4, lam_heads, dk) f32 if accumulate,

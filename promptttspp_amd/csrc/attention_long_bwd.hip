@@ -4,8 +4,8 @@
 //   attn_long_dkv_kernel  owns 128 keys, streams queries and dout:   dk, dv, per-block sums of the table's gradient
 //   attn_long_fin_kernel  adds the per-block sums of dtable and dlam in a fixed order
 // The price of the second pass is 2 of 7 products (4 of 14 units with two maps); one pass would need f32 atomics on dq.
-// 24 x 761-1250 of 4 x 64 bf16: dq 79, dk / dv 123 us (380 and 325 TFLOP/s; 800 blocks on 768 and 512 places); 8 x 1317-2000
-// differential: 132 and 265 us (dk / dv: its accumulators leave one wave per SIMD).  Counters of the former dk / dv: vector unit 33 %, matrix
+// 24 x 761-1250 of 4 x 64 bf16, calls back to back: dq 78, dk / dv 119 us (385 and 336 TFLOP/s; 800 blocks on 768 and 512 places);
+// 8 x 1317-2000 differential: 129 and 253 us (dk / dv: its accumulators leave one wave per SIMD).  Counters of the former dk / dv: vector unit 33 %, matrix
 // 18 %, LDS 17 % busy, no bank conflicts, 1.45 waves per SIMD on average -- the second, partly empty round of blocks.
 //
 // D_m: rows of dout . out_m give it only to the rounding of the kept 16-bit context.  That is enough to centre dS where a row sees many keys

@@ -7,7 +7,8 @@
 namespace {
 
 // ---- the softmax of one 32 x 32 patch of scores, a lane = one query and 16 of the keys -----------------------------------
-// No running maximum yet: far below every score that a matrix instruction of finite operands gives, and still a finite reference
+// No running maximum yet: far below every score that a matrix instruction of finite operands gives, and still a finite reference.  A table entry
+// of -1e30 (-1.44e30 in base 2) stays below it for good: it hides its keys
 constexpr float LA_NONE = -1.0e30f;
 // The reference is raised only when a score passes it by more than this (base 2): probabilities up to 2^6 are as exact in every
 // element type, and the rescaling of the context -- as many operations as there are scores -- almost never happens (with two waves per
@@ -66,8 +67,9 @@ __device__ __forceinline__ float la_probs(f32x16& s, float mul, float add) {
 
 // One block = 128 query rows of one (utterance, head), a wave = 32 of them; keys and values stream through LDS in tiles of 64,
 // the next tile's LDS-DMA under the current tile's products.  Bound by the vector unit: about 120 instructions and 16 exponentials (a quarter
-// of the rate) per 32 x 32 patch of 64 channels, 617 cycles against 256 of matrix work.  2 x 6001 of 8 x 64 f16 200 us, 740 TFLOP/s;
-// 24 x 761-1250 of 4 x 64 bf16 62 us (800 blocks on 768 places); 8 x 1317-2000 differential 127 us.
+// of the rate) per 32 x 32 patch of 64 channels, 617 cycles against 256 of matrix work.  In calls back to
+// back 2 x 6001 of 8 x 64 f16 210 us, 700 TFLOP/s; 24 x 761-1250 of 4 x 64 bf16 62 us (800 blocks on 768 places); 8 x 1317-2000
+// differential 117 us.
 template <typename E, int DK, int DV, int MAPS, bool BIAS>
 __global__ __launch_bounds__(256, sizeof(E) == 4 ? 1 : 2) void attn_long_fwd_kernel(const LongP p) {
   constexpr int CH = LOp<E>::CH, KS = DK / (2 * CH), PS = 16 / CH, NT = DV / 32;
@@ -233,7 +235,7 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 ? 1 : 2) void attn_long_fwd_ker
 // each streaming its own chunks through its own two LDS buffers (no block barrier in the loop), and join at the end.  With more
 // than one range the blocks leave unnormalised sums and (max, sum) for the join kernel.  A step is HBM-bound: every key and value is
 // read once, two chunks per wave on their way (one query on 16 x 4001, differential f16: 51 us with one chunk ahead, 47 us with two;
-// on 32 x 8191 of 12 heads on 4 x 64 bf16: 39 us, 5.5 TB/s).
+// on 32 x 8191 of 12 heads on 4 x 64 bf16: 40 us, 5.4 TB/s).
 template <typename E, int DK, int DV, int MAPS, bool BIAS, bool REST>
 __global__ __launch_bounds__((LSplit<E, DK, DV, MAPS>::W * 64), sizeof(E) == 4 || MAPS * DV == 256 ? 1 : 2) void attn_long_split_kernel(const LongP p) {
   typedef LSplit<E, DK, DV, MAPS> S_;

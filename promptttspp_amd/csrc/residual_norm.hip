@@ -8,7 +8,7 @@
 // whole row: every tensor element is touched once, means and squared deviations are two passes over registers.  In backward a lane
 // group walks over rows of one utterance with the column sums in registers; the block adds its groups in a fixed order and writes
 // one partial row per sum, a finishing launch adds the partial rows (no atomics: the same bits on every run).  24 x 875-1250 of 256 bf16:
-// forward 19 us (2.9 TB/s), backward 31 + 5 us; 8 x 1638-2048 of 1024 f16: forward 31 us (4.1 TB/s), backward 65 + 4.5 us (3 TB/s).
+// forward 19 us (2.9 TB/s), backward 30 + 5 us; 8 x 1638-2048 of 1024 f16: forward 30 us (4.2 TB/s), backward 67 + 4.3 us (2.9 TB/s).
 #include "ptpp_common.h"
 
 namespace {

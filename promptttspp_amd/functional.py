@@ -1126,16 +1126,22 @@ def attention_bucket(q, k, v, table, heads, kv_heads=None, max_distance=128, bid
                      causal=False, scale=None):
     """Attention with a learned relative-position bias by buckets: softmax(scale * q k^T + table[bucket(j - i), head]) v -> (B, Tq, H * dk).
 
-    q (B, Tq, heads * dk), k / v (B, Tk, kv_heads * dk): contiguous channels, any row and batch stride, 16-byte aligned rows (slices of
-    a fused projection as they are); ``k = v = None``: q is the fused (B, T, q | k | v) projection of self-attention.  Query head h
+    q (B, Tq, heads * dk), k / v (B, Tk, kv_heads * dk): contiguous channels, 16-byte aligned rows that do not overlap, any batch stride (slices
+    of a fused projection as they are); ``k = v = None``: q is the fused (B, T, q | k | v) projection of self-attention.  Query head h
     reads key / value head h // (heads // kv_heads).  dk: a multiple of 8, at most 128; f32, bf16 or f16.  ``table`` (buckets, heads):
     bucket of a distance as ``ops.bucket_edges`` (two-sided; ``bidirectional=False``: later keys share bucket 0).
     ``lengths`` (B): valid keys (None: all); ``q_lengths`` (B): valid queries, the others give zeros (None: as ``lengths`` for the fused
     form, else all); rows behind them are never read.  ``q_start`` (B): position of the first query among the keys (None: 0) -- a step
     of one query against a kept memory of n keys has ``q_start = n - 1``; ``causal``: only keys at or before the query's position.
-    A query that sees no key gives zeros; a table entry of -inf (or below -1e30) hides its keys like a mask.  Keys behind the lengths, and for
-    ``causal`` keys behind the last query, are not read in forward; a value that only ``causal`` hides from an earlier query has to be finite,
-    as has a gradient: it may still be multiplied by zero.  ``scale``: positive, default dk ** -0.5.  Memory O(Tq + Tk) in both directions."""
+    A query that sees no key gives zeros; a table entry of -inf, or of -1e30 and lower, hides its keys like a mask (a finite one of -1e5 or
+    lower for every key that a row sees leaves its f32 statistics too few digits: the row's gradients are off).  Keys behind the lengths, and
+    for ``causal`` keys behind the last query, are not read in forward; a value that only ``causal`` or the table hides has to be finite, as
+    has a gradient: it may still be multiplied by zero.  ``scale``: positive, default dk ** -0.5.  Memory O(Tq + Tk) in both directions.
+
+    Scores, softmax statistics and all sums are f32.  bf16 / f16: probabilities and dS are rounded once to the element type as operands of
+    the matrix instructions, beside the rounding of the result: errors of about 1.4 times the latter (without a gradient, where there are few
+    queries: probabilities as two operands, errors of the result's rounding alone).  ``lengths``, ``q_lengths`` and ``q_start`` are saved for backward: int32 tensors on the device
+    must not be refilled in place before it (it raises)."""
     if table is None:
         raise ValueError("attention_bucket: needs a position table")
     cfg = _attention_cfg(1, heads, kv_heads, max_distance, bidirectional, 0.0, causal, scale)
@@ -1149,7 +1155,7 @@ def attention_diff(q, k, v, lam, lam_init, heads, kv_heads=None, table=None, max
 
     q (B, Tq, heads * 2 dk), k / v (B, Tk, kv_heads * 2 dk): a head's two maps lie side by side in q and k, its value is 2 dk wide; dk a
     multiple of 8, at most 64.  ``lam`` (4, 1 or heads, dk).  ``table`` (optional): the position bias of ``attention_bucket``, the same for
-    both maps.  Everything else as there.  The norm over a head that usually follows is ``residual_norm`` without a residual."""
+    both maps.  Everything else, roundings included, as there (for backward the second map's context is kept in the element type).  The norm over a head that usually follows is ``residual_norm`` without a residual."""
     if lam is None:
         raise ValueError("attention_diff: needs the lam vectors")
     cfg = _attention_cfg(2, heads, kv_heads, max_distance, bidirectional, lam_init, causal, scale)
@@ -1221,8 +1227,8 @@ def residual_norm(f, x=None, gate=None, post=None, pre=None, scale=1.0, eps=1e-5
     f: a block's output, x: the residual stream (None: y = scale * gate * u), both (B, T, C) of one dtype (f32, bf16, f16), C a multiple
     of 4, at most 4096.  ``post`` / ``pre``: (gamma, beta) of the norm behind the block and of the norm before the next one, or None (no
     such norm; without ``pre`` z is None); ``kind``: "layer", or "rms" (beta None).  ``gate``: None, (C,) or one row per utterance (B, C),
-    f32.  Rows at or behind ``lengths`` (B) are not read, give zeros and get zero gradients.  y is rounded to the tensors' dtype once; z is
-    computed from the unrounded y."""
+    f32.  Rows at or behind ``lengths`` (B) are not read, give zeros and get zero gradients (an int32 tensor on the device is saved for backward:
+    refilled in place before it, backward raises).  y is rounded to the tensors' dtype once; z is computed from the unrounded y."""
     post_g, post_b = post if post is not None else (None, None)
     pre_g, pre_b = pre if pre is not None else (None, None)
     cfg = SimpleNamespace(scale=_number(scale, "residual_norm: scale"), eps=_number(eps, "residual_norm: eps"), kind=kind)
