@@ -13,7 +13,7 @@
 // corrects it.  But the table's
 // gradient is a sum with heavy cancellation (every row of dS adds up to zero), so the dq pass also sums P_m (dP - D_m') in f32 and
 // the dk / dv pass uses the corrected D_m.  lam's gradient adds the D_1 of all rows (50000 of 8 x 1317-2000, of either sign), and takes that
-// sum as exact as its terms are, at no operation per pair (EXACT; error of such a D_1 against 64 bits 1.7e-7 -> 0.9e-7, of dlam 1.8e-4 -> 0.34e-4
+// sum as exact as its terms are, at no operation per pair (EXACT; error of such a D_1 against 64 bits 1.7e-7 -> 0.9e-7, of dlam 1.8e-4 -> 0.46e-4
 // where plain f32 has 0.9e-4; backward of 8 x 1333-2000 bf16 385 -> 389 us):
 //   - D' rounded to the grid of dP's largest values (la_grid): dP - D' is then exact, else it is rounded the same way for all pairs of a row;
 //   - P taken against lse - log2(keys) / 2, a whole number, instead of lse (la_half_lse): a row spread over n keys has scores log2(n) below lse,
@@ -147,9 +147,13 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
 #pragma unroll
       for (int s = 0; s < VS; ++s) vn += la_dot<E>(vf[s], vf[s]);
       vn = la_half_sum(vn);
+      float lg = vn > 0.f ? log2f(vn) : 0.f, cnt = vn > 0.f ? 1.f : 0.f;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) vn = fmaxf(vn, __shfl_xor(vn, o, 64));
-      size = sqrtf(la_half_sum(dn)) * sqrtf(vn);
+      for (int o = 16; o > 0; o >>= 1) {  // (the geometric mean: one key of another size must not coarsen the others' grid)
+        lg += __shfl_xor(lg, o, 64);
+        cnt += __shfl_xor(cnt, o, 64);
+      }
+      size = 2.f * sqrtf(la_half_sum(dn)) * exp2f(0.5f * lg / fmaxf(cnt, 1.f));
     }
     if constexpr (FLIP) {
       const uint32_t flip = lq & 1 ? 0x80008000u : 0u;

@@ -422,6 +422,34 @@ def test_query_gradients_of_short_rows(dev, dtype, maps, dk, B, T, causal):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("maps,dk", [(1, 64), (2, 32), (2, 64)])
+@pytest.mark.parametrize("B,T,at", [(2, 300, 0), (2, 300, 200), (60, 140, 0)])
+def test_one_value_of_another_size(dev, maps, dk, B, T, at):
+    """a key that next to no query sees, with values 10^4 times the others': nothing of it shows in the others' gradients (f32)"""
+    H = 2
+    q, k, v, table, lam, dout = make(maps, torch.float32, B, T, T, H, H, dk, 16, seed=21)
+    q.view(B, T, H, maps, dk)[..., 0] = 20.0
+    k.view(B, T, H, maps, dk)[..., 0] = 0.0
+    k.view(B, T, H, maps, dk)[:, at, ..., 0] = -4.0 * dk ** 0.5   # 80 below the others: seen with 10^-34
+    v[:, at] *= 1e4
+    ref = RefAttention(q, k, v, table, lam, 0.35, dout, H, H, maps)
+    leaves = [t.to(dev).requires_grad_() for t in (q, k, v, table) + ((lam,) if maps == 2 else ())]
+    full = leaves + [None] * (5 - len(leaves))
+    grads = torch.autograd.grad(call(maps, *full, H), leaves, dout.to(dev))
+    seen = torch.ones(T, dtype=torch.bool)
+    seen[at] = False
+    for n, t in zip(("dq", "dk", "dv"), grads):
+        rows = slice(None) if n == "dq" else seen
+        within(t[:, rows], ref.g[n][:, rows], ref.b[n][:, rows], n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("maps", [1, 2])
+def test_table_entries_of_minus_1e30_hide_keys(dev, maps):
+    test_table_entries_that_hide_keys(dev, maps, -1e30, 150, 150)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("dk", [32, 64])
 @pytest.mark.parametrize("B", [4, 12])
