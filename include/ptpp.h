@@ -411,8 +411,8 @@ int ptpp_attention_win_bwd(const void* q, const void* k, const void* v, const fl
  *   of contiguous channels, row strides ld* and batch strides s* in elements, 16-byte aligned; a head's maps lie side by side.
  *   Hk divides H: query head h reads key / value head h / (H / Hk).  dk % 8 == 0, dk <= 128 (maps == 1) / 64 (maps == 2).
  *   k_lengths / q_lengths (B) int32: keys at or behind k_lengths[b] are never read; query rows at or behind q_lengths[b] give
- *   zeros and receive zeros, whatever the keys hold.  q_start (B) int32: position of query 0 (NULL: 0), qpos_i = q_start + i.  causal: a query sees the
- *   keys j <= qpos_i.  A query that sees no key gives zeros.
+ *   zeros and receive zeros, whatever the keys hold.  q_start (B) int32: position of query 0 (NULL: 0), qpos_i = q_start + i.
+ *   causal: a query sees the keys j <= qpos_i.  A query that sees no key gives zeros.
  *   Buckets (table (nbuckets, H) f32; Raffel et al. 2020, section 2.1): bidirectional: nbuckets / 2 for j <= qpos, the others
  *   for j > qpos; else all for the distance qpos - j (0 for later keys).  Of such a set of n buckets the first nexact = n / 2
  *   distances have one each, distance d >= nexact lies in bucket nexact + #{t : d >= edges[t]}; edges: HOST, ascending,

@@ -5,16 +5,15 @@
 //   attn_long_fin_kernel  adds the per-block sums of dtable and dlam in a fixed order
 // The price of the second pass is 2 of 7 products (4 of 14 units with two maps); one pass would need f32 atomics on dq.
 // 24 x 761-1250 of 4 x 64 bf16, calls back to back: dq 78, dk / dv 119 us (385 and 336 TFLOP/s; 800 blocks on 768 and 512 places);
-// 8 x 1317-2000 differential: 129 and 253 us (dk / dv: its accumulators leave one wave per SIMD).  Counters of the former dk / dv: vector unit 33 %, matrix
-// 18 %, LDS 17 % busy, no bank conflicts, 1.45 waves per SIMD on average -- the second, partly empty round of blocks.
+// 8 x 1317-2000 differential: 129 and 253 us (dk / dv: its accumulators leave one wave per SIMD).  Counters of the former dk / dv: vector
+// unit 33 %, matrix 18 %, LDS 17 % busy, no bank conflicts, 1.45 waves per SIMD on average -- the second, partly empty round of blocks.
 //
-// D_m: rows of dout . out_m give it only to the rounding of the kept 16-bit context.  That is enough to centre dS where a row sees many keys
-// (in dq the centre's error is multiplied by the mean of their k), not where it sees few: up to LA_TWICE of them a first sweep of the block
-// corrects it.  But the table's
-// gradient is a sum with heavy cancellation (every row of dS adds up to zero), so the dq pass also sums P_m (dP - D_m') in f32 and
-// the dk / dv pass uses the corrected D_m.  lam's gradient adds the D_1 of all rows (50000 of 8 x 1317-2000, of either sign), and takes that
-// sum as exact as its terms are, at no operation per pair (EXACT; error of such a D_1 against 64 bits 1.7e-7 -> 0.9e-7, of dlam 1.8e-4 -> 0.46e-4
-// where plain f32 has 0.9e-4; backward of 8 x 1333-2000 bf16 385 -> 389 us):
+// D_m: rows of dout . out_m give it only to the rounding of the kept 16-bit context.  That is enough to centre dS where a row sees many keys (in
+// dq the centre's error is multiplied by the mean of their k); where a block sees few, up to LA_TWICE, a first sweep corrects it.  The table's
+// gradient is a sum with heavy cancellation (every row of dS adds up to zero), so the dq pass also sums P_m (dP - D_m') in f32 and the dk / dv
+// pass uses the corrected D_m.  lam's gradient adds the D_1 of all rows (50000 of 8 x 1317-2000, of either sign), and takes that sum as exact as
+// its terms are, at no operation per pair (EXACT; error of such a D_1 against 64 bits 1.7e-7 -> 0.9e-7, of dlam 1.8e-4 -> 0.46e-4 where plain
+// f32 has 0.9e-4; backward of 8 x 1333-2000 bf16 385 -> 389 us):
 //   - D' rounded to the grid of dP's largest values (la_grid): dP - D' is then exact, else it is rounded the same way for all pairs of a row;
 //   - P taken against lse - log2(keys) / 2, a whole number, instead of lse (la_half_lse): a row spread over n keys has scores log2(n) below lse,
 //     whose rounding would grow with that; the factor is applied to the row's sums;
@@ -118,7 +117,7 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
     const E* o2 = reinterpret_cast<const E*>(p.out2) + ((int64_t)b * p.Tq + iq) * ((int64_t)p.H * dv) + (int64_t)h * dv;
     float d0 = 0.f, d1 = 0.f, dn = 0.f, vn = 0.f;
     uint4 vf[EXACT ? VS : 1];
-    if constexpr (EXACT) {  // |v| of the first 32 keys and |dout|: dP's size
+    if constexpr (EXACT) {  // |v| of the first 32 keys, and |dout|: dP's size
 #pragma unroll
       for (int s = 0; s < VS; ++s) {
         const int c = (2 * s + hw) * CH;

@@ -1070,6 +1070,9 @@ def _attention_cfg(maps, heads, kv_heads, max_distance, bidirectional, lam_init,
                            scale=None if scale is None else _number(scale, "attention: scale"))
 
 
+_ATTENTION_INPUTS = ("q", "table", "lam", "k_lengths", "q_lengths", "q_start", "k", "v")
+
+
 class AttentionLongFn(Function):
     @staticmethod
     def forward(ctx, q, k, v, table, lam, lengths, q_lengths, q_start, cfg):
@@ -1089,8 +1092,7 @@ class AttentionLongFn(Function):
     def backward(ctx, dout):
         q, k, v, table, lam, out, lse, out2, *rows = ctx.saved_tensors
         op = ctx.op
-        names = ("q", "table", "lam", "k_lengths", "q_lengths", "q_start") if k is None else ("q", "table", "lam", "k_lengths", "q_lengths", "q_start", "k", "v")
-        if not _still(op.args, names, (q, table, lam, *rows, k, v)):
+        if not _still(op.args, _ATTENTION_INPUTS[:6] if k is None else _ATTENTION_INPUTS, (q, table, lam, *rows, k, v)):
             op = _attention_long_op(q, k, v, _f32_view(table), _f32_view(lam), rows, ctx.cfg)
         dout = _packed(dout)
         direct = ctx.direct is not None
@@ -1140,8 +1142,8 @@ def attention_bucket(q, k, v, table, heads, kv_heads=None, max_distance=128, bid
 
     Scores, softmax statistics and all sums are f32.  bf16 / f16: probabilities and dS are rounded once to the element type as operands of
     the matrix instructions, beside the rounding of the result: errors of about 1.4 times the latter (without a gradient, where there are few
-    queries: probabilities as two operands, errors of the result's rounding alone).  ``lengths``, ``q_lengths`` and ``q_start`` are saved for backward: int32 tensors on the device
-    must not be refilled in place before it (it raises)."""
+    queries: probabilities as two operands, errors of the result's rounding alone).  ``lengths``, ``q_lengths`` and ``q_start`` are saved for
+    backward: int32 tensors on the device must not be refilled in place before it (it raises)."""
     if table is None:
         raise ValueError("attention_bucket: needs a position table")
     cfg = _attention_cfg(1, heads, kv_heads, max_distance, bidirectional, 0.0, causal, scale)
@@ -1155,7 +1157,8 @@ def attention_diff(q, k, v, lam, lam_init, heads, kv_heads=None, table=None, max
 
     q (B, Tq, heads * 2 dk), k / v (B, Tk, kv_heads * 2 dk): a head's two maps lie side by side in q and k, its value is 2 dk wide; dk a
     multiple of 8, at most 64.  ``lam`` (4, 1 or heads, dk).  ``table`` (optional): the position bias of ``attention_bucket``, the same for
-    both maps.  Everything else, roundings included, as there (for backward the second map's context is kept in the element type).  The norm over a head that usually follows is ``residual_norm`` without a residual."""
+    both maps.  Everything else, roundings included, as there (for backward the second map's context is kept in the element type).  The norm
+    over a head that usually follows is ``residual_norm`` without a residual."""
     if lam is None:
         raise ValueError("attention_diff: needs the lam vectors")
     cfg = _attention_cfg(2, heads, kv_heads, max_distance, bidirectional, lam_init, causal, scale)
