@@ -9,7 +9,7 @@
 // unit 33 %, matrix 18 %, LDS 17 % busy, no bank conflicts, 1.45 waves per SIMD on average -- the second, partly empty round of blocks.
 //
 // D_m: rows of dout . out_m give it only to the rounding of the kept 16-bit context.  That is enough to centre dS where a row sees many keys (in
-// dq the centre's error is multiplied by the mean of their k); where a block sees few, up to LA_TWICE, a first sweep corrects it.  The table's
+// dq the centre's error is multiplied by the mean of their k); where a block's rows see few, up to LA_TWICE, a first sweep corrects it.  The table's
 // gradient is a sum with heavy cancellation (every row of dS adds up to zero), so the dq pass also sums P_m (dP - D_m') in f32 and the dk / dv
 // pass uses the corrected D_m.  lam's gradient adds the D_1 of all rows (50000 of 8 x 1317-2000, of either sign), and takes that sum as exact as
 // its terms are, at no operation per pair (EXACT; error of such a D_1 against 64 bits 1.7e-7 -> 0.9e-7, of dlam 1.8e-4 -> 0.46e-4 where plain
@@ -37,7 +37,7 @@ struct LBwd {
   static constexpr int NB = FEW ? LSplit<E, DK, DV, MAPS>::NB : 2;
 };
 
-// Most keys of a block, 16-bit, for which the centre is corrected before dq is summed.  Error of dq against 64 bits, in units of its output's
+// Most keys of a row, 16-bit, for which the centre is corrected before dq is summed.  Error of dq against 64 bits, in units of its output's
 // rounding, without and with: 2-12 keys 1.6-3.4 and 1.4, 16-41 keys 1.5-1.6 and 1.4, 63-128 keys 1.5 and 1.4.  Backward, us: 32 x 64 of
 // 2 x 128 27.8 and 29.9, 200 x 64 of 4 x 64 49 and 53; up to 128 keys 200 x 128 of 4 x 64 would go from 74 to 82.
 constexpr int LA_TWICE = 64;
@@ -251,7 +251,7 @@ __global__ __launch_bounds__((LBwd<E, DK, DV, MAPS, FEW>::W * 64), sizeof(E) == 
   };
   if constexpr (FEW && BIAS) la_barrier();  // (the table; the loop itself has no barrier)
   if constexpr (sizeof(E) == 2) {
-    if (kend <= LA_TWICE) {  // (the whole block: kend is the same in all its waves)
+    if (kend <= LA_TWICE || (p.causal && qs + ib < LA_TWICE)) {  // (the whole block; causal: its first rows see few, and it is a short one)
       sweep(std::true_type{});
 #pragma unroll
       for (int m = 0; m < MAPS; ++m) {

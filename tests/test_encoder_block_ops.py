@@ -389,12 +389,12 @@ def test_f16_gradients_of_any_size(dev, maps, dk, B, T, power):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("maps,dk", [(1, 64), (1, 128), (2, 32), (2, 64)])
-@pytest.mark.parametrize("B,T", [(3, 2), (3, 7), (3, 33), (3, 64), (90, 64)])
-@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("B,T,causal", [(3, 2, False), (3, 2, True), (3, 7, False), (3, 7, True), (3, 33, False), (3, 33, True), (3, 64, False), (3, 64, True),
+                                        (90, 64, False), (90, 64, True), (2, 300, True), (50, 150, True)])
 def test_query_gradients_of_short_rows(dev, dtype, maps, dk, B, T, causal):
     """Where a row sees few keys the centre D of dS must not carry the rounding of the kept 16-bit context: dq is off by the f32 errors (those of
     the f32 form), by dS rounded once as an operand -- half a step of sum |dS| |k| -- and by its own rounding; a row with one key gives next
-    to nothing"""
+    to nothing.  Long sequences: the first 64 rows under the causal rule"""
     dt, H = DT[dtype], 2
     u, tiny = half_ulp(dt), 2.0 ** -25 if dtype == "f16" else 0.0
     q, k, v, _, lam, dout = make(maps, dt, B, T, T, H, H, dk, 0, seed=13)
@@ -418,7 +418,8 @@ def test_query_gradients_of_short_rows(dev, dtype, maps, dk, B, T, causal):
     rows = torch.tensor(lens, device=dev, dtype=torch.int32)
     out = call(maps, *leaves, None if table is None else table.to(dev), None if lam is None else lam.to(dev), H, lengths=rows, q_lengths=rows, causal=causal)
     (dq,) = torch.autograd.grad(out, leaves[:1], dout.to(dev))
-    within(dq, ref.g["dq"], ref.b["dq"] + half.reshape(B, T, -1) + u * ref.g["dq"].abs() + tiny, "dq")
+    bound = ref.b["dq"] + half.reshape(B, T, -1) + u * ref.g["dq"].abs() + tiny
+    within(dq[:, :64], ref.g["dq"][:, :64], bound[:, :64], "dq")
 
 
 @pytest.mark.gpu
